@@ -101,6 +101,29 @@ int tb200_rms_norm_bwd(void* dx, void* dweight, void* dbias /*nullable*/, const 
                        int64_t col_stride, int64_t partial_cols, float eps, int dtype,
                        void* stream);
 
+/* ---- Gated residual RMSNorm ----------------------------------------------
+ * The step between two blocks (not in the reference, which has RMSNorm alone):
+ *   n = x / (rms(x) + eps) * w1   (w1 null: n = x)
+ *   y = residual_scale * r + gate * n   (gate null: 1)
+ *   h = y / (rms(y) + eps) * w2,   rms(v) = sqrt(mean(v^2))
+ * x, r, y, h are contiguous [rows, cols]; w1, w2 [cols]; gate is [cols] (rows_per_gate 0) or
+ * [rows / rows_per_gate, cols]. rms1 (unused without w1) and rms2 [rows] are kept for backward. */
+int tb200_gated_residual_rms_norm_fwd(void* h, void* y, float* rms1, float* rms2, const void* x, const void* r,
+                                      const void* w1 /*nullable*/, const void* w2, const void* gate /*nullable*/,
+                                      int64_t rows, int64_t cols, int64_t rows_per_gate, float residual_scale,
+                                      float eps, int dtype, void* stream);
+/* dx, dr and (each nullable) dw1, dw2, dgate (shaped as gate) from dh and dy, one of which may be
+ * null (zero). The workspace holds per-CTA column partials; none is needed when dw1, dw2 and dgate
+ * are null, or for a dgate with rows_per_gate 1 alone. */
+size_t tb200_gated_residual_rms_norm_bwd_workspace(int64_t rows, int64_t cols, int64_t rows_per_gate);
+int tb200_gated_residual_rms_norm_bwd(void* dx, void* dr, void* dw1 /*nullable*/, void* dw2 /*nullable*/,
+                                      void* dgate /*nullable*/, const void* dh /*nullable*/,
+                                      const void* dy /*nullable*/, const void* x, const void* r,
+                                      const void* w1 /*nullable*/, const void* w2, const void* gate /*nullable*/,
+                                      const float* rms1, const float* rms2, void* workspace, size_t workspace_bytes,
+                                      int64_t rows, int64_t cols, int64_t rows_per_gate, float residual_scale,
+                                      float eps, int dtype, void* stream);
+
 /* ---- Softmax / MaskedSoftmax -------------------------------------------
  * Replaces kernel.Softmax.forward (trident/kernel/softmax.py:29-106, launched at
  * trident/operation/softmax.py:57) and kernel.MaskedSoftmax.forward

@@ -5,6 +5,7 @@ the current CUDA stream, and raises on a non-zero status. There is no CPU or PyT
 fallback: without the built library, or without a CUDA device, the calls fail loudly.
 """
 
+import contextlib
 import ctypes
 import os
 
@@ -39,6 +40,12 @@ SIGNATURES = {
     "tb200_rms_norm_fwd": (c_int, [c_ptr] * 5 + [c_i64] * 5 + [c_f32, c_int, c_ptr]),
     "tb200_rms_norm_bwd_workspace": (c_size, [c_i64, c_i64]),
     "tb200_rms_norm_bwd": (c_int, [c_ptr] * 8 + [c_size] + [c_i64] * 5 + [c_f32, c_int, c_ptr]),
+    "tb200_gated_residual_rms_norm_fwd": (c_int, [c_ptr] * 9 + [c_i64] * 3 + [c_f32] * 2 + [c_int, c_ptr]),
+    "tb200_gated_residual_rms_norm_bwd_workspace": (c_size, [c_i64] * 3),
+    "tb200_gated_residual_rms_norm_bwd": (
+        c_int,
+        [c_ptr] * 15 + [c_size] + [c_i64] * 3 + [c_f32] * 2 + [c_int, c_ptr],
+    ),
     "tb200_reduce_fwd": (c_int, [c_ptr] * 3 + [c_i64] * 4 + [c_int, c_f32, c_int, c_ptr]),
     "tb200_reduce_bwd": (c_int, [c_ptr] * 4 + [c_i64] * 4 + [c_int, c_f32, c_int, c_ptr]),
     "tb200_softmax_fwd": (c_int, [c_ptr] * 3 + [c_i64] * 6 + [c_int, c_ptr]),
@@ -151,6 +158,21 @@ def _require_cuda(*tensors):
             raise Tb200Error("trident_b200 kernels run on CUDA tensors only (no CPU fallback)")
 
 
+def _on_device(tensor):
+    """Context in which `tensor`'s device is the current one (a launch goes to the current device)."""
+    if torch.cuda.current_device() == tensor.device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(tensor.device)
+
+
+def require_one_device(**tensors):
+    """All given tensors (None allowed) lie on one CUDA device."""
+    _require_cuda(*tensors.values())
+    devices = {t.device for t in tensors.values() if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{', '.join(n for n, t in tensors.items() if t is not None)} should be on the same device.")
+
+
 def _strides4(t):
     return (c_i64 * 4)(*t.stride())
 
@@ -224,6 +246,37 @@ def rms_norm_bwd(dx, dweight, dbias, dy, x, weight, rms, workspace, rows, cols, 
         ),
         "tb200_rms_norm_bwd",
     )
+
+
+def gated_residual_rms_norm_fwd(h, y, rms1, rms2, x, r, w1, w2, gate, rows, cols, rows_per_gate, scale, eps):
+    _require_cuda(h, y, x, r, w1, w2, gate)
+    with _on_device(x):
+        _check(
+            load().tb200_gated_residual_rms_norm_fwd(
+                _ptr(h), _ptr(y), _ptr(rms1), _ptr(rms2), _ptr(x), _ptr(r), _ptr(w1), _ptr(w2), _ptr(gate),
+                rows, cols, rows_per_gate, scale, eps, dtype_code(x.dtype), _stream(x),
+            ),
+            "tb200_gated_residual_rms_norm_fwd",
+        )
+
+
+def gated_residual_rms_norm_bwd_workspace(rows, cols, rows_per_gate):
+    return load().tb200_gated_residual_rms_norm_bwd_workspace(rows, cols, rows_per_gate)
+
+
+def gated_residual_rms_norm_bwd(dx, dr, dw1, dw2, dgate, dh, dy, x, r, w1, w2, gate, rms1, rms2, workspace, rows,
+                                cols, rows_per_gate, scale, eps):
+    _require_cuda(dx, dr, dw1, dw2, dgate, dh, dy, x, r, w1, w2, gate)
+    with _on_device(x):
+        _check(
+            load().tb200_gated_residual_rms_norm_bwd(
+                _ptr(dx), _ptr(dr), _ptr(dw1), _ptr(dw2), _ptr(dgate), _ptr(dh), _ptr(dy), _ptr(x), _ptr(r),
+                _ptr(w1), _ptr(w2), _ptr(gate), _ptr(rms1), _ptr(rms2), _ptr(workspace),
+                0 if workspace is None else workspace.numel() * workspace.element_size(),
+                rows, cols, rows_per_gate, scale, eps, dtype_code(x.dtype), _stream(x),
+            ),
+            "tb200_gated_residual_rms_norm_bwd",
+        )
 
 
 REDUCE_KINDS = {"sum": 0, "mean": 1, "var": 2, "var_mean": 3}

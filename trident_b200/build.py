@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(HERE, "libtb200.so")
 SOURCES = [
     "api.cu",
     "row_norm.cu",
+    "residual_norm.cu",
     "softmax.cu",
     "reduce.cu",
     "gemm_simt.cu",

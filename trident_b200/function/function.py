@@ -8,6 +8,7 @@ import torch
 from trident_b200 import operation
 
 __all__ = [
+    "gated_residual_rms_norm",
     "geglu",
     "layer_norm",
     "linear",
@@ -21,6 +22,31 @@ __all__ = [
     "var",
     "var_mean",
 ]
+
+
+def gated_residual_rms_norm(
+    input: torch.Tensor,
+    residual: torch.Tensor,
+    post_weight: torch.Tensor = None,
+    pre_weight: torch.Tensor = None,
+    gate: torch.Tensor = None,
+    residual_scale: float = 1.0,
+    eps: float = 1e-08,
+):
+    """
+    Applies the step between two blocks of a transformer (not in the reference): the norm after a block,
+    its gate, the scaled residual and the norm before the next block.
+
+        output_residual = residual_scale * residual + gate * rms_norm(input, -1.0, post_weight)
+        output = rms_norm(output_residual, -1.0, pre_weight)
+
+    Without post_weight the input is not normalised, without gate it is not scaled. The gate holds one
+    value per feature ([features]), or has the dimensions of the input with ones from some dimension on
+    ([batch, 1, features]: one vector per sequence). Returns (output, output_residual).
+
+    See GatedResidualRMSNorm for details.
+    """
+    return operation.GatedResidualRMSNorm.apply(input, residual, post_weight, pre_weight, gate, residual_scale, eps)
 
 
 def geglu(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None, use_accelerator: bool = False):

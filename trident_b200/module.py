@@ -9,7 +9,7 @@ import torch
 
 from trident_b200 import function, util
 
-__all__ = ["GEGLU", "LayerNorm", "Linear", "MaskedSoftmax", "Mean", "RMSNorm", "ScaledDotProductAttention",
+__all__ = ["GatedResidualRMSNorm", "GEGLU", "LayerNorm", "Linear", "MaskedSoftmax", "Mean", "RMSNorm", "ScaledDotProductAttention",
            "Softmax", "Sum", "Var", "VarMean"]
 
 
@@ -172,6 +172,60 @@ class RMSNorm(torch.nn.Module):
             f"p={self.p}, "
             f"eps={self.eps}, "
             f"bias={self.bias is not None}, "
+            f"backend=Trident"
+        )
+
+
+class GatedResidualRMSNorm(torch.nn.Module):
+    """Module form of function.gated_residual_rms_norm: the norm after a block (left out with
+    post_norm=False), a gate with one value per feature (left out with gate=False; another gate can be
+    passed to forward), the residual and the norm before the next block. Returns (output, residual)."""
+
+    def __init__(
+        self,
+        normalized_shape: int,
+        post_norm: bool = True,
+        gate: bool = True,
+        residual_scale: float = 1.0,
+        eps: float = 1e-05,
+        device=None,
+        dtype=None,
+    ):
+        super().__init__()
+        factory_kwargs = {"device": device, "dtype": dtype}
+        self.normalized_shape = _shape_tuple(normalized_shape)
+        self.residual_scale = residual_scale
+        self.eps = eps
+        for name, used in (("post_weight", post_norm), ("pre_weight", True), ("gate", gate)):
+            if used:
+                setattr(self, name, torch.nn.Parameter(torch.empty(self.normalized_shape, **factory_kwargs)))
+            else:
+                self.register_parameter(name, None)
+        self.reset_parameters()
+
+    def forward(self, input: torch.Tensor, residual: torch.Tensor, gate: torch.Tensor = None):
+        return function.gated_residual_rms_norm(
+            input,
+            residual,
+            self.post_weight,
+            self.pre_weight,
+            self.gate if gate is None else gate,
+            self.residual_scale,
+            self.eps,
+        )
+
+    def reset_parameters(self):
+        for parameter in (self.post_weight, self.pre_weight, self.gate):
+            if parameter is not None:
+                util.fill(parameter, 1.0)
+
+    def extra_repr(self):
+        return (
+            f"{tuple(self.normalized_shape)}, "
+            f"post_norm={self.post_weight is not None}, "
+            f"gate={self.gate is not None}, "
+            f"residual_scale={self.residual_scale}, "
+            f"eps={self.eps}, "
             f"backend=Trident"
         )
 

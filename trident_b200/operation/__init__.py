@@ -1,4 +1,5 @@
 from .attention import Attention
+from .gated_residual_rms_norm import GatedResidualRMSNorm
 from .geglu import GEGLU
 from .layer_norm import LayerNorm
 from .linear import Linear
@@ -9,5 +10,6 @@ from .rms_norm_geglu import RMSNormGEGLU
 from .softmax import Softmax
 
 __all__ = [
-    "Attention", "GEGLU", "LayerNorm", "Linear", "MaskedSoftmax", "Mean", "RMSNorm", "RMSNormGEGLU", "Softmax", "Sum", "Var", "VarMean",
+    "Attention", "GatedResidualRMSNorm", "GEGLU", "LayerNorm", "Linear", "MaskedSoftmax", "Mean", "RMSNorm",
+    "RMSNormGEGLU", "Softmax", "Sum", "Var", "VarMean",
 ]
