@@ -255,6 +255,61 @@ int tb200_attention_bwd(void* dq, void* dk, void* dv, void* dmask /*nullable*/,
                         const int64_t* out_strides, const int64_t* mask_strides,
                         int is_causal, float softmax_scale, int dtype, void* stream);
 
+/* ---- Window attention (not in the reference) ------------------------------
+ * Causal attention of a query at position i over the keys j <= i with i - j < window or j < sinks
+ * (the first `sinks` tokens stay visible). q, out: [B,H,S,D]; k, v: [B,KV,S,D], H a multiple of KV
+ * (at most 64 times): query head h uses key head h / (H / KV). All with element strides (4 each).
+ * lse [B,H,S]: natural-log sum of exponentials of a score row (float32), kept for backward. Keys and
+ * values have to be finite: a NaN or infinity may reach queries near it that do not see it. */
+int tb200_window_attention_fwd(void* out, float* lse, const void* q, const void* k, const void* v, int64_t B,
+                               int64_t H, int64_t KV, int64_t S, int64_t D, const int64_t* q_strides,
+                               const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
+                               int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream);
+/* dq [B,H,S,D], dk, dv [B,KV,S,D] (summed over the query heads of a key head) from dout. No atomics:
+ * the same inputs give the same bits. The workspace (16-byte aligned) holds a float per score row and
+ * the parts of the sinks' gradients. */
+size_t tb200_window_attention_bwd_workspace(int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D, int64_t window,
+                                            int64_t sinks, int dtype);
+int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k,
+                               const void* v, const void* out, const float* lse, void* workspace,
+                               size_t workspace_bytes, int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D,
+                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                               const int64_t* out_strides, const int64_t* dout_strides, const int64_t* dq_strides,
+                               const int64_t* dk_strides, const int64_t* dv_strides, int64_t window, int64_t sinks,
+                               float softmax_scale, int dtype, void* stream);
+
+/* ---- Paged attention (not in the reference) --------------------------------
+ * Keys and values of n sequences lie in pages of a pool, key_cache and value_cache
+ * [pages, page, KV, D] (element strides, 4 each): the key at position x of sequence s is row
+ * x % page of page table[s][x / page]. context[s] counts a sequence's keys, its new tokens
+ * included; its new tokens are the rows [starts[s], starts[s+1]) of q [T,H,D] (3 strides; starts
+ * null: token s), and the i-th of t new tokens has position context - t + i. It sees the positions
+ * up to its own, with a window (> 0) those less than `window` back and the first `sinks`.
+ * A token without a visible key (position below 0) gets zeros. Rows that belong to no sequence (behind
+ * starts[n]) are left alone, or set to zero with zero_tail != 0. table, context and starts are read on
+ * the device; values out of range are cut to the buffers (a page outside the pool reads as zeros), and
+ * table entries of blocks that no query sees are not read. max_query_length: no sequence has more new
+ * tokens. max_context_length: the longest context expected (longer ones are still right). The workspace
+ * holds the parts of walks that are cut along the keys. */
+size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t H, int64_t KV, int64_t D,
+                                       int64_t max_query_length, int64_t max_context_length, int64_t window,
+                                       int64_t sinks, int dtype);
+int tb200_paged_attention(void* out, const void* q, const void* key_cache, const void* value_cache,
+                          const int32_t* table, const int32_t* context, const int32_t* starts /*nullable*/,
+                          void* workspace, size_t workspace_bytes, int64_t T, int64_t n, int64_t H, int64_t KV,
+                          int64_t D, int64_t page, int64_t pages, int64_t table_cols, int64_t table_stride,
+                          const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                          const int64_t* out_strides, int64_t max_query_length, int64_t max_context_length,
+                          int64_t window, int64_t sinks, float softmax_scale, int zero_tail, int dtype, void* stream);
+/* Writes the keys and values of the new tokens, k and v [T,KV,D] (3 strides), to their places in the
+ * pages (same table, context and starts). Tokens at positions below 0, beyond the table or on pages
+ * outside the pool are left out. */
+int tb200_paged_cache_append(void* key_cache, void* value_cache, const void* k, const void* v, const int32_t* table,
+                             const int32_t* context, const int32_t* starts /*nullable*/, int64_t T, int64_t n,
+                             int64_t KV, int64_t D, int64_t page, int64_t pages, int64_t table_cols,
+                             int64_t table_stride, const int64_t* kc_strides, const int64_t* vc_strides,
+                             const int64_t* k_strides, const int64_t* v_strides, int dtype, void* stream);
+
 /* ---- introspection used by the tests and the bench ----------------------
  * Name of the kernel family the last successful call on this thread dispatched to
  * ("row_vec", "row_generic", "gemm_tcgen05", "gemm_simt", "attn_tcgen05", "attn_simt", ...)

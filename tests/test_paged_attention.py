@@ -1,0 +1,376 @@
+"""Attention over a paged cache and the write into it, against the formula in 64 bits."""
+
+import pytest
+import torch
+
+import trident_b200 as trident
+from tests import local_reference as ref
+from tests import util
+from trident_b200 import _lib
+
+attend = trident.function.paged_attention
+append = trident.function.paged_cache_append
+
+
+class Cache:
+    """A pool of pages in random order, with the sequences' keys and values in it; everything else in the
+    pool (the rest of last pages, spare pages) is NaN, and unused table entries are -1."""
+
+    def __init__(self, context, KV, D, page, dtype, device, seed=0, poison=float("nan")):
+        self.context, self.page = context, page
+        g = util.seeded(seed)
+        blocks = [-(-c // page) for c in context]
+        pages = sum(blocks) + 2
+        order = torch.randperm(pages, generator=g)
+        self.table = torch.full((len(context), max(blocks + [1]) + 1), -1, dtype=torch.int32)
+        self.keys, self.values = [], []
+        kc, vc = (torch.full((pages, page, KV, D), poison) for _ in range(2))
+        at = 0
+        for s, (c, b) in enumerate(zip(context, blocks)):
+            self.table[s, :b] = order[at:at + b].to(torch.int32)
+            at += b
+            k, v = (torch.randn(c, KV, D, generator=g).to(dtype) for _ in range(2))
+            self.keys.append(k)
+            self.values.append(v)
+            for cache, rows in ((kc, k), (vc, v)):
+                x = torch.arange(c)
+                cache[self.table[s, (x // page)].long(), x % page] = rows.float()
+        self.key_cache, self.value_cache = kc.to(dtype).to(device), vc.to(dtype).to(device)
+        self.table_dev = self.table.to(device)
+        self.context_dev = torch.tensor(context, dtype=torch.int32, device=device)
+
+
+def _offsets(new, device):
+    return torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32, device=device)
+
+
+def _want(q, cache, new, window, sinks, scale, dtype):
+    """Values and bounds [T, H, D]."""
+    T, H, D = q.shape
+    KV = cache.key_cache.shape[2]
+    G = H // KV
+    value, bound = (torch.zeros(T, H, D, dtype=torch.float64) for _ in range(2))
+    at = 0
+    for s, t in enumerate(new):
+        c = cache.context[s]
+        pos = torch.arange(c - t, c)
+        for h in range(KV):
+            one = ref.attention(q[at:at + t, h * G:(h + 1) * G].double().transpose(0, 1), cache.keys[s][:, h].double(),
+                                cache.values[s][:, h].double(), pos, window, sinks, scale, dtype)["out"]
+            value[at:at + t, h * G:(h + 1) * G] = one[0].transpose(0, 1)
+            bound[at:at + t, h * G:(h + 1) * G] = one[1].transpose(0, 1)
+        at += t
+    return value, bound
+
+
+def _compare(context, new, KV, G, D, page, dtype, device, window=None, sinks=0, seed=0, decode=False, **more):
+    cache = Cache(context, KV, D, page, dtype, device, seed)
+    q = util.randn(sum(new), KV * G, D, seed=seed + 1000).to(dtype)
+    got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev,
+                 None if decode else _offsets(new, device), window_size=window, num_sinks=sinks, **more)
+    ref.check(got, _want(q, cache, new, window or 0, sinks, D ** -0.5, dtype), "out")
+    assert _lib.device_status() == 0
+    return got
+
+
+# ------------------------------------------------------------------------------------ no GPU
+def _cpu_call(**change):
+    args = dict(query=torch.randn(3, 4, 16), key_cache=torch.randn(5, 8, 2, 16), value_cache=torch.randn(5, 8, 2, 16),
+                block_table=torch.zeros(2, 3, dtype=torch.int32), context_lengths=torch.ones(2, dtype=torch.int32),
+                query_offsets=torch.tensor([0, 1, 3], dtype=torch.int32))
+    args.update(change)
+    return args
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(query=torch.randn(3, 64)), "dimension of query"),
+    (dict(key_cache=torch.randn(5, 8, 32)), "dimension of key_cache"),
+    (dict(value_cache=torch.randn(5, 4, 2, 16)), "same shape"),
+    (dict(key_cache=torch.randn(5, 0, 2, 16), value_cache=torch.randn(5, 0, 2, 16)), "at least one token"),
+    (dict(query=torch.randn(3, 4, 32)), "same head size"),
+    (dict(query=torch.randn(3, 3, 16)), "multiple"),
+    (dict(block_table=torch.zeros(2, 3)), "torch.int32"),
+    (dict(context_lengths=torch.ones(2, dtype=torch.int64)), "torch.int32"),
+    (dict(context_lengths=torch.ones(3, dtype=torch.int32)), r"\[sequences\]"),
+    (dict(query_offsets=torch.tensor([0, 3], dtype=torch.int32)), r"sequences \+ 1"),
+    (dict(query_offsets=None), "one new token per sequence"),
+    (dict(query=torch.randn(3, 4, 16).half()), "same dtype"),
+    (dict(window_size=0), "window_size"),
+    (dict(num_sinks=2), "needs a window_size"),
+    (dict(window_size=4, num_sinks=-1), "num_sinks"),
+    (dict(max_query_length=-1), "max_query_length"),
+    (dict(max_context_length=-1), "max_context_length"),
+    (dict(output=torch.empty(2, 4, 16)), "output and query"),
+    (dict(query=torch.randn(3, 4, 16, requires_grad=True)), "no backward"),
+])
+def test_refusals(change, match):
+    with pytest.raises(ValueError, match=match):
+        attend(**_cpu_call(**change))
+
+
+def test_append_refusals():
+    args = _cpu_call()
+    del args["query"]
+    k = torch.randn(3, 2, 16)
+    for key, value, match in ((k, k[:2], "same shape"), (k[0], k[0], "same shape"), (k[:, :1], k[:, :1], "same heads"),
+                              (k.half(), k.half(), "same dtype")):
+        with pytest.raises(ValueError, match=match):
+            append(key, value, **args)
+    with pytest.raises(_lib.Tb200Error, match="CUDA tensors only"):
+        append(k, k, **args)
+    with pytest.raises(_lib.Tb200Error, match="CUDA tensors only"):
+        attend(**_cpu_call())
+
+
+# ------------------------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("page", [1, 8, 16, 24, 64, 100, 256])
+def test_single_tokens(page, D, dtype, device):
+    _compare([1, 7, 64, 129, 500], [1] * 5, 2, 4, D, page, dtype, device, decode=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 24, 128, 37])
+@pytest.mark.parametrize("window, sinks", [(None, 0), (50, 3), (1, 0), (200, 140)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_chunks(D, window, sinks, page, dtype, device):
+    _compare([300, 33, 513, 1], [40, 33, 130, 1], 2, 3, D, page, dtype, device, window, sinks, seed=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("KV, G", [(1, 1), (3, 1), (1, 8), (2, 16), (1, 7), (1, 64), (1, 40)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_head_groups(KV, G, D, dtype, device):
+    _compare([200, 90], [1, 1], KV, G, D, 16, dtype, device, decode=True, seed=2)
+    _compare([200, 90], [30, 20], KV, G, D, 16, dtype, device, 60, 2, seed=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G, t", [(1, 1), (4, 1), (4, 9), (8, 40)])
+@pytest.mark.parametrize("window, sinks", [(None, 0), (3000, 5), (700, 600)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_contexts_of_few_sequences(D, window, sinks, G, t, dtype, device):
+    """Few rows and many keys: the walk along the keys is cut and joined."""
+    _compare([5000], [t], 1, G, D, 32, dtype, device, window, sinks, seed=4)
+    _compare([4100, 70], [t, t], 2, G, D, 16, dtype, device, window, sinks, seed=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_announced_lengths_only_change_the_speed(D, device):
+    """Contexts longer than announced are still right, and so is every announced number."""
+    for announced in (None, 1, 300, 3000, 10 ** 6):
+        _compare([2500, 40], [1, 1], 1, 4, D, 16, torch.bfloat16, device, decode=True, seed=6, max_context_length=announced)
+        _compare([2500, 40], [3, 7], 1, 4, D, 16, torch.bfloat16, device, seed=6, max_query_length=7, max_context_length=announced)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_sequences_without_tokens_or_keys(D, dtype, device):
+    """No new tokens, no keys, more new tokens than keys (positions below zero see nothing)."""
+    cache = Cache([50, 0, 20, 3], 2, D, 16, dtype, device, seed=7)
+    new = [0, 2, 5, 6]
+    q = util.randn(13, 4, D, seed=8).to(dtype)
+    got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, _offsets(new, device))
+    want = _want(q, cache, new, 0, 0, D ** -0.5, dtype)
+    ref.check(got, want, "out")
+    assert torch.all(got[:2] == 0) and torch.all(got[7:10] == 0)  # the second sequence, and the last one's first three
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_rows_behind_the_last_sequence(D, dtype, device):
+    cache = Cache([30, 45], 1, D, 8, dtype, device, seed=9)
+    q = util.randn(300, 2, D, seed=10).to(dtype)
+    offsets = _offsets([4, 6], device)
+    got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, offsets)
+    ref.check(got[:10], _want(q[:10], cache, [4, 6], 0, 0, D ** -0.5, dtype), "out")
+    assert torch.all(got[10:] == 0)
+    mine = torch.full_like(got, 5.0)
+    back = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, offsets, output=mine)
+    assert back is mine and torch.equal(mine[:10], got[:10]) and torch.all(mine[10:] == 5.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_released_pages_are_not_read(D, dtype, device):
+    """Blocks that lie wholly outside window and sinks may carry any table entry and any content."""
+    context, window, sinks, page = [900], 100, 20, 16
+    for t in (1, 30):
+        cache = Cache(context, 2, D, page, dtype, device, seed=11)
+        q = util.randn(t, 4, D, seed=12).to(dtype)
+        first = context[0] - t - window + 1
+        gone = [b for b in range(-(-context[0] // page)) if b * page >= sinks and (b + 1) * page <= first]
+        assert len(gone) > 40
+        for mode in ("poisoned", "missing"):
+            table = cache.table_dev.clone()
+            kc, vc = cache.key_cache.clone(), cache.value_cache.clone()
+            for b in gone:
+                if mode == "missing":
+                    table[0, b] = (-1, 10 ** 9)[b % 2]
+                else:
+                    kc[table[0, b].long()] = float("nan")
+                    vc[table[0, b].long()] = float("inf")
+            got = attend(q.to(device), kc, vc, table, cache.context_dev, _offsets([t], device), window_size=window, num_sinks=sinks)
+            ref.check(got, _want(q, cache, [t], window, sinks, D ** -0.5, dtype), mode)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_bad_pages_and_offsets_touch_nothing_else(D, dtype, device):
+    """Table entries outside the pool that a token sees read as zeros; offsets and contexts out of range are cut."""
+    cache = Cache([64], 1, D, 16, dtype, device, seed=13)
+    q = util.randn(2, 2, D, seed=14).to(dtype)
+    table = cache.table_dev.clone()
+    table[0, 1], table[0, 2] = -5, 2 ** 31 - 1
+    cache.keys[0][16:48], cache.values[0][16:48] = 0.0, 0.0
+    got = attend(q.to(device), cache.key_cache, cache.value_cache, table, cache.context_dev, _offsets([2], device))
+    ref.check(got, _want(q, cache, [2], 0, 0, D ** -0.5, dtype), "bad pages")
+    wild = torch.tensor([-7, 10 ** 9], dtype=torch.int32, device=device)
+    got = attend(q.to(device), cache.key_cache, cache.value_cache, table, cache.context_dev, wild)
+    ref.check(got, _want(q, cache, [2], 0, 0, D ** -0.5, dtype), "wild offsets")
+    # a context beyond the table counts as what the table holds (here 5 blocks, the last of which is missing)
+    long = attend(q.to(device), cache.key_cache, cache.value_cache, table, torch.full_like(cache.context_dev, 10 ** 9), wild)
+    assert torch.isfinite(long.float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_layouts(D, dtype, device):
+    """A pool that keeps heads before positions, a strided query, a table that is a slice."""
+    cache = Cache([100, 260], 2, D, 32, dtype, device, seed=15)
+    q = util.randn(2, 8, D, seed=16).to(dtype)
+    want = _want(q, cache, [1, 1], 0, 0, D ** -0.5, dtype)
+    kc, vc = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (cache.key_cache, cache.value_cache))
+    wide = torch.stack([q, q], 2).to(device)[:, :, 0]
+    table = torch.cat([cache.table_dev, cache.table_dev], 1)[:, : cache.table_dev.shape[1]]
+    ref.check(attend(wide, kc, vc, table, cache.context_dev), want, "layouts")
+    both = torch.stack([cache.key_cache, cache.value_cache], 1)  # [pages, 2, page, KV, D]
+    ref.check(attend(q.to(device), both[:, 0], both[:, 1], cache.table_dev.t().contiguous().t(), cache.context_dev), want, "joint pool")
+    out = torch.empty(8, 2, D, dtype=dtype, device=device).transpose(0, 1)
+    ref.check(attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, output=out), want, "strided output")
+    odd_k, odd_v = (torch.empty(t.numel() + 1, dtype=dtype, device=device)[1:].view(t.shape).copy_(t) for t in (cache.key_cache, cache.value_cache))
+    ref.check(attend(q.to(device), odd_k, odd_v, cache.table_dev, cache.context_dev), want, "unaligned pool")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 16, 24, 64])
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_append(D, page, dtype, device):
+    context, new = [20, 70, 3, 0, 9], [20, 5, 1, 0, 12]
+    cache = Cache(context, 2, D, page, dtype, device, seed=17)
+    k, v = (util.randn(sum(new) + 4, 2, D, seed=18 + i).to(dtype).to(device) for i in range(2))
+    kc, vc = cache.key_cache.clone(), cache.value_cache.clone()
+    append(k, v, kc, vc, cache.table_dev, cache.context_dev, _offsets(new, device))
+    want_k, want_v = cache.key_cache.clone(), cache.value_cache.clone()
+    at = 0
+    for s, t in enumerate(new):
+        for i in range(t):
+            pos = context[s] - t + i
+            if pos >= 0:
+                where = cache.table[s, pos // page].long().item(), pos % page
+                want_k[where], want_v[where] = k[at + i], v[at + i]
+        at += t
+    assert torch.equal(kc.view(torch.uint8 if dtype != torch.float32 else torch.int32), want_k.view(torch.uint8 if dtype != torch.float32 else torch.int32))
+    assert torch.equal(torch.nan_to_num(vc), torch.nan_to_num(want_v))
+    # one token each, strided rows, and pages outside the pool left out
+    table = cache.table_dev.clone()
+    table[0] = torch.tensor([-1, 2 ** 31 - 1], dtype=torch.int32, device=device)[torch.arange(table.shape[1], device=device) % 2]
+    kc, vc = cache.key_cache.clone(), cache.value_cache.clone()
+    joint = torch.cat([k, v], 1)[:5]
+    append(joint[:, :2], joint[:, 2:], kc, vc, table, cache.context_dev)
+    want_k = cache.key_cache.clone()
+    for s, c in enumerate(context):
+        if s > 0 and c > 0:
+            want_k[cache.table[s, (c - 1) // page].long(), (c - 1) % page] = k[s]
+    assert torch.equal(torch.nan_to_num(kc), torch.nan_to_num(want_k))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_captured_decode_grows(dt, device):
+    """One captured step (write, attend) replayed while the contexts grow; two graphs live side by side."""
+    D, KV, G, page = 64, 2, 2, 16
+    cache = Cache([300, 40], KV, D, page, dt, device, seed=20)
+    spare = [int(p) for p in range(cache.key_cache.shape[0]) if p not in set(cache.table[cache.table >= 0].tolist())]
+    for s, c in enumerate(cache.context):  # room for the next tokens
+        if cache.table[s, c // page] < 0:
+            cache.table[s, c // page] = spare.pop()
+    cache.table_dev.copy_(cache.table)
+    q = torch.zeros(2, KV * G, D, dtype=dt, device=device)
+    k, v = (torch.zeros(2, KV, D, dtype=dt, device=device) for _ in range(2))
+
+    def step():
+        append(k, v, cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev)
+        return attend(q, cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, max_context_length=320)
+
+    cache.context_dev += 1
+    step()
+    torch.cuda.synchronize()
+    cache.context_dev -= 1
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(step())
+    for i in range(4):
+        fresh = [util.randn(*t.shape, seed=30 + 3 * i + j).to(dt) for j, t in enumerate((q, k, v))]
+        for dst, src in zip((q, k, v), fresh):
+            dst.copy_(src)
+        cache.context_dev += 1
+        for s in range(2):
+            cache.context[s] += 1
+            cache.keys[s] = torch.cat([cache.keys[s], fresh[1][s:s + 1]])
+            cache.values[s] = torch.cat([cache.values[s], fresh[2][s:s + 1]])
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        ref.check(outs[i % 2], _want(fresh[0], cache, [1, 1], 0, 0, D ** -0.5, dt), f"step {i}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_same_bits_every_time_and_two_streams(D, dtype, device):
+    cache = Cache([3000, 900], 1, D, 16, dtype, device, seed=40)
+    q = util.randn(2, 4, D, seed=41).to(dtype).to(device)
+
+    def call():
+        return attend(q, cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, max_context_length=3000)
+
+    first = call()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(call())
+    for s in streams:
+        s.synchronize()
+    assert all(torch.equal(first, r) for r in results)
+
+
+@pytest.mark.gpu
+def test_module(device, dtype):
+    D = 64
+    cache = Cache([40, 12], 2, D, 16, dtype, device, seed=50, poison=0.0)
+    q, k, v = (util.randn(2, h, D, seed=51 + h).to(dtype).to(device) for h in (4, 2, 2))
+    m = trident.PagedAttention(window_size=20, num_sinks=2)
+    with torch.no_grad():
+        got = m(q, k, v, cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev)
+    for s in range(2):
+        cache.keys[s][-1], cache.values[s][-1] = k[s].cpu(), v[s].cpu()
+    ref.check(got, _want(q.cpu(), cache, [1, 1], 20, 2, D ** -0.5, dtype), "module")
+    assert "backend=Trident" in repr(m)
+
+
+@pytest.mark.gpu
+def test_nothing_to_do(device):
+    kc = torch.zeros(2, 8, 1, 64, device=device)
+    table = torch.zeros(0, 1, dtype=torch.int32, device=device)
+    none = torch.zeros(0, dtype=torch.int32, device=device)
+    assert attend(torch.zeros(0, 2, 64, device=device), kc, kc, table, none).shape == (0, 2, 64)
+    out = attend(torch.ones(3, 2, 64, device=device), kc, kc, table, none, torch.zeros(1, dtype=torch.int32, device=device))
+    assert torch.all(out == 0)
+    append(torch.zeros(0, 1, 64, device=device), torch.zeros(0, 1, 64, device=device), kc, kc, table, none)

@@ -1,0 +1,291 @@
+"""Window attention with sinks against its formula in 64 bits, forward and backward."""
+
+import pytest
+import torch
+
+import trident_b200 as trident
+from tests import local_reference as ref
+from tests import util
+from trident_b200 import _lib
+
+F = trident.function.sliding_window_attention
+
+
+def _problem(B, KV, G, S, D, dtype, seed=0, q_std=1.0):
+    q, dout = (util.randn(B, KV * G, S, D, seed=seed + i, std=s).to(dtype) for i, s in ((0, q_std), (1, 1.0)))
+    k, v = (util.randn(B, KV, S, D, seed=seed + 2 + i).to(dtype) for i in range(2))
+    return q, k, v, dout
+
+
+def _run(problem, window, sinks, device, scale=None):
+    q, k, v = (t.to(device).requires_grad_(True) for t in problem[:3])
+    out = F(q, k, v, window, sinks, scale)
+    out.backward(problem[3].to(device))
+    return {"out": out, "dq": q.grad, "dk": k.grad, "dv": v.grad}
+
+
+def _compare(problem, window, sinks, device, scale=None):
+    q, k, v, dout = problem
+    want = ref.batched(q, k, v, window, sinks, q.shape[-1] ** -0.5 if scale is None else scale, q.dtype, dout)
+    got = _run(problem, window, sinks, device, scale)
+    for name in ("out", "dv", "dq", "dk"):
+        ref.check(got[name], want[name], name)
+    assert _lib.device_status() == 0
+
+
+# ------------------------------------------------------------------------------------ no GPU
+def test_the_reference_agrees_with_autograd():
+    q, k, v, dout = (t.double() for t in _problem(1, 2, 3, 23, 16, torch.float64))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    seen = ref.visible(torch.arange(23), 23, 5, 2)
+    s = leaves[0] @ leaves[1].repeat_interleave(3, 1).transpose(-1, -2) * 0.25
+    out = torch.softmax(s.masked_fill(~seen, float("-inf")), -1) @ leaves[2].repeat_interleave(3, 1)
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = ref.batched(q, k, v, 5, 2, 0.25, torch.float32, dout)
+    for name, value in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        assert torch.allclose(want[name][0], value, rtol=1e-10, atol=1e-12), name
+
+
+def test_refusals():
+    q, k = torch.randn(1, 4, 8, 16), torch.randn(1, 2, 8, 16)
+    for args, match in (
+        ((q[0], k, k, 4), "dimension"),
+        ((q, k, k[:, :1], 4), "key and value"),
+        ((q, k[:, :, :4], k[:, :, :4], 4), "same batch, length"),
+        ((q[:, :3], k, k, 4), "multiple"),
+        ((q[:, :0], k, k, 4), "1 to 64"),
+        ((q, k[:, :0], k[:, :0], 4), "multiple"),
+        ((q[..., :12], k[..., :12], k[..., :12], 4), "head size"),
+        ((q, k, k, 0), "window_size"),
+        ((q, k, k, 2.0), "window_size"),
+        ((q, k, k, True), "window_size"),
+        ((q, k, k, 4, -1), "num_sinks"),
+        ((q, k.half(), k.half(), 4), "same dtype"),
+        ((q.double(), k.double(), k.double(), 4), "Unable to convert"),
+        ((torch.randn(1, 65, 2, 16), k[:, :1, :2], k[:, :1, :2], 4), "1 to 64"),
+    ):
+        with pytest.raises(ValueError, match=match):
+            F(*args)
+    with pytest.raises(_lib.Tb200Error, match="CUDA tensors only"):
+        F(q, k, k, 4)
+
+
+def test_library_refuses_before_launch():
+    import ctypes
+
+    lib = _lib.load()
+    s = (ctypes.c_int64 * 4)(1, 1, 1, 1)
+    call = lambda *a: lib.tb200_window_attention_fwd(*a)  # noqa: E731
+    assert call(None, None, None, None, None, 1, 1, 1, 8, 16, s, s, s, s, 4, 0, 1.0, 0, None) == -1
+    assert call(8, 8, 8, 8, 8, 1, 3, 2, 8, 16, s, s, s, s, 4, 0, 1.0, 0, None) == -1
+    assert call(8, 8, 8, 8, 8, 1, 2, 2, 8, 24, s, s, s, s, 4, 0, 1.0, 0, None) == -2
+    assert call(8, 8, 8, 8, 8, 1, 2, 2, 8, 16, s, s, s, s, 0, 0, 1.0, 0, None) == -1
+    assert call(8, 8, 8, 8, 8, 1, 2, 2, 8, 16, s, s, s, None, 4, 0, 1.0, 0, None) == -1
+
+
+# ------------------------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize(
+    "S, window, sinks", [(1, 1, 0), (2, 1, 1), (65, 16, 3), (130, 500, 0), (300, 100, 70), (257, 1, 0), (400, 129, 1)]
+)
+def test_lengths(S, window, sinks, D, dtype, device):
+    _compare(_problem(1, 2, 2, S, D, dtype), window, sinks, device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, KV, G", [(1, 1, 1), (3, 1, 3), (2, 3, 5), (1, 1, 8), (1, 2, 16), (1, 1, 7), (1, 1, 64), (1, 1, 33)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_head_groups(B, KV, G, D, device, dtype):
+    _compare(_problem(B, KV, G, 150, D, dtype, seed=10), 40, 2, device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S, window, sinks", [(1000, 200, 4), (1000, 64, 200), (640, 640, 5), (777, 128, 128), (513, 255, 0), (900, 1000, 0)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_tiles(S, window, sinks, D, dtype, device):
+    _compare(_problem(1, 1, 2, S, D, dtype, seed=20), window, sinks, device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_large_scores(D, device, dtype):
+    """Scores of hundreds: one key takes almost all the weight, the running maximum moves by large steps."""
+    _compare(_problem(1, 1, 2, 400, D, dtype, seed=30, q_std=25.0), 150, 3, device)
+
+
+@pytest.mark.gpu
+def test_scale_is_taken(device):
+    _compare(_problem(1, 1, 2, 100, 64, torch.bfloat16, seed=40), 30, 1, device, scale=0.5)
+    _compare(_problem(1, 1, 2, 100, 64, torch.bfloat16, seed=40), 30, 1, device, scale=-0.25)
+    _compare(_problem(1, 1, 2, 100, 64, torch.float32, seed=40), 30, 1, device, scale=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_strides(D, device, dtype):
+    """[batch, length, heads, size] projections, one joint projection, odd offsets, expanded gradients."""
+    q, k, v, dout = _problem(2, 2, 2, 140, D, dtype, seed=50)
+    want = ref.batched(q, k, v, 50, 3, D ** -0.5, dtype, dout)
+    names = ("out", "dq", "dk", "dv")
+
+    def run(q, k, v, dout):
+        q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+        out = F(q, k, v, 50, 3)
+        return dict(zip(names, (out, *torch.autograd.grad(out, (q, k, v), dout))))
+
+    swapped = [t.to(device).transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v, dout)]
+    got = run(*swapped)
+    assert got["out"].stride() == swapped[0].stride()  # laid out as the query is
+    joint = torch.cat([t.to(device).transpose(1, 2) for t in (q, k, v)], 2)
+    slices = [joint[:, :, a:b].transpose(1, 2) for a, b in ((0, 4), (4, 6), (6, 8))]
+    got_joint = run(*slices, dout.to(device))
+
+    def off(t):
+        base = torch.empty(t.numel() + 1, dtype=dtype, device=device)[1:]
+        return base.view(t.shape).copy_(t)
+
+    got_off = run(*(off(t) for t in (q, k, v, dout)))
+    wide = [torch.stack([t, t + 1], -1).to(device)[..., 0] for t in (q, k, v, dout)]  # feature stride 2
+    got_wide = run(*wide)
+    for g in (got, got_joint, got_off, got_wide):
+        for name in names:
+            ref.check(g[name], want[name], name)
+    one = torch.ones_like(dout)
+    want = ref.batched(q, k, v, 50, 3, D ** -0.5, dtype, one)
+    got = run(*(t.to(device) for t in (q, k, v)), torch.ones((), dtype=dtype, device=device).expand(one.shape))
+    for name in names:
+        ref.check(got[name], want[name], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_same_bits_every_time_and_on_another_stream(D, device, dtype):
+    problem = _problem(2, 2, 3, 700, D, dtype, seed=60)
+    first = _run(problem, 130, 4, device)
+    for _ in range(3):
+        again = _run(problem, 130, 4, device)
+        assert all(torch.equal(first[n], again[n]) for n in first)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        again = _run(problem, 130, 4, device)
+    stream.synchronize()
+    assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_whole_window_is_causal_attention(D, device):
+    """With a window as long as the sequence the result is that of the dense causal attention."""
+    dt = torch.bfloat16
+    q, k, v, _ = _problem(1, 4, 1, 512, D, dt, seed=70)
+    dense = trident.function.scaled_dot_product_attention(*(t.to(device) for t in (q, k, v)), is_causal=True)
+    want = ref.batched(q, k, v, 512, 0, D ** -0.5, dt)["out"]
+    ref.check(dense, want, "dense")
+    ref.check(F(*(t.to(device) for t in (q, k, v)), 512), want, "window")
+    assert torch.equal(F(*(t.to(device) for t in (q, k, v)), 512), F(*(t.to(device) for t in (q, k, v)), 10 ** 30, 10 ** 30))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_window_forgets(D, device, dtype):
+    """What lies outside window and sinks has no influence, to the last bit."""
+    q, k, v, _ = (t.to(device) for t in _problem(1, 1, 2, 600, D, dtype, seed=80))
+    before = F(q, k, v, 100, 4)
+    k2, v2 = k.clone(), v.clone()
+    k2[:, :, 4:300], v2[:, :, 4:300] = 7.0, -3.0
+    after = F(q, k2, v2, 100, 4)
+    assert torch.equal(before[:, :, 400:], after[:, :, 400:])
+    assert not torch.equal(before[:, :, 300:399], after[:, :, 300:399])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_guarded_buffers(D, device, dtype):
+    """Nothing is written outside the outputs: the library is called on slices of one poisoned buffer."""
+    B, KV, G, S = 1, 2, 3, 131
+    q, k, v, dout = (t.to(device) for t in _problem(B, KV, G, S, D, dtype, seed=90))
+    pad = 4096
+
+    def guarded(t, dt=None):
+        dt = t.dtype if dt is None else dt
+        buf = torch.full((t.numel() + 2 * pad,), 123.0, dtype=dt, device=device)
+        return buf, buf[pad:-pad].view(t.shape)
+
+    bufs, views = zip(*(guarded(t, dt) for t, dt in ((q, None), (q[..., 0], torch.float32), (q, None), (k, None), (v, None))))
+    out, lse, dq, dk, dv = views
+    _lib.window_attention_fwd(out, lse, q, k, v, 40, 3, D ** -0.5)
+    size = _lib.window_attention_bwd_workspace(q, k, 40, 3)
+    ws = torch.full((size + 2 * pad,), 77, dtype=torch.uint8, device=device)
+    _lib.window_attention_bwd(dq, dk, dv, dout, q, k, v, out, lse, ws[pad:-pad], 40, 3, D ** -0.5)
+    torch.cuda.synchronize()
+    for buf in bufs:
+        assert torch.all(buf[:pad] == 123.0) and torch.all(buf[-pad:] == 123.0)
+    assert torch.all(ws[:pad] == 77) and torch.all(ws[-pad:] == 77)
+    want = ref.batched(*(t.cpu() for t in (q, k, v)), 40, 3, D ** -0.5, dtype, dout.cpu())
+    for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        ref.check(got, want[name], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_captured_step(dt, device):
+    """Forward and backward captured into a CUDA graph, replayed on new values."""
+    problem = [t.to(device) for t in _problem(1, 2, 2, 300, 64, dt, seed=100)]
+    leaves = [t.clone().requires_grad_(True) for t in problem[:3]]
+
+    def step():
+        out = F(*leaves, 90, 2)
+        return (out, *torch.autograd.grad(out, leaves, problem[3]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    fresh = _problem(1, 2, 2, 300, 64, dt, seed=110)
+    with torch.no_grad():
+        for dst, src in zip(leaves + [problem[3]], fresh):
+            dst.copy_(src)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = ref.batched(*fresh[:3], 90, 2, 0.125, dt, fresh[3])
+    for name, got in zip(("out", "dq", "dk", "dv"), outs):
+        ref.check(got, want[name], name)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(device):
+    q, k, v, dout = (t.to(device) for t in _problem(1, 1, 2, 40, 16, torch.float32, seed=120))
+    grads = _run((q, k, v, dout), 9, 2, device)
+    step = 2.0 ** -6
+    for i, name in enumerate(("dq", "dk", "dv")):
+        direction = util.randn(*(q, k, v)[i].shape, seed=130 + i, device=device)
+        up, down = [q, k, v], [q, k, v]
+        up[i], down[i] = up[i] + step * direction, down[i] - step * direction
+        slope = ((F(*up, 9, 2) - F(*down, 9, 2)).double() * dout.double()).sum() / (2 * step)
+        want = (grads[name].double() * direction.double()).sum()
+        # third-order term of the difference (step^2 = 2.4e-4 of the terms) and fp32 noise
+        assert abs(slope - want) <= 5e-3 * (grads[name].double() * direction.double()).abs().sum(), name
+
+
+@pytest.mark.gpu
+def test_empty(device):
+    q, k = torch.empty(2, 4, 0, 64, device=device, requires_grad=True), torch.empty(2, 2, 0, 64, device=device)
+    out = F(q, k, k, 5, 1)
+    out.sum().backward()
+    assert out.shape == q.shape and q.grad.shape == q.shape
+    assert F(torch.empty(0, 4, 7, 64, device=device), torch.empty(0, 2, 7, 64, device=device), torch.empty(0, 2, 7, 64, device=device), 5).shape == (0, 4, 7, 64)
+
+
+@pytest.mark.gpu
+def test_module(device, dtype):
+    m = trident.SlidingWindowAttention(16, 2)
+    q, k, v, dout = (t.to(device) for t in _problem(1, 2, 2, 50, 64, dtype, seed=140))
+    assert torch.equal(m(q, k, v), F(q, k, v, 16, 2))
+    assert "backend=Trident" in repr(m)

@@ -68,6 +68,18 @@ SIGNATURES = {
         c_int,
         [c_ptr] * 12 + [c_size] + [c_i64] * 4 + [c_ptr] * 5 + [c_int, c_f32, c_int, c_ptr],
     ),
+    "tb200_window_attention_fwd": (c_int, [c_ptr] * 5 + [c_i64] * 5 + [c_ptr] * 4 + [c_i64] * 2 + [c_f32, c_int, c_ptr]),
+    "tb200_window_attention_bwd_workspace": (c_size, [c_i64] * 7 + [c_int]),
+    "tb200_window_attention_bwd": (
+        c_int,
+        [c_ptr] * 10 + [c_size] + [c_i64] * 5 + [c_ptr] * 8 + [c_i64] * 2 + [c_f32, c_int, c_ptr],
+    ),
+    "tb200_paged_attention_workspace": (c_size, [c_i64] * 9 + [c_int]),
+    "tb200_paged_attention": (
+        c_int,
+        [c_ptr] * 8 + [c_size] + [c_i64] * 9 + [c_ptr] * 4 + [c_i64] * 4 + [c_f32, c_int, c_int, c_ptr],
+    ),
+    "tb200_paged_cache_append": (c_int, [c_ptr] * 7 + [c_i64] * 8 + [c_ptr] * 4 + [c_int, c_ptr]),
 }
 
 _lib = None
@@ -175,6 +187,10 @@ def require_one_device(**tensors):
 
 def _strides4(t):
     return (c_i64 * 4)(*t.stride())
+
+
+def _strides3(t):
+    return (c_i64 * 3)(*t.stride())
 
 
 # --------------------------------------------------------------------------- row ops
@@ -481,3 +497,76 @@ def attention_bwd(dq, dk, dv, dmask, dout, q, k, v, out, lse, mask, workspace, i
         ),
         "tb200_attention_bwd",
     )
+
+
+def window_attention_fwd(out, lse, q, k, v, window, sinks, scale):
+    B, H, S, D = q.shape
+    with _on_device(q):
+        _check(
+            load().tb200_window_attention_fwd(
+                _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), B, H, k.shape[1], S, D,
+                _strides4(q), _strides4(k), _strides4(v), _strides4(out), window, sinks, scale,
+                dtype_code(q.dtype), _stream(q),
+            ),
+            "tb200_window_attention_fwd",
+        )
+
+
+def window_attention_bwd_workspace(q, k, window, sinks):
+    B, H, S, D = q.shape
+    with _on_device(q):
+        return load().tb200_window_attention_bwd_workspace(B, H, k.shape[1], S, D, window, sinks, dtype_code(q.dtype))
+
+
+def window_attention_bwd(dq, dk, dv, dout, q, k, v, out, lse, workspace, window, sinks, scale):
+    B, H, S, D = q.shape
+    with _on_device(q):
+        _check(
+            load().tb200_window_attention_bwd(
+                _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
+                _ptr(workspace), workspace.numel() * workspace.element_size(), B, H, k.shape[1], S, D,
+                _strides4(q), _strides4(k), _strides4(v), _strides4(out), _strides4(dout), _strides4(dq),
+                _strides4(dk), _strides4(dv), window, sinks, scale, dtype_code(q.dtype), _stream(q),
+            ),
+            "tb200_window_attention_bwd",
+        )
+
+
+def paged_attention_workspace(q, kv_heads, n, max_query_length, max_context_length, window, sinks):
+    T, H, D = q.shape
+    with _on_device(q):
+        return load().tb200_paged_attention_workspace(
+            T, n, H, kv_heads, D, max_query_length, max_context_length, window, sinks, dtype_code(q.dtype)
+        )
+
+
+def paged_attention(out, q, key_cache, value_cache, table, context, starts, workspace, max_query_length,
+                    max_context_length, window, sinks, scale, zero_tail):
+    T, H, D = q.shape
+    pages, page, kv_heads, _ = key_cache.shape
+    with _on_device(q):
+        _check(
+            load().tb200_paged_attention(
+                _ptr(out), _ptr(q), _ptr(key_cache), _ptr(value_cache), _ptr(table), _ptr(context), _ptr(starts),
+                _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+                T, table.shape[0], H, kv_heads, D, page, pages, table.shape[1], table.stride(0),
+                _strides3(q), _strides4(key_cache), _strides4(value_cache), _strides3(out), max_query_length,
+                max_context_length, window, sinks, scale, int(zero_tail), dtype_code(q.dtype), _stream(q),
+            ),
+            "tb200_paged_attention",
+        )
+
+
+def paged_cache_append(key_cache, value_cache, k, v, table, context, starts):
+    T, kv_heads, D = k.shape
+    pages, page = key_cache.shape[:2]
+    with _on_device(k):
+        _check(
+            load().tb200_paged_cache_append(
+                _ptr(key_cache), _ptr(value_cache), _ptr(k), _ptr(v), _ptr(table), _ptr(context), _ptr(starts),
+                T, table.shape[0], kv_heads, D, page, pages, table.shape[1], table.stride(0),
+                _strides4(key_cache), _strides4(value_cache), _strides3(k), _strides3(v), dtype_code(k.dtype),
+                _stream(k),
+            ),
+            "tb200_paged_cache_append",
+        )

@@ -24,6 +24,8 @@ SOURCES = [
     "attention_simt.cu",
     "attention_fwd_tc.cu",
     "attention_bwd_tc.cu",
+    "local_attention.cu",
+    "local_attention_simt.cu",
 ]
 
 NVCC_FLAGS = [

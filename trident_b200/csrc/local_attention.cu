@@ -1,0 +1,303 @@
+// Entry points of local attention (window and sinks), training and serving, and the cache write:
+// validate, pick a kernel family, launch.
+#include "local_attention.cuh"
+
+namespace tb200 {
+namespace {
+
+// New keys and values into their pages, one thread per 16 bytes (or per element where strides or
+// alignment do not allow that). Bounded by HBM: reads and writes each element once.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(256)
+    cache_append(T* kc, T* vc, const T* k, const T* v, const LocalArgs a, const int64_t sk0, const int64_t sk1,
+                 const int64_t sk2, const int64_t sv0, const int64_t sv1, const int64_t sv2) {
+  constexpr int N = VECTOR ? Traits<T>::VEC : 1;
+  const int s = blockIdx.z;
+  const Sequence sq = load_sequence(a, s);
+  const int per_row = a.D / N, per_token = a.KV * per_row;
+  const int base = sq.kv_len - sq.q_len;
+  const int64_t total = (int64_t)sq.q_len * per_token;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int t = (int)(i / per_token), rest = (int)(i % per_token), h = rest / per_row, d = rest % per_row * N;
+    const int pos = base + t;
+    if (pos < 0) continue;
+    const int page = a.table[s * a.table_stride + pos / a.page];
+    if (page < 0 || page >= a.pages) continue;
+    const int64_t off = pos % a.page, tok = sq.q_begin + t;
+    T* dk = kc + (int64_t)page * a.ks[0] + h * a.ks[1] + off * a.ks[2] + d * a.ks[3];
+    T* dv = vc + (int64_t)page * a.vs[0] + h * a.vs[1] + off * a.vs[2] + d * a.vs[3];
+    const T* pk = k + tok * sk0 + h * sk1 + d * sk2;
+    const T* pv = v + tok * sv0 + h * sv1 + d * sv2;
+    if constexpr (VECTOR) {
+      const uint4 x = ld_stream(pk), y = ld_stream(pv);
+      *reinterpret_cast<uint4*>(dk) = x;
+      *reinterpret_cast<uint4*>(dv) = y;
+    } else {
+      *dk = *pk;
+      *dv = *pv;
+    }
+  }
+}
+
+int check_heads(const char* who, int64_t H, int64_t KV, int64_t D) {
+  TB200_REQUIRE(H > 0 && KV > 0 && H % KV == 0, TB200_ERR_INVALID, "%s: %lld query heads are no multiple of %lld key heads",
+                who, (long long)H, (long long)KV);
+  TB200_REQUIRE(H / KV <= 64 && KV <= 65535, TB200_ERR_UNSUPPORTED, "%s: more than 64 query heads per key head", who);
+  TB200_REQUIRE(D == 16 || D == 32 || D == 64 || D == 128, TB200_ERR_UNSUPPORTED, "%s: head size %lld not in {16,32,64,128}",
+                who, (long long)D);
+  return 0;
+}
+
+void copy4(int64_t* dst, const int64_t* src) {
+  for (int i = 0; i < 4; ++i) dst[i] = src[i];
+}
+
+int fill_window(LocalArgs* a, const char* who, int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D, const int64_t* qs,
+                const int64_t* ks, const int64_t* vs, const int64_t* os, int64_t window, int64_t sinks, float scale) {
+  if (int rc = check_heads(who, H, KV, D)) return rc;
+  TB200_REQUIRE(B >= 0 && S >= 0, TB200_ERR_INVALID, "%s: negative size", who);
+  TB200_REQUIRE(B <= 65535 && S < (1ll << 30), TB200_ERR_UNSUPPORTED, "%s: more than 65535 sequences or 2^30 tokens", who);
+  TB200_REQUIRE(window >= 1 && sinks >= 0, TB200_ERR_INVALID, "%s: window %lld, sinks %lld", who, (long long)window,
+                (long long)sinks);
+  TB200_REQUIRE(qs && ks && vs && os, TB200_ERR_INVALID, "%s: null stride array", who);
+  a->n = (int)B; a->H = (int)H; a->KV = (int)KV; a->G = (int)(H / KV); a->D = (int)D;
+  a->tokens = (int)S;
+  a->window = window >= S ? NO_WINDOW : (int)window;
+  a->sinks = (int)(sinks < S ? sinks : S);
+  a->scale = scale;
+  copy4(a->qs, qs); copy4(a->ks, ks); copy4(a->vs, vs); copy4(a->os, os);
+  return 0;
+}
+
+// Far pieces of the backward pass (see LocalBwdArgs), each about as long as a key tile's walk inside
+// the window.
+void plan_far(LocalBwdArgs* b, int key_tile) {
+  const LocalArgs& a = b->f;
+  b->sink_tiles = b->far = 0;
+  if (a.window == NO_WINDOW || a.sinks == 0) return;
+  const int st = (a.sinks + key_tile - 1) / key_tile;
+  while (b->sink_tiles < st && near_end(a, b->sink_tiles, key_tile) < a.tokens) ++b->sink_tiles;
+  if (b->sink_tiles == 0) return;
+  const int64_t span = a.tokens - near_end(a, 0, key_tile), walk = (int64_t)a.window + key_tile;
+  const int64_t pieces = ceil_div(span, walk);
+  b->far = (int)(pieces < 64 ? pieces : 64);
+}
+size_t far_bytes(const LocalBwdArgs& b, int key_tile) {
+  return (size_t)b.f.n * b.f.KV * b.sink_tiles * (b.far + 1) * 2 * key_tile * b.f.D * sizeof(float);
+}
+size_t row_bytes(const LocalArgs& a) { return ((size_t)a.n * a.H * a.tokens * sizeof(float) + 255) & ~(size_t)255; }
+
+// Parts of a split walk. One row tile of a sequence and key head is one CTA; where those are too few
+// for the GPU the walk along the keys is cut. Single tokens (few rows): parts for 4 CTAs an SM, so that
+// sequences of unequal length even out; the parts' outputs are small next to the keys. Chunks: only as
+// many parts as leave no SM without a CTA. A part is at least 256 keys.
+void plan_split(LocalArgs* a, int64_t max_q, int64_t max_ctx, int row_tile, int key_tile) {
+  a->splits = 1;
+  a->split_tiles = 0;
+  const int64_t row_tiles = ceil_div(max_q, row_tile / a->G), units = (int64_t)a->n * a->KV * row_tiles;
+  int64_t keys = max_ctx;
+  if (a->window != NO_WINDOW) {
+    const int64_t seen = (int64_t)a->window + row_tile / a->G + 2 * key_tile + (a->sinks > 0 ? a->sinks + key_tile : 0);
+    if (seen < keys) keys = seen;
+  }
+  const int64_t tiles = ceil_div(keys, key_tile), least = 256 / key_tile;
+  const int64_t target = (int64_t)sm_count() * (row_tiles == 1 ? 4 : 1);
+  if (units >= target || tiles < 2 * least) return;
+  int64_t splits = ceil_div(target, units);
+  if (splits > tiles / least) splits = tiles / least;
+  if (splits * a->n > 65535) splits = 65535 / a->n;
+  if (splits < 2) return;
+  a->split_tiles = (int)ceil_div(tiles, splits);
+  a->splits = (int)ceil_div(ceil_div(max_ctx, key_tile), a->split_tiles);  // (a walk is never longer than the context)
+  if (a->window != NO_WINDOW) a->splits = (int)ceil_div(tiles, a->split_tiles);
+}
+size_t split_bytes(const LocalArgs& a) {
+  return a.split_tiles == 0 ? 0 : (size_t)a.splits * a.tokens * a.H * (a.D + 1) * sizeof(float);
+}
+
+int fill_paged(LocalArgs* a, const char* who, int64_t T, int64_t n, int64_t H, int64_t KV, int64_t D, const void* table,
+               const int32_t* context, const int32_t* starts, int64_t table_cols, int64_t table_stride, int64_t page,
+               int64_t pages, const int64_t* ks, const int64_t* vs) {
+  if (int rc = check_heads(who, H, KV, D)) return rc;
+  TB200_REQUIRE(T >= 0 && n >= 0 && page > 0 && pages >= 0 && table_cols >= 0, TB200_ERR_INVALID, "%s: bad size", who);
+  TB200_REQUIRE(n <= 65535 && T < (1ll << 30) && pages < (1ll << 31) && page < (1ll << 30) && table_cols < (1ll << 31),
+                TB200_ERR_UNSUPPORTED, "%s: more than 65535 sequences, 2^30 tokens or keys per page, or 2^31 pages", who);
+  TB200_REQUIRE(starts || T == n || n == 0, TB200_ERR_INVALID, "%s: %lld tokens for %lld sequences without starts", who,
+                (long long)T, (long long)n);
+  TB200_REQUIRE((table && context) || n == 0 || T == 0, TB200_ERR_INVALID, "%s: null pointer", who);
+  TB200_REQUIRE(ks && vs, TB200_ERR_INVALID, "%s: null stride array", who);
+  a->n = (int)n; a->H = (int)H; a->KV = (int)KV; a->G = (int)(H / KV); a->D = (int)D;
+  a->tokens = (int)T;
+  a->table = (const int*)table; a->context = context; a->starts = starts;
+  a->table_cols = (int)table_cols; a->table_stride = table_stride;
+  a->page = (int)page; a->pages = (int)pages;
+  const int to[4] = {0, 2, 1, 3};  // [pages, page, KV, D] -> (page, head, position, feature)
+  for (int i = 0; i < 4; ++i) {
+    a->ks[to[i]] = ks[i];
+    a->vs[to[i]] = vs[i];
+  }
+  return 0;
+}
+
+void set_window(LocalArgs* a, int64_t window, int64_t sinks) {
+  a->window = window <= 0 || window >= NO_WINDOW ? NO_WINDOW : (int)window;
+  a->sinks = a->window == NO_WINDOW ? 0 : (int)(sinks < (1 << 30) ? sinks : (1 << 30));
+}
+
+}  // namespace
+}  // namespace tb200
+
+using namespace tb200;
+
+extern "C" int tb200_window_attention_fwd(void* out, float* lse, const void* q, const void* k, const void* v, int64_t B,
+                                          int64_t H, int64_t KV, int64_t S, int64_t D, const int64_t* q_strides,
+                                          const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
+                                          int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream) {
+  LocalArgs a;
+  if (int rc = fill_window(&a, "window_attention_fwd", B, H, KV, S, D, q_strides, k_strides, v_strides, out_strides, window,
+                           sinks, softmax_scale))
+    return rc;
+  if (B == 0 || S == 0) return 0;
+  TB200_REQUIRE(out && lse && q && k && v, TB200_ERR_INVALID, "window_attention_fwd: null pointer");
+  int rc = launch_local_fwd_simt(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream);
+  if (rc == 0) note_kernel("local_simt", 1);
+  return rc;
+}
+
+extern "C" size_t tb200_window_attention_bwd_workspace(int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D,
+                                                       int64_t window, int64_t sinks, int dtype) {
+  (void)dtype;
+  const int64_t st[4] = {0, 0, 0, 0};
+  LocalBwdArgs b;
+  if (fill_window(&b.f, "window_attention_bwd", B, H, KV, S, D, st, st, st, st, window, sinks, 1.f)) return 0;
+  plan_far(&b, local_simt_key_tile());
+  return row_bytes(b.f) + far_bytes(b, local_simt_key_tile());
+}
+
+extern "C" int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k,
+                                          const void* v, const void* out, const float* lse, void* workspace,
+                                          size_t workspace_bytes, int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D,
+                                          const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                          const int64_t* out_strides, const int64_t* dout_strides,
+                                          const int64_t* dq_strides, const int64_t* dk_strides,
+                                          const int64_t* dv_strides, int64_t window, int64_t sinks, float softmax_scale,
+                                          int dtype, void* stream) {
+  LocalBwdArgs b;
+  if (int rc = fill_window(&b.f, "window_attention_bwd", B, H, KV, S, D, q_strides, k_strides, v_strides, out_strides, window,
+                           sinks, softmax_scale))
+    return rc;
+  TB200_REQUIRE(dout_strides && dq_strides && dk_strides && dv_strides, TB200_ERR_INVALID,
+                "window_attention_bwd: null stride array");
+  if (B == 0 || S == 0) return 0;
+  TB200_REQUIRE(dq && dk && dv && dout && q && k && v && out && lse && workspace, TB200_ERR_INVALID,
+                "window_attention_bwd: null pointer");
+  copy4(b.dos, dout_strides); copy4(b.dqs, dq_strides); copy4(b.dks, dk_strides); copy4(b.dvs, dv_strides);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int key_tile = local_simt_key_tile();
+  plan_far(&b, key_tile);
+  const size_t need = row_bytes(b.f) + far_bytes(b, key_tile);
+  TB200_REQUIRE(workspace_bytes >= need, TB200_ERR_WORKSPACE, "window_attention_bwd: workspace of %zu bytes, %zu needed",
+                workspace_bytes, need);
+  TB200_REQUIRE(aligned16(workspace), TB200_ERR_INVALID, "window_attention_bwd: workspace must be 16-byte aligned");
+  float* delta = (float*)workspace;
+  b.part = (float*)((char*)workspace + row_bytes(b.f));
+  if (int rc = launch_local_delta(delta, out, dout, b.dos, b.f, dtype, st)) return rc;
+  if (int rc = launch_local_bwd_simt(dq, dk, dv, dout, q, k, v, lse, delta, b, dtype, st)) return rc;
+  int launches = 3;
+  if (b.sink_tiles > 0) {
+    if (int rc = launch_local_far_sum(dk, dv, b, key_tile, dtype, st)) return rc;
+    ++launches;
+  }
+  note_kernel("local_simt", launches);
+  return 0;
+}
+
+extern "C" size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t H, int64_t KV, int64_t D,
+                                                  int64_t max_query_length, int64_t max_context_length, int64_t window,
+                                                  int64_t sinks, int dtype) {
+  (void)dtype;
+  const int64_t st[4] = {0, 0, 0, 0};
+  LocalArgs a;
+  if (T <= 0 || n <= 0) return 0;
+  const int32_t some = 0;
+  if (fill_paged(&a, "paged_attention", T, n, H, KV, D, &some, &some, &some, 1, 1, 1, 1, st, st)) return 0;
+  set_window(&a, window, sinks);
+  const int max_q = (int)(max_query_length < T ? max_query_length : T);
+  if (max_q <= 0) return 0;
+  plan_split(&a, max_q, max_context_length, local_simt_row_tile(a, max_q), local_simt_key_tile());
+  return split_bytes(a);
+}
+
+extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_cache, const void* value_cache,
+                                     const int32_t* table, const int32_t* context, const int32_t* starts, void* workspace,
+                                     size_t workspace_bytes, int64_t T, int64_t n, int64_t H, int64_t KV, int64_t D,
+                                     int64_t page, int64_t pages, int64_t table_cols, int64_t table_stride,
+                                     const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                     const int64_t* out_strides, int64_t max_query_length, int64_t max_context_length,
+                                     int64_t window, int64_t sinks, float softmax_scale, int zero_tail, int dtype,
+                                     void* stream) {
+  LocalArgs a;
+  if (int rc = fill_paged(&a, "paged_attention", T, n, H, KV, D, table, context, starts, table_cols, table_stride, page,
+                          pages, k_strides, v_strides))
+    return rc;
+  TB200_REQUIRE(q_strides && out_strides, TB200_ERR_INVALID, "paged_attention: null stride array");
+  TB200_REQUIRE(sinks >= 0, TB200_ERR_INVALID, "paged_attention: %lld sinks", (long long)sinks);
+  TB200_REQUIRE(max_query_length > 0 && max_query_length < (1ll << 30) && max_context_length >= 0 &&
+                max_context_length < (1ll << 31), TB200_ERR_INVALID, "paged_attention: bad longest query or context");
+  if (T == 0 || n == 0) return 0;
+  TB200_REQUIRE(out && q && key_cache && value_cache, TB200_ERR_INVALID, "paged_attention: null pointer");
+  for (int i = 0; i < 3; ++i) {  // (head, token, feature) of q and out come as (token, head, feature)
+    const int to[3] = {2, 1, 3};
+    a.qs[to[i]] = q_strides[i];
+    a.os[to[i]] = out_strides[i];
+  }
+  set_window(&a, window, sinks);
+  a.scale = softmax_scale;
+  a.zero_tail = zero_tail;
+  cudaStream_t st = (cudaStream_t)stream;
+  const int max_q = (int)(max_query_length < T ? max_query_length : T);
+  const int row_tile = local_simt_row_tile(a, max_q), key_tile = local_simt_key_tile();
+  plan_split(&a, max_q, max_context_length, row_tile, key_tile);
+  TB200_REQUIRE(workspace_bytes >= split_bytes(a) && (workspace || a.split_tiles == 0), TB200_ERR_WORKSPACE,
+                "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, split_bytes(a));
+  a.part_out = (float*)workspace;
+  a.part_lse = a.part_out + (size_t)a.splits * a.tokens * a.H * a.D;
+  if (int rc = launch_local_fwd_simt(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st)) return rc;
+  if (a.split_tiles > 0)
+    if (int rc = launch_local_combine(out, a, max_q, row_tile / a.G, key_tile, dtype, st)) return rc;
+  note_kernel("local_simt", a.split_tiles > 0 ? 2 : 1);
+  return 0;
+}
+
+extern "C" int tb200_paged_cache_append(void* key_cache, void* value_cache, const void* k, const void* v,
+                                        const int32_t* table, const int32_t* context, const int32_t* starts, int64_t T,
+                                        int64_t n, int64_t KV, int64_t D, int64_t page, int64_t pages, int64_t table_cols,
+                                        int64_t table_stride, const int64_t* kc_strides, const int64_t* vc_strides,
+                                        const int64_t* k_strides, const int64_t* v_strides, int dtype, void* stream) {
+  LocalArgs a;
+  if (int rc = fill_paged(&a, "paged_cache_append", T, n, KV, KV, D, table, context, starts, table_cols, table_stride, page,
+                          pages, kc_strides, vc_strides))
+    return rc;
+  TB200_REQUIRE(k_strides && v_strides, TB200_ERR_INVALID, "paged_cache_append: null stride array");
+  if (T == 0 || n == 0) return 0;
+  TB200_REQUIRE(key_cache && value_cache && k && v, TB200_ERR_INVALID, "paged_cache_append: null pointer");
+  return dispatch_dtype(dtype, [&](auto tag) -> int {
+    using T_ = decltype(tag);
+    constexpr int VEC = Traits<T_>::VEC;
+    auto fits = [](const void* p, const int64_t* s, int last) {
+      bool ok = aligned16(p) && s[last] == 1;
+      for (int i = 0; i < last; ++i) ok = ok && s[i] % VEC == 0;
+      return ok;
+    };
+    const bool vec = fits(key_cache, a.ks, 3) && fits(value_cache, a.vs, 3) && fits(k, k_strides, 2) && fits(v, v_strides, 2);
+    // enough CTAs for all tokens in one sequence, at most 8 an SM over all sequences
+    const int64_t work = ceil_div(T * KV * D / (vec ? VEC : 1), 256), cap = ceil_div((int64_t)sm_count() * 8, n);
+    const dim3 grid((unsigned)(work < cap ? (work > 0 ? work : 1) : cap), 1, (unsigned)n);
+    auto kern = vec ? cache_append<T_, true> : cache_append<T_, false>;
+    kern<<<grid, 256, 0, (cudaStream_t)stream>>>((T_*)key_cache, (T_*)value_cache, (const T_*)k, (const T_*)v, a, k_strides[0],
+                                                 k_strides[1], k_strides[2], v_strides[0], v_strides[1], v_strides[2]);
+    const int rc = launch_status("cache_append");
+    if (rc == 0) note_kernel("cache_append", 1);
+    return rc;
+  });
+}

@@ -16,7 +16,10 @@ __all__ = [
     "rms_norm",
     "rms_norm_geglu",
     "mean",
+    "paged_attention",
+    "paged_cache_append",
     "scaled_dot_product_attention",
+    "sliding_window_attention",
     "softmax",
     "sum",
     "var",
@@ -130,6 +133,63 @@ def rms_norm_geglu(
     return out.view(*shape[:-1], out.shape[-1])
 
 
+def paged_attention(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lengths: torch.Tensor,
+    query_offsets: torch.Tensor = None,
+    max_query_length: int = None,
+    max_context_length: int = None,
+    window_size: int = None,
+    num_sinks: int = 0,
+    softmax_scale: float = None,
+    output: torch.Tensor = None,
+):
+    """
+    Computes attention of each sequence's newest tokens over the keys and values of a paged cache (not in
+    the reference): one token per sequence, or a chunk of a prompt, in one call.
+
+    key_cache and value_cache are [pages, page size, key heads, head size]; the key at position x of
+    sequence s is row x % page size of page block_table[s][x // page size]. context_lengths counts the
+    keys of each sequence, its new tokens included (paged_cache_append writes them first, with the same
+    arguments). The new tokens of sequence s are rows query_offsets[s] to query_offsets[s + 1] of query
+    [tokens, heads, head size]; without query_offsets there is one per sequence. A token sees the positions
+    up to its own; with window_size, those less than window_size back and the first num_sinks, and table
+    entries of blocks that no token sees may be anything. block_table, context_lengths and query_offsets
+    are int32 tensors on the device and are not read by the host.
+
+    No sequence may have more than max_query_length new tokens (default: all); max_context_length is the
+    longest context expected (default: what the table holds) and only chooses how the work is split. Both
+    have to be given for the best speed, and stay what they are in a captured graph. Rows of query that
+    belong to no sequence give zeros, or leave `output`, where it is given, as it was.
+    """
+    scale = 1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None else softmax_scale
+    return operation.paged_attention(
+        query, key_cache, value_cache, block_table, context_lengths, query_offsets, max_query_length,
+        max_context_length, window_size, num_sinks, scale, output,
+    )
+
+
+def paged_cache_append(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lengths: torch.Tensor,
+    query_offsets: torch.Tensor = None,
+):
+    """
+    Writes the keys and values [tokens, key heads, head size] of new tokens into the pages of a cache, in
+    place: the i-th of t new tokens of a sequence goes to position context_length - t + i.
+
+    See paged_attention for the other arguments.
+    """
+    operation.paged_cache_append(key, value, key_cache, value_cache, block_table, context_lengths, query_offsets)
+
+
 def scaled_dot_product_attention(
     query: torch.Tensor,
     key: torch.Tensor,
@@ -149,6 +209,28 @@ def scaled_dot_product_attention(
     return operation.Attention.apply(
         query, key, value, attn_mask, dropout_p, is_causal, 1.0 / math.sqrt(key.shape[-1]), use_accelerator
     )
+
+
+def sliding_window_attention(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    window_size: int,
+    num_sinks: int = 0,
+    softmax_scale: float = None,
+):
+    """
+    Computes causal attention in which a query sees its last window_size positions (its own among them)
+    and the first num_sinks tokens (not in the reference, whose attention is dense).
+
+    query is [batch, heads, length, head size], key and value [batch, key heads, length, head size]; each
+    key head serves heads / key heads consecutive query heads. The softmax scale is 1/sqrt(head size)
+    unless given. Any strides are taken; the output is laid out as query is.
+
+    See WindowAttention for more details.
+    """
+    scale = 1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None else softmax_scale
+    return operation.WindowAttention.apply(query, key, value, window_size, num_sinks, scale)
 
 
 def softmax(input: torch.Tensor, dim: int = None):

@@ -9,8 +9,8 @@ import torch
 
 from trident_b200 import function, util
 
-__all__ = ["GatedResidualRMSNorm", "GEGLU", "LayerNorm", "Linear", "MaskedSoftmax", "Mean", "RMSNorm", "ScaledDotProductAttention",
-           "Softmax", "Sum", "Var", "VarMean"]
+__all__ = ["GatedResidualRMSNorm", "GEGLU", "LayerNorm", "Linear", "MaskedSoftmax", "Mean", "PagedAttention", "RMSNorm",
+           "ScaledDotProductAttention", "SlidingWindowAttention", "Softmax", "Sum", "Var", "VarMean"]
 
 
 def _shape_tuple(shape: Union[int, Tuple[int, ...]]) -> Tuple[int, ...]:
@@ -247,6 +247,57 @@ class ScaledDotProductAttention(torch.nn.Module):
 
     def extra_repr(self):
         return f"dropout_p={self.dropout_p}, is_causal={self.is_causal}, use_accelerator={self.use_accelerator}"
+
+
+class SlidingWindowAttention(torch.nn.Module):
+    """Module form of function.sliding_window_attention."""
+
+    def __init__(self, window_size: int, num_sinks: int = 0, softmax_scale: float = None):
+        super().__init__()
+        self.window_size = window_size
+        self.num_sinks = num_sinks
+        self.softmax_scale = softmax_scale
+
+    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor):
+        return function.sliding_window_attention(
+            query, key, value, self.window_size, self.num_sinks, self.softmax_scale
+        )
+
+    def extra_repr(self):
+        return f"window_size={self.window_size}, num_sinks={self.num_sinks}, backend=Trident"
+
+
+class PagedAttention(torch.nn.Module):
+    """Keys and values of new tokens into the pages of a cache, then the tokens' attention over it
+    (function.paged_cache_append and function.paged_attention with the same arguments)."""
+
+    def __init__(self, window_size: int = None, num_sinks: int = 0, softmax_scale: float = None):
+        super().__init__()
+        self.window_size = window_size
+        self.num_sinks = num_sinks
+        self.softmax_scale = softmax_scale
+
+    def forward(
+        self,
+        query: torch.Tensor,
+        key: torch.Tensor,
+        value: torch.Tensor,
+        key_cache: torch.Tensor,
+        value_cache: torch.Tensor,
+        block_table: torch.Tensor,
+        context_lengths: torch.Tensor,
+        query_offsets: torch.Tensor = None,
+        max_query_length: int = None,
+        max_context_length: int = None,
+    ):
+        function.paged_cache_append(key, value, key_cache, value_cache, block_table, context_lengths, query_offsets)
+        return function.paged_attention(
+            query, key_cache, value_cache, block_table, context_lengths, query_offsets, max_query_length,
+            max_context_length, self.window_size, self.num_sinks, self.softmax_scale,
+        )
+
+    def extra_repr(self):
+        return f"window_size={self.window_size}, num_sinks={self.num_sinks}, backend=Trident"
 
 
 class Softmax(torch.nn.Module):
