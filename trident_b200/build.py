@@ -26,6 +26,7 @@ SOURCES = [
     "attention_bwd_tc.cu",
     "local_attention.cu",
     "local_attention_simt.cu",
+    "local_attention_fwd_tc.cu",
 ]
 
 NVCC_FLAGS = [

@@ -1,6 +1,6 @@
 // Entry points of local attention (window and sinks), training and serving, and the cache write:
 // validate, pick a kernel family, launch.
-#include "local_attention.cuh"
+#include "local_attention_tc.cuh"
 
 namespace tb200 {
 namespace {
@@ -159,8 +159,10 @@ extern "C" int tb200_window_attention_fwd(void* out, float* lse, const void* q, 
     return rc;
   if (B == 0 || S == 0) return 0;
   TB200_REQUIRE(out && lse && q && k && v, TB200_ERR_INVALID, "window_attention_fwd: null pointer");
-  int rc = launch_local_fwd_simt(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream);
-  if (rc == 0) note_kernel("local_simt", 1);
+  const bool tc = local_tc_supported(a, dtype, q, k, v, out);
+  int rc = tc ? launch_local_fwd_tc(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream)
+              : launch_local_fwd_simt(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream);
+  if (rc == 0) note_kernel(tc ? "local_tcgen05" : "local_simt", 1);
   return rc;
 }
 
@@ -224,8 +226,11 @@ extern "C" size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t 
   set_window(&a, window, sinks);
   const int max_q = (int)(max_query_length < T ? max_query_length : T);
   if (max_q <= 0) return 0;
+  // (which kernel family takes the call depends on strides and alignment: enough for either)
+  LocalArgs b = a;
   plan_split(&a, max_q, max_context_length, local_simt_row_tile(a, max_q), local_simt_key_tile());
-  return split_bytes(a);
+  plan_split(&b, max_q, max_context_length, 2 * LOCAL_TC_TILE, LOCAL_TC_TILE);
+  return split_bytes(a) > split_bytes(b) ? split_bytes(a) : split_bytes(b);
 }
 
 extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_cache, const void* value_cache,
@@ -256,16 +261,22 @@ extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_c
   a.zero_tail = zero_tail;
   cudaStream_t st = (cudaStream_t)stream;
   const int max_q = (int)(max_query_length < T ? max_query_length : T);
-  const int row_tile = local_simt_row_tile(a, max_q), key_tile = local_simt_key_tile();
+  const bool tc = local_tc_supported(a, dtype, q, key_cache, value_cache, out);
+  const int row_tile = tc ? 2 * LOCAL_TC_TILE : local_simt_row_tile(a, max_q);
+  const int key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
   plan_split(&a, max_q, max_context_length, row_tile, key_tile);
   TB200_REQUIRE(workspace_bytes >= split_bytes(a) && (workspace || a.split_tiles == 0), TB200_ERR_WORKSPACE,
                 "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, split_bytes(a));
   a.part_out = (float*)workspace;
   a.part_lse = a.part_out + (size_t)a.splits * a.tokens * a.H * a.D;
-  if (int rc = launch_local_fwd_simt(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st)) return rc;
-  if (a.split_tiles > 0)
-    if (int rc = launch_local_combine(out, a, max_q, row_tile / a.G, key_tile, dtype, st)) return rc;
-  note_kernel("local_simt", a.split_tiles > 0 ? 2 : 1);
+  int rc = tc ? launch_local_fwd_tc(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st)
+              : launch_local_fwd_simt(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st);
+  if (rc) return rc;
+  if (a.split_tiles > 0) {
+    const int row_tokens = tc ? local_tc_row_tokens(a) : row_tile / a.G;
+    if ((rc = launch_local_combine(out, a, max_q, row_tokens, key_tile, dtype, st))) return rc;
+  }
+  note_kernel(tc ? "local_tcgen05" : "local_simt", a.split_tiles > 0 ? 2 : 1);
   return 0;
 }
 

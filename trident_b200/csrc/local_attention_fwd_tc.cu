@@ -1,0 +1,711 @@
+// tcgen05 forward of local attention (window and sinks), training and serving form, for 16-bit operands
+// with head size 64 or 128.
+//
+// A CTA owns two adjacent tiles of 128 packed query rows (token * G + head of the group) of one sequence
+// and key head, and walks the key tiles that any of them sees (KeyRange), or one part of that walk. Both
+// score tiles and both output accumulators live in tensor memory (S0, S1: 128 fp32 columns each; O0, O1: D
+// columns each), so the tensor pipe works on one query tile while the softmax warps work on the other; a
+// key tile that only one of the two sees is walked by that one alone.
+//
+//   warp 0      producer: Q0, Q1 once, then rings of two K and two V tiles. A tile of keys is 128 rows of
+//               a sequence (training), or 128 / R pieces of R rows, R the largest divisor of the page size
+//               and of 128: one lane per piece looks its page up and issues its copies. Pieces that no row
+//               sees, or whose page is outside the pool, are read at a page index past the end: zeros.
+//   warp 1      MMA issuer: S_t = Q_t K^T, O_t += P_t V (P_t from tensor memory)
+//   warp 2      tensor-memory allocation
+//   warp 3      serving form: zeroes the rows of the last V tile behind the sequence's end (a probability
+//               of 0 times what an unused row holds, which may be NaN, would not be 0)
+//   warps 4-7   softmax of query tile 0, warps 8-11 of tile 1: one thread per row; scores stay in registers
+//               between maximum and exponentials. Warps without a row of the sequence only pass the
+//               barriers (a single new token is G rows of one tile).
+//
+// Only tiles at a border of the window, of the sinks or of the diagonal are masked per element, with a
+// 32-bit mask per 32 columns. The running maximum used in the exponent moves only when the true one has moved
+// by more than 8 (log2 units): the final division by the row sum undoes it exactly. The row sum adds the
+// fp32 probabilities; P is rounded to 16 bits for the product with V, as the tensor cores take it.
+//
+// Bound, by size of the problem: exponentials (128 x 128 of them take the 16 units of an SM 1024 cycles a
+// tile pair, both products together 512 at D = 128) for chunks and training, HBM for single tokens.
+#include <mutex>
+#include <type_traits>
+
+#include "attn_math.cuh"
+#include "local_attention_tc.cuh"
+#include "ptx.cuh"
+
+namespace tb200 {
+namespace {
+
+constexpr int TILE = LOCAL_TC_TILE;
+constexpr int FWD_THREADS = 384;
+// (launch registers x threads is the pool that setmaxnreg.inc draws on; checked below and by the host)
+constexpr int REGS_LAUNCH = 168, REGS_SERVICE = 72, REGS_SOFTMAX = 216;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float RESCALE_THRESHOLD = 8.f;
+
+struct FwdParams {
+  LocalArgs a;
+  void* out;
+  float* lse;
+  float scale_log2;
+  int tile_tokens;  // tokens of a query tile
+  int piece;        // R: rows of one copy of keys
+  int reverse;      // walk lengths grow with the tile index: longest first
+  uint32_t wait_units;
+};
+
+__device__ inline void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(ptx::smem_u32(dst)), "l"(map), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ inline void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w, int u) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(ptx::smem_u32(dst)), "l"(map), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u)
+      : "memory");
+}
+// the lowest n bits
+__device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(FWD_THREADS, 1)
+    local_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v, const FwdParams p) {
+  constexpr int TILE_BYTES = TILE * D * 2;
+  constexpr int NBOX = D / 64;
+  constexpr int BOX_BYTES = TILE * 64 * 2;
+  constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t IDESC_QK = ptx::make_idesc(IS_BF16, false, false, TILE, TILE);
+  constexpr uint32_t IDESC_PV = ptx::make_idesc(IS_BF16, false, true, TILE, D);
+  constexpr uint32_t TMEM_COLS = 512;
+  constexpr uint32_t COL_S = 0, COL_O = 256;
+  // At D = 64 the accumulators leave 128 columns free: P gets columns of its own, and the next score
+  // product is issued as soon as the softmax threads hold the current scores in registers.
+  constexpr bool P_SPLIT = D == 64;
+  constexpr uint32_t COL_P = 384;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_smem = smem;                    // [2][TILE_BYTES]
+  uint8_t* k_smem = smem + 2 * TILE_BYTES;   // [2][TILE_BYTES]
+  uint8_t* v_smem = smem + 4 * TILE_BYTES;   // [2][TILE_BYTES]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * TILE_BYTES);
+  // Hand-overs. A ring barrier completes once per step of the walk, a barrier of query tile t once per
+  // step that t takes part in (its count c): the waiter of phase c passes parity c & 1.
+  //   k/v_full    copies (complete_tx), or warp 3 after its zeroes   MMA issuer
+  //   k/v_empty   tcgen05.commit after the last product that reads   producer
+  //   s_full[t]   tcgen05.commit after Q_t K^T                       softmax: load of S_t
+  //   s_free[t]   128 softmax threads after the load of S_t (D = 64) MMA issuer: next Q_t K^T over S_t
+  //   p_full[t]   128 softmax threads after the store of P_t         MMA issuer: P_t V
+  //   o_done[t]   tcgen05.commit after P_t V                         softmax: rescale, P_t over P_t, epilogue
+  uint64_t* q_full = bars;           // [2]
+  uint64_t* k_full = bars + 2;       // [2]
+  uint64_t* k_empty = bars + 4;      // [2]
+  uint64_t* v_full = bars + 6;       // [2]
+  uint64_t* v_empty = bars + 8;      // [2]
+  uint64_t* s_full = bars + 10;      // [2]
+  uint64_t* p_full = bars + 12;      // [2]
+  uint64_t* o_done = bars + 14;      // [2]
+  uint64_t* s_free = bars + 16;      // [2]
+  uint64_t* v_raw = bars + 18;       // the copies of a V tile that warp 3 completes
+  uint64_t* mma_drained = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  volatile uint32_t* abort_flag = tmem_slot + 1;  // [0] abort flag, [1] wait limit (ptx::mbar_wait)
+
+  const LocalArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int s = blockIdx.z / a.splits, split = blockIdx.z % a.splits, hk = blockIdx.y;
+  const Sequence seq = load_sequence(a, s);
+  if (PAGED && a.zero_tail && s == a.n - 1 && hk == 0 && split == 0) zero_tail_rows(reinterpret_cast<T*>(p.out), a, seq);
+  const int pair = p.reverse ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
+  const int t0 = pair * 2 * p.tile_tokens;  // first token (within the sequence) of query tile 0
+  if (t0 >= seq.q_len) return;
+  const int base = seq.kv_len - seq.q_len;
+  const int last_token = min(t0 + 2 * p.tile_tokens, seq.q_len) - 1;
+  const KeyRange kr = key_range(a, base + t0, base + last_token, seq.kv_len, TILE);
+  int m0, m1;
+  split_range(a, kr.count, split, &m0, &m1);
+  if (split > 0 && m0 >= m1) return;
+  const bool whole = a.split_tiles == 0 || kr.count <= a.split_tiles;
+  // the walk of one query tile: key tiles below `st` (sinks) or from lo on, up to hi
+  const int st_tiles = a.window != NO_WINDOW && a.sinks > 0 ? (a.sinks + TILE - 1) / TILE : 0;
+  auto lowest = [&](int t) { return first_key(a, max(base + t0 + t * p.tile_tokens, 0)) / TILE; };
+  auto highest = [&](int t) {
+    const int first = t0 + t * p.tile_tokens, last = min(first + p.tile_tokens, seq.q_len) - 1;
+    return first <= last && base + last >= 0 ? (base + last) / TILE : -1;
+  };
+  const int lo0 = lowest(0), lo1 = lowest(1), hi0 = highest(0), hi1 = highest(1);
+  auto active = [&](int t, int j) { return (j < st_tiles || j >= (t ? lo1 : lo0)) && j <= (t ? hi1 : hi0); };
+  // the last V tile has rows behind the sequence's end that its copies do not fill with zeros
+  const bool fix = PAGED && m1 > m0 && kr.tile(m1 - 1) == (seq.kv_len - 1) / TILE && seq.kv_len % p.piece != 0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 12; ++i) ptx::mbar_init(&bars[i], 1);
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(&p_full[t], 128);
+      ptx::mbar_init(&o_done[t], 1);
+      ptx::mbar_init(&s_free[t], 128);
+    }
+    ptx::mbar_init(v_raw, 1);
+    ptx::mbar_init(mma_drained, 1);
+    abort_flag[0] = 0;
+    abort_flag[1] = p.wait_units;
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&map_q);
+    ptx::prefetch_tensormap(&map_k);
+    ptx::prefetch_tensormap(&map_v);
+  }
+  if (warp == 2) {
+    ptx::tmem_alloc(tmem_slot, TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  static_assert(REGS_LAUNCH * FWD_THREADS <= 65536, "launch allocation");
+  static_assert(4 * 32 * REGS_SERVICE + 8 * 32 * REGS_SOFTMAX <= REGS_LAUNCH * FWD_THREADS,
+                "register pool of the CTA exceeded: setmaxnreg.inc would never return");
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_SERVICE));
+    if (warp == 0) {
+      // -------------------------------------------------------------- producer (whole warp)
+      const int pieces = TILE / p.piece;
+      if (m1 > m0 && lane == 0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if ((t ? hi1 : hi0) < 0) continue;
+          ptx::mbar_expect_tx(&q_full[t], NBOX * p.tile_tokens * a.G * 128);
+#pragma unroll
+          for (int c = 0; c < NBOX; ++c)
+            tma_load_5d(q_smem + t * TILE_BYTES + c * BOX_BYTES, &map_q, &q_full[t], c * 64, 0,
+                        seq.q_begin + t0 + t * p.tile_tokens, hk, PAGED ? 0 : s);
+        }
+      }
+      const int from = first_key(a, max(base + t0, 0));
+      // page and row of this lane's piece of key tile j (index `pages`: zeros)
+      auto locate = [&](int j, int* page, int* row) {
+        if constexpr (PAGED) {
+          const int p0 = j * TILE + lane * p.piece;
+          int id = -1;
+          if (lane < pieces && p0 < seq.kv_len && (p0 + p.piece > from || p0 < a.sinks))
+            id = a.table[s * a.table_stride + p0 / a.page];
+          *page = id < 0 || id >= a.pages ? a.pages : id;
+          *row = p0 % a.page;
+        } else {
+          *page = s;
+          *row = j * TILE;
+        }
+      };
+      int page = 0, row = 0;
+      if (m1 > m0) locate(kr.tile(m0), &page, &row);
+      for (int m = m0; m < m1; ++m) {
+        const int st = (m - m0) & 1;
+        const uint32_t ph = ((m - m0) >> 1) & 1;
+        int next_page = 0, next_row = 0;  // (looked up while this step's copies wait for their stage)
+        if (m + 1 < m1) locate(kr.tile(m + 1), &next_page, &next_row);
+        if (lane == 0) {
+          ptx::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, 61);
+          ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
+        }
+        __syncwarp();
+        if (lane < pieces) {
+#pragma unroll
+          for (int c = 0; c < NBOX; ++c)
+            tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, &map_k, &k_full[st], c * 64, row, hk,
+                        page);
+        }
+        uint64_t* vbar = fix && m + 1 == m1 ? v_raw : &v_full[st];
+        if (lane == 0) {
+          ptx::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, 62);
+          ptx::mbar_expect_tx(vbar, TILE_BYTES);
+        }
+        __syncwarp();
+        if (lane < pieces) {
+#pragma unroll
+          for (int c = 0; c < NBOX; ++c)
+            tma_load_4d(v_smem + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, &map_v, vbar, c * 64, row, hk, page);
+        }
+        page = next_page;
+        row = next_row;
+      }
+      // Drain: every copy has landed before the CTA gives up its shared memory.
+      if (lane == 0 && m1 > m0) {
+        for (int t = 0; t < 2; ++t)
+          if ((t ? hi1 : hi0) >= 0) ptx::mbar_wait_drain(&q_full[t], 0, abort_flag, a.status, 63);
+        for (int m = m1 - m0 > 2 ? m1 - 2 : m0; m < m1; ++m) {
+          const int st = (m - m0) & 1;
+          const uint32_t ph = ((m - m0) >> 1) & 1;
+          ptx::mbar_wait_drain(&k_full[st], ph, abort_flag, a.status, 64);
+          if (fix && m + 1 == m1)
+            ptx::mbar_wait_drain(v_raw, 0, abort_flag, a.status, 65);
+          else
+            ptx::mbar_wait_drain(&v_full[st], ph, abort_flag, a.status, 65);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // -------------------------------------------------------------- MMA issuer
+      const bool elected = ptx::elect_one();
+      auto wait_ = [&](uint64_t* bar, uint32_t parity, int code) {
+        if (elected) ptx::mbar_wait(bar, parity, abort_flag, a.status, code);
+        __syncwarp();
+      };
+      auto commit_ = [&](uint64_t* bar) {
+        if (elected) ptx::umma_commit(bar);
+      };
+      const uint64_t dq0 = ptx::make_smem_desc(ptx::smem_u32(q_smem), 16, 1024);
+      const uint64_t dk0 = ptx::make_smem_desc(ptx::smem_u32(k_smem), 16, 1024);
+      const uint64_t dv0 = ptx::make_smem_desc(ptx::smem_u32(v_smem), BOX_BYTES, 1024);
+      constexpr uint64_t NEXT_TILE = static_cast<uint64_t>(TILE_BYTES >> 4);
+      auto issue_qk = [&](int t, int st) {
+        const uint64_t qd = dq0 + (t ? NEXT_TILE : 0), kd = dk0 + (st ? NEXT_TILE : 0);
+        const uint32_t d_tmem = tmem_base + COL_S + t * 128;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint64_t off = static_cast<uint64_t>(((ks >> 2) * BOX_BYTES + (ks & 3) * 32) >> 4);
+          if (elected) ptx::umma_ss(d_tmem, qd + off, kd + off, IDESC_QK, ks != 0);
+        }
+      };
+      auto issue_pv = [&](int t, int st, bool accumulate) {
+        const uint64_t vd = dv0 + (st ? NEXT_TILE : 0);
+        const uint32_t d_tmem = tmem_base + COL_O + t * D;
+        const uint32_t p_tmem = tmem_base + (P_SPLIT ? COL_P + t * 64 : COL_S + t * 128);
+#pragma unroll
+        for (int ks = 0; ks < TILE / 16; ++ks) {
+          if (elected)
+            ptx::umma_ts(d_tmem, p_tmem + ks * 8, vd + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_PV,
+                         accumulate || ks != 0);
+        }
+      };
+      if (m1 > m0) {
+        int scores[2] = {0, 0}, values[2] = {0, 0};  // products issued so far, per query tile
+        // S of step m for query tile t
+        auto do_scores = [&](int t, int m) {
+          const int st = (m - m0) & 1;
+          if (scores[t] == 0) wait_(&q_full[t], 0, 71 + t);
+          if (P_SPLIT && scores[t] > 0) wait_(&s_free[t], (scores[t] - 1) & 1, 73 + t);
+          wait_(&k_full[st], ((m - m0) >> 1) & 1, 75);
+          ptx::tc_fence_after();
+          issue_qk(t, st);
+          commit_(&s_full[t]);
+          ++scores[t];
+        };
+        auto do_values = [&](int t, int m) {
+          const int st = (m - m0) & 1;
+          wait_(&p_full[t], values[t] & 1, 76 + t);
+          wait_(&v_full[st], ((m - m0) >> 1) & 1, 78);
+          ptx::tc_fence_after();
+          issue_pv(t, st, values[t] > 0);
+          commit_(&o_done[t]);
+          ++values[t];
+        };
+        {
+          const int j = kr.tile(m0);
+          if (active(0, j)) do_scores(0, m0);
+          if (active(1, j)) do_scores(1, m0);
+          commit_(&k_empty[0]);
+        }
+        for (int m = m0; m < m1; ++m) {
+          const int j = kr.tile(m), nj = m + 1 < m1 ? kr.tile(m + 1) : 0;
+          const bool more = m + 1 < m1;
+          if constexpr (P_SPLIT) {
+            // next scores of a tile before its values
+            if (more && active(0, nj)) do_scores(0, m + 1);
+            if (active(0, j)) do_values(0, m);
+            if (more && active(1, nj)) do_scores(1, m + 1);
+            if (more) commit_(&k_empty[(m + 1 - m0) & 1]);
+            if (active(1, j)) do_values(1, m);
+            commit_(&v_empty[(m - m0) & 1]);
+          } else {
+            // P overwrites S: the next scores follow the values on the in-order pipe
+            if (active(0, j)) do_values(0, m);
+            if (more && active(0, nj)) do_scores(0, m + 1);
+            if (active(1, j)) do_values(1, m);
+            commit_(&v_empty[(m - m0) & 1]);
+            if (more && active(1, nj)) do_scores(1, m + 1);
+            if (more) commit_(&k_empty[(m + 1 - m0) & 1]);
+          }
+        }
+      }
+      // everything issued has completed before tensor memory is freed
+      commit_(mma_drained);
+      if (elected) ptx::mbar_wait_drain(mma_drained, 0, abort_flag, a.status, 79);
+      __syncwarp();
+    } else if (PAGED && warp == 3 && fix) {
+      // -------------------------------------------------------------- zeros behind the sequence's end
+      const int st = (m1 - 1 - m0) & 1;
+      ptx::mbar_wait(v_raw, 0, abort_flag, a.status, 66);
+      const int first = seq.kv_len % TILE, end = min(TILE, ((first + p.piece - 1) / p.piece) * p.piece);
+      // (whole pieces behind the end were read as zeros)
+      for (int r = first; r < end; ++r)
+#pragma unroll
+        for (int c = 0; c < NBOX; ++c)
+          if (lane < 8) *reinterpret_cast<uint4*>(v_smem + st * TILE_BYTES + c * BOX_BYTES + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&v_full[st]);
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax + epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    const int t = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const int first_token = t0 + t * p.tile_tokens;
+    const int tokens = min(p.tile_tokens, seq.q_len - first_token);
+    const int rows = tokens > 0 ? tokens * a.G : 0;
+    const bool warp_live = quarter * 32 < rows, live = r < rows;
+    const int token = first_token + r / a.G;  // of the sequence
+    const int pos = live ? base + token : -1;
+    const int pmin = base + first_token, pmax = base + first_token + tokens - 1;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_off + COL_S + t * 128;
+    const uint32_t o_addr = tmem_base + lane_off + COL_O + t * D;
+    const uint32_t p_addr = tmem_base + lane_off + (P_SPLIT ? COL_P + t * 64 : COL_S + t * 128);
+    float m_used = -INFINITY, l = 0.f;
+    int count = 0;
+    for (int m = m0; m < m1; ++m) {
+      const int j = kr.tile(m);
+      if (!active(t, j)) continue;
+      const int c = count++;
+      ptx::mbar_wait(&s_full[t], c & 1, abort_flag, a.status, 81);
+      ptx::tc_fence_after();
+      if (!warp_live) {
+        if constexpr (P_SPLIT) ptx::mbar_arrive(&s_free[t]);
+        // (P(c) of these rows is never read into a stored result; the barrier's phases stay in step)
+        if (P_SPLIT && c > 0) ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 82);
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(&p_full[t]);
+        continue;
+      }
+      const int j0 = j * TILE;
+      // every row of the tile sees every key of it
+      const bool plain = j0 + TILE - 1 <= pmin && (pmax - j0 < a.window || j0 + TILE <= a.sinks);
+      uint32_t sr[4][32];
+      float mx = -INFINITY;
+      if (plain) {
+        float x0 = -INFINITY, x1 = -INFINITY;
+        auto reduce32 = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            x0 = am::max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            x1 = am::max3(x1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+          }
+        };
+        ptx::tmem_ld32(s_addr, sr[0]);
+        am::tmem_ld_wait_dep(sr[0]);
+        ptx::tmem_ld32(s_addr + 32, sr[1]);
+        reduce32(sr[0]);
+        am::tmem_ld_wait_dep(sr[1]);
+        ptx::tmem_ld32(s_addr + 64, sr[2]);
+        reduce32(sr[1]);
+        am::tmem_ld_wait_dep(sr[2]);
+        ptx::tmem_ld32(s_addr + 96, sr[3]);
+        reduce32(sr[2]);
+        am::tmem_ld_wait_dep(sr[3]);
+        reduce32(sr[3]);
+        if (p.scale_log2 < 0.f) {  // (the largest score is the smallest product)
+          x0 = x1 = INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x0 = fminf(x0, __uint_as_float(sr[q][i]));
+        } else {
+          x0 = fmaxf(x0, x1);
+        }
+        mx = x0 * p.scale_log2;
+      } else {
+        const int high = min(pos, seq.kv_len - 1) - j0 + 1;  // columns below `high` are not in the future
+        const int64_t low64 = (int64_t)pos - a.window + 1 - j0;
+        const int low = low64 < 0 ? 0 : (int)low64;          // columns from `low` on are in the window
+        const int sink = a.sinks - j0;                       // columns below `sink` are sinks
+        auto scale32 = [&](uint32_t (&v)[32], int q) {
+          const uint32_t seen = low_bits(high - 32 * q) & (~low_bits(low - 32 * q) | low_bits(sink - 32 * q));
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float sc = (seen >> i) & 1u ? __uint_as_float(v[i]) * p.scale_log2 : -INFINITY;
+            mx = fmaxf(mx, sc);
+            v[i] = __float_as_uint(sc);
+          }
+        };
+        ptx::tmem_ld32(s_addr, sr[0]);
+        am::tmem_ld_wait_dep(sr[0]);
+        ptx::tmem_ld32(s_addr + 32, sr[1]);
+        scale32(sr[0], 0);
+        am::tmem_ld_wait_dep(sr[1]);
+        ptx::tmem_ld32(s_addr + 64, sr[2]);
+        scale32(sr[1], 1);
+        am::tmem_ld_wait_dep(sr[2]);
+        ptx::tmem_ld32(s_addr + 96, sr[3]);
+        scale32(sr[2], 2);
+        am::tmem_ld_wait_dep(sr[3]);
+        scale32(sr[3], 3);
+      }
+      if constexpr (P_SPLIT) {
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(&s_free[t]);
+      }
+      const float m_new = fmaxf(m_used, mx);
+      if (c == 0) {
+        m_used = m_new;
+      } else {
+        const bool need = m_new > m_used + RESCALE_THRESHOLD;
+        if (__any_sync(0xffffffffu, need)) {
+          ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 83);
+          ptx::tc_fence_after();
+          const float factor = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t v[32];
+            ptx::tmem_ld32(o_addr + q * 32, v);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
+            ptx::tmem_st32(o_addr + q * 32, v);
+          }
+          ptx::tmem_st_wait();
+          l *= factor;
+          m_used = m_new;
+        }
+      }
+      const float m_safe = m_used == -INFINITY ? 0.f : m_used;
+      {
+        const float to_log2 = plain ? p.scale_log2 : 1.f;
+        const uint64_t scale2 = am::pack2f(to_log2, to_log2);
+        const uint64_t negm2 = am::pack2f(-m_safe, -m_safe);
+        uint64_t lsum = am::pack2f(0.f, 0.f), lsum_b = am::pack2f(0.f, 0.f);
+        auto exp32 = [&](const uint32_t (&v)[32], int q) {
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            am::unpack2f(am::fma2(am::pack2u(v[i], v[i + 1]), scale2, negm2), x[i], x[i + 1]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = am::ex2(x[i]);
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            lsum = am::add2(lsum, am::pack2f(x[i], x[i + 1]));
+            lsum_b = am::add2(lsum_b, am::pack2f(x[i + 2], x[i + 3]));
+            packed[i >> 1] = am::cvt_pair<T>(x[i], x[i + 1]);
+            packed[(i >> 1) + 1] = am::cvt_pair<T>(x[i + 2], x[i + 3]);
+          }
+          ptx::tmem_st16(p_addr + q * 16, packed);
+        };
+        if constexpr (P_SPLIT) {
+          if (c > 0) {  // P(c) goes over P(c-1)
+            ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 84);
+            ptx::tc_fence_after();
+          }
+        }
+        exp32(sr[0], 0);
+        exp32(sr[1], 1);
+        exp32(sr[2], 2);
+        exp32(sr[3], 3);
+        float l0, l1;
+        am::unpack2f(am::add2(lsum, lsum_b), l0, l1);
+        l += l0 + l1;
+      }
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(&p_full[t]);
+    }
+    if (warp_live) {
+      if (count > 0) {
+        ptx::mbar_wait(&o_done[t], (count - 1) & 1, abort_flag, a.status, 85);
+        ptx::tc_fence_after();
+      }
+      const int head = hk * a.G + r % a.G;
+      const long long tok = seq.q_begin + token;
+      const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys: zeros
+      const float ls = l > 0.f ? m_used * LN2 + logf(l) : -INFINITY;
+      T* orow = reinterpret_cast<T*>(p.out) + (long long)s * a.os[0] + head * a.os[1] + tok * a.os[2];
+      const long long prow = ((long long)split * a.tokens + tok) * a.H + head;
+#pragma unroll 1
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t v[32];
+        __syncwarp();
+        if (count > 0) {
+          ptx::tmem_ld32(o_addr + q * 32, v);
+          ptx::tmem_ld_wait();
+        }
+        if (!(l > 0.f)) {  // (nothing was accumulated: the columns hold what was there before)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0;
+        }
+        if (live && whole) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 o;
+            o.x = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv);
+            o.y = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv);
+            o.z = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv);
+            o.w = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv);
+            *reinterpret_cast<uint4*>(orow + q * 32 + g * 8) = o;
+          }
+        } else if (live && l > 0.f) {  // (a part without keys is known by its lse)
+          float4* dst = reinterpret_cast<float4*>(a.part_out + prow * D + q * 32);
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            dst[g] = make_float4(__uint_as_float(v[g * 4]) * inv, __uint_as_float(v[g * 4 + 1]) * inv,
+                                 __uint_as_float(v[g * 4 + 2]) * inv, __uint_as_float(v[g * 4 + 3]) * inv);
+        }
+      }
+      if (live) {
+        if (!whole) a.part_lse[prow] = ls;
+        else if (!PAGED) p.lse[((long long)s * a.H + head) * a.tokens + tok] = ls;
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(sym);
+    else
+      cudaGetLastError();
+  });
+  return fn;
+}
+
+bool encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box, const char* what) {
+  bind_primary_context();
+  cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides,
+                                 box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return true;
+  set_error("local attention: tensor map of %s refused with CUresult %d", what, (int)r);
+  return false;
+}
+
+int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
+
+// stride of a dimension; one of extent 1 may carry any
+cuuint64_t stride_of(int64_t st, int64_t extent) { return (cuuint64_t)(extent > 1 ? st : 64) * 2; }
+
+bool stride_ok(int64_t st, int64_t extent) { return extent <= 1 || (st > 0 && st % 8 == 0 && st < (1ll << 38)); }
+
+}  // namespace
+
+// packed rows of q (or a tensor laid out like it): [features, head of the group, token, key head, sequence],
+// box of one query tile
+bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, const char* what) {
+  const bool paged = a.table != nullptr;
+  const cuuint64_t dims[5] = {(cuuint64_t)a.D, (cuuint64_t)a.G, (cuuint64_t)a.tokens, (cuuint64_t)a.KV,
+                              (cuuint64_t)(paged ? 1 : a.n)};
+  const cuuint64_t strides[4] = {stride_of(st[1], a.G), stride_of(st[2], a.tokens), stride_of(st[1] * a.G, a.KV),
+                                 stride_of(st[0], paged ? 1 : a.n)};
+  const cuuint32_t box[5] = {64, (cuuint32_t)a.G, (cuuint32_t)(LOCAL_TC_TILE / a.G), 1, 1};
+  return encode(map, 5, q, dims, strides, box, what);
+}
+// keys (or values): [features, position (of a page), key head, sequence or page], box of one piece
+bool local_map_keys(CUtensorMap* map, const void* k, const int64_t* st, const LocalArgs& a, int piece, const char* what) {
+  const bool paged = a.table != nullptr;
+  const int64_t rows = paged ? a.page : a.tokens, outer = paged ? a.pages : a.n;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)rows, (cuuint64_t)a.KV, (cuuint64_t)outer};
+  const cuuint64_t strides[3] = {stride_of(st[2], rows), stride_of(st[1], a.KV), stride_of(st[0], outer)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)piece, 1, 1};
+  return encode(map, 4, k, dims, strides, box, what);
+}
+bool local_rows_ok(const void* p, const int64_t* st, const LocalArgs& a) {
+  return aligned16(p) && st[3] == 1 && stride_ok(st[1], a.H) && stride_ok(st[2], a.tokens) &&
+         (a.table || stride_ok(st[0], a.n)) && st[1] * (int64_t)a.G < (1ll << 38);
+}
+bool local_keys_ok(const void* p, const int64_t* st, const LocalArgs& a) {
+  return aligned16(p) && st[3] == 1 && stride_ok(st[1], a.KV) && stride_ok(st[2], a.table ? a.page : a.tokens) &&
+         stride_ok(st[0], a.table ? a.pages : a.n);
+}
+int local_piece(const LocalArgs& a) { return a.table ? gcd(a.page, LOCAL_TC_TILE) : LOCAL_TC_TILE; }
+
+bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void* k, const void* v, const void* out) {
+  if (dtype != TB200_F16 && dtype != TB200_BF16) return false;
+  if (a.D != 64 && a.D != 128) return false;
+  if (a.table && (local_piece(a) < 8 || a.pages == 0)) return false;
+  return local_rows_ok(q, a.qs, a) && local_rows_ok(out, a.os, a) && local_keys_ok(k, a.ks, a) && local_keys_ok(v, a.vs, a) &&
+         encode_fn() != nullptr;
+}
+
+namespace {
+
+template <typename T, int D, bool PAGED>
+int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdParams& p, int max_q,
+               cudaStream_t st) {
+  constexpr int SMEM = 6 * TILE * D * 2 + 1024 + 256;
+  static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+  auto kern = local_fwd_tc_kernel<T, D, PAGED>;
+  static std::atomic<unsigned long long> optin_done{0};
+  static std::atomic<int> regs_cached{0};
+  cudaError_t e = smem_optin_per_device(optin_done, reinterpret_cast<const void*>(kern), SMEM);
+  int regs = regs_cached.load(std::memory_order_relaxed);
+  if (e == cudaSuccess && regs == 0) {
+    cudaFuncAttributes fa;
+    if ((e = cudaFuncGetAttributes(&fa, kern)) == cudaSuccess) {
+      regs = fa.numRegs;
+      regs_cached.store(regs, std::memory_order_relaxed);
+    }
+  }
+  if (e != cudaSuccess) {
+    set_error("local_fwd_tc: cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
+    return (int)e;
+  }
+  // (the register allowances of the kernel's warps come from its launch allocation)
+  if (regs * FWD_THREADS < 4 * 32 * REGS_SERVICE + 8 * 32 * REGS_SOFTMAX) {
+    set_error("local_fwd_tc: kernel compiled with %d registers per thread, the register rebalancing needs %d", regs, REGS_LAUNCH);
+    return TB200_ERR_UNSUPPORTED;
+  }
+  const dim3 grid((unsigned)ceil_div(max_q, 2 * p.tile_tokens), (unsigned)p.a.KV, (unsigned)(p.a.n * p.a.splits));
+  kern<<<grid, FWD_THREADS, SMEM, st>>>(mq, mk, mv, p);
+  return launch_status("local_fwd_tc");
+}
+
+}  // namespace
+
+int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, const void* v, const LocalArgs& a, int max_q,
+                        int dtype, cudaStream_t st) {
+  FwdParams p;
+  p.a = a;
+  p.a.status = device_status_ptr();
+  p.out = out;
+  p.lse = lse;
+  p.scale_log2 = a.scale * LOG2E;
+  p.tile_tokens = TILE / a.G;
+  p.piece = local_piece(a);
+  p.reverse = a.window == NO_WINDOW;
+  p.wait_units = ptx::WAIT_LIMIT_UNITS;
+  CUtensorMap mq, mk, mv;
+  if (!local_map_rows(&mq, q, a.qs, a, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
+      !local_map_keys(&mv, v, a.vs, a, p.piece, "v"))
+    return TB200_ERR_UNSUPPORTED;
+  auto go = [&](auto tag, auto dsel) -> int {
+    using T = decltype(tag);
+    constexpr int D = decltype(dsel)::value;
+    return a.table ? launch_fwd<T, D, true>(mq, mk, mv, p, max_q, st) : launch_fwd<T, D, false>(mq, mk, mv, p, max_q, st);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (dtype == TB200_BF16) return a.D == 128 ? go(__nv_bfloat16{}, D128{}) : go(__nv_bfloat16{}, D64{});
+  return a.D == 128 ? go(__half{}, D128{}) : go(__half{}, D64{});
+}
+
+}  // namespace tb200

@@ -294,11 +294,10 @@ __global__ void __launch_bounds__(256)
   for (int p = 0; p < parts; ++p) {
     const float w = expf(a.part_lse[row + p * step] - safe);
     total += w;
-    if (live) {
+    if (live && w > 0.f) {  // (a part without keys has no output)
       const float* src = a.part_out + (row + p * step) * D + lane * PER;
       float f[PER];
       load_w<PER>(f, src);
-      // (a part without keys has weight 0 and an output of zeros)
 #pragma unroll
       for (int i = 0; i < PER; ++i) acc[i] = fmaf(w, f[i], acc[i]);
     }
