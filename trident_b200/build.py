@@ -27,6 +27,7 @@ SOURCES = [
     "local_attention.cu",
     "local_attention_simt.cu",
     "local_attention_fwd_tc.cu",
+    "local_attention_bwd_tc.cu",
 ]
 
 NVCC_FLAGS = [

@@ -85,7 +85,16 @@ void plan_far(LocalBwdArgs* b, int key_tile) {
 size_t far_bytes(const LocalBwdArgs& b, int key_tile) {
   return (size_t)b.f.n * b.f.KV * b.sink_tiles * (b.far + 1) * 2 * key_tile * b.f.D * sizeof(float);
 }
-size_t row_bytes(const LocalArgs& a) { return ((size_t)a.n * a.H * a.tokens * sizeof(float) + 255) & ~(size_t)255; }
+// delta of each score row (CUDA cores), or -lse and -delta by query tile (tensor cores)
+size_t row_bytes(const LocalArgs& a, bool tc) {
+  const int64_t floats = tc ? 2 * local_tc_rows(a) : (int64_t)a.n * a.H * a.tokens;
+  return ((size_t)floats * sizeof(float) + 255) & ~(size_t)255;
+}
+size_t bwd_bytes(LocalBwdArgs b, bool tc) {
+  const int key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
+  plan_far(&b, key_tile);
+  return row_bytes(b.f, tc) + far_bytes(b, key_tile);
+}
 
 // Parts of a split walk. One row tile of a sequence and key head is one CTA; where those are too few
 // for the GPU the walk along the keys is cut. Single tokens (few rows): parts for 4 CTAs an SM, so that
@@ -172,8 +181,9 @@ extern "C" size_t tb200_window_attention_bwd_workspace(int64_t B, int64_t H, int
   const int64_t st[4] = {0, 0, 0, 0};
   LocalBwdArgs b;
   if (fill_window(&b.f, "window_attention_bwd", B, H, KV, S, D, st, st, st, st, window, sinks, 1.f)) return 0;
-  plan_far(&b, local_simt_key_tile());
-  return row_bytes(b.f) + far_bytes(b, local_simt_key_tile());
+  // (which kernel family takes the call depends on strides and alignment: enough for either)
+  const size_t simt = bwd_bytes(b, false), tc = bwd_bytes(b, true);
+  return simt > tc ? simt : tc;
 }
 
 extern "C" int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k,
@@ -195,22 +205,27 @@ extern "C" int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const vo
                 "window_attention_bwd: null pointer");
   copy4(b.dos, dout_strides); copy4(b.dqs, dq_strides); copy4(b.dks, dk_strides); copy4(b.dvs, dv_strides);
   cudaStream_t st = (cudaStream_t)stream;
-  const int key_tile = local_simt_key_tile();
+  const bool tc = local_bwd_tc_supported(b, dtype, q, k, v, out, dout, dq, dk, dv);
+  const int key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
+  const size_t need = bwd_bytes(b, tc);
   plan_far(&b, key_tile);
-  const size_t need = row_bytes(b.f) + far_bytes(b, key_tile);
   TB200_REQUIRE(workspace_bytes >= need, TB200_ERR_WORKSPACE, "window_attention_bwd: workspace of %zu bytes, %zu needed",
                 workspace_bytes, need);
   TB200_REQUIRE(aligned16(workspace), TB200_ERR_INVALID, "window_attention_bwd: workspace must be 16-byte aligned");
-  float* delta = (float*)workspace;
-  b.part = (float*)((char*)workspace + row_bytes(b.f));
-  if (int rc = launch_local_delta(delta, out, dout, b.dos, b.f, dtype, st)) return rc;
-  if (int rc = launch_local_bwd_simt(dq, dk, dv, dout, q, k, v, lse, delta, b, dtype, st)) return rc;
+  float* row_scratch = (float*)workspace;
+  b.part = (float*)((char*)workspace + row_bytes(b.f, tc));
+  if (tc) {
+    if (int rc = launch_local_bwd_tc(dq, dk, dv, dout, q, k, v, out, lse, row_scratch, b, dtype, st)) return rc;
+  } else {
+    if (int rc = launch_local_delta(row_scratch, out, dout, b.dos, b.f, dtype, st)) return rc;
+    if (int rc = launch_local_bwd_simt(dq, dk, dv, dout, q, k, v, lse, row_scratch, b, dtype, st)) return rc;
+  }
   int launches = 3;
   if (b.sink_tiles > 0) {
     if (int rc = launch_local_far_sum(dk, dv, b, key_tile, dtype, st)) return rc;
     ++launches;
   }
-  note_kernel("local_simt", launches);
+  note_kernel(tc ? "local_tcgen05" : "local_simt", launches);
   return 0;
 }
 

@@ -24,8 +24,8 @@
 // by more than 8 (log2 units): the final division by the row sum undoes it exactly. The row sum adds the
 // fp32 probabilities; P is rounded to 16 bits for the product with V, as the tensor cores take it.
 //
-// Bound, by size of the problem: exponentials (128 x 128 of them take the 16 units of an SM 1024 cycles a
-// tile pair, both products together 512 at D = 128) for chunks and training, HBM for single tokens.
+// Bound, by size of the problem: exponentials (the 128 x 128 of a tile pair take the 16 units of an SM 1024
+// cycles, as both products together at D = 128) for chunks and training, HBM for single tokens.
 #include <mutex>
 #include <type_traits>
 

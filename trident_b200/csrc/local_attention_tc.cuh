@@ -1,5 +1,7 @@
 // Tensor maps and launch entry points of the tcgen05 kernels of local attention.
 #pragma once
+#include <cuda.h>
+
 #include "local_attention.cuh"
 
 namespace tb200 {
@@ -11,6 +13,22 @@ constexpr int LOCAL_TC_TILE = 128;  // packed query rows and keys of a tile
 bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void* k, const void* v, const void* out);
 int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, const void* v, const LocalArgs& a, int max_q,
                         int dtype, cudaStream_t st);
+// Tensor maps (false with the error text set when the driver refuses one) and what they take.
+bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, const char* what);
+bool local_map_keys(CUtensorMap* map, const void* k, const int64_t* st, const LocalArgs& a, int piece, const char* what);
+bool local_rows_ok(const void* p, const int64_t* st, const LocalArgs& a);
+bool local_keys_ok(const void* p, const int64_t* st, const LocalArgs& a);
+
+// Backward pass of the training form. row_scratch: two float arrays of local_tc_rows(a) elements.
+bool local_bwd_tc_supported(const LocalBwdArgs& b, int dtype, const void* q, const void* k, const void* v, const void* out,
+                            const void* dout, const void* dq, const void* dk, const void* dv);
+int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k, const void* v,
+                        const void* out, const float* lse, float* row_scratch, const LocalBwdArgs& b, int dtype,
+                        cudaStream_t st);
+// packed rows of all query tiles, unused ones included
+static inline int64_t local_tc_rows(const LocalArgs& a) {
+  return (int64_t)a.n * a.KV * ceil_div(a.tokens, LOCAL_TC_TILE / a.G) * LOCAL_TC_TILE;
+}
 // tokens of the two query tiles of a CTA
 static inline int local_tc_row_tokens(const LocalArgs& a) { return 2 * (LOCAL_TC_TILE / a.G); }
 
