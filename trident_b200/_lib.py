@@ -5,8 +5,8 @@ the current CUDA stream, and raises on a non-zero status. There is no CPU or PyT
 fallback: without the built library, or without a CUDA device, the calls fail loudly.
 """
 
-import contextlib
 import ctypes
+import functools
 import os
 
 import torch
@@ -170,27 +170,53 @@ def _require_cuda(*tensors):
             raise Tb200Error("trident_b200 kernels run on CUDA tensors only (no CPU fallback)")
 
 
-def _on_device(tensor):
-    """Context in which `tensor`'s device is the current one (a launch goes to the current device)."""
-    if torch.cuda.current_device() == tensor.device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(tensor.device)
+def _call(name, like, *args):
+    """Calls entry point `name` on the device of tensor `like`, made current if it is not (a launch goes
+    to the current device), and that device's current stream. (The raw handles of torch._C: a Stream
+    object and a device context cost more host time than the launch of a small kernel.)"""
+    function = getattr(load(), name)
+    index = like.device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        status = function(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            status = function(*args, stream)
+    if status != 0:
+        _check(status, name)
 
 
-def require_one_device(**tensors):
+@functools.lru_cache(maxsize=4096)
+def _workspace(name, index, *args):
+    """Bytes of workspace that entry point `name` asks for (a function of sizes and of the device)."""
+    with torch.cuda.device(index):
+        return getattr(load(), name)(*args)
+
+
+def require_one_device(*tensors):
     """All given tensors (None allowed) lie on one CUDA device."""
-    _require_cuda(*tensors.values())
-    devices = {t.device for t in tensors.values() if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"{', '.join(n for n, t in tensors.items() if t is not None)} should be on the same device.")
+    first = None
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                _require_cuda(t)
+            if first is None:
+                first = t.device
+            elif t.device != first:
+                raise ValueError(f"All tensors should be on the same device, got {first} and {t.device}.")
+
+
+@functools.lru_cache(maxsize=4096)
+def _stride_array(strides):
+    """The strides as a C array (made once per layout: the library only reads it)."""
+    return (c_i64 * len(strides))(*strides)
 
 
 def _strides4(t):
-    return (c_i64 * 4)(*t.stride())
+    return _stride_array(t.stride())
 
 
-def _strides3(t):
-    return (c_i64 * 3)(*t.stride())
+_strides3 = _strides4
 
 
 # --------------------------------------------------------------------------- row ops
@@ -264,35 +290,27 @@ def rms_norm_bwd(dx, dweight, dbias, dy, x, weight, rms, workspace, rows, cols, 
     )
 
 
-def gated_residual_rms_norm_fwd(h, y, rms1, rms2, x, r, w1, w2, gate, rows, cols, rows_per_gate, scale, eps):
-    _require_cuda(h, y, x, r, w1, w2, gate)
-    with _on_device(x):
-        _check(
-            load().tb200_gated_residual_rms_norm_fwd(
-                _ptr(h), _ptr(y), _ptr(rms1), _ptr(rms2), _ptr(x), _ptr(r), _ptr(w1), _ptr(w2), _ptr(gate),
-                rows, cols, rows_per_gate, scale, eps, dtype_code(x.dtype), _stream(x),
-            ),
-            "tb200_gated_residual_rms_norm_fwd",
-        )
+def gated_residual_rms_norm_fwd(h, y, rms, x, r, w1, w2, gate, rows, cols, rows_per_gate, scale, eps):
+    """rms: [2, rows], of x and of y."""
+    rms1 = rms.data_ptr()
+    _call(
+        "tb200_gated_residual_rms_norm_fwd", x, _ptr(h), _ptr(y), rms1, rms1 + 4 * rows, _ptr(x), _ptr(r), _ptr(w1),
+        _ptr(w2), _ptr(gate), rows, cols, rows_per_gate, scale, eps, dtype_code(x.dtype),
+    )
 
 
-def gated_residual_rms_norm_bwd_workspace(rows, cols, rows_per_gate):
-    return load().tb200_gated_residual_rms_norm_bwd_workspace(rows, cols, rows_per_gate)
+def gated_residual_rms_norm_bwd_workspace(like, rows, cols, rows_per_gate):
+    return _workspace("tb200_gated_residual_rms_norm_bwd_workspace", like.device.index, rows, cols, rows_per_gate)
 
 
-def gated_residual_rms_norm_bwd(dx, dr, dw1, dw2, dgate, dh, dy, x, r, w1, w2, gate, rms1, rms2, workspace, rows,
-                                cols, rows_per_gate, scale, eps):
-    _require_cuda(dx, dr, dw1, dw2, dgate, dh, dy, x, r, w1, w2, gate)
-    with _on_device(x):
-        _check(
-            load().tb200_gated_residual_rms_norm_bwd(
-                _ptr(dx), _ptr(dr), _ptr(dw1), _ptr(dw2), _ptr(dgate), _ptr(dh), _ptr(dy), _ptr(x), _ptr(r),
-                _ptr(w1), _ptr(w2), _ptr(gate), _ptr(rms1), _ptr(rms2), _ptr(workspace),
-                0 if workspace is None else workspace.numel() * workspace.element_size(),
-                rows, cols, rows_per_gate, scale, eps, dtype_code(x.dtype), _stream(x),
-            ),
-            "tb200_gated_residual_rms_norm_bwd",
-        )
+def gated_residual_rms_norm_bwd(dx, dr, dw1, dw2, dgate, dh, dy, x, r, w1, w2, gate, rms, workspace, rows, cols,
+                                rows_per_gate, scale, eps):
+    rms1 = rms.data_ptr()
+    _call(
+        "tb200_gated_residual_rms_norm_bwd", x, _ptr(dx), _ptr(dr), _ptr(dw1), _ptr(dw2), _ptr(dgate), _ptr(dh),
+        _ptr(dy), _ptr(x), _ptr(r), _ptr(w1), _ptr(w2), _ptr(gate), rms1, rms1 + 4 * rows, _ptr(workspace),
+        0 if workspace is None else workspace.numel(), rows, cols, rows_per_gate, scale, eps, dtype_code(x.dtype),
+    )
 
 
 REDUCE_KINDS = {"sum": 0, "mean": 1, "var": 2, "var_mean": 3}
@@ -501,72 +519,58 @@ def attention_bwd(dq, dk, dv, dmask, dout, q, k, v, out, lse, mask, workspace, i
 
 def window_attention_fwd(out, lse, q, k, v, window, sinks, scale):
     B, H, S, D = q.shape
-    with _on_device(q):
-        _check(
-            load().tb200_window_attention_fwd(
-                _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), B, H, k.shape[1], S, D,
-                _strides4(q), _strides4(k), _strides4(v), _strides4(out), window, sinks, scale,
-                dtype_code(q.dtype), _stream(q),
-            ),
-            "tb200_window_attention_fwd",
-        )
+    _call(
+        "tb200_window_attention_fwd", q, _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), B, H, k.shape[1], S, D,
+        _strides4(q), _strides4(k), _strides4(v), _strides4(out), window, sinks, scale, dtype_code(q.dtype),
+    )
 
 
 def window_attention_bwd_workspace(q, k, window, sinks):
     B, H, S, D = q.shape
-    with _on_device(q):
-        return load().tb200_window_attention_bwd_workspace(B, H, k.shape[1], S, D, window, sinks, dtype_code(q.dtype))
+    return _workspace(
+        "tb200_window_attention_bwd_workspace", q.device.index, B, H, k.shape[1], S, D, window, sinks,
+        dtype_code(q.dtype),
+    )
 
 
 def window_attention_bwd(dq, dk, dv, dout, q, k, v, out, lse, workspace, window, sinks, scale):
     B, H, S, D = q.shape
-    with _on_device(q):
-        _check(
-            load().tb200_window_attention_bwd(
-                _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
-                _ptr(workspace), workspace.numel() * workspace.element_size(), B, H, k.shape[1], S, D,
-                _strides4(q), _strides4(k), _strides4(v), _strides4(out), _strides4(dout), _strides4(dq),
-                _strides4(dk), _strides4(dv), window, sinks, scale, dtype_code(q.dtype), _stream(q),
-            ),
-            "tb200_window_attention_bwd",
-        )
+    _call(
+        "tb200_window_attention_bwd", q, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(q), _ptr(k), _ptr(v),
+        _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel(), B, H, k.shape[1], S, D, _strides4(q), _strides4(k),
+        _strides4(v), _strides4(out), _strides4(dout), _strides4(dq), _strides4(dk), _strides4(dv), window, sinks,
+        scale, dtype_code(q.dtype),
+    )
 
 
 def paged_attention_workspace(q, kv_heads, n, max_query_length, max_context_length, window, sinks):
     T, H, D = q.shape
-    with _on_device(q):
-        return load().tb200_paged_attention_workspace(
-            T, n, H, kv_heads, D, max_query_length, max_context_length, window, sinks, dtype_code(q.dtype)
-        )
+    return _workspace(
+        "tb200_paged_attention_workspace", q.device.index, T, n, H, kv_heads, D, max_query_length,
+        max_context_length, window, sinks, dtype_code(q.dtype),
+    )
 
 
 def paged_attention(out, q, key_cache, value_cache, table, context, starts, workspace, max_query_length,
                     max_context_length, window, sinks, scale, zero_tail):
     T, H, D = q.shape
     pages, page, kv_heads, _ = key_cache.shape
-    with _on_device(q):
-        _check(
-            load().tb200_paged_attention(
-                _ptr(out), _ptr(q), _ptr(key_cache), _ptr(value_cache), _ptr(table), _ptr(context), _ptr(starts),
-                _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-                T, table.shape[0], H, kv_heads, D, page, pages, table.shape[1], table.stride(0),
-                _strides3(q), _strides4(key_cache), _strides4(value_cache), _strides3(out), max_query_length,
-                max_context_length, window, sinks, scale, int(zero_tail), dtype_code(q.dtype), _stream(q),
-            ),
-            "tb200_paged_attention",
-        )
+    n, blocks = table.shape
+    _call(
+        "tb200_paged_attention", q, _ptr(out), _ptr(q), _ptr(key_cache), _ptr(value_cache), _ptr(table),
+        _ptr(context), _ptr(starts), _ptr(workspace), 0 if workspace is None else workspace.numel(), T, n, H,
+        kv_heads, D, page, pages, blocks, table.stride(0), _strides3(q), _strides4(key_cache),
+        _strides4(value_cache), _strides3(out), max_query_length, max_context_length, window, sinks, scale,
+        zero_tail, dtype_code(q.dtype),
+    )
 
 
 def paged_cache_append(key_cache, value_cache, k, v, table, context, starts):
     T, kv_heads, D = k.shape
     pages, page = key_cache.shape[:2]
-    with _on_device(k):
-        _check(
-            load().tb200_paged_cache_append(
-                _ptr(key_cache), _ptr(value_cache), _ptr(k), _ptr(v), _ptr(table), _ptr(context), _ptr(starts),
-                T, table.shape[0], kv_heads, D, page, pages, table.shape[1], table.stride(0),
-                _strides4(key_cache), _strides4(value_cache), _strides3(k), _strides3(v), dtype_code(k.dtype),
-                _stream(k),
-            ),
-            "tb200_paged_cache_append",
-        )
+    n, blocks = table.shape
+    _call(
+        "tb200_paged_cache_append", k, _ptr(key_cache), _ptr(value_cache), _ptr(k), _ptr(v), _ptr(table),
+        _ptr(context), _ptr(starts), T, n, kv_heads, D, page, pages, blocks, table.stride(0), _strides4(key_cache),
+        _strides4(value_cache), _strides3(k), _strides3(v), dtype_code(k.dtype),
+    )

@@ -26,6 +26,7 @@
 // reads x, r, dy, dh and writes dx, dr (6 e).
 #include <type_traits>
 
+#include "ptx.cuh"
 #include "row_common.cuh"
 
 namespace tb200 {
@@ -160,6 +161,296 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// ------------------------------------------------------------------ rows of 16-byte vectors
+// Forward: a row stays in registers (a warp or a CTA owns it, RowPlan); x, r, the weights and the gate
+// are requested together before the first reduction.
+template <typename T, int CHUNKS, bool CTA_ROW>
+__global__ void __launch_bounds__(CTA_ROW ? 512 : 256, CTA_ROW ? 2 : 4)
+    resnorm_fwd_vec(T* __restrict__ h, T* __restrict__ y, float* __restrict__ rms1, float* __restrict__ rms2,
+                    const T* __restrict__ x, const T* __restrict__ r, const T* __restrict__ w1, const T* __restrict__ w2,
+                    const T* __restrict__ gate, const ResNormArgs a) {
+  constexpr int VEC = Traits<T>::VEC, PAIRS = VEC / 2;
+  __shared__ float slot[64];
+  int phase = 0;
+  RowThread<CTA_ROW> rt;
+  const int cols = (int)a.cols;
+  const float inv_n = 1.f / (float)cols;
+  pdl_wait();
+  pdl_release();
+  for (int64_t row = rt.first_row(); row < a.rows; row += rt.row_step()) {
+    const int64_t off = row * a.cols;
+    const T* g = gate ? gate + gate_index(a, row) * a.cols : nullptr;
+    uint4 xr[CHUNKS], rr[CHUNKS];
+    uint64_t v[CHUNKS][PAIRS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = rt.template col<VEC>(c);
+      const bool in = col < cols;
+      xr[c] = in ? ld_stream(x + off + col) : make_uint4(0, 0, 0, 0);
+      rr[c] = in ? ld_stream(r + off + col) : make_uint4(0, 0, 0, 0);
+    }
+    float i1 = 1.f;
+    if (w1) {
+      uint64_t s2 = 0ull;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        unpack2<T>(xr[c], v[c]);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) s2 = am::fma2(v[c][i], v[c][i], s2);
+      }
+      const float rms = sqrtf(row_reduce<CTA_ROW, false>(hsum2(s2), slot, phase) * inv_n);
+      i1 = 1.f / (rms + a.eps);
+      if (rt.tid == 0) rms1[row] = rms;
+    }
+    const uint64_t i1_2 = splat2(i1), scale2 = splat2(a.scale);
+    uint64_t s2 = 0ull;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = rt.template col<VEC>(c);
+      unpack2<T>(xr[c], v[c]);
+      if (col < cols) {
+        uint64_t t[PAIRS];
+        if (w1) {
+          unpack2<T>(ld_cached(w1 + col), t);
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) v[c][i] = am::mul2(am::mul2(v[c][i], i1_2), t[i]);
+        }
+        if (g) {
+          unpack2<T>(ld_cached(g + col), t);
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) v[c][i] = am::mul2(v[c][i], t[i]);
+        }
+        unpack2<T>(rr[c], t);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          v[c][i] = am::fma2(scale2, t[i], v[c][i]);
+          s2 = am::fma2(v[c][i], v[c][i], s2);
+        }
+        st_stream(y + off + col, pack2<T>(v[c]));
+      }
+    }
+    const float rms = sqrtf(row_reduce<CTA_ROW, false>(hsum2(s2), slot, phase) * inv_n);
+    const uint64_t i2_2 = splat2(1.f / (rms + a.eps));
+    if (rt.tid == 0) rms2[row] = rms;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = rt.template col<VEC>(c);
+      if (col < cols) {
+        uint64_t t[PAIRS];
+        unpack2<T>(ld_cached(w2 + col), t);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) v[c][i] = am::mul2(am::mul2(v[c][i], i2_2), t[i]);
+        st_stream(h + off + col, pack2<T>(v[c]));
+      }
+    }
+  }
+}
+
+// Backward: a CTA walks its part of the rows. x, r, dy and dh of a row arrive in a ring of shared-memory
+// stages by bulk copies (one thread issues them stages ahead, so loads stay in flight across the two
+// reductions of a row); a thread takes its vectors into registers, and keeps the column sums of its
+// columns in registers.
+template <typename T, int CHUNKS>
+__global__ void __launch_bounds__(512)
+    resnorm_bwd_vec(T* __restrict__ dx, T* __restrict__ dr, T* __restrict__ dgate_rows, float* __restrict__ part_a,
+                    float* __restrict__ part_b, const T* __restrict__ dh, const T* __restrict__ dy, const T* __restrict__ x,
+                    const T* __restrict__ r, const T* __restrict__ w1, const T* __restrict__ w2, const T* __restrict__ gate,
+                    const float* __restrict__ rms1, const float* __restrict__ rms2, const ResNormArgs a, int per_row,
+                    int stages, int* status) {
+  constexpr int VEC = Traits<T>::VEC, PAIRS = VEC / 2;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float slot[64];
+  __shared__ uint64_t full[4];
+  __shared__ uint32_t abort_words[2];
+  volatile uint32_t* abort_flag = abort_words;
+  const int cols = (int)a.cols;
+  const int bytes = cols * (int)sizeof(T);
+  const int64_t n = gridDim.x, begin = part_begin(blockIdx.x, n, a.rows), end = part_begin(blockIdx.x + 1, n, a.rows);
+  const int count = (int)(end - begin);
+  const float inv_n = 1.f / (float)cols;
+  int phase = 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) ptx::mbar_init(&full[i], 1);
+    abort_flag[0] = 0;
+    abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
+    ptx::fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_release();
+  const int tensors = 2 + (dh ? 1 : 0) + (dy ? 1 : 0);
+  auto request = [&](int i) {  // (thread 0) row begin + i into its stage
+    const int st = i % stages;
+    uint8_t* dst = ring + (size_t)st * 4 * bytes;
+    const int64_t off = (begin + i) * a.cols;
+    ptx::mbar_expect_tx(&full[st], (uint32_t)(tensors * bytes));
+    auto copy = [&](const T* src, int k) {
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       ptx::smem_u32(dst + (size_t)k * bytes)),
+                   "l"(src + off), "r"(bytes), "r"(ptx::smem_u32(&full[st]))
+                   : "memory");
+    };
+    copy(x, 0);
+    copy(r, 1);
+    if (dh) copy(dh, 2);
+    if (dy) copy(dy, 3);
+  };
+  if (threadIdx.x == 0)
+    for (int i = 0; i < stages && i < count; ++i) request(i);
+
+  uint64_t acc_a[CHUNKS][PAIRS], acc_b[CHUNKS][PAIRS];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) acc_a[c][i] = acc_b[c][i] = 0ull;
+  auto col_of = [&](int c) { return (c * (int)blockDim.x + (int)threadIdx.x) * VEC; };
+  auto flush = [&](float* dst, uint64_t (&acc)[CHUNKS][PAIRS]) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = col_of(c);
+      if (col < cols)
+#pragma unroll
+        for (int i = 0; i < PAIRS; i += 2) {
+          float f0, f1, f2, f3;
+          am::unpack2f(acc[c][i], f0, f1);
+          am::unpack2f(acc[c][i + 1], f2, f3);
+          *reinterpret_cast<float4*>(dst + col + i * 2) = make_float4(f0, f1, f2, f3);
+          acc[c][i] = acc[c][i + 1] = 0ull;
+        }
+    }
+  };
+  int64_t current = gate_index(a, begin);
+  for (int i = 0; i < count; ++i) {
+    const int64_t row = begin + i, off = row * a.cols, gi = gate_index(a, row);
+    if (part_a && !per_row && gi != current) {  // the previous rows' stretch of one gate vector ends
+      flush(part_a + ((int64_t)blockIdx.x + current) * a.cols, acc_a);
+      current = gi;
+    }
+    const T* g = gate ? gate + gi * a.cols : nullptr;
+    const float m1 = w1 ? rms1[row] : 1.f, m2 = rms2[row];
+    const float i1 = w1 ? 1.f / (m1 + a.eps) : 1.f, i2 = 1.f / (m2 + a.eps);
+    const uint64_t i1_2 = splat2(i1), i2_2 = splat2(i2), scale2 = splat2(a.scale);
+    const int st = i % stages;
+    const uint8_t* src = ring + (size_t)st * 4 * bytes;
+    ptx::mbar_wait(&full[st], (i / stages) & 1, abort_flag, status, 141);
+    // t = dh w2 (then dY), u = x, v = y
+    uint64_t t[CHUNKS][PAIRS], u[CHUNKS][PAIRS], v[CHUNKS][PAIRS];
+    uint4 dyr[CHUNKS];
+    uint64_t s2 = 0ull;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = col_of(c);
+      if (col < cols) {
+        const uint8_t* at = src + col * (int)sizeof(T);
+        uint64_t w[PAIRS];
+        unpack2<T>(*reinterpret_cast<const uint4*>(at), u[c]);
+        unpack2<T>(*reinterpret_cast<const uint4*>(at + bytes), v[c]);
+        dyr[c] = dy ? *reinterpret_cast<const uint4*>(at + 3 * (size_t)bytes) : make_uint4(0, 0, 0, 0);
+        uint64_t b[PAIRS];  // the branch n * gate
+        if (w1) {
+          unpack2<T>(ld_cached(w1 + col), w);
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) b[k] = am::mul2(am::mul2(u[c][k], i1_2), w[k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) b[k] = u[c][k];
+        }
+        if (g) {
+          unpack2<T>(ld_cached(g + col), w);
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) b[k] = am::mul2(b[k], w[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) v[c][k] = am::fma2(scale2, v[c][k], b[k]);
+        if (dh) {
+          unpack2<T>(*reinterpret_cast<const uint4*>(at + 2 * (size_t)bytes), t[c]);
+          unpack2<T>(ld_cached(w2 + col), w);
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) {
+            acc_b[c][k] = am::fma2(t[c][k], am::mul2(v[c][k], i2_2), acc_b[c][k]);
+            t[c][k] = am::mul2(t[c][k], w[k]);
+            s2 = am::fma2(t[c][k], v[c][k], s2);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) t[c][k] = 0ull;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) t[c][k] = u[c][k] = v[c][k] = 0ull;
+        dyr[c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    // (the reduction's barrier also says that every thread has taken its part of the stage)
+    ptx::fence_proxy_async_smem();
+    const float sum2 = row_reduce<true, false>(hsum2(s2), slot, phase);
+    if (threadIdx.x == 0 && i + stages < count) request(i + stages);
+    const float k2 = m2 > 0.f ? sum2 * i2 * i2 * inv_n / m2 : 0.f;
+    const uint64_t nk2 = splat2(-k2);
+    uint64_t s1 = 0ull;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = col_of(c);
+      if (col < cols) {
+        uint64_t w[PAIRS];
+        unpack2<T>(dyr[c], w);
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+          // dY = dy + dh w2 i2 - y k2
+          t[c][k] = am::fma2(t[c][k], i2_2, am::fma2(v[c][k], nk2, w[k]));
+          v[c][k] = am::mul2(scale2, t[c][k]);
+        }
+        st_stream(dr + off + col, pack2<T>(v[c]));
+        // column sum A: dY x i1 (times a gate of its own per row); v = dY g w1
+        uint64_t ax[PAIRS];
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) ax[k] = am::mul2(t[c][k], am::mul2(u[c][k], i1_2));
+        if (dgate_rows) {
+          uint64_t dg[PAIRS];
+          if (w1) unpack2<T>(ld_cached(w1 + col), w);
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) dg[k] = w1 ? am::mul2(ax[k], w[k]) : ax[k];
+          st_stream(dgate_rows + off + col, pack2<T>(dg));
+        }
+        if (g) {
+          unpack2<T>(ld_cached(g + col), w);
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) {
+            t[c][k] = am::mul2(t[c][k], w[k]);
+            if (per_row) ax[k] = am::mul2(ax[k], w[k]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) acc_a[c][k] = am::add2(acc_a[c][k], ax[k]);
+        if (w1) {
+          unpack2<T>(ld_cached(w1 + col), w);
+#pragma unroll
+          for (int k = 0; k < PAIRS; ++k) {
+            t[c][k] = am::mul2(t[c][k], w[k]);
+            s1 = am::fma2(t[c][k], u[c][k], s1);
+          }
+        }
+      }
+    }
+    uint64_t nk1 = 0ull;
+    if (w1) {
+      const float sum1 = row_reduce<true, false>(hsum2(s1), slot, phase);
+      nk1 = splat2(m1 > 0.f ? -(sum1 * i1 * i1 * inv_n / m1) : 0.f);
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = col_of(c);
+      if (col < cols) {
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) t[c][k] = am::fma2(u[c][k], nk1, am::mul2(t[c][k], i1_2));
+        st_stream(dx + off + col, pack2<T>(t[c]));
+      }
+    }
+  }
+  if (part_a) flush(part_a + ((int64_t)blockIdx.x + (per_row ? 0 : current)) * a.cols, acc_a);
+  if (part_b) flush(part_b + (int64_t)blockIdx.x * a.cols, acc_b);
+}
+
 // blockIdx.y 0: dw1 (and dgate where one vector serves all rows), 1: dw2, 2..: dgate of one vector each.
 // Block (32, 32): threadIdx.x walks columns, threadIdx.y splits the partial rows.
 template <typename T>
@@ -249,6 +540,27 @@ int64_t backward_parts(int64_t rows, int64_t per_sm) {
 }
 constexpr int64_t MAX_PARTS_PER_SM = 16;
 
+// Shape of the vector kernel of the backward pass (chunks 0: the generic one). Up to three rows of
+// the four tensors are in flight per CTA; CTAs per SM by shared memory and 1024 threads.
+struct BackwardPlan {
+  int chunks = 0, threads = 0, stages = 0, per_sm = 0;
+};
+constexpr int RING_BYTES = 200 * 1024;
+template <typename T>
+BackwardPlan plan_backward(int64_t cols, bool ptrs_ok) {
+  BackwardPlan p;
+  constexpr int VEC = Traits<T>::VEC;
+  if (!ptrs_ok || cols % VEC != 0 || cols > 2048 * VEC) return p;
+  const int64_t vecs = cols / VEC, stage = 4 * cols * (int64_t)sizeof(T);
+  p.chunks = vecs <= 512 ? 1 : (vecs <= 1024 ? 2 : 4);
+  p.threads = (int)(ceil_div(ceil_div(vecs, p.chunks), 32) * 32);
+  p.stages = (int)(RING_BYTES / stage < 3 ? RING_BYTES / stage : 3);
+  int64_t per_sm = 220 * 1024 / (p.stages * stage + 2048);
+  if (per_sm > 1024 / p.threads) per_sm = 1024 / p.threads;
+  p.per_sm = (int)(per_sm < 1 ? 1 : (per_sm > MAX_PARTS_PER_SM ? MAX_PARTS_PER_SM : per_sm));
+  return p;
+}
+
 int check(const char* who, const ResNormArgs& a, const void* gate) {
   TB200_REQUIRE(a.rows >= 0 && a.cols > 0, TB200_ERR_INVALID, "%s: bad shape", who);
   TB200_REQUIRE(a.rows < (1ll << 31) && a.cols < (1ll << 30), TB200_ERR_UNSUPPORTED, "%s: more than 2^31 rows or 2^30 columns", who);
@@ -276,6 +588,19 @@ extern "C" int tb200_gated_residual_rms_norm_fwd(void* h, void* y, float* rms1, 
   cudaStream_t st = (cudaStream_t)stream;
   return dispatch_dtype(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
+    const bool ok = aligned16(h) && aligned16(y) && aligned16(x) && aligned16(r) && aligned16(w2) && (!w1 || aligned16(w1)) &&
+                    (!gate || aligned16(gate));
+    const RowPlan plan = plan_rows<T>(cols, ok);
+    if (plan.vec) {
+      const int rc = dispatch_plan<T>(plan, [&](auto c, auto cta) -> int {
+        (void)launch_pdl(resnorm_fwd_vec<T, decltype(c)::value, decltype(cta)::value>,
+                         dim3((unsigned)ceil_div(rows, plan.rows_per_cta)), dim3(plan.threads), 0, st, false, (T*)h, (T*)y, rms1,
+                         rms2, (const T*)x, (const T*)r, (const T*)w1, (const T*)w2, (const T*)gate, a);
+        return launch_status("resnorm_fwd_vec");
+      });
+      if (rc == 0) note_kernel("row_vec", 1);
+      return rc;
+    }
     resnorm_fwd_generic<T><<<(unsigned)rows, 256, 0, st>>>((T*)h, (T*)y, rms1, rms2, (const T*)x, (const T*)r,
                                                            (const T*)w1, (const T*)w2, (const T*)gate, a);
     const int rc = launch_status("resnorm_fwd_generic");
@@ -320,25 +645,49 @@ extern "C" int tb200_gated_residual_rms_norm_bwd(void* dx, void* dr, void* dw1, 
   return dispatch_dtype(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     const int64_t vectors = a.rows_per_gate > 1 ? rows / a.rows_per_gate : 1;
-    const int64_t n = backward_parts(rows, 4);
+    const bool ok = aligned16(dx) && aligned16(dr) && aligned16(x) && aligned16(r) && aligned16(w2) && (!dh || aligned16(dh)) &&
+                    (!dy || aligned16(dy)) && (!w1 || aligned16(w1)) && (!gate || aligned16(gate)) && (!dgate || aligned16(dgate)) &&
+                    (!workspace || aligned16(workspace));
+    const BackwardPlan plan = plan_backward<T>(cols, ok);
+    const int64_t n = backward_parts(rows, plan.chunks ? plan.per_sm : 4);
     float* part_a = want_a ? (float*)workspace : nullptr;
     float* part_b = want_b ? (float*)workspace + (n + vectors) * cols : nullptr;
-    resnorm_bwd_generic<T><<<(unsigned)n, 256, 0, st>>>(
-        (T*)dx, (T*)dr, per_row ? (T*)dgate : nullptr, part_a, part_b, (const T*)dh, (const T*)dy, (const T*)x, (const T*)r,
-        (const T*)w1, (const T*)w2, (const T*)gate, rms1, rms2, a, per_row ? 1 : 0);
-    int rc = launch_status("resnorm_bwd_generic");
+    int rc = 0;
+    if (plan.chunks) {
+      auto go = [&](auto c) -> int {
+        auto kern = resnorm_bwd_vec<T, decltype(c)::value>;
+        static std::atomic<unsigned long long> done{0};
+        const cudaError_t e = smem_optin_per_device(done, reinterpret_cast<const void*>(kern), RING_BYTES);
+        if (e != cudaSuccess) {
+          set_error("gated_residual_rms_norm_bwd: cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
+          return (int)e;
+        }
+        (void)launch_pdl(kern, dim3((unsigned)n), dim3(plan.threads), (size_t)plan.stages * 4 * cols * sizeof(T), st, false,
+                         (T*)dx, (T*)dr, per_row ? (T*)dgate : nullptr, part_a, part_b, (const T*)dh, (const T*)dy, (const T*)x,
+                         (const T*)r, (const T*)w1, (const T*)w2, (const T*)gate, rms1, rms2, a, per_row ? 1 : 0, plan.stages,
+                         device_status_ptr());
+        return launch_status("resnorm_bwd_vec");
+      };
+      rc = plan.chunks == 1 ? go(IntC<1>{}) : plan.chunks == 2 ? go(IntC<2>{}) : go(IntC<4>{});
+    } else {
+      resnorm_bwd_generic<T><<<(unsigned)n, 256, 0, st>>>(
+          (T*)dx, (T*)dr, per_row ? (T*)dgate : nullptr, part_a, part_b, (const T*)dh, (const T*)dy, (const T*)x, (const T*)r,
+          (const T*)w1, (const T*)w2, (const T*)gate, rms1, rms2, a, per_row ? 1 : 0);
+      rc = launch_status("resnorm_bwd_generic");
+    }
     if (rc) return rc;
     int launches = 1;
     if (want_a || want_b) {
       const bool groups = dgate && !per_row && a.rows_per_gate > 0;
       const int64_t gy = groups ? 2 + (vectors < 4096 ? vectors : 4096) : 2;
-      resnorm_finalize<T><<<dim3((unsigned)ceil_div(cols, 32), (unsigned)gy), dim3(32, 32), 0, st>>>(
-          (T*)dw1, (T*)dw2, per_row ? nullptr : (T*)dgate, part_a, part_b, (const T*)w1, (const T*)gate, n, a, per_row ? 1 : 0);
+      (void)launch_pdl(resnorm_finalize<T>, dim3((unsigned)ceil_div(cols, 32), (unsigned)gy), dim3(32, 32), 0, st, false, (T*)dw1,
+                       (T*)dw2, per_row ? (T*)nullptr : (T*)dgate, part_a, part_b, (const T*)w1, (const T*)gate, n, a,
+                       per_row ? 1 : 0);
       rc = launch_status("resnorm_finalize");
       if (rc) return rc;
       ++launches;
     }
-    note_kernel("row_generic", launches);
+    note_kernel(plan.chunks ? "row_vec" : "row_generic", launches);
     return 0;
   });
 }

@@ -55,9 +55,7 @@ class GatedResidualRMSNorm(torch.autograd.Function):
             if tensor is not None and tensor.dtype != input.dtype:
                 raise ValueError("input, residual, weights and gate should have the same dtype.")
         _lib.dtype_code(input.dtype)
-        _lib.require_one_device(
-            input=input, residual=residual, post_weight=post_weight, pre_weight=pre_weight, gate=gate
-        )
+        _lib.require_one_device(input, residual, post_weight, pre_weight, gate)
 
         util.push_trace("GatedResidualRMSNorm.__forward")
         input, residual, post_weight, pre_weight, gate = (
@@ -71,8 +69,7 @@ class GatedResidualRMSNorm(torch.autograd.Function):
         _lib.gated_residual_rms_norm_fwd(
             output,
             output_residual,
-            rms[0],
-            rms[1],
+            rms,
             input,
             residual,
             post_weight,
@@ -137,7 +134,7 @@ class GatedResidualRMSNorm(torch.autograd.Function):
         workspace = None
         if any(t is not None for t in (grad_post_weight, grad_pre_weight, grad_gate)):
             workspace = torch.empty(
-                max(_lib.gated_residual_rms_norm_bwd_workspace(y_size, x_size, group), 16),
+                max(_lib.gated_residual_rms_norm_bwd_workspace(input, y_size, x_size, group), 16),
                 dtype=torch.uint8,
                 device=input.device,
             )
@@ -156,8 +153,7 @@ class GatedResidualRMSNorm(torch.autograd.Function):
             post_weight,
             pre_weight,
             gate,
-            rms[0],
-            rms[1],
+            rms,
             workspace,
             y_size,
             x_size,

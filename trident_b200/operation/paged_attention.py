@@ -23,17 +23,21 @@ def _check_cache(key_cache, value_cache, block_table, context_lengths, query_off
             raise ValueError("Without query_offsets there should be one new token per sequence.")
     elif query_offsets.dim() != 1 or query_offsets.shape[0] != block_table.shape[0] + 1:
         raise ValueError("query_offsets should be [sequences + 1].")
-    for name, tensor in (
-        ("block_table", block_table),
-        ("context_lengths", context_lengths),
-        ("query_offsets", query_offsets),
-    ):
+    for tensor in (block_table, context_lengths, query_offsets):
         if tensor is not None and tensor.dtype != torch.int32:
-            raise ValueError(f"{name} should have the dtype torch.int32.")
-    if any(t.dtype != key_cache.dtype for t in (value_cache, *tensors.values())):
+            raise ValueError(
+                "block_table, context_lengths and query_offsets should have the dtype torch.int32."
+            )
+    grad = key_cache.requires_grad or value_cache.requires_grad
+    dtype = key_cache.dtype
+    same = value_cache.dtype == dtype
+    for tensor in tensors.values():
+        same = same and tensor.dtype == dtype
+        grad = grad or tensor.requires_grad
+    if not same:
         raise ValueError(f"{', '.join(tensors)}, key_cache and value_cache should have the same dtype.")
-    _lib.dtype_code(key_cache.dtype)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (key_cache, value_cache, *tensors.values())):
+    _lib.dtype_code(dtype)
+    if grad and torch.is_grad_enabled():
         raise ValueError("Paged attention has no backward pass: call it under torch.no_grad().")
 
 
@@ -83,8 +87,7 @@ def paged_attention(
     elif max_context_length < 0:
         raise ValueError("max_context_length should not be negative.")
     _lib.require_one_device(
-        key_cache=key_cache, value_cache=value_cache, block_table=block_table, context_lengths=context_lengths,
-        query_offsets=query_offsets, **tensors,
+        key_cache, value_cache, block_table, context_lengths, query_offsets, *tensors.values()
     )
     max_query_length = max(1, min(max_query_length, tokens, MOST_TOKENS))
     max_context_length = min(max_context_length, MOST_TOKENS)
@@ -134,8 +137,7 @@ def paged_cache_append(key, value, key_cache, value_cache, block_table, context_
         raise ValueError("key and key_cache should have the same heads and head size.")
     check_heads(key.shape[1], key.shape[1], key.shape[2])
     _lib.require_one_device(
-        key_cache=key_cache, value_cache=value_cache, block_table=block_table, context_lengths=context_lengths,
-        query_offsets=query_offsets, **tensors,
+        key_cache, value_cache, block_table, context_lengths, query_offsets, *tensors.values()
     )
     if key.shape[0] == 0 or block_table.shape[0] == 0:
         return

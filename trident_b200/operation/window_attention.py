@@ -46,7 +46,7 @@ class WindowAttention(torch.autograd.Function):
         if query.dtype != key.dtype or query.dtype != value.dtype:
             raise ValueError("query, key and value should have the same dtype.")
         _lib.dtype_code(query.dtype)
-        _lib.require_one_device(query=query, key=key, value=value)
+        _lib.require_one_device(query, key, value)
         # beyond the length of the sequence both mean the same (and any integer fits the library's types)
         window_size, num_sinks = min(window_size, max(y_size, 1)), min(num_sinks, y_size)
 
