@@ -85,7 +85,7 @@ void plan_far(LocalBwdArgs* b, int key_tile) {
 size_t far_bytes(const LocalBwdArgs& b, int key_tile) {
   return (size_t)b.f.n * b.f.KV * b.sink_tiles * (b.far + 1) * 2 * key_tile * b.f.D * sizeof(float);
 }
-// delta of each score row (CUDA cores), or -lse and -delta by query tile (tensor cores)
+// delta of each score row (CUDA cores), or -lse and -delta by column tile (tensor cores)
 size_t row_bytes(const LocalArgs& a, bool tc) {
   const int64_t floats = tc ? 2 * local_tc_rows(a) : (int64_t)a.n * a.H * a.tokens;
   return ((size_t)floats * sizeof(float) + 255) & ~(size_t)255;
@@ -220,7 +220,7 @@ extern "C" int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const vo
     if (int rc = launch_local_delta(row_scratch, out, dout, b.dos, b.f, dtype, st)) return rc;
     if (int rc = launch_local_bwd_simt(dq, dk, dv, dout, q, k, v, lse, row_scratch, b, dtype, st)) return rc;
   }
-  int launches = 3;
+  int launches = tc ? 2 : 3;
   if (b.sink_tiles > 0) {
     if (int rc = launch_local_far_sum(dk, dv, b, key_tile, dtype, st)) return rc;
     ++launches;

@@ -4,24 +4,27 @@
 // give the same bits (one kernel for all three gradients would need 5 products a tile pair instead of 7,
 // but has to add dQ across CTAs):
 //
-//   dK, dV  a CTA owns 128 keys (K_j, V_j resident) and walks the tiles of 128 packed query rows (token *
-//           G + head) that see any of them; the sum over the heads of a group is part of the walk. All
+//   dQ      tiles of 128 packed query rows (token * G + head); a persistent CTA takes every gridDim-th of
+//           them. Q and dO of the tile are put into tensor memory as operands (their products then read only
+//           K or V from shared memory: with both operands there, the four 4 KB reads of an instruction pair
+//           took the pipe 120 cycles an instruction instead of 64); along the keys of the tile's walk
+//             S = Q K^T, dP = dO V^T, P = exp2(S scale log2e - lse log2e), dS = P (dP - delta), dQ += dS K
+//           (dS 16-bit in tensor memory over dP). S(i+1) is computed as soon as S(i) is in registers, dP(i+1)
+//           after dQ(i), so that exponentials and score gradients follow each other without a pause. The
+//           threads that load dO also compute delta = sum_d out dout, for themselves and for the other kernel.
+//   dK, dV  a CTA owns 128 keys (K_j, V_j resident in shared memory) and walks the tiles of 96 packed query
+//           rows that see any of them; the sum over the heads of a group is part of the walk. All
 //           transposed, keys on the tensor-memory lanes:
-//             S^T = K_j Q^T, dP^T = V_j dO^T, P^T = exp2(S^T scale log2e - lse log2e), dS^T = P^T (dP^T - delta),
-//             dV += P^T dO, dK += dS^T Q   (P^T, dS^T 16-bit in tensor memory over S^T and dP^T)
-//           The tensor pipe runs dP^T(s) | dV(s) | S^T(s+1) | dK(s): while the compute warps are in one
-//           of their two stages (exponentials; score gradients) it has the other's products to run.
-//   dQ      a CTA owns a tile of 128 packed query rows (Q, dO resident) and walks the keys it sees:
-//             S = Q K^T (two buffers), dP = dO V^T, dS = P (dP - delta) over S, dQ += dS K
+//             S^T = K_j Q^T, dP^T = V_j dO^T, dV += P^T dO, dK += dS^T Q
+//           96 rows because dV, dK, S^T, dP^T and a P^T of its own then fit into the 512 columns: with P^T
+//           over S^T (128 rows) the chain exponentials -> dV -> S^T -> exponentials bounded a step at 4100
+//           cycles.
 //
 // The queries beyond the window of a key tile that holds sinks ("far", LocalBwdArgs) are cut into pieces
 // about as long as a walk inside the window, each a CTA of its own: a single CTA would walk all queries.
 //
-// A first kernel computes -delta = -sum_d out dout and -lse log2e, laid out by query tile; rows that do
-// not exist get -lse = -inf, so that their probabilities are 0.
-//
-// Bound by the tensor pipe and, next to it, the exponentials: at D = 128 the four products of a step of
-// the first kernel take 2048 cycles, the three of the second 1536, the 16 K exponentials of either 1024.
+// Bound by the compute warps' exponentials and score gradients (the 16 K exponentials of a 128 x 128 tile
+// pair take 1024 cycles), next to them shared-memory reads of the operands and the tensor pipe.
 #include <type_traits>
 
 #include "attn_math.cuh"
@@ -32,17 +35,22 @@ namespace tb200 {
 namespace {
 
 constexpr int TILE = LOCAL_TC_TILE;
+constexpr int COLS = LOCAL_TC_COLS;  // packed query rows of a step of the dK, dV kernel
 constexpr int THREADS = 384;  // 4 service warps, 8 compute warps: two threads per row, 64 columns each
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct BwdParams {
   LocalBwdArgs b;
-  void *dq, *dk, *dv;
-  const float* nlse2;   // [n * KV][query tiles][128]  -lse * log2(e)
-  const float* ndelta;  // [n * KV][query tiles][128]
+  void *dk, *dv;
+  const void *q, *out, *dout;
+  const float* lse;
+  float* nlse2;         // [n * KV][column tiles][96]  -lse * log2(e), written by the dQ kernel for the other
+  float* ndelta;        // [n * KV][column tiles][96]  -delta
   float scale_log2;
-  int tile_tokens;      // tokens of a query tile
-  int query_tiles, key_tiles;
+  int tile_tokens;      // tokens of a row tile (dQ)
+  int row_tiles;
+  int col_tokens;       // tokens of a column tile (dK, dV)
+  int col_tiles, key_tiles;
   int* status;
 };
 
@@ -64,18 +72,14 @@ __device__ inline void bulk_load(void* dst, const void* src, uint32_t bytes, uin
                "l"(src), "r"(bytes), "r"(ptx::smem_u32(bar))
                : "memory");
 }
-__device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+// the lowest n bits
+__device__ inline uint64_t low_bits64(int n) { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull); }
 __device__ inline int saturate(int64_t v) { return v < -(1 << 20) ? -(1 << 20) : (v > (1 << 20) ? (1 << 20) : (int)v); }
-// Column of the packed 16-bit copy of the 32 columns `c` of a score row: each compute thread packs into
-// the 64 columns it has read itself.
-__host__ __device__ constexpr uint32_t packed_col(int c) { return static_cast<uint32_t>((c >> 1) * 64 + (c & 1) * 16); }
-
-// Rows [rows, 128) of `tiles` swizzled tiles set to zero (rows that no copy writes, but products read).
-template <int NBOX>
-__device__ inline void zero_rows(uint8_t* smem, int tiles, int rows) {
-  const int per_box = (TILE - rows) * 8;  // 16-byte chunks
-  for (int i = threadIdx.x; i < tiles * NBOX * per_box; i += THREADS)
-    *reinterpret_cast<uint4*>(smem + (i / per_box) * (TILE * 128) + rows * 128 + (i % per_box) * 16) = make_uint4(0, 0, 0, 0);
+// Rows [rows, 96) of `boxes` swizzled boxes set to zero (rows that no copy writes, but products read).
+__device__ inline void zero_rows(uint8_t* smem, int boxes, int rows) {
+  const int per_box = (COLS - rows) * 8;  // 16-byte chunks
+  for (int i = threadIdx.x; i < boxes * per_box; i += THREADS)
+    *reinterpret_cast<uint4*>(smem + (i / per_box) * (COLS * 128) + rows * 128 + (i % per_box) * 16) = make_uint4(0, 0, 0, 0);
 }
 
 // ------------------------------------------------------------------ dK, dV
@@ -84,56 +88,63 @@ __global__ void __launch_bounds__(THREADS, 1)
     local_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                         const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const BwdParams p) {
-  constexpr int TILE_BYTES = TILE * D * 2, NBOX = D / 64, BOX_BYTES = TILE * 128;
+  constexpr int STAGES = 3;
+  constexpr int KEY_BYTES = TILE * D * 2, COL_BYTES = COLS * D * 2, NBOX = D / 64;
+  constexpr int KEY_BOX = TILE * 128, COL_BOX = COLS * 128;
+  constexpr int HALF = COLS / 2;  // columns of a compute thread
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr uint32_t IDESC_S = ptx::make_idesc(IS_BF16, false, false, TILE, TILE);
+  constexpr uint32_t IDESC_S = ptx::make_idesc(IS_BF16, false, false, TILE, COLS);
   constexpr uint32_t IDESC_D = ptx::make_idesc(IS_BF16, false, true, TILE, D);
-  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_P = 128, COL_DV = 256, COL_DK = 256 + D;
+  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = COLS, COL_P = 2 * COLS, COL_DV = 256, COL_DK = 256 + D;
+  static_assert(COL_P + COLS / 2 <= COL_DV, "tensor memory");
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* k_smem = smem;
-  uint8_t* v_smem = smem + TILE_BYTES;
-  uint8_t* q_smem = smem + 2 * TILE_BYTES;   // [2]
-  uint8_t* do_smem = smem + 4 * TILE_BYTES;  // [2]
-  float* nlse_smem = reinterpret_cast<float*>(smem + 6 * TILE_BYTES);  // [2][128]
-  float* ndelta_smem = nlse_smem + 256;                                // [2][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ndelta_smem + 256);
+  uint8_t* v_smem = smem + KEY_BYTES;
+  uint8_t* q_smem = smem + 2 * KEY_BYTES;           // [STAGES]
+  uint8_t* do_smem = q_smem + STAGES * COL_BYTES;   // [STAGES]
+  float* nlse_smem = reinterpret_cast<float*>(do_smem + STAGES * COL_BYTES);  // [STAGES][96]
+  float* ndelta_smem = nlse_smem + STAGES * COLS;                             // [STAGES][96]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ndelta_smem + STAGES * COLS);
   uint64_t* kv_full = bars;
-  uint64_t* qdo_full = bars + 1;   // [2]
-  uint64_t* qdo_empty = bars + 3;  // [2]
-  uint64_t* s_ready = bars + 5;    // S^T(s) computed
-  uint64_t* p_ready = bars + 6;    // P^T(s) written      (256 arrivals)
-  uint64_t* dp_ready = bars + 7;   // dP^T(s) computed
-  uint64_t* ds_ready = bars + 8;   // dS^T(s) written     (256 arrivals)
-  uint64_t* all_done = bars + 9;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 10);
+  uint64_t* qdo_full = bars + 1;             // [STAGES]
+  uint64_t* qdo_empty = bars + 1 + STAGES;   // [STAGES]
+  uint64_t* s_ready = bars + 1 + 2 * STAGES; // S^T(i) computed
+  uint64_t* dp_ready = s_ready + 1;          // dP^T(i) computed
+  uint64_t* dv_done = s_ready + 2;           // dV(i) has read P^T(i)
+  uint64_t* all_done = s_ready + 3;
+  uint64_t* s_free = s_ready + 4;            // S^T(i) read          (256 arrivals)
+  uint64_t* p_ready = s_ready + 5;           // P^T(i) written       (256 arrivals)
+  uint64_t* ds_ready = s_ready + 6;          // dS^T(i) over dP^T(i) (256 arrivals)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_ready + 7);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const LocalArgs& a = p.b.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int s = blockIdx.z, hk = blockIdx.y;
-  // the walk: query tiles [i0, i0 + steps)
+  // the walk: column tiles [i0, i0 + steps)
   int jt = blockIdx.x, piece = -1, i0, i1;
   const bool far = jt >= p.key_tiles;
   if (far) {
     piece = (jt - p.key_tiles) % p.b.far;
     jt = (jt - p.key_tiles) / p.b.far;
   }
-  const int beyond = (near_end(a, jt, TILE) + p.tile_tokens - 1) / p.tile_tokens;  // first query tile beyond the window
+  const int beyond = (near_end(a, jt, TILE) + p.col_tokens - 1) / p.col_tokens;  // first column tile beyond the window
   if (far) {
-    const int64_t span = p.query_tiles - beyond;
+    const int64_t span = p.col_tiles - beyond;
     i0 = beyond + (int)(span * piece / p.b.far);
     i1 = beyond + (int)(span * (piece + 1) / p.b.far);
   } else {
-    i0 = jt * TILE / p.tile_tokens;
+    i0 = jt * TILE / p.col_tokens;
     i1 = beyond;
   }
   const int steps = i1 - i0;
-  const int rows = p.tile_tokens * a.G;
+  const int rows = p.col_tokens * a.G;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 10; ++i) ptx::mbar_init(&bars[i], (i == 6 || i == 8) ? 256 : 1);
+    for (int i = 0; i < 1 + 2 * STAGES + 4; ++i) ptx::mbar_init(&bars[i], 1);
+    for (int i = 0; i < 3; ++i) ptx::mbar_init(s_free + i, 256);
     abort_flag[0] = 0;
     abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
     ptx::fence_barrier_init();
@@ -146,8 +157,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     ptx::tmem_alloc(tmem_slot, TMEM_COLS);
     ptx::tmem_relinquish();
   }
-  if (rows < TILE) {
-    zero_rows<NBOX>(q_smem, 4, rows);
+  if (rows < COLS) {
+    zero_rows(q_smem, 2 * STAGES * NBOX, rows);
     ptx::fence_proxy_async_smem();
   }
   ptx::tc_fence_before();
@@ -157,35 +168,37 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0 && steps > 0) {
-      ptx::mbar_expect_tx(kv_full, 2 * TILE_BYTES);
+      ptx::mbar_expect_tx(kv_full, 2 * KEY_BYTES);
 #pragma unroll
       for (int c = 0; c < NBOX; ++c) {
-        tma_load_4d(k_smem + c * BOX_BYTES, &map_k, kv_full, c * 64, jt * TILE, hk, s);
-        tma_load_4d(v_smem + c * BOX_BYTES, &map_v, kv_full, c * 64, jt * TILE, hk, s);
+        tma_load_4d(k_smem + c * KEY_BOX, &map_k, kv_full, c * 64, jt * TILE, hk, s);
+        tma_load_4d(v_smem + c * KEY_BOX, &map_v, kv_full, c * 64, jt * TILE, hk, s);
       }
       for (int i = 0; i < steps; ++i) {
-        const int st = i & 1, it = i0 + i;
-        ptx::mbar_wait(&qdo_empty[st], ((i >> 1) & 1) ^ 1, abort_flag, p.status, 101);
-        ptx::mbar_expect_tx(&qdo_full[st], 2 * NBOX * rows * 128 + 2 * 512);
+        const int st = i % STAGES, it = i0 + i;
+        ptx::mbar_wait(&qdo_empty[st], ((i / STAGES) & 1) ^ 1, abort_flag, p.status, 101);
+        ptx::mbar_expect_tx(&qdo_full[st], 2 * NBOX * rows * 128 + 2 * COLS * 4);
 #pragma unroll
         for (int c = 0; c < NBOX; ++c) {
-          tma_load_5d(q_smem + st * TILE_BYTES + c * BOX_BYTES, &map_q, &qdo_full[st], c * 64, 0, it * p.tile_tokens, hk, s);
-          tma_load_5d(do_smem + st * TILE_BYTES + c * BOX_BYTES, &map_do, &qdo_full[st], c * 64, 0, it * p.tile_tokens, hk, s);
+          tma_load_5d(q_smem + st * COL_BYTES + c * COL_BOX, &map_q, &qdo_full[st], c * 64, 0, it * p.col_tokens, hk, s);
+          tma_load_5d(do_smem + st * COL_BYTES + c * COL_BOX, &map_do, &qdo_full[st], c * 64, 0, it * p.col_tokens, hk, s);
         }
-        const int64_t row0 = (((int64_t)s * a.KV + hk) * p.query_tiles + it) * TILE;
-        bulk_load(nlse_smem + st * 128, p.nlse2 + row0, 512, &qdo_full[st]);
-        bulk_load(ndelta_smem + st * 128, p.ndelta + row0, 512, &qdo_full[st]);
+        const int64_t row0 = (((int64_t)s * a.KV + hk) * p.col_tiles + it) * COLS;
+        bulk_load(nlse_smem + st * COLS, p.nlse2 + row0, COLS * 4, &qdo_full[st]);
+        bulk_load(ndelta_smem + st * COLS, p.ndelta + row0, COLS * 4, &qdo_full[st]);
       }
       // every copy has landed before the CTA gives up its shared memory
       ptx::mbar_wait_drain(kv_full, 0, abort_flag, p.status, 102);
-      for (int i = steps > 2 ? steps - 2 : 0; i < steps; ++i)
-        ptx::mbar_wait_drain(&qdo_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 102);
+      for (int i = steps > STAGES ? steps - STAGES : 0; i < steps; ++i)
+        ptx::mbar_wait_drain(&qdo_full[i % STAGES], (i / STAGES) & 1, abort_flag, p.status, 102);
     }
     __syncwarp();
   } else if (warp == 1) {
+    // The whole warp walks the loop and waits; one elected lane issues. (With the waits in the elected lane
+    // alone, a commit was seen to take effect only after that lane's next wait had given up.)
     const bool elected = ptx::elect_one();
     auto wait_ = [&](uint64_t* bar, uint32_t parity, int code) {
-      if (elected) ptx::mbar_wait(bar, parity, abort_flag, p.status, code);
+      ptx::mbar_wait(bar, parity, abort_flag, p.status, code);
       __syncwarp();
     };
     auto commit_ = [&](uint64_t* bar) {
@@ -193,22 +206,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     const uint64_t dk = ptx::make_smem_desc(ptx::smem_u32(k_smem), 16, 1024), dv = ptx::make_smem_desc(ptx::smem_u32(v_smem), 16, 1024);
     const uint64_t dq = ptx::make_smem_desc(ptx::smem_u32(q_smem), 16, 1024), dd = ptx::make_smem_desc(ptx::smem_u32(do_smem), 16, 1024);
-    const uint64_t dq_t = ptx::make_smem_desc(ptx::smem_u32(q_smem), BOX_BYTES, 1024);   // read along the rows
-    const uint64_t dd_t = ptx::make_smem_desc(ptx::smem_u32(do_smem), BOX_BYTES, 1024);
-    constexpr uint64_t NEXT = static_cast<uint64_t>(TILE_BYTES >> 4);
+    const uint64_t dq_t = ptx::make_smem_desc(ptx::smem_u32(q_smem), COL_BOX, 1024);  // read along the rows
+    const uint64_t dd_t = ptx::make_smem_desc(ptx::smem_u32(do_smem), COL_BOX, 1024);
+    constexpr uint64_t STAGE = static_cast<uint64_t>(COL_BYTES >> 4);
     auto score = [&](uint32_t col, uint64_t ad, uint64_t bd) {  // [keys][rows] = A B^T over the features
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        const uint64_t off = static_cast<uint64_t>(((ks >> 2) * BOX_BYTES + (ks & 3) * 32) >> 4);
-        if (elected) ptx::umma_ss(tmem_base + col, ad + off, bd + off, IDESC_S, ks != 0);
+        const uint64_t oa = static_cast<uint64_t>(((ks >> 2) * KEY_BOX + (ks & 3) * 32) >> 4);
+        const uint64_t ob = static_cast<uint64_t>(((ks >> 2) * COL_BOX + (ks & 3) * 32) >> 4);
+        if (elected) ptx::umma_ss(tmem_base + col, ad + oa, bd + ob, IDESC_S, ks != 0);
       }
-    };
-    auto gather = [&](uint32_t col, uint32_t from, uint64_t bd, bool accumulate) {  // [keys][features] += P B over the rows
-#pragma unroll
-      for (int ks = 0; ks < TILE / 16; ++ks)
-        if (elected)
-          ptx::umma_ts(tmem_base + col, tmem_base + from + packed_col(ks >> 1) + (ks & 1) * 8,
-                       bd + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_D, accumulate || ks != 0);
     };
     if (steps > 0) {
       wait_(kv_full, 0, 103);
@@ -216,116 +223,134 @@ __global__ void __launch_bounds__(THREADS, 1)
       ptx::tc_fence_after();
       score(COL_S, dk, dq);
       commit_(s_ready);
+      score(COL_DP, dv, dd);
+      commit_(dp_ready);
       for (int i = 0; i < steps; ++i) {
         const uint32_t ph = i & 1;
-        const uint64_t cur = (i & 1) ? NEXT : 0, nxt = (i & 1) ? 0 : NEXT;
-        score(COL_P, dv, dd + cur);  // dP^T(i): dK(i-1), issued before, has read dS^T(i-1)
-        commit_(dp_ready);
-        wait_(p_ready, ph, 105);
-        ptx::tc_fence_after();
-        gather(COL_DV, COL_S, dd_t + cur, i > 0);
+        const uint64_t cur = (i % STAGES) * STAGE, nxt = ((i + 1) % STAGES) * STAGE;
         if (i + 1 < steps) {
-          wait_(&qdo_full[(i + 1) & 1], ((i + 1) >> 1) & 1, 106);
+          wait_(s_free, ph, 105);
+          wait_(&qdo_full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1, 106);
           ptx::tc_fence_after();
-          score(COL_S, dk, dq + nxt);  // (over P^T(i), which dV(i) reads first on the in-order pipe)
+          score(COL_S, dk, dq + nxt);
           commit_(s_ready);
         }
-        wait_(ds_ready, ph, 107);
+        wait_(p_ready, ph, 107);
         ptx::tc_fence_after();
-        gather(COL_DK, COL_P, dq_t + cur, i > 0);
-        commit_(&qdo_empty[i & 1]);
+#pragma unroll
+        for (int ks = 0; ks < COLS / 16; ++ks)
+          if (elected)
+            ptx::umma_ts(tmem_base + COL_DV, tmem_base + COL_P + ks * 8, dd_t + cur + static_cast<uint64_t>((ks * 2048) >> 4),
+                         IDESC_D, (i | ks) != 0);
+        commit_(dv_done);
+        wait_(ds_ready, ph, 108);
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < COLS / 16; ++ks)  // (a thread packs dS^T into the first half of its own columns)
+          if (elected)
+            ptx::umma_ts(tmem_base + COL_DK, tmem_base + COL_DP + (ks / (HALF / 16)) * HALF + (ks % (HALF / 16)) * 8,
+                         dq_t + cur + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_D, (i | ks) != 0);
+        commit_(&qdo_empty[i % STAGES]);
+        if (i + 1 < steps) {
+          score(COL_DP, dv, dd + nxt);  // over dS^T(i), which dK(i) reads first on the in-order pipe
+          commit_(dp_ready);
+        }
       }
     }
     commit_(all_done);
-    if (elected) ptx::mbar_wait_drain(all_done, 0, abort_flag, p.status, 108);
+    ptx::mbar_wait_drain(all_done, 0, abort_flag, p.status, 109);
     __syncwarp();
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane, key = jt * TILE + r;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem_base + lane_off + COL_S + half * 64, p_addr = tmem_base + lane_off + COL_P + half * 64;
+    const uint32_t s_addr = tmem_base + lane_off + COL_S + half * HALF, dp_addr = tmem_base + lane_off + COL_DP + half * HALF;
+    const uint32_t p_addr = tmem_base + lane_off + COL_P + half * (HALF / 2);
     const uint64_t scale2 = am::pack2f(p.scale_log2, p.scale_log2);
-    const uint32_t always = key < a.sinks ? 0xffffffffu : 0u;
+    const uint64_t always = key < a.sinks ? ~0ull : 0ull;
     for (int i = 0; i < steps; ++i) {
-      const int st = i & 1, it = i0 + i;
-      const int token0 = it * p.tile_tokens, token1 = token0 + p.tile_tokens - 1;
+      const int st = i % STAGES, it = i0 + i;
+      const int token0 = it * p.col_tokens, token1 = token0 + p.col_tokens - 1;
       // every query of the tile sees every key of this one
       const bool plain = token0 >= jt * TILE + TILE - 1 && (token1 - jt * TILE < a.window || (jt + 1) * TILE <= a.sinks);
-      const float4* nlse4 = reinterpret_cast<const float4*>(nlse_smem + st * 128 + half * 64);
-      const float4* ndel4 = reinterpret_cast<const float4*>(ndelta_smem + st * 128 + half * 64);
-      float pr[64];
-      ptx::mbar_wait(&qdo_full[st], (i >> 1) & 1, abort_flag, p.status, 109);
-      ptx::mbar_wait(s_ready, i & 1, abort_flag, p.status, 110);
+      const float4* nlse4 = reinterpret_cast<const float4*>(nlse_smem + st * COLS + half * HALF);
+      const float4* ndel4 = reinterpret_cast<const float4*>(ndelta_smem + st * COLS + half * HALF);
+      float pr[HALF];
+      uint32_t ra[32], rb[16];
+      ptx::mbar_wait(&qdo_full[st], (i / STAGES) & 1, abort_flag, p.status, 110);
+      ptx::mbar_wait(s_ready, i & 1, abort_flag, p.status, 111);
       ptx::tc_fence_after();
-      {
-        uint32_t ra[32], rb[32];
+      ptx::tmem_ld32(s_addr, ra);
+      ptx::tmem_ld16(s_addr + 32, rb);
+      am::tmem_ld_wait_dep(ra);
+      am::tmem_ld_wait_dep(rb);
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(s_free);
+      auto scaled = [&](int g, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+        const float4 nl = nlse4[g];
+        am::unpack2f(am::fma2(am::pack2u(v0, v1), scale2, am::pack2f(nl.x, nl.y)), pr[g * 4], pr[g * 4 + 1]);
+        am::unpack2f(am::fma2(am::pack2u(v2, v3), scale2, am::pack2f(nl.z, nl.w)), pr[g * 4 + 2], pr[g * 4 + 3]);
+      };
+#pragma unroll
+      for (int g = 0; g < 8; ++g) scaled(g, ra[g * 4], ra[g * 4 + 1], ra[g * 4 + 2], ra[g * 4 + 3]);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) scaled(8 + g, rb[g * 4], rb[g * 4 + 1], rb[g * 4 + 2], rb[g * 4 + 3]);
+#pragma unroll
+      for (int e = 0; e < HALF; ++e) pr[e] = am::ex2(pr[e]);
+      if (!plain) {
         // columns from `low` on are not before the key, those below `high` are within its window
-        const int low = saturate((int64_t)(key - token0) * a.G) - half * 64;
-        const int high = saturate(((int64_t)key + a.window - token0) * a.G) - half * 64;
-        auto exp32 = [&](const uint32_t (&v)[32], int q) {
+        const int low = saturate((int64_t)(key - token0) * a.G) - half * HALF;
+        const int high = saturate(((int64_t)key + a.window - token0) * a.G) - half * HALF;
+        const uint64_t seen = ~low_bits64(low) & (low_bits64(high) | always);
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const float4 nl = nlse4[q * 8 + g];
-            am::unpack2f(am::fma2(am::pack2u(v[g * 4], v[g * 4 + 1]), scale2, am::pack2f(nl.x, nl.y)), pr[q * 32 + g * 4],
-                         pr[q * 32 + g * 4 + 1]);
-            am::unpack2f(am::fma2(am::pack2u(v[g * 4 + 2], v[g * 4 + 3]), scale2, am::pack2f(nl.z, nl.w)),
-                         pr[q * 32 + g * 4 + 2], pr[q * 32 + g * 4 + 3]);
-          }
+        for (int e = 0; e < HALF; ++e)
+          if (!((seen >> e) & 1u)) pr[e] = 0.f;
+      }
+      {
+        uint32_t pa[16], pb[8];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) pr[q * 32 + e] = am::ex2(pr[q * 32 + e]);
-          if (!plain) {
-            const uint32_t seen = ~low_bits(low - 32 * q) & (low_bits(high - 32 * q) | always);
+        for (int e = 0; e < 16; ++e) pa[e] = am::cvt_pair<T>(pr[2 * e], pr[2 * e + 1]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((seen >> e) & 1u)) pr[q * 32 + e] = 0.f;
-          }
-          uint32_t packed[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) packed[e] = am::cvt_pair<T>(pr[q * 32 + 2 * e], pr[q * 32 + 2 * e + 1]);
-          ptx::tmem_st16(s_addr + q * 16, packed);
-        };
-        ptx::tmem_ld32(s_addr, ra);
-        am::tmem_ld_wait_dep(ra);
-        ptx::tmem_ld32(s_addr + 32, rb);
-        am::tmem_ld_wait_dep(rb);  // (both blocks are read before the packed copy goes over them)
-        exp32(ra, 0);
-        exp32(rb, 1);
+        for (int e = 0; e < 8; ++e) pb[e] = am::cvt_pair<T>(pr[32 + 2 * e], pr[33 + 2 * e]);
+        if (i > 0) {  // P^T(i) goes over P^T(i-1)
+          ptx::mbar_wait(dv_done, (i - 1) & 1, abort_flag, p.status, 112);
+          ptx::tc_fence_after();
+        }
+        ptx::tmem_st16(p_addr, pa);
+        ptx::tmem_st8(p_addr + 16, pb);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         ptx::mbar_arrive(p_ready);
       }
-      ptx::mbar_wait(dp_ready, i & 1, abort_flag, p.status, 111);
+      ptx::mbar_wait(dp_ready, i & 1, abort_flag, p.status, 113);
       ptx::tc_fence_after();
+      ptx::tmem_ld32(dp_addr, ra);
+      ptx::tmem_ld16(dp_addr + 32, rb);
+      am::tmem_ld_wait_dep(ra);
+      am::tmem_ld_wait_dep(rb);
       {
-        uint32_t ra[32], rb[32];
-        auto grad32 = [&](const uint32_t (&v)[32], int q) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const float4 nd = ndel4[q * 8 + g];
-            float d0, d1, d2, d3;
-            am::unpack2f(am::mul2(am::pack2f(pr[q * 32 + g * 4], pr[q * 32 + g * 4 + 1]),
-                                  am::add2(am::pack2u(v[g * 4], v[g * 4 + 1]), am::pack2f(nd.x, nd.y))), d0, d1);
-            am::unpack2f(am::mul2(am::pack2f(pr[q * 32 + g * 4 + 2], pr[q * 32 + g * 4 + 3]),
-                                  am::add2(am::pack2u(v[g * 4 + 2], v[g * 4 + 3]), am::pack2f(nd.z, nd.w))), d2, d3);
-            packed[g * 2] = am::cvt_pair<T>(d0, d1);
-            packed[g * 2 + 1] = am::cvt_pair<T>(d2, d3);
-          }
-          ptx::tmem_st16(p_addr + q * 16, packed);
+        uint32_t pa[16], pb[8];
+        auto grad = [&](int g, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, uint32_t& o0, uint32_t& o1) {
+          const float4 nd = ndel4[g];
+          float d0, d1, d2, d3;
+          am::unpack2f(am::mul2(am::pack2f(pr[g * 4], pr[g * 4 + 1]), am::add2(am::pack2u(v0, v1), am::pack2f(nd.x, nd.y))), d0, d1);
+          am::unpack2f(am::mul2(am::pack2f(pr[g * 4 + 2], pr[g * 4 + 3]), am::add2(am::pack2u(v2, v3), am::pack2f(nd.z, nd.w))), d2, d3);
+          o0 = am::cvt_pair<T>(d0, d1);
+          o1 = am::cvt_pair<T>(d2, d3);
         };
-        ptx::tmem_ld32(p_addr, ra);
-        am::tmem_ld_wait_dep(ra);
-        ptx::tmem_ld32(p_addr + 32, rb);
-        am::tmem_ld_wait_dep(rb);
-        grad32(ra, 0);
-        grad32(rb, 1);
+#pragma unroll
+        for (int g = 0; g < 8; ++g) grad(g, ra[g * 4], ra[g * 4 + 1], ra[g * 4 + 2], ra[g * 4 + 3], pa[g * 2], pa[g * 2 + 1]);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) grad(8 + g, rb[g * 4], rb[g * 4 + 1], rb[g * 4 + 2], rb[g * 4 + 3], pb[g * 2], pb[g * 2 + 1]);
+        ptx::tmem_st16(dp_addr, pa);
+        ptx::tmem_st8(dp_addr + 16, pb);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         ptx::mbar_arrive(ds_ready);
       }
     }
     // epilogue: the first half of the warps writes dV, the second dK
-    ptx::mbar_wait(all_done, 0, abort_flag, p.status, 112);
+    ptx::mbar_wait(all_done, 0, abort_flag, p.status, 114);
     ptx::tc_fence_after();
     const bool is_k = half == 1, parted = jt < p.b.sink_tiles;
     const float mul = is_k ? a.scale : 1.f;
@@ -373,49 +398,61 @@ __global__ void __launch_bounds__(THREADS, 1)
 // ------------------------------------------------------------------ dQ
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
-    local_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                       const BwdParams p) {
+    local_dq_tc_kernel(const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v, const BwdParams p) {
+  constexpr int STAGES = 3;
   constexpr int TILE_BYTES = TILE * D * 2, NBOX = D / 64, BOX_BYTES = TILE * 128;
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t IDESC_S = ptx::make_idesc(IS_BF16, false, false, TILE, TILE);
   constexpr uint32_t IDESC_D = ptx::make_idesc(IS_BF16, false, true, TILE, D);
-  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 256, COL_DQ = 384;
+  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256, COL_Q = 384, COL_DO = 448;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_smem = smem;
-  uint8_t* do_smem = smem + TILE_BYTES;
-  uint8_t* k_smem = smem + 2 * TILE_BYTES;  // [2]
-  uint8_t* v_smem = smem + 4 * TILE_BYTES;  // [2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * TILE_BYTES);
-  uint64_t* qdo_full = bars;
-  uint64_t* k_full = bars + 1;    // [2]
-  uint64_t* v_full = bars + 3;    // [2]
-  uint64_t* kv_empty = bars + 5;  // [2]
-  uint64_t* s_ready = bars + 7;   // [2] S(i) computed, by buffer i & 1
-  uint64_t* ds_ready = bars + 9;  // [2] dS(i) written over S(i)   (256 arrivals)
-  uint64_t* dp_ready = bars + 11; // dP(i) computed
-  uint64_t* dp_free = bars + 12;  // dP(i) read                    (256 arrivals)
-  uint64_t* all_done = bars + 13;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  uint8_t* k_smem = smem;                             // [STAGES]
+  uint8_t* v_smem = smem + STAGES * TILE_BYTES;       // [STAGES]
+  uint8_t* stage_smem = smem + 2 * STAGES * TILE_BYTES;  // dQ tile on its way out
+  float* delta_smem = reinterpret_cast<float*>(stage_smem + TILE_BYTES);  // [128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(delta_smem + TILE);
+  uint64_t* k_full = bars;                 // [STAGES]
+  uint64_t* v_full = bars + STAGES;        // [STAGES]
+  uint64_t* kv_empty = bars + 2 * STAGES;  // [STAGES]
+  // Per step (g counts the steps of all tiles of this CTA): parity g & 1. Per tile (u): parity u & 1.
+  uint64_t* s_ready = bars + 3 * STAGES;   // S(g) computed
+  uint64_t* dp_ready = s_ready + 1;        // dP(g) computed
+  uint64_t* tile_done = s_ready + 2;       // all products of tile u done
+  uint64_t* s_free = s_ready + 3;          // S(g) read               (256 arrivals)
+  uint64_t* ds_ready = s_ready + 4;        // dS(g) written over dP(g) (256 arrivals)
+  uint64_t* q_ready = s_ready + 5;         // Q, dO of tile u in tensor memory, dQ of tile u - 1 read (256 arrivals)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_ready + 6);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const LocalArgs& a = p.b.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int s = blockIdx.z, hk = blockIdx.y;
-  const int it = (int)gridDim.x - 1 - (int)blockIdx.x;  // longest walks first
-  const int t0 = it * p.tile_tokens, ntok = min(p.tile_tokens, a.tokens - t0);
-  const KeyRange kr = key_range(a, t0, t0 + ntok - 1, a.tokens, TILE);
-  const int steps = kr.count;  // (at least one: a query sees itself)
+  const int units = a.n * a.KV * p.row_tiles;
+  // tile `unit`: longest walks (last tokens) of a sequence and key head first
+  struct Unit {
+    int s, hk, t0, ntok;
+    KeyRange kr;
+  };
+  auto unit_at = [&](int unit) {
+    Unit w;
+    const int sh = unit / p.row_tiles, it = p.row_tiles - 1 - unit % p.row_tiles;
+    w.s = sh / a.KV;
+    w.hk = sh % a.KV;
+    w.t0 = it * p.tile_tokens;
+    w.ntok = min(p.tile_tokens, a.tokens - w.t0);
+    w.kr = key_range(a, w.t0, w.t0 + w.ntok - 1, a.tokens, TILE);  // (at least one tile: a query sees itself)
+    return w;
+  };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 14; ++i) ptx::mbar_init(&bars[i], (i == 9 || i == 10 || i == 12) ? 256 : 1);
+    for (int i = 0; i < 3 * STAGES + 3; ++i) ptx::mbar_init(&bars[i], 1);
+    for (int i = 0; i < 3; ++i) ptx::mbar_init(s_free + i, 256);
     abort_flag[0] = 0;
     abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
     ptx::fence_barrier_init();
-    ptx::prefetch_tensormap(&map_q);
-    ptx::prefetch_tensormap(&map_do);
+    ptx::prefetch_tensormap(&map_dq);
     ptx::prefetch_tensormap(&map_k);
     ptx::prefetch_tensormap(&map_v);
   }
@@ -430,213 +467,249 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t bytes = NBOX * p.tile_tokens * a.G * 128;
-      ptx::mbar_expect_tx(qdo_full, 2 * bytes);
+      int g = 0;
+      for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const Unit w = unit_at(unit);
+        for (int i = 0; i < w.kr.count; ++i, ++g) {
+          const int st = g % STAGES, j0 = w.kr.tile(i) * TILE;
+          ptx::mbar_wait(&kv_empty[st], ((g / STAGES) & 1) ^ 1, abort_flag, p.status, 121);
+          ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
 #pragma unroll
-      for (int c = 0; c < NBOX; ++c) {
-        tma_load_5d(q_smem + c * BOX_BYTES, &map_q, qdo_full, c * 64, 0, t0, hk, s);
-        tma_load_5d(do_smem + c * BOX_BYTES, &map_do, qdo_full, c * 64, 0, t0, hk, s);
+          for (int c = 0; c < NBOX; ++c) tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES, &map_k, &k_full[st], c * 64, j0, w.hk, w.s);
+          ptx::mbar_expect_tx(&v_full[st], TILE_BYTES);
+#pragma unroll
+          for (int c = 0; c < NBOX; ++c) tma_load_4d(v_smem + st * TILE_BYTES + c * BOX_BYTES, &map_v, &v_full[st], c * 64, j0, w.hk, w.s);
+        }
       }
-      for (int i = 0; i < steps; ++i) {
-        const int st = i & 1, j0 = kr.tile(i) * TILE;
-        ptx::mbar_wait(&kv_empty[st], ((i >> 1) & 1) ^ 1, abort_flag, p.status, 121);
-        ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
-#pragma unroll
-        for (int c = 0; c < NBOX; ++c) tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES, &map_k, &k_full[st], c * 64, j0, hk, s);
-        ptx::mbar_expect_tx(&v_full[st], TILE_BYTES);
-#pragma unroll
-        for (int c = 0; c < NBOX; ++c) tma_load_4d(v_smem + st * TILE_BYTES + c * BOX_BYTES, &map_v, &v_full[st], c * 64, j0, hk, s);
-      }
-      ptx::mbar_wait_drain(qdo_full, 0, abort_flag, p.status, 122);
-      for (int i = steps > 2 ? steps - 2 : 0; i < steps; ++i) {
-        ptx::mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 122);
-        ptx::mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 122);
+      // every copy has landed before the CTA gives up its shared memory
+      for (int i = g > STAGES ? g - STAGES : 0; i < g; ++i) {
+        ptx::mbar_wait_drain(&k_full[i % STAGES], (i / STAGES) & 1, abort_flag, p.status, 122);
+        ptx::mbar_wait_drain(&v_full[i % STAGES], (i / STAGES) & 1, abort_flag, p.status, 122);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
+    // The whole warp walks the loop and waits; one elected lane issues. (With the waits in the elected lane
+    // alone, a commit was seen to take effect only after that lane's next wait had given up.)
     const bool elected = ptx::elect_one();
     auto wait_ = [&](uint64_t* bar, uint32_t parity, int code) {
-      if (elected) ptx::mbar_wait(bar, parity, abort_flag, p.status, code);
+      ptx::mbar_wait(bar, parity, abort_flag, p.status, code);
       __syncwarp();
     };
     auto commit_ = [&](uint64_t* bar) {
       if (elected) ptx::umma_commit(bar);
     };
-    const uint64_t dq = ptx::make_smem_desc(ptx::smem_u32(q_smem), 16, 1024), dd = ptx::make_smem_desc(ptx::smem_u32(do_smem), 16, 1024);
     const uint64_t dk = ptx::make_smem_desc(ptx::smem_u32(k_smem), 16, 1024), dv = ptx::make_smem_desc(ptx::smem_u32(v_smem), 16, 1024);
     const uint64_t dk_t = ptx::make_smem_desc(ptx::smem_u32(k_smem), BOX_BYTES, 1024);  // read along the keys
-    constexpr uint64_t NEXT = static_cast<uint64_t>(TILE_BYTES >> 4);
-    auto score = [&](uint32_t col, uint64_t ad, uint64_t bd) {
+    constexpr uint64_t STAGE = static_cast<uint64_t>(TILE_BYTES >> 4);
+    auto score = [&](uint32_t col, uint32_t from, uint64_t bd) {
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint64_t off = static_cast<uint64_t>(((ks >> 2) * BOX_BYTES + (ks & 3) * 32) >> 4);
-        if (elected) ptx::umma_ss(tmem_base + col, ad + off, bd + off, IDESC_S, ks != 0);
-      }
+      for (int ks = 0; ks < D / 16; ++ks)
+        if (elected)
+          ptx::umma_ts(tmem_base + col, tmem_base + from + ks * 8, bd + static_cast<uint64_t>(((ks >> 2) * BOX_BYTES + (ks & 3) * 32) >> 4),
+                       IDESC_S, ks != 0);
     };
-    auto scores_of = [&](int i) {
-      wait_(&k_full[i & 1], (i >> 1) & 1, 123);
+    auto scores_of = [&](int g) {
+      if (g > 0) wait_(s_free, (g - 1) & 1, 123);
+      wait_(&k_full[g % STAGES], (g / STAGES) & 1, 124);
       ptx::tc_fence_after();
-      score(COL_S + (i & 1) * 128, dq, dk + ((i & 1) ? NEXT : 0));
-      commit_(&s_ready[i & 1]);
+      score(COL_S, COL_Q, dk + (g % STAGES) * STAGE);
+      commit_(s_ready);
     };
-    auto gradients_of = [&](int i) {
-      wait_(&v_full[i & 1], (i >> 1) & 1, 124);
+    auto gradients_of = [&](int g) {  // (over dS(g-1), which dQ(g-1) reads first on the in-order pipe)
+      wait_(&v_full[g % STAGES], (g / STAGES) & 1, 125);
       ptx::tc_fence_after();
-      score(COL_DP, dd, dv + ((i & 1) ? NEXT : 0));
+      score(COL_DP, COL_DO, dv + (g % STAGES) * STAGE);
       commit_(dp_ready);
     };
-    wait_(qdo_full, 0, 125);
-    scores_of(0);
-    gradients_of(0);
-    for (int i = 0; i < steps; ++i) {
-      if (i + 1 < steps) {
-        scores_of(i + 1);  // (over dS(i-1), which dQ(i-1) reads first on the in-order pipe)
-        wait_(dp_free, i & 1, 126);
-        ptx::tc_fence_after();
-        gradients_of(i + 1);
-      }
-      wait_(&ds_ready[i & 1], (i >> 1) & 1, 127);
+    int g = 0, u = 0;
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
+      const int steps = unit_at(unit).kr.count;
+      wait_(q_ready, u & 1, 126);
       ptx::tc_fence_after();
+      scores_of(g);
+      gradients_of(g);
+      for (int i = 0; i < steps; ++i, ++g) {
+        if (i + 1 < steps) scores_of(g + 1);
+        wait_(ds_ready, g & 1, 127);
+        ptx::tc_fence_after();
 #pragma unroll
-      for (int ks = 0; ks < TILE / 16; ++ks)
-        if (elected)
-          ptx::umma_ts(tmem_base + COL_DQ, tmem_base + COL_S + (i & 1) * 128 + packed_col(ks >> 1) + (ks & 1) * 8,
-                       dk_t + ((i & 1) ? NEXT : 0) + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_D, (i | ks) != 0);
-      commit_(&kv_empty[i & 1]);
+        for (int ks = 0; ks < TILE / 16; ++ks)  // (a thread packs dS into the first half of its own 64 columns)
+          if (elected)
+            ptx::umma_ts(tmem_base + COL_DQ, tmem_base + COL_DP + (ks >> 2) * 64 + (ks & 3) * 8,
+                         dk_t + (g % STAGES) * STAGE + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_D, (i | ks) != 0);
+        commit_(&kv_empty[g % STAGES]);
+        if (i + 1 < steps) gradients_of(g + 1);
+      }
+      commit_(tile_done);
     }
-    commit_(all_done);
-    if (elected) ptx::mbar_wait_drain(all_done, 0, abort_flag, p.status, 128);
+    // everything issued has completed before tensor memory is freed
+    if (u > 0) ptx::mbar_wait_drain(tile_done, (u - 1) & 1, abort_flag, p.status, 128);
     __syncwarp();
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
-    const bool live = r < ntok * a.G;
-    const int pos = live ? t0 + r / a.G : -1;
+    const int group = r % a.G, row_token = r / a.G;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + COL_S + half * 64, dp_addr = tmem_base + lane_off + COL_DP + half * 64;
-    const int64_t row = (((int64_t)s * a.KV + hk) * p.query_tiles + it) * TILE + r;
-    const float nlse = p.nlse2[row], ndelta = p.ndelta[row];
-    const uint64_t scale2 = am::pack2f(p.scale_log2, p.scale_log2), nlse_2 = am::pack2f(nlse, nlse), ndelta_2 = am::pack2f(ndelta, ndelta);
-    for (int i = 0; i < steps; ++i) {
-      const int j0 = kr.tile(i) * TILE;
-      const bool plain = j0 + TILE - 1 <= t0 && (t0 + ntok - 1 - j0 < a.window || j0 + TILE <= a.sinks);
-      float pr[64];
-      ptx::mbar_wait(&s_ready[i & 1], (i >> 1) & 1, abort_flag, p.status, 129);
-      ptx::tc_fence_after();
-      {
-        uint32_t ra[32], rb[32];
-        const int high = pos - j0 + 1 - half * 64;  // columns below `high` are not in the future
-        const int low = saturate((int64_t)pos - a.window + 1 - j0) - half * 64, sink = a.sinks - j0 - half * 64;
-        auto exp32 = [&](const uint32_t (&v)[32], int q) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            am::unpack2f(am::fma2(am::pack2u(v[e], v[e + 1]), scale2, nlse_2), pr[q * 32 + e], pr[q * 32 + e + 1]);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) pr[q * 32 + e] = am::ex2(pr[q * 32 + e]);
-          if (!plain) {
-            const uint32_t seen = low_bits(high - 32 * q) & (~low_bits(low - 32 * q) | low_bits(sink - 32 * q));
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((seen >> e) & 1u)) pr[q * 32 + e] = 0.f;
-          }
-        };
-        ptx::tmem_ld32(s_addr + (i & 1) * 128, ra);
-        am::tmem_ld_wait_dep(ra);
-        ptx::tmem_ld32(s_addr + (i & 1) * 128 + 32, rb);
-        exp32(ra, 0);
-        am::tmem_ld_wait_dep(rb);
-        exp32(rb, 1);
+    const uint64_t scale2 = am::pack2f(p.scale_log2, p.scale_log2);
+    // entries of column tiles that belong to no row: zeros (the products that meet them see rows of zeros)
+    {
+      const int64_t tiles = (int64_t)a.n * a.KV * p.col_tiles;
+      for (int64_t t = (int64_t)blockIdx.x * 256 + (threadIdx.x - 128); t < tiles; t += (int64_t)gridDim.x * 256) {
+        const int left = a.tokens - (int)(t % p.col_tiles) * p.col_tokens;
+        for (int c = min(left, p.col_tokens) * a.G; c < COLS; ++c) p.nlse2[t * COLS + c] = p.ndelta[t * COLS + c] = 0.f;
       }
-      ptx::mbar_wait(dp_ready, i & 1, abort_flag, p.status, 130);
-      ptx::tc_fence_after();
-      {
-        uint32_t ra[32], rb[32];
-        auto grad32 = [&](const uint32_t (&v)[32], int q) {
-          uint32_t packed[16];
+    }
+    // half 0 brings the rows of Q, half 1 those of dO
+    uint4 raw[D / 8];
+    auto fetch = [&](const Unit& w) {
+      const bool live = r < w.ntok * a.G;
+      const int64_t* st = half ? p.b.dos : a.qs;
+      const T* src = reinterpret_cast<const T*>(half ? p.dout : p.q) + (int64_t)w.s * st[0] + (int64_t)(w.hk * a.G + group) * st[1] +
+                     (int64_t)(w.t0 + row_token) * st[2];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float d0, d1;
-            am::unpack2f(am::mul2(am::pack2f(pr[q * 32 + e], pr[q * 32 + e + 1]), am::add2(am::pack2u(v[e], v[e + 1]), ndelta_2)),
-                         d0, d1);
-            packed[e >> 1] = am::cvt_pair<T>(d0, d1);
+      for (int c = 0; c < D / 8; ++c) raw[c] = live ? ld_stream(src + c * 8) : make_uint4(0, 0, 0, 0);
+    };
+    int g = 0, u = 0;
+    if ((int)blockIdx.x < units) fetch(unit_at(blockIdx.x));
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
+      const Unit w = unit_at(unit);
+      const bool live = r < w.ntok * a.G;
+      const int pos = live ? w.t0 + row_token : -1, head = w.hk * a.G + group;
+      // rows into tensor memory (the products that read the previous tile's are done: tile_done)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t v[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e * 4] = raw[c * 8 + e].x;
+          v[e * 4 + 1] = raw[c * 8 + e].y;
+          v[e * 4 + 2] = raw[c * 8 + e].z;
+          v[e * 4 + 3] = raw[c * 8 + e].w;
+        }
+        ptx::tmem_st32(tmem_base + lane_off + (half ? COL_DO : COL_Q) + c * 32, v);
+      }
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(q_ready);
+      const float nlse = live ? -p.lse[((int64_t)w.s * a.H + head) * a.tokens + pos] * LOG2E : 0.f;
+      float ndelta = 0.f;
+      if (half) {
+        const T* src = reinterpret_cast<const T*>(p.out) + (int64_t)w.s * a.os[0] + (int64_t)head * a.os[1] + (int64_t)pos * a.os[2];
+#pragma unroll
+        for (int c = 0; c < D / 8; c += 4) {
+          uint4 o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = live ? ld_stream(src + (c + e) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x[8], y[8];
+            unpack<T>(o[e], x);
+            unpack<T>(raw[c + e], y);
+#pragma unroll
+            for (int f = 0; f < 8; ++f) ndelta = fmaf(x[f], -y[f], ndelta);
           }
-          ptx::tmem_st16(s_addr + (i & 1) * 128 + q * 16, packed);
-        };
+        }
+        delta_smem[r] = ndelta;
+        if (live) {
+          const int64_t at = (((int64_t)w.s * a.KV + w.hk) * p.col_tiles + pos / p.col_tokens) * COLS + (pos % p.col_tokens) * a.G + group;
+          p.nlse2[at] = nlse;
+          p.ndelta[at] = ndelta;
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      ndelta = delta_smem[r];
+      const uint64_t nlse_2 = am::pack2f(nlse, nlse), ndelta_2 = am::pack2f(ndelta, ndelta);
+      for (int i = 0; i < w.kr.count; ++i, ++g) {
+        const int j0 = w.kr.tile(i) * TILE;
+        const bool plain = j0 + TILE - 1 <= w.t0 && (w.t0 + w.ntok - 1 - j0 < a.window || j0 + TILE <= a.sinks);
+        float pr[64];
+        uint32_t ra[32], rb[32];
+        ptx::mbar_wait(s_ready, g & 1, abort_flag, p.status, 129);
+        ptx::tc_fence_after();
+        ptx::tmem_ld32(s_addr, ra);
+        ptx::tmem_ld32(s_addr + 32, rb);
+        am::tmem_ld_wait_dep(ra);
+        am::tmem_ld_wait_dep(rb);
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(s_free);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          am::unpack2f(am::fma2(am::pack2u(ra[e], ra[e + 1]), scale2, nlse_2), pr[e], pr[e + 1]);
+          am::unpack2f(am::fma2(am::pack2u(rb[e], rb[e + 1]), scale2, nlse_2), pr[32 + e], pr[33 + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 64; ++e) pr[e] = am::ex2(pr[e]);
+        if (!plain) {
+          const int high = pos - j0 + 1 - half * 64;  // columns below `high` are not in the future
+          const int low = saturate((int64_t)pos - a.window + 1 - j0) - half * 64, sink = a.sinks - j0 - half * 64;
+          const uint64_t seen = low_bits64(high) & (~low_bits64(low) | low_bits64(sink));
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (!((seen >> e) & 1u)) pr[e] = 0.f;
+        }
+        ptx::mbar_wait(dp_ready, g & 1, abort_flag, p.status, 130);
+        ptx::tc_fence_after();
         ptx::tmem_ld32(dp_addr, ra);
         ptx::tmem_ld32(dp_addr + 32, rb);
         am::tmem_ld_wait_dep(ra);
         am::tmem_ld_wait_dep(rb);
-        ptx::tc_fence_before();
-        ptx::mbar_arrive(dp_free);
-        grad32(ra, 0);
-        grad32(rb, 1);
+        uint32_t packed[32];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float d0, d1;
+          am::unpack2f(am::mul2(am::pack2f(pr[e], pr[e + 1]), am::add2(am::pack2u(ra[e], ra[e + 1]), ndelta_2)), d0, d1);
+          packed[e >> 1] = am::cvt_pair<T>(d0, d1);
+          am::unpack2f(am::mul2(am::pack2f(pr[32 + e], pr[33 + e]), am::add2(am::pack2u(rb[e], rb[e + 1]), ndelta_2)), d0, d1);
+          packed[16 + (e >> 1)] = am::cvt_pair<T>(d0, d1);
+        }
+        ptx::tmem_st32(dp_addr, packed);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
-        ptx::mbar_arrive(&ds_ready[i & 1]);
+        ptx::mbar_arrive(ds_ready);
       }
-    }
-    // epilogue: each half of the warps writes half of the features
-    ptx::mbar_wait(all_done, 0, abort_flag, p.status, 131);
-    ptx::tc_fence_after();
-    T* out = reinterpret_cast<T*>(p.dq) + (int64_t)s * p.b.dqs[0] + (int64_t)(hk * a.G + r % a.G) * p.b.dqs[1] +
-             (int64_t)(t0 + r / a.G) * p.b.dqs[2] + half * (D / 2);
-#pragma unroll 1
-    for (int c = 0; c < D / 64; ++c) {
-      uint32_t v[32];
-      __syncwarp();
-      ptx::tmem_ld32(tmem_base + lane_off + COL_DQ + half * (D / 2) + c * 32, v);
-      ptx::tmem_ld_wait();
-      if (live) {
+      // the next tile's rows are requested while this one's last products run
+      if (unit + (int)gridDim.x < units) fetch(unit_at(unit + gridDim.x));
+      // dQ out, through shared memory (its previous tile's copy has been read): each half of the warps
+      // takes half of the features
+      if (threadIdx.x == 128) ptx::bulk_wait_read();
+      ptx::mbar_wait(tile_done, u & 1, abort_flag, p.status, 131);
+      ptx::tc_fence_after();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t v[32];
+        ptx::tmem_ld32(tmem_base + lane_off + COL_DQ + half * (D / 2) + c * 32, v);
+        ptx::tmem_ld_wait();
+        const int chunk0 = (half * (D / 2) + c * 32) / 8;  // first 16-byte chunk of the row
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
           uint4 o;
-          o.x = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 0]) * a.scale, __uint_as_float(v[g * 8 + 1]) * a.scale);
-          o.y = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 2]) * a.scale, __uint_as_float(v[g * 8 + 3]) * a.scale);
-          o.z = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 4]) * a.scale, __uint_as_float(v[g * 8 + 5]) * a.scale);
-          o.w = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 6]) * a.scale, __uint_as_float(v[g * 8 + 7]) * a.scale);
-          *reinterpret_cast<uint4*>(out + c * 32 + g * 8) = o;
+          o.x = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 0]) * a.scale, __uint_as_float(v[e * 8 + 1]) * a.scale);
+          o.y = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 2]) * a.scale, __uint_as_float(v[e * 8 + 3]) * a.scale);
+          o.z = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 4]) * a.scale, __uint_as_float(v[e * 8 + 5]) * a.scale);
+          o.w = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 6]) * a.scale, __uint_as_float(v[e * 8 + 7]) * a.scale);
+          const int chunk = chunk0 + e;
+          *reinterpret_cast<uint4*>(stage_smem + (chunk >> 3) * BOX_BYTES + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = o;
         }
       }
+      ptx::tc_fence_before();
+      ptx::fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (threadIdx.x == 128) {
+#pragma unroll
+        for (int c = 0; c < NBOX; ++c) ptx::tma_store_5d(&map_dq, stage_smem + c * BOX_BYTES, c * 64, 0, w.t0, w.hk, w.s);
+        ptx::bulk_commit();
+      }
     }
+    if (threadIdx.x == 128) ptx::bulk_wait_done();
   }
   ptx::tc_fence_before();
   __syncthreads();
   if (warp == 2) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem_base, TMEM_COLS);
-  }
-}
-
-// ------------------------------------------------------------------ -lse log2e and -delta by query tile
-// D / 8 threads a row, each one 16-byte load of out and one of dout.
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
-    local_bwd_prep(float* __restrict__ nlse2, float* __restrict__ ndelta, const T* __restrict__ out, const T* __restrict__ dout,
-                   const float* __restrict__ lse, const LocalBwdArgs b, int tile_tokens, int query_tiles) {
-  constexpr int TPR = D / 8;
-  const LocalArgs& a = b.f;
-  const int sub = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  const int64_t total = (int64_t)a.n * a.KV * query_tiles * TILE;
-  const int c = (int)(row % TILE), it = (int)(row / TILE % query_tiles);
-  const int64_t sh = row / TILE / query_tiles;
-  const int hk = (int)(sh % a.KV), head = hk * a.G + c % a.G, t = it * tile_tokens + c / a.G;
-  const int64_t s = sh / a.KV;
-  const bool live = row < total && c < tile_tokens * a.G && t < a.tokens;
-  float acc = 0.f;
-  if (live) {
-    float o[8], g[8];
-    unpack<T>(ld_stream(out + s * a.os[0] + head * a.os[1] + t * a.os[2] + sub * 8), o);
-    unpack<T>(ld_stream(dout + s * b.dos[0] + head * b.dos[1] + t * b.dos[2] + sub * 8), g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc = fmaf(o[i], g[i], acc);
-  }
-#pragma unroll
-  for (int off = TPR / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-  if (row < total && sub == 0) {
-    nlse2[row] = live ? -lse[(s * a.H + head) * a.tokens + t] * LOG2E : -INFINITY;
-    ndelta[row] = -acc;
   }
 }
 
@@ -652,7 +725,8 @@ int optin(Kernel kern, int bytes, std::atomic<unsigned long long>& done) {
 
 bool local_bwd_tc_supported(const LocalBwdArgs& b, int dtype, const void* q, const void* k, const void* v, const void* out,
                             const void* dout, const void* dq, const void* dk, const void* dv) {
-  return local_tc_supported(b.f, dtype, q, k, v, out) && local_rows_ok(dout, b.dos, b.f) && local_rows_ok(dq, b.dqs, b.f) &&
+  return (int64_t)b.f.n * b.f.KV * ceil_div(b.f.tokens, LOCAL_TC_TILE / b.f.G) < (1ll << 31) - (1 << 20) &&
+         local_tc_supported(b.f, dtype, q, k, v, out) && local_rows_ok(dout, b.dos, b.f) && local_rows_ok(dq, b.dqs, b.f) &&
          local_keys_ok(dk, b.dks, b.f) && local_keys_ok(dv, b.dvs, b.f);
 }
 
@@ -660,40 +734,45 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
                         const void* out, const float* lse, float* row_scratch, const LocalBwdArgs& b, int dtype,
                         cudaStream_t st) {
   const LocalArgs& a = b.f;
-  CUtensorMap mq, md, mk, mv;
-  if (!local_map_rows(&mq, q, a.qs, a, "q") || !local_map_rows(&md, dout, b.dos, a, "dout") ||
-      !local_map_keys(&mk, k, a.ks, a, TILE, "k") || !local_map_keys(&mv, v, a.vs, a, TILE, "v"))
+  const int col_tokens = COLS / a.G;
+  CUtensorMap mq, md, mk, mv, mdq;
+  if (!local_map_rows(&mq, q, a.qs, a, col_tokens, "q") || !local_map_rows(&md, dout, b.dos, a, col_tokens, "dout") ||
+      !local_map_rows(&mdq, dq, b.dqs, a, TILE / a.G, "dq") || !local_map_keys(&mk, k, a.ks, a, TILE, "k") ||
+      !local_map_keys(&mv, v, a.vs, a, TILE, "v"))
     return TB200_ERR_UNSUPPORTED;
-  const int64_t rows = local_tc_rows(a);
   BwdParams p;
   p.b = b;
-  p.dq = dq;
   p.dk = dk;
   p.dv = dv;
+  p.q = q;
+  p.out = out;
+  p.dout = dout;
+  p.lse = lse;
   p.nlse2 = row_scratch;
-  p.ndelta = row_scratch + rows;
+  p.ndelta = row_scratch + local_tc_rows(a);
   p.scale_log2 = a.scale * LOG2E;
   p.tile_tokens = TILE / a.G;
-  p.query_tiles = (int)ceil_div(a.tokens, p.tile_tokens);
+  p.row_tiles = (int)ceil_div(a.tokens, p.tile_tokens);
+  p.col_tokens = col_tokens;
+  p.col_tiles = (int)ceil_div(a.tokens, col_tokens);
   p.key_tiles = (int)ceil_div(a.tokens, TILE);
   p.status = device_status_ptr();
   auto go = [&](auto tag, auto dsel) -> int {
     using T = decltype(tag);
     constexpr int D = decltype(dsel)::value;
-    constexpr int DKV_SMEM = 6 * TILE * D * 2 + 2048 + 256 + 1024, DQ_SMEM = 6 * TILE * D * 2 + 256 + 1024;
-    static_assert(DKV_SMEM <= 227 * 1024, "shared memory of one CTA");
+    constexpr int DKV_SMEM = 2 * TILE * D * 2 + 6 * COLS * D * 2 + 6 * COLS * 4 + 256 + 1024;
+    constexpr int DQ_SMEM = 7 * TILE * D * 2 + TILE * 4 + 256 + 1024;
+    static_assert(DKV_SMEM <= 227 * 1024 && DQ_SMEM <= 227 * 1024, "shared memory of one CTA");
     auto kkv = local_dkv_tc_kernel<T, D>;
     auto kq = local_dq_tc_kernel<T, D>;
     static std::atomic<unsigned long long> done_kv{0}, done_q{0};
     if (int rc = optin(kkv, DKV_SMEM, done_kv)) return rc;
     if (int rc = optin(kq, DQ_SMEM, done_q)) return rc;
-    local_bwd_prep<T, D><<<(unsigned)ceil_div(rows, 256 / (D / 8)), 256, 0, st>>>(
-        row_scratch, row_scratch + rows, (const T*)out, (const T*)dout, lse, b, p.tile_tokens, p.query_tiles);
-    if (int rc = launch_status("local_bwd_prep")) return rc;
+    const int64_t units = (int64_t)a.n * a.KV * p.row_tiles;
+    kq<<<(unsigned)(units < sm_count() ? units : sm_count()), THREADS, DQ_SMEM, st>>>(mdq, mk, mv, p);
+    if (int rc = launch_status("local_dq_tc")) return rc;
     kkv<<<dim3((unsigned)(p.key_tiles + b.sink_tiles * b.far), (unsigned)a.KV, (unsigned)a.n), THREADS, DKV_SMEM, st>>>(mq, md, mk, mv, p);
-    if (int rc = launch_status("local_dkv_tc")) return rc;
-    kq<<<dim3((unsigned)p.query_tiles, (unsigned)a.KV, (unsigned)a.n), THREADS, DQ_SMEM, st>>>(mq, md, mk, mv, p);
-    return launch_status("local_dq_tc");
+    return launch_status("local_dkv_tc");
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

@@ -250,9 +250,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       __syncwarp();
     } else if (warp == 1) {
       // -------------------------------------------------------------- MMA issuer
+      // The whole warp walks the loop and waits; one elected lane issues. (With the waits in the elected lane
+      // alone, a commit was seen to take effect only after that lane's next wait had given up.)
       const bool elected = ptx::elect_one();
       auto wait_ = [&](uint64_t* bar, uint32_t parity, int code) {
-        if (elected) ptx::mbar_wait(bar, parity, abort_flag, a.status, code);
+        ptx::mbar_wait(bar, parity, abort_flag, a.status, code);
         __syncwarp();
       };
       auto commit_ = [&](uint64_t* bar) {
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       }
       // everything issued has completed before tensor memory is freed
       commit_(mma_drained);
-      if (elected) ptx::mbar_wait_drain(mma_drained, 0, abort_flag, a.status, 79);
+      ptx::mbar_wait_drain(mma_drained, 0, abort_flag, a.status, 79);
       __syncwarp();
     } else if (PAGED && warp == 3 && fix) {
       // -------------------------------------------------------------- zeros behind the sequence's end
@@ -609,14 +611,14 @@ bool stride_ok(int64_t st, int64_t extent) { return extent <= 1 || (st > 0 && st
 }  // namespace
 
 // packed rows of q (or a tensor laid out like it): [features, head of the group, token, key head, sequence],
-// box of one query tile
-bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, const char* what) {
+// box of `tokens` tokens of one key head
+bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, int tokens, const char* what) {
   const bool paged = a.table != nullptr;
   const cuuint64_t dims[5] = {(cuuint64_t)a.D, (cuuint64_t)a.G, (cuuint64_t)a.tokens, (cuuint64_t)a.KV,
                               (cuuint64_t)(paged ? 1 : a.n)};
   const cuuint64_t strides[4] = {stride_of(st[1], a.G), stride_of(st[2], a.tokens), stride_of(st[1] * a.G, a.KV),
                                  stride_of(st[0], paged ? 1 : a.n)};
-  const cuuint32_t box[5] = {64, (cuuint32_t)a.G, (cuuint32_t)(LOCAL_TC_TILE / a.G), 1, 1};
+  const cuuint32_t box[5] = {64, (cuuint32_t)a.G, (cuuint32_t)tokens, 1, 1};
   return encode(map, 5, q, dims, strides, box, what);
 }
 // keys (or values): [features, position (of a page), key head, sequence or page], box of one piece
@@ -694,7 +696,7 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   p.reverse = a.window == NO_WINDOW;
   p.wait_units = ptx::WAIT_LIMIT_UNITS;
   CUtensorMap mq, mk, mv;
-  if (!local_map_rows(&mq, q, a.qs, a, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
+  if (!local_map_rows(&mq, q, a.qs, a, p.tile_tokens, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
       !local_map_keys(&mv, v, a.vs, a, p.piece, "v"))
     return TB200_ERR_UNSUPPORTED;
   auto go = [&](auto tag, auto dsel) -> int {

@@ -7,6 +7,7 @@
 namespace tb200 {
 
 constexpr int LOCAL_TC_TILE = 128;  // packed query rows and keys of a tile
+constexpr int LOCAL_TC_COLS = 96;   // packed query rows of a step of the dK, dV kernel
 
 // What the tensor-core kernels take: 16-bit operands, head size 64 or 128, unit feature strides, other
 // strides multiples of 16 bytes, and (serving form) a page size that shares a factor of at least 8 with 128.
@@ -14,7 +15,8 @@ bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void
 int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, const void* v, const LocalArgs& a, int max_q,
                         int dtype, cudaStream_t st);
 // Tensor maps (false with the error text set when the driver refuses one) and what they take.
-bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, const char* what);
+// (rows: boxes of `tokens` tokens with the heads of a group)
+bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, int tokens, const char* what);
 bool local_map_keys(CUtensorMap* map, const void* k, const int64_t* st, const LocalArgs& a, int piece, const char* what);
 bool local_rows_ok(const void* p, const int64_t* st, const LocalArgs& a);
 bool local_keys_ok(const void* p, const int64_t* st, const LocalArgs& a);
@@ -25,9 +27,9 @@ bool local_bwd_tc_supported(const LocalBwdArgs& b, int dtype, const void* q, con
 int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k, const void* v,
                         const void* out, const float* lse, float* row_scratch, const LocalBwdArgs& b, int dtype,
                         cudaStream_t st);
-// packed rows of all query tiles, unused ones included
+// packed rows of all column tiles, unused ones included
 static inline int64_t local_tc_rows(const LocalArgs& a) {
-  return (int64_t)a.n * a.KV * ceil_div(a.tokens, LOCAL_TC_TILE / a.G) * LOCAL_TC_TILE;
+  return (int64_t)a.n * a.KV * ceil_div(a.tokens, LOCAL_TC_COLS / a.G) * LOCAL_TC_COLS;
 }
 // tokens of the two query tiles of a CTA
 static inline int local_tc_row_tokens(const LocalArgs& a) { return 2 * (LOCAL_TC_TILE / a.G); }

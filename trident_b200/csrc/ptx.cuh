@@ -105,6 +105,16 @@ __device__ inline void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint6
       ::"r"(smem_u32(smem_dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// Tiled bulk store shared -> global (elements outside the tensor are left out), and the waits of the
+// issuing thread: until the shared memory has been read, until the writes are done.
+__device__ inline void tma_store_5d(const CUtensorMap* map, const void* smem_src, int x, int y, int z, int w, int u) {
+  asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];" ::"l"(map),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u)
+               : "memory");
+}
+__device__ inline void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ inline void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ inline void bulk_wait_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // L2 eviction priorities for bulk tensor loads: a tile that only one CTA ever reads (its own Q
 // tiles in the attention forward, its K/V tile in the backward) is marked as the first to go.
 __device__ inline uint64_t l2_policy_evict_first() {
@@ -222,6 +232,11 @@ __device__ inline void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
         "r"(taddr)
       : "memory");
+}
+__device__ inline void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+               : "memory");
 }
 __device__ inline void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
