@@ -10,8 +10,8 @@
 //           took the pipe 120 cycles an instruction instead of 64); along the keys of the tile's walk
 //             S = Q K^T, dP = dO V^T, P = exp2(S scale log2e - lse log2e), dS = P (dP - delta), dQ += dS K
 //           (dS 16-bit in tensor memory over dP). S(i+1) is computed as soon as S(i) is in registers, dP(i+1)
-//           after dQ(i), so that exponentials and score gradients follow each other without a pause. The
-//           threads that load dO also compute delta = sum_d out dout, for themselves and for the other kernel.
+//           after dQ(i), so that exponentials and score gradients follow each other without a pause. Two
+//           more warps compute delta = sum_d out dout of the next tile, also for the other kernel.
 //   dK, dV  a CTA owns 128 keys (K_j, V_j resident in shared memory) and walks the tiles of 96 packed query
 //           rows that see any of them; the sum over the heads of a group is part of the walk. All
 //           transposed, keys on the tensor-memory lanes:
@@ -42,7 +42,6 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct BwdParams {
   LocalBwdArgs b;
   void *dk, *dv;
-  const void *q, *out, *dout;
   const float* lse;
   float* nlse2;         // [n * KV][column tiles][96]  -lse * log2(e), written by the dQ kernel for the other
   float* ndelta;        // [n * KV][column tiles][96]  -delta
@@ -73,7 +72,7 @@ __device__ inline void bulk_load(void* dst, const void* src, uint32_t bytes, uin
                : "memory");
 }
 // the lowest n bits
-__device__ inline uint64_t low_bits64(int n) { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull); }
+__device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 __device__ inline int saturate(int64_t v) { return v < -(1 << 20) ? -(1 << 20) : (v > (1 << 20) ? (1 << 20) : (int)v); }
 // Rows [rows, 96) of `boxes` swizzled boxes set to zero (rows that no copy writes, but products read).
 __device__ inline void zero_rows(uint8_t* smem, int boxes, int rows) {
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t s_addr = tmem_base + lane_off + COL_S + half * HALF, dp_addr = tmem_base + lane_off + COL_DP + half * HALF;
     const uint32_t p_addr = tmem_base + lane_off + COL_P + half * (HALF / 2);
     const uint64_t scale2 = am::pack2f(p.scale_log2, p.scale_log2);
-    const uint64_t always = key < a.sinks ? ~0ull : 0ull;
+    const uint32_t always = key < a.sinks ? 0xffffffffu : 0u;
     for (int i = 0; i < steps; ++i) {
       const int st = i % STAGES, it = i0 + i;
       const int token0 = it * p.col_tokens, token1 = token0 + p.col_tokens - 1;
@@ -301,10 +300,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         // columns from `low` on are not before the key, those below `high` are within its window
         const int low = saturate((int64_t)(key - token0) * a.G) - half * HALF;
         const int high = saturate(((int64_t)key + a.window - token0) * a.G) - half * HALF;
-        const uint64_t seen = ~low_bits64(low) & (low_bits64(high) | always);
 #pragma unroll
-        for (int e = 0; e < HALF; ++e)
-          if (!((seen >> e) & 1u)) pr[e] = 0.f;
+        for (int q = 0; q < HALF; q += 32) {
+          const uint32_t seen = ~low_bits(low - q) & (low_bits(high - q) | always);
+#pragma unroll
+          for (int e = 0; e < 32 && q + e < HALF; ++e)
+            if (!(seen & (1u << e))) pr[q + e] = 0.f;
+        }
       }
       {
         uint32_t pa[16], pb[8];
@@ -396,45 +398,54 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // ------------------------------------------------------------------ dQ
+// warp 0: producer (rings of two K and two V tiles across all tiles of the CTA; Q, dO and out of the next tile
+// land in shared memory during this one); warp 1: MMA issuer; warps 2, 3: -lse log2e and -delta of the next
+// tile's rows, also for the other kernel; warps 4-11: compute.
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
-    local_dq_tc_kernel(const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const BwdParams p) {
-  constexpr int STAGES = 3;
+    local_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                       const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_dq,
+                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const BwdParams p) {
   constexpr int TILE_BYTES = TILE * D * 2, NBOX = D / 64, BOX_BYTES = TILE * 128;
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t IDESC_S = ptx::make_idesc(IS_BF16, false, false, TILE, TILE);
   constexpr uint32_t IDESC_D = ptx::make_idesc(IS_BF16, false, true, TILE, D);
   constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256, COL_Q = 384, COL_DO = 448;
 
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* k_smem = smem;                             // [STAGES]
-  uint8_t* v_smem = smem + STAGES * TILE_BYTES;       // [STAGES]
-  uint8_t* stage_smem = smem + 2 * STAGES * TILE_BYTES;  // dQ tile on its way out
-  float* delta_smem = reinterpret_cast<float*>(stage_smem + TILE_BYTES);  // [128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(delta_smem + TILE);
-  uint64_t* k_full = bars;                 // [STAGES]
-  uint64_t* v_full = bars + STAGES;        // [STAGES]
-  uint64_t* kv_empty = bars + 2 * STAGES;  // [STAGES]
-  // Per step (g counts the steps of all tiles of this CTA): parity g & 1. Per tile (u): parity u & 1.
-  uint64_t* s_ready = bars + 3 * STAGES;   // S(g) computed
-  uint64_t* dp_ready = s_ready + 1;        // dP(g) computed
-  uint64_t* tile_done = s_ready + 2;       // all products of tile u done
-  uint64_t* s_free = s_ready + 3;          // S(g) read               (256 arrivals)
-  uint64_t* ds_ready = s_ready + 4;        // dS(g) written over dP(g) (256 arrivals)
-  uint64_t* q_ready = s_ready + 5;         // Q, dO of tile u in tensor memory, dQ of tile u - 1 read (256 arrivals)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_ready + 6);
+  // (at D = 128 the tiles leave 3 KB: the window starts at the CTA's shared memory, checked below)
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* k_smem = smem;                     // [2]
+  uint8_t* v_smem = smem + 2 * TILE_BYTES;    // [2]
+  uint8_t* land_smem = smem + 4 * TILE_BYTES; // Q, dO of the next tile
+  uint8_t* out_smem = smem + 6 * TILE_BYTES;  // dQ of the last tile on its way out, then out of the next one
+  float* stats = reinterpret_cast<float*>(smem + 7 * TILE_BYTES);  // [2][nlse, ndelta][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + 4 * TILE);
+  // Per step (g counts the steps of all tiles of this CTA), per tile (u): parity of g or u; rings: of g / 2.
+  uint64_t* k_full = bars;           // [2]
+  uint64_t* k_empty = bars + 2;      // [2] dQ(g) done
+  uint64_t* v_full = bars + 4;       // [2]
+  uint64_t* v_empty = bars + 6;      // [2] dP(g) done
+  uint64_t* land_full = bars + 8;    // Q, dO of tile u have landed
+  uint64_t* s_ready = bars + 9;      // S(g) computed
+  uint64_t* dp_ready = bars + 10;    // dP(g) computed
+  uint64_t* tile_done = bars + 11;   // all products of tile u done
+  uint64_t* s_free = bars + 12;      // S(g) read                (256 arrivals)
+  uint64_t* ds_ready = bars + 13;    // dS(g) written over dP(g) (256 arrivals)
+  uint64_t* q_ready = bars + 14;     // Q, dO of tile u in tensor memory, dQ of tile u - 1 read (256 arrivals)
+  uint64_t* stats_empty = bars + 15; // [2] (256 arrivals)
+  uint64_t* stats_full = bars + 17;  // [2] (64 arrivals)
+  uint64_t* out_free = bars + 19;    // dQ of tile u - 1 has left shared memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const LocalArgs& a = p.b.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = a.n * a.KV * p.row_tiles;
-  // tile `unit`: longest walks (last tokens) of a sequence and key head first
   struct Unit {
     int s, hk, t0, ntok;
-    KeyRange kr;
   };
+  // tile `unit`: longest walks (last tokens) of a sequence and key head first
   auto unit_at = [&](int unit) {
     Unit w;
     const int sh = unit / p.row_tiles, it = p.row_tiles - 1 - unit % p.row_tiles;
@@ -442,21 +453,30 @@ __global__ void __launch_bounds__(THREADS, 1)
     w.hk = sh % a.KV;
     w.t0 = it * p.tile_tokens;
     w.ntok = min(p.tile_tokens, a.tokens - w.t0);
-    w.kr = key_range(a, w.t0, w.t0 + w.ntok - 1, a.tokens, TILE);  // (at least one tile: a query sees itself)
     return w;
   };
+  // (at least one key tile: a query sees itself)
+  auto walk_of = [&](const Unit& w) { return key_range(a, w.t0, w.t0 + w.ntok - 1, a.tokens, TILE); };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 3 * STAGES + 3; ++i) ptx::mbar_init(&bars[i], 1);
-    for (int i = 0; i < 3; ++i) ptx::mbar_init(s_free + i, 256);
+    for (int i = 0; i < 12; ++i) ptx::mbar_init(&bars[i], 1);
+    for (int i = 12; i < 17; ++i) ptx::mbar_init(&bars[i], 256);
+    for (int i = 17; i < 19; ++i) ptx::mbar_init(&bars[i], 64);
+    ptx::mbar_init(out_free, 1);
     abort_flag[0] = 0;
     abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
+    if ((ptx::smem_u32(smem) & 1023u) != 0) {  // swizzled tiles need a 1024-byte aligned base
+      abort_flag[0] = 1;
+      atomicCAS(p.status, 0, 120);
+    }
     ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&map_q);
+    ptx::prefetch_tensormap(&map_do);
     ptx::prefetch_tensormap(&map_dq);
     ptx::prefetch_tensormap(&map_k);
     ptx::prefetch_tensormap(&map_v);
   }
-  if (warp == 2) {
+  if (warp == 1) {
     ptx::tmem_alloc(tmem_slot, TMEM_COLS);
     ptx::tmem_relinquish();
   }
@@ -467,24 +487,45 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int g = 0;
-      for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+      auto land = [&](int unit) {
         const Unit w = unit_at(unit);
-        for (int i = 0; i < w.kr.count; ++i, ++g) {
-          const int st = g % STAGES, j0 = w.kr.tile(i) * TILE;
-          ptx::mbar_wait(&kv_empty[st], ((g / STAGES) & 1) ^ 1, abort_flag, p.status, 121);
+        ptx::mbar_expect_tx(land_full, 3 * NBOX * p.tile_tokens * a.G * 128);
+#pragma unroll
+        for (int c = 0; c < NBOX; ++c) {
+          tma_load_5d(land_smem + c * BOX_BYTES, &map_q, land_full, c * 64, 0, w.t0, w.hk, w.s);
+          tma_load_5d(land_smem + TILE_BYTES + c * BOX_BYTES, &map_do, land_full, c * 64, 0, w.t0, w.hk, w.s);
+          tma_load_5d(out_smem + c * BOX_BYTES, &map_out, land_full, c * 64, 0, w.t0, w.hk, w.s);
+        }
+      };
+      int g = 0, u = 0;
+      land(blockIdx.x);
+      for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
+        const Unit w = unit_at(unit);
+        const KeyRange kr = walk_of(w);
+        for (int i = 0; i < kr.count; ++i, ++g) {
+          const int st = g & 1, j0 = kr.tile(i) * TILE;
+          ptx::mbar_wait(&k_empty[st], ((g >> 1) & 1) ^ 1, abort_flag, p.status, 121);
           ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
 #pragma unroll
           for (int c = 0; c < NBOX; ++c) tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES, &map_k, &k_full[st], c * 64, j0, w.hk, w.s);
+          ptx::mbar_wait(&v_empty[st], ((g >> 1) & 1) ^ 1, abort_flag, p.status, 122);
           ptx::mbar_expect_tx(&v_full[st], TILE_BYTES);
 #pragma unroll
           for (int c = 0; c < NBOX; ++c) tma_load_4d(v_smem + st * TILE_BYTES + c * BOX_BYTES, &map_v, &v_full[st], c * 64, j0, w.hk, w.s);
+          // the next tile's rows, once this tile's have been taken out (after the copies that are needed first)
+          if (i == min(1, kr.count - 1) && unit + (int)gridDim.x < units) {
+            ptx::mbar_wait(q_ready, u & 1, abort_flag, p.status, 123);
+            ptx::mbar_wait(&stats_full[u & 1], (u >> 1) & 1, abort_flag, p.status, 123);
+            ptx::mbar_wait(out_free, u & 1, abort_flag, p.status, 123);
+            land(unit + gridDim.x);
+          }
         }
       }
       // every copy has landed before the CTA gives up its shared memory
-      for (int i = g > STAGES ? g - STAGES : 0; i < g; ++i) {
-        ptx::mbar_wait_drain(&k_full[i % STAGES], (i / STAGES) & 1, abort_flag, p.status, 122);
-        ptx::mbar_wait_drain(&v_full[i % STAGES], (i / STAGES) & 1, abort_flag, p.status, 122);
+      ptx::mbar_wait_drain(land_full, (u - 1) & 1, abort_flag, p.status, 124);
+      for (int i = g > 2 ? g - 2 : 0; i < g; ++i) {
+        ptx::mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 124);
+        ptx::mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 124);
       }
     }
     __syncwarp();
@@ -510,123 +551,146 @@ __global__ void __launch_bounds__(THREADS, 1)
                        IDESC_S, ks != 0);
     };
     auto scores_of = [&](int g) {
-      if (g > 0) wait_(s_free, (g - 1) & 1, 123);
-      wait_(&k_full[g % STAGES], (g / STAGES) & 1, 124);
+      if (g > 0) wait_(s_free, (g - 1) & 1, 125);
+      wait_(&k_full[g & 1], (g >> 1) & 1, 126);
       ptx::tc_fence_after();
-      score(COL_S, COL_Q, dk + (g % STAGES) * STAGE);
+      score(COL_S, COL_Q, dk + (g & 1) * STAGE);
       commit_(s_ready);
     };
     auto gradients_of = [&](int g) {  // (over dS(g-1), which dQ(g-1) reads first on the in-order pipe)
-      wait_(&v_full[g % STAGES], (g / STAGES) & 1, 125);
+      wait_(&v_full[g & 1], (g >> 1) & 1, 127);
       ptx::tc_fence_after();
-      score(COL_DP, COL_DO, dv + (g % STAGES) * STAGE);
+      score(COL_DP, COL_DO, dv + (g & 1) * STAGE);
       commit_(dp_ready);
+      commit_(&v_empty[g & 1]);
     };
     int g = 0, u = 0;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
-      const int steps = unit_at(unit).kr.count;
-      wait_(q_ready, u & 1, 126);
+      const int steps = walk_of(unit_at(unit)).count;
+      wait_(q_ready, u & 1, 128);
       ptx::tc_fence_after();
       scores_of(g);
       gradients_of(g);
       for (int i = 0; i < steps; ++i, ++g) {
         if (i + 1 < steps) scores_of(g + 1);
-        wait_(ds_ready, g & 1, 127);
+        wait_(ds_ready, g & 1, 129);
         ptx::tc_fence_after();
 #pragma unroll
         for (int ks = 0; ks < TILE / 16; ++ks)  // (a thread packs dS into the first half of its own 64 columns)
           if (elected)
             ptx::umma_ts(tmem_base + COL_DQ, tmem_base + COL_DP + (ks >> 2) * 64 + (ks & 3) * 8,
-                         dk_t + (g % STAGES) * STAGE + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_D, (i | ks) != 0);
-        commit_(&kv_empty[g % STAGES]);
+                         dk_t + (g & 1) * STAGE + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_D, (i | ks) != 0);
+        commit_(&k_empty[g & 1]);
         if (i + 1 < steps) gradients_of(g + 1);
       }
       commit_(tile_done);
     }
     // everything issued has completed before tensor memory is freed
-    if (u > 0) ptx::mbar_wait_drain(tile_done, (u - 1) & 1, abort_flag, p.status, 128);
+    ptx::mbar_wait_drain(tile_done, (u - 1) & 1, abort_flag, p.status, 130);
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    // -------------------------------------------------------------- -lse log2e, -delta
+    // entries of column tiles that belong to no row: zeros (the products that meet them see rows of zeros)
+    const int t = threadIdx.x - 64;
+    {
+      const int64_t tiles = (int64_t)a.n * a.KV * p.col_tiles;
+      for (int64_t i = (int64_t)blockIdx.x * 64 + t; i < tiles; i += (int64_t)gridDim.x * 64) {
+        const int left = a.tokens - (int)(i % p.col_tiles) * p.col_tokens;
+        for (int c = min(left, p.col_tokens) * a.G; c < COLS; ++c) p.nlse2[i * COLS + c] = p.ndelta[i * COLS + c] = 0.f;
+      }
+    }
+    int u = 0;
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
+      const Unit w = unit_at(unit);
+      float nlse[2], ndelta[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // rows t and t + 64
+        const int r = t + 64 * i;
+        nlse[i] = r < w.ntok * a.G ? -p.lse[((int64_t)w.s * a.H + w.hk * a.G + r % a.G) * a.tokens + w.t0 + r / a.G] * LOG2E : 0.f;
+      }
+      ptx::mbar_wait(land_full, u & 1, abort_flag, p.status, 131);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = t + 64 * i;
+        float acc = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          const int at = (c >> 3) * BOX_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          float x[8], y[8];
+          unpack<T>(*reinterpret_cast<const uint4*>(out_smem + at), x);
+          unpack<T>(*reinterpret_cast<const uint4*>(land_smem + TILE_BYTES + at), y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc = fmaf(x[e], y[e], acc);
+        }
+        ndelta[i] = -acc;
+      }
+      ptx::mbar_wait(&stats_empty[u & 1], ((u >> 1) & 1) ^ 1, abort_flag, p.status, 131);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = t + 64 * i;
+        stats[(u & 1) * 2 * TILE + r] = nlse[i];
+        stats[((u & 1) * 2 + 1) * TILE + r] = ndelta[i];
+        if (r < w.ntok * a.G) {
+          const int pos = w.t0 + r / a.G;
+          const int64_t at = (((int64_t)w.s * a.KV + w.hk) * p.col_tiles + pos / p.col_tokens) * COLS + (pos % p.col_tokens) * a.G + r % a.G;
+          p.nlse2[at] = nlse[i];
+          p.ndelta[at] = ndelta[i];
+        }
+      }
+      ptx::fence_proxy_async_smem();  // (the landing zone is next written by copies)
+      ptx::mbar_arrive(&stats_full[u & 1]);
+    }
+  } else {
+    // -------------------------------------------------------------- compute
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
-    const int group = r % a.G, row_token = r / a.G;
+    const int row_token = r / a.G;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + COL_S + half * 64, dp_addr = tmem_base + lane_off + COL_DP + half * 64;
     const uint64_t scale2 = am::pack2f(p.scale_log2, p.scale_log2);
-    // entries of column tiles that belong to no row: zeros (the products that meet them see rows of zeros)
-    {
-      const int64_t tiles = (int64_t)a.n * a.KV * p.col_tiles;
-      for (int64_t t = (int64_t)blockIdx.x * 256 + (threadIdx.x - 128); t < tiles; t += (int64_t)gridDim.x * 256) {
-        const int left = a.tokens - (int)(t % p.col_tiles) * p.col_tokens;
-        for (int c = min(left, p.col_tokens) * a.G; c < COLS; ++c) p.nlse2[t * COLS + c] = p.ndelta[t * COLS + c] = 0.f;
-      }
-    }
-    // half 0 brings the rows of Q, half 1 those of dO
-    uint4 raw[D / 8];
-    auto fetch = [&](const Unit& w) {
-      const bool live = r < w.ntok * a.G;
-      const int64_t* st = half ? p.b.dos : a.qs;
-      const T* src = reinterpret_cast<const T*>(half ? p.dout : p.q) + (int64_t)w.s * st[0] + (int64_t)(w.hk * a.G + group) * st[1] +
-                     (int64_t)(w.t0 + row_token) * st[2];
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) raw[c] = live ? ld_stream(src + c * 8) : make_uint4(0, 0, 0, 0);
-    };
     int g = 0, u = 0;
-    if ((int)blockIdx.x < units) fetch(unit_at(blockIdx.x));
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
       const Unit w = unit_at(unit);
+      const KeyRange kr = walk_of(w);
       const bool live = r < w.ntok * a.G;
-      const int pos = live ? w.t0 + row_token : -1, head = w.hk * a.G + group;
-      // rows into tensor memory (the products that read the previous tile's are done: tile_done)
+      const int pos = live ? w.t0 + row_token : -1;
+      // half 0 puts the rows of Q into tensor memory, half 1 those of dO (the products that read the
+      // previous tile's are done: tile_done)
+      ptx::mbar_wait(land_full, u & 1, abort_flag, p.status, 132);
+      {
+        const uint8_t* src = land_smem + half * TILE_BYTES + r * 128;
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t v[32];
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t v[32];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e * 4] = raw[c * 8 + e].x;
-          v[e * 4 + 1] = raw[c * 8 + e].y;
-          v[e * 4 + 2] = raw[c * 8 + e].z;
-          v[e * 4 + 3] = raw[c * 8 + e].w;
-        }
-        ptx::tmem_st32(tmem_base + lane_off + (half ? COL_DO : COL_Q) + c * 32, v);
-      }
-      ptx::tmem_st_wait();
-      ptx::tc_fence_before();
-      ptx::mbar_arrive(q_ready);
-      const float nlse = live ? -p.lse[((int64_t)w.s * a.H + head) * a.tokens + pos] * LOG2E : 0.f;
-      float ndelta = 0.f;
-      if (half) {
-        const T* src = reinterpret_cast<const T*>(p.out) + (int64_t)w.s * a.os[0] + (int64_t)head * a.os[1] + (int64_t)pos * a.os[2];
-#pragma unroll
-        for (int c = 0; c < D / 8; c += 4) {
-          uint4 o[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = live ? ld_stream(src + (c + e) * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x[8], y[8];
-            unpack<T>(o[e], x);
-            unpack<T>(raw[c + e], y);
-#pragma unroll
-            for (int f = 0; f < 8; ++f) ndelta = fmaf(x[f], -y[f], ndelta);
+          for (int e = 0; e < 8; ++e) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + c * BOX_BYTES + ((e ^ (r & 7)) << 4));
+            v[e * 4] = x.x;
+            v[e * 4 + 1] = x.y;
+            v[e * 4 + 2] = x.z;
+            v[e * 4 + 3] = x.w;
           }
+          ptx::tmem_st32(tmem_base + lane_off + (half ? COL_DO : COL_Q) + c * 32, v);
         }
-        delta_smem[r] = ndelta;
-        if (live) {
-          const int64_t at = (((int64_t)w.s * a.KV + w.hk) * p.col_tiles + pos / p.col_tokens) * COLS + (pos % p.col_tokens) * a.G + group;
-          p.nlse2[at] = nlse;
-          p.ndelta[at] = ndelta;
-        }
+        ptx::tmem_st_wait();
+        ptx::fence_proxy_async_smem();  // (the landing zone is next written by copies)
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(q_ready);
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      ndelta = delta_smem[r];
+      if (threadIdx.x == 128) {
+        ptx::bulk_wait_read();
+        ptx::mbar_arrive(out_free);
+      }
+      ptx::mbar_wait(&stats_full[u & 1], (u >> 1) & 1, abort_flag, p.status, 133);
+      const float nlse = stats[(u & 1) * 2 * TILE + r], ndelta = stats[((u & 1) * 2 + 1) * TILE + r];
+      ptx::mbar_arrive(&stats_empty[u & 1]);
       const uint64_t nlse_2 = am::pack2f(nlse, nlse), ndelta_2 = am::pack2f(ndelta, ndelta);
-      for (int i = 0; i < w.kr.count; ++i, ++g) {
-        const int j0 = w.kr.tile(i) * TILE;
+      for (int i = 0; i < kr.count; ++i, ++g) {
+        const int j0 = kr.tile(i) * TILE;
         const bool plain = j0 + TILE - 1 <= w.t0 && (w.t0 + w.ntok - 1 - j0 < a.window || j0 + TILE <= a.sinks);
         float pr[64];
         uint32_t ra[32], rb[32];
-        ptx::mbar_wait(s_ready, g & 1, abort_flag, p.status, 129);
+        ptx::mbar_wait(s_ready, g & 1, abort_flag, p.status, 134);
         ptx::tc_fence_after();
         ptx::tmem_ld32(s_addr, ra);
         ptx::tmem_ld32(s_addr + 32, rb);
@@ -634,22 +698,41 @@ __global__ void __launch_bounds__(THREADS, 1)
         am::tmem_ld_wait_dep(rb);
         ptx::tc_fence_before();
         ptx::mbar_arrive(s_free);
+        if (plain) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          am::unpack2f(am::fma2(am::pack2u(ra[e], ra[e + 1]), scale2, nlse_2), pr[e], pr[e + 1]);
-          am::unpack2f(am::fma2(am::pack2u(rb[e], rb[e + 1]), scale2, nlse_2), pr[32 + e], pr[33 + e]);
+          for (int e = 0; e < 32; e += 2) {
+            am::unpack2f(am::fma2(am::pack2u(ra[e], ra[e + 1]), scale2, nlse_2), pr[e], pr[e + 1]);
+            am::unpack2f(am::fma2(am::pack2u(rb[e], rb[e + 1]), scale2, nlse_2), pr[32 + e], pr[33 + e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 64; ++e) pr[e] = am::ex2(pr[e]);
+        } else {
+          // by blocks of 32 columns: those that no row sees cost nothing, those that all rows see no mask
+          auto block = [&](const uint32_t (&v)[32], int q) {
+            const int b0 = j0 + half * 64 + 32 * q, last = w.t0 + w.ntok - 1;
+            const bool none = b0 > last || (w.t0 - (b0 + 31) >= a.window && b0 >= a.sinks);
+            const bool all = b0 + 31 <= w.t0 && (last - b0 < a.window || b0 + 32 <= a.sinks);
+            if (none) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) pr[q * 32 + e] = 0.f;
+              return;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              am::unpack2f(am::fma2(am::pack2u(v[e], v[e + 1]), scale2, nlse_2), pr[q * 32 + e], pr[q * 32 + e + 1]);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pr[q * 32 + e] = am::ex2(pr[q * 32 + e]);
+            if (all) return;
+            // columns below pos + 1 - b0 are not in the future, those from pos - window + 1 - b0 on in the window
+            const uint32_t seen = low_bits(pos + 1 - b0) & (~low_bits(saturate((int64_t)pos - a.window + 1 - b0)) | low_bits(a.sinks - b0));
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen & (1u << e))) pr[q * 32 + e] = 0.f;
+          };
+          block(ra, 0);
+          block(rb, 1);
         }
-#pragma unroll
-        for (int e = 0; e < 64; ++e) pr[e] = am::ex2(pr[e]);
-        if (!plain) {
-          const int high = pos - j0 + 1 - half * 64;  // columns below `high` are not in the future
-          const int low = saturate((int64_t)pos - a.window + 1 - j0) - half * 64, sink = a.sinks - j0 - half * 64;
-          const uint64_t seen = low_bits64(high) & (~low_bits64(low) | low_bits64(sink));
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (!((seen >> e) & 1u)) pr[e] = 0.f;
-        }
-        ptx::mbar_wait(dp_ready, g & 1, abort_flag, p.status, 130);
+        ptx::mbar_wait(dp_ready, g & 1, abort_flag, p.status, 135);
         ptx::tc_fence_after();
         ptx::tmem_ld32(dp_addr, ra);
         ptx::tmem_ld32(dp_addr + 32, rb);
@@ -669,14 +752,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         ptx::tc_fence_before();
         ptx::mbar_arrive(ds_ready);
       }
-      // the next tile's rows are requested while this one's last products run
-      if (unit + (int)gridDim.x < units) fetch(unit_at(unit + gridDim.x));
-      // dQ out, through shared memory (its previous tile's copy has been read): each half of the warps
-      // takes half of the features
-      if (threadIdx.x == 128) ptx::bulk_wait_read();
-      ptx::mbar_wait(tile_done, u & 1, abort_flag, p.status, 131);
+      // dQ out through shared memory, where `out` of the next tile has been read (its statistics are there):
+      // each half of the warps takes half of the features
+      if (unit + (int)gridDim.x < units)
+        ptx::mbar_wait(&stats_full[(u + 1) & 1], ((u + 1) >> 1) & 1, abort_flag, p.status, 137);
+      ptx::mbar_wait(tile_done, u & 1, abort_flag, p.status, 136);
       ptx::tc_fence_after();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         uint32_t v[32];
@@ -691,7 +772,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           o.z = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 4]) * a.scale, __uint_as_float(v[e * 8 + 5]) * a.scale);
           o.w = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 6]) * a.scale, __uint_as_float(v[e * 8 + 7]) * a.scale);
           const int chunk = chunk0 + e;
-          *reinterpret_cast<uint4*>(stage_smem + (chunk >> 3) * BOX_BYTES + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = o;
+          *reinterpret_cast<uint4*>(out_smem + (chunk >> 3) * BOX_BYTES + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = o;
         }
       }
       ptx::tc_fence_before();
@@ -699,7 +780,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (threadIdx.x == 128) {
 #pragma unroll
-        for (int c = 0; c < NBOX; ++c) ptx::tma_store_5d(&map_dq, stage_smem + c * BOX_BYTES, c * 64, 0, w.t0, w.hk, w.s);
+        for (int c = 0; c < NBOX; ++c) ptx::tma_store_5d(&map_dq, out_smem + c * BOX_BYTES, c * 64, 0, w.t0, w.hk, w.s);
         ptx::bulk_commit();
       }
     }
@@ -707,7 +788,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == 2) {
+  if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem_base, TMEM_COLS);
   }
@@ -735,8 +816,10 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
                         cudaStream_t st) {
   const LocalArgs& a = b.f;
   const int col_tokens = COLS / a.G;
-  CUtensorMap mq, md, mk, mv, mdq;
+  CUtensorMap mq, md, mq128, md128, mo128, mk, mv, mdq;
   if (!local_map_rows(&mq, q, a.qs, a, col_tokens, "q") || !local_map_rows(&md, dout, b.dos, a, col_tokens, "dout") ||
+      !local_map_rows(&mq128, q, a.qs, a, TILE / a.G, "q") || !local_map_rows(&md128, dout, b.dos, a, TILE / a.G, "dout") ||
+      !local_map_rows(&mo128, out, a.os, a, TILE / a.G, "out") ||
       !local_map_rows(&mdq, dq, b.dqs, a, TILE / a.G, "dq") || !local_map_keys(&mk, k, a.ks, a, TILE, "k") ||
       !local_map_keys(&mv, v, a.vs, a, TILE, "v"))
     return TB200_ERR_UNSUPPORTED;
@@ -744,9 +827,6 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
   p.b = b;
   p.dk = dk;
   p.dv = dv;
-  p.q = q;
-  p.out = out;
-  p.dout = dout;
   p.lse = lse;
   p.nlse2 = row_scratch;
   p.ndelta = row_scratch + local_tc_rows(a);
@@ -761,7 +841,7 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
     using T = decltype(tag);
     constexpr int D = decltype(dsel)::value;
     constexpr int DKV_SMEM = 2 * TILE * D * 2 + 6 * COLS * D * 2 + 6 * COLS * 4 + 256 + 1024;
-    constexpr int DQ_SMEM = 7 * TILE * D * 2 + TILE * 4 + 256 + 1024;
+    constexpr int DQ_SMEM = 7 * TILE * D * 2 + 4 * TILE * 4 + 256;
     static_assert(DKV_SMEM <= 227 * 1024 && DQ_SMEM <= 227 * 1024, "shared memory of one CTA");
     auto kkv = local_dkv_tc_kernel<T, D>;
     auto kq = local_dq_tc_kernel<T, D>;
@@ -769,7 +849,7 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
     if (int rc = optin(kkv, DKV_SMEM, done_kv)) return rc;
     if (int rc = optin(kq, DQ_SMEM, done_q)) return rc;
     const int64_t units = (int64_t)a.n * a.KV * p.row_tiles;
-    kq<<<(unsigned)(units < sm_count() ? units : sm_count()), THREADS, DQ_SMEM, st>>>(mdq, mk, mv, p);
+    kq<<<(unsigned)(units < sm_count() ? units : sm_count()), THREADS, DQ_SMEM, st>>>(mq128, md128, mo128, mdq, mk, mv, p);
     if (int rc = launch_status("local_dq_tc")) return rc;
     kkv<<<dim3((unsigned)(p.key_tiles + b.sink_tiles * b.far), (unsigned)a.KV, (unsigned)a.n), THREADS, DKV_SMEM, st>>>(mq, md, mk, mv, p);
     return launch_status("local_dkv_tc");
