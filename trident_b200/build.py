@@ -28,6 +28,7 @@ SOURCES = [
     "local_attention_simt.cu",
     "local_attention_fwd_tc.cu",
     "local_attention_bwd_tc.cu",
+    "local_attention_few_tc.cu",
 ]
 
 NVCC_FLAGS = [

@@ -96,29 +96,45 @@ size_t bwd_bytes(LocalBwdArgs b, bool tc) {
   return row_bytes(b.f, tc) + far_bytes(b, key_tile);
 }
 
-// Parts of a split walk. One row tile of a sequence and key head is one CTA; where those are too few
-// for the GPU the walk along the keys is cut. Single tokens (few rows): parts for 4 CTAs an SM, so that
-// sequences of unequal length even out; the parts' outputs are small next to the keys. Chunks: only as
-// many parts as leave no SM without a CTA. A part is at least 256 keys.
-void plan_split(LocalArgs* a, int64_t max_q, int64_t max_ctx, int row_tile, int key_tile) {
+// Parts of a split walk. One row tile of a sequence and key head is one CTA (or unit of work); where those
+// are too few for the GPU the walk along the keys is cut into parts for `target` CTAs: with one row tile
+// per sequence (few rows) that is several times what runs at once, so that sequences of unequal length even
+// out (the parts' outputs are small next to the keys); with more, only as many as leave no SM without work.
+// A part is at least 256 keys.
+void plan_split(LocalArgs* a, int64_t max_q, int64_t max_ctx, int row_tile, int key_tile, int64_t target) {
   a->splits = 1;
   a->split_tiles = 0;
   const int64_t row_tiles = ceil_div(max_q, row_tile / a->G), units = (int64_t)a->n * a->KV * row_tiles;
+  if (row_tiles > 1) target = sm_count();
   int64_t keys = max_ctx;
   if (a->window != NO_WINDOW) {
     const int64_t seen = (int64_t)a->window + row_tile / a->G + 2 * key_tile + (a->sinks > 0 ? a->sinks + key_tile : 0);
     if (seen < keys) keys = seen;
   }
   const int64_t tiles = ceil_div(keys, key_tile), least = 256 / key_tile;
-  const int64_t target = (int64_t)sm_count() * (row_tiles == 1 ? 4 : 1);
   if (units >= target || tiles < 2 * least) return;
   int64_t splits = ceil_div(target, units);
   if (splits > tiles / least) splits = tiles / least;
   if (splits * a->n > 65535) splits = 65535 / a->n;
   if (splits < 2) return;
   a->split_tiles = (int)ceil_div(tiles, splits);
-  a->splits = (int)ceil_div(ceil_div(max_ctx, key_tile), a->split_tiles);  // (a walk is never longer than the context)
-  if (a->window != NO_WINDOW) a->splits = (int)ceil_div(tiles, a->split_tiles);
+  a->splits = (int)ceil_div(tiles, a->split_tiles);
+}
+// The kernel family of a serving call and its tiles.
+struct PagedPlan {
+  bool tc = false;
+  int few = 0;  // columns of the kernel for few rows
+  int row_tile = 0, key_tile = 0, row_tokens = 0;
+};
+PagedPlan plan_paged(LocalArgs* a, int64_t max_q, int64_t max_ctx, bool tc) {
+  PagedPlan p;
+  p.tc = tc;
+  p.few = tc ? local_few_rows(*a, (int)max_q) : 0;
+  p.row_tile = p.few ? p.few : (tc ? 2 * LOCAL_TC_TILE : local_simt_row_tile(*a, (int)max_q));
+  p.key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
+  p.row_tokens = p.few || !tc ? p.row_tile / a->G : local_tc_row_tokens(*a);
+  plan_split(a, max_q, max_ctx, p.row_tile, p.key_tile, (int64_t)sm_count() * (p.few ? 8 : 4));
+  return p;
 }
 size_t split_bytes(const LocalArgs& a) {
   return a.split_tiles == 0 ? 0 : (size_t)a.splits * a.tokens * a.H * (a.D + 1) * sizeof(float);
@@ -243,8 +259,8 @@ extern "C" size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t 
   if (max_q <= 0) return 0;
   // (which kernel family takes the call depends on strides and alignment: enough for either)
   LocalArgs b = a;
-  plan_split(&a, max_q, max_context_length, local_simt_row_tile(a, max_q), local_simt_key_tile());
-  plan_split(&b, max_q, max_context_length, 2 * LOCAL_TC_TILE, LOCAL_TC_TILE);
+  plan_paged(&a, max_q, max_context_length, false);
+  plan_paged(&b, max_q, max_context_length, true);
   return split_bytes(a) > split_bytes(b) ? split_bytes(a) : split_bytes(b);
 }
 
@@ -276,22 +292,18 @@ extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_c
   a.zero_tail = zero_tail;
   cudaStream_t st = (cudaStream_t)stream;
   const int max_q = (int)(max_query_length < T ? max_query_length : T);
-  const bool tc = local_tc_supported(a, dtype, q, key_cache, value_cache, out);
-  const int row_tile = tc ? 2 * LOCAL_TC_TILE : local_simt_row_tile(a, max_q);
-  const int key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
-  plan_split(&a, max_q, max_context_length, row_tile, key_tile);
+  const PagedPlan plan = plan_paged(&a, max_q, max_context_length, local_tc_supported(a, dtype, q, key_cache, value_cache, out));
   TB200_REQUIRE(workspace_bytes >= split_bytes(a) && (workspace || a.split_tiles == 0), TB200_ERR_WORKSPACE,
                 "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, split_bytes(a));
   a.part_out = (float*)workspace;
   a.part_lse = a.part_out + (size_t)a.splits * a.tokens * a.H * a.D;
-  int rc = tc ? launch_local_fwd_tc(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st)
-              : launch_local_fwd_simt(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st);
+  int rc = plan.few ? launch_local_few_tc(out, q, key_cache, value_cache, a, plan.few, dtype, st)
+           : plan.tc ? launch_local_fwd_tc(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st)
+                     : launch_local_fwd_simt(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st);
   if (rc) return rc;
-  if (a.split_tiles > 0) {
-    const int row_tokens = tc ? local_tc_row_tokens(a) : row_tile / a.G;
-    if ((rc = launch_local_combine(out, a, max_q, row_tokens, key_tile, dtype, st))) return rc;
-  }
-  note_kernel(tc ? "local_tcgen05" : "local_simt", a.split_tiles > 0 ? 2 : 1);
+  if (a.split_tiles > 0)
+    if ((rc = launch_local_combine(out, a, max_q, plan.row_tokens, plan.key_tile, dtype, st))) return rc;
+  note_kernel(plan.tc ? "local_tcgen05" : "local_simt", a.split_tiles > 0 ? 2 : 1);
   return 0;
 }
 

@@ -1,31 +1,37 @@
 // tcgen05 forward of local attention (window and sinks), training and serving form, for 16-bit operands
 // with head size 64 or 128.
 //
-// A CTA owns two adjacent tiles of 128 packed query rows (token * G + head of the group) of one sequence
-// and key head, and walks the key tiles that any of them sees (KeyRange), or one part of that walk. Both
-// score tiles and both output accumulators live in tensor memory (S0, S1: 128 fp32 columns each; O0, O1: D
-// columns each), so the tensor pipe works on one query tile while the softmax warps work on the other; a
-// key tile that only one of the two sees is walked by that one alone.
+// A unit of work is two adjacent tiles of 128 packed query rows (token * G + head of the group) of one sequence
+// and key head, along the key tiles that any of them sees (KeyRange), or one part of that walk. A persistent
+// CTA takes every gridDim-th unit: the next unit's queries, keys and first scores are under way while the
+// last one's output is written (a CTA per unit spent 9500 of 51000 cycles on its start and end at a window
+// of 1024). Both score tiles and both output accumulators live in tensor memory (S0, S1: 128 fp32 columns each;
+// O0, O1: D columns each), so the tensor pipe works on one query tile while the softmax warps work on the
+// other; a key tile that only one of the two sees is walked by that one alone.
 //
-//   warp 0      producer: Q0, Q1 once, then rings of two K and two V tiles. A tile of keys is 128 rows of
-//               a sequence (training), or 128 / R pieces of R rows, R the largest divisor of the page size
+//   warp 0      producer: Q0, Q1 of a unit, rings of two K and two V tiles. A tile of keys is 128 rows of a
+//               sequence (training), or 128 / R pieces of R rows, R the largest divisor of the page size
 //               and of 128: one lane per piece looks its page up and issues its copies. Pieces that no row
 //               sees, or whose page is outside the pool, are read at a page index past the end: zeros.
-//   warp 1      MMA issuer: S_t = Q_t K^T, O_t += P_t V (P_t from tensor memory)
+//   warp 1      MMA issuer: S_t = Q_t K^T, O_t += P_t V (P_t from tensor memory, in two parts: the product
+//               starts when three quarters of P_t are there)
 //   warp 2      tensor-memory allocation
 //   warp 3      serving form: zeroes the rows of the last V tile behind the sequence's end (a probability
 //               of 0 times what an unused row holds, which may be NaN, would not be 0)
 //   warps 4-7   softmax of query tile 0, warps 8-11 of tile 1: one thread per row; scores stay in registers
 //               between maximum and exponentials. Warps without a row of the sequence only pass the
-//               barriers (a single new token is G rows of one tile).
+//               barriers (a single new token is G rows of one tile). Output tiles leave through shared memory
+//               and bulk copies (by the threads themselves where a tile is not full or the walk is cut).
 //
-// Only tiles at a border of the window, of the sinks or of the diagonal are masked per element, with a
-// 32-bit mask per 32 columns. The running maximum used in the exponent moves only when the true one has moved
-// by more than 8 (log2 units): the final division by the row sum undoes it exactly. The row sum adds the
-// fp32 probabilities; P is rounded to 16 bits for the product with V, as the tensor cores take it.
+// Masks by blocks of 32 columns and warps of 32 rows: a block that no row of the warp sees costs nothing, one
+// that all rows see no mask, the others a 32-bit mask per row. The running maximum used in the exponent moves
+// only when the true one has moved by more than 8 (log2 units): the final division by the row sum undoes it
+// exactly. The row sum adds the fp32 probabilities; P is rounded to 16 bits for the product with V, as the
+// tensor cores take it.
 //
-// Bound, by size of the problem: exponentials (the 128 x 128 of a tile pair take the 16 units of an SM 1024
-// cycles, as both products together at D = 128) for chunks and training, HBM for single tokens.
+// Bound, by size of the problem: the chain scores -> maximum -> exponentials -> P V of each of the two tiles
+// (exponentials of a tile pair take the 16 units of an SM 1024 cycles, as both products together at D = 128)
+// for chunks and training, HBM for single tokens.
 #include <mutex>
 #include <type_traits>
 
@@ -51,7 +57,8 @@ struct FwdParams {
   float scale_log2;
   int tile_tokens;  // tokens of a query tile
   int piece;        // R: rows of one copy of keys
-  int reverse;      // walk lengths grow with the tile index: longest first
+  int pairs, units; // pairs of query tiles per sequence and key head; pairs * KV * sequences * parts
+  int longest_first;
   uint32_t wait_units;
 };
 
@@ -70,10 +77,63 @@ __device__ inline void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* 
 // the lowest n bits
 __device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
+// A unit of work, as all roles of the CTA see it.
+struct Unit {
+  int s, hk, split, t0;   // t0: first token (within the sequence) of query tile 0
+  Sequence seq;
+  int base;               // position of the sequence's first new token
+  KeyRange kr;
+  int m0, m1;             // steps of the walk
+  bool whole;
+  int st_tiles, lo0, lo1, hi0, hi1;
+  // whether query tile t takes part in key tile j: tiles below st_tiles (sinks) or from lo on, up to hi
+  __device__ bool active(int t, int j) const { return (j < st_tiles || j >= (t ? lo1 : lo0)) && j <= (t ? hi1 : hi0); }
+};
+// false: nothing to do
+template <bool PAGED>
+__device__ inline bool unit_at(const FwdParams& p, int unit, Unit* w) {
+  const LocalArgs& a = p.a;
+  int pair, rest;
+  if (PAGED || p.longest_first) {
+    const int each = p.units / p.pairs;
+    pair = unit / each;
+    if (p.longest_first) pair = p.pairs - 1 - pair;
+    rest = unit % each;
+  } else {  // (neighbouring tiles share keys)
+    pair = unit % p.pairs;
+    rest = unit / p.pairs;
+  }
+  w->hk = rest % a.KV;
+  rest /= a.KV;
+  w->s = rest / a.splits;
+  w->split = rest % a.splits;
+  w->seq = load_sequence(a, w->s);
+  w->t0 = pair * 2 * p.tile_tokens;
+  if (w->t0 >= w->seq.q_len) return false;
+  w->base = w->seq.kv_len - w->seq.q_len;
+  const int last_token = min(w->t0 + 2 * p.tile_tokens, w->seq.q_len) - 1;
+  w->kr = key_range(a, w->base + w->t0, w->base + last_token, w->seq.kv_len, TILE);
+  split_range(a, w->kr.count, w->split, &w->m0, &w->m1);
+  if (w->split > 0 && w->m0 >= w->m1) return false;
+  w->whole = a.split_tiles == 0 || w->kr.count <= a.split_tiles;
+  w->st_tiles = a.window != NO_WINDOW && a.sinks > 0 ? (a.sinks + TILE - 1) / TILE : 0;
+  auto lowest = [&](int t) { return first_key(a, max(w->base + w->t0 + t * p.tile_tokens, 0)) / TILE; };
+  auto highest = [&](int t) {
+    const int first = w->t0 + t * p.tile_tokens, last = min(first + p.tile_tokens, w->seq.q_len) - 1;
+    return first <= last && w->base + last >= 0 ? (w->base + last) / TILE : -1;
+  };
+  w->lo0 = lowest(0);
+  w->lo1 = lowest(1);
+  w->hi0 = highest(0);
+  w->hi1 = highest(1);
+  return true;
+}
+
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
     local_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                        const __grid_constant__ CUtensorMap map_v, const FwdParams p) {
+                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+                        const FwdParams p) {
   constexpr int TILE_BYTES = TILE * D * 2;
   constexpr int NBOX = D / 64;
   constexpr int BOX_BYTES = TILE * 64 * 2;
@@ -86,77 +146,68 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   // product is issued as soon as the softmax threads hold the current scores in registers.
   constexpr bool P_SPLIT = D == 64;
   constexpr uint32_t COL_P = 384;
+  constexpr int P_FIRST = 6;  // steps of 16 keys in the first part of P V
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_smem = smem;                    // [2][TILE_BYTES]
-  uint8_t* k_smem = smem + 2 * TILE_BYTES;   // [2][TILE_BYTES]
-  uint8_t* v_smem = smem + 4 * TILE_BYTES;   // [2][TILE_BYTES]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * TILE_BYTES);
-  // Hand-overs. A ring barrier completes once per step of the walk, a barrier of query tile t once per
-  // step that t takes part in (its count c): the waiter of phase c passes parity c & 1.
+  uint8_t* q_smem = smem;                      // [2][TILE_BYTES]
+  uint8_t* k_smem = smem + 2 * TILE_BYTES;     // [2][TILE_BYTES]
+  uint8_t* v_smem = smem + 4 * TILE_BYTES;     // [2][TILE_BYTES]
+  uint8_t* out_smem = smem + 6 * TILE_BYTES;   // an output tile on its way out
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 7 * TILE_BYTES);
+  // Hand-overs. A ring barrier completes once per step of the walks, a barrier of query tile t once per step
+  // that t takes part in, or once per unit: the waiter of phase c passes parity c & 1.
   //   k/v_full    copies (complete_tx), or warp 3 after its zeroes   MMA issuer
   //   k/v_empty   tcgen05.commit after the last product that reads   producer
+  //   q_full[t]   copies, per unit in which t takes part             MMA issuer
+  //   q_empty[t]  tcgen05.commit after the unit's last Q_t K^T       producer
   //   s_full[t]   tcgen05.commit after Q_t K^T                       softmax: load of S_t
   //   s_free[t]   128 softmax threads after the load of S_t (D = 64) MMA issuer: next Q_t K^T over S_t
-  //   p_full[t]   128 softmax threads after the store of P_t         MMA issuer: P_t V
+  //   p_part[t]   128 softmax threads, first part of P_t stored      MMA issuer: first part of P_t V
+  //   p_full[t]   128 softmax threads, all of P_t stored             MMA issuer: the rest
   //   o_done[t]   tcgen05.commit after P_t V                         softmax: rescale, P_t over P_t, epilogue
+  //   o_free[t]   128 softmax threads after the unit's O_t is read   MMA issuer: first P_t V of the next
+  //   turn[t]     128 softmax threads, per unit, the one that issued softmax of the other tile: output tile
+  //               the copy of output tile t once that has been read  into shared memory
+  // (Every barrier's next completion needs all its waiters to have seen the last one. turn counts all threads
+  // of a tile for that: with one arrival per tile, a warp without rows could be two units behind.)
   uint64_t* q_full = bars;           // [2]
   uint64_t* k_full = bars + 2;       // [2]
   uint64_t* k_empty = bars + 4;      // [2]
   uint64_t* v_full = bars + 6;       // [2]
   uint64_t* v_empty = bars + 8;      // [2]
   uint64_t* s_full = bars + 10;      // [2]
-  uint64_t* p_full = bars + 12;      // [2]
-  uint64_t* o_done = bars + 14;      // [2]
-  uint64_t* s_free = bars + 16;      // [2]
-  uint64_t* v_raw = bars + 18;       // the copies of a V tile that warp 3 completes
-  uint64_t* mma_drained = bars + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* o_done = bars + 12;      // [2]
+  uint64_t* q_empty = bars + 14;     // [2]
+  uint64_t* v_raw = bars + 16;       // [2] the copies of a V tile that warp 3 completes (by stage: the
+                                     // producer may be two tiles ahead, both of them such)
+  uint64_t* mma_drained = bars + 18;
+  uint64_t* p_full = bars + 19;      // [2]
+  uint64_t* p_part = bars + 21;      // [2]
+  uint64_t* s_free = bars + 23;      // [2]
+  uint64_t* o_free = bars + 25;      // [2]
+  uint64_t* turn = bars + 27;        // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
   volatile uint32_t* abort_flag = tmem_slot + 1;  // [0] abort flag, [1] wait limit (ptx::mbar_wait)
 
   const LocalArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int s = blockIdx.z / a.splits, split = blockIdx.z % a.splits, hk = blockIdx.y;
-  const Sequence seq = load_sequence(a, s);
-  if (PAGED && a.zero_tail && s == a.n - 1 && hk == 0 && split == 0) zero_tail_rows(reinterpret_cast<T*>(p.out), a, seq);
-  const int pair = p.reverse ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
-  const int t0 = pair * 2 * p.tile_tokens;  // first token (within the sequence) of query tile 0
-  if (t0 >= seq.q_len) return;
-  const int base = seq.kv_len - seq.q_len;
-  const int last_token = min(t0 + 2 * p.tile_tokens, seq.q_len) - 1;
-  const KeyRange kr = key_range(a, base + t0, base + last_token, seq.kv_len, TILE);
-  int m0, m1;
-  split_range(a, kr.count, split, &m0, &m1);
-  if (split > 0 && m0 >= m1) return;
-  const bool whole = a.split_tiles == 0 || kr.count <= a.split_tiles;
-  // the walk of one query tile: key tiles below `st` (sinks) or from lo on, up to hi
-  const int st_tiles = a.window != NO_WINDOW && a.sinks > 0 ? (a.sinks + TILE - 1) / TILE : 0;
-  auto lowest = [&](int t) { return first_key(a, max(base + t0 + t * p.tile_tokens, 0)) / TILE; };
-  auto highest = [&](int t) {
-    const int first = t0 + t * p.tile_tokens, last = min(first + p.tile_tokens, seq.q_len) - 1;
-    return first <= last && base + last >= 0 ? (base + last) / TILE : -1;
-  };
-  const int lo0 = lowest(0), lo1 = lowest(1), hi0 = highest(0), hi1 = highest(1);
-  auto active = [&](int t, int j) { return (j < st_tiles || j >= (t ? lo1 : lo0)) && j <= (t ? hi1 : hi0); };
+  if (PAGED && a.zero_tail) zero_tail_rows(reinterpret_cast<T*>(p.out), a, load_sequence(a, a.n - 1));
   // the last V tile has rows behind the sequence's end that its copies do not fill with zeros
-  const bool fix = PAGED && m1 > m0 && kr.tile(m1 - 1) == (seq.kv_len - 1) / TILE && seq.kv_len % p.piece != 0;
+  auto needs_fix = [&](const Unit& w) {
+    return PAGED && w.m1 > w.m0 && w.kr.tile(w.m1 - 1) == (w.seq.kv_len - 1) / TILE && w.seq.kv_len % p.piece != 0;
+  };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 12; ++i) ptx::mbar_init(&bars[i], 1);
-    for (int t = 0; t < 2; ++t) {
-      ptx::mbar_init(&p_full[t], 128);
-      ptx::mbar_init(&o_done[t], 1);
-      ptx::mbar_init(&s_free[t], 128);
-    }
-    ptx::mbar_init(v_raw, 1);
-    ptx::mbar_init(mma_drained, 1);
+    for (int i = 0; i < 19; ++i) ptx::mbar_init(&bars[i], 1);
+    for (int i = 19; i < 29; ++i) ptx::mbar_init(&bars[i], 128);
     abort_flag[0] = 0;
     abort_flag[1] = p.wait_units;
     ptx::fence_barrier_init();
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
     ptx::prefetch_tensormap(&map_v);
+    ptx::prefetch_tensormap(&map_out);
   }
   if (warp == 2) {
     ptx::tmem_alloc(tmem_slot, TMEM_COLS);
@@ -175,76 +226,85 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     if (warp == 0) {
       // -------------------------------------------------------------- producer (whole warp)
       const int pieces = TILE / p.piece;
-      if (m1 > m0 && lane == 0) {
+      int g = 0, queries0 = 0, queries1 = 0;  // steps, units of each query tile so far
+      uint32_t fixed = 0;                     // bit s: the last V tile of stage s is completed by warp 3
+      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+        Unit w;
+        if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
+        const bool fix = needs_fix(w);
+        const int from = first_key(a, max(w.base + w.t0, 0));
+        // page and row of this lane's piece of key tile j (index `pages`: zeros)
+        auto locate = [&](int j, int* page, int* row) {
+          if constexpr (PAGED) {
+            const int p0 = j * TILE + lane * p.piece;
+            int id = -1;
+            if (lane < pieces && p0 < w.seq.kv_len && (p0 + p.piece > from || p0 < a.sinks))
+              id = a.table[w.s * a.table_stride + p0 / a.page];
+            *page = id < 0 || id >= a.pages ? a.pages : id;
+            *row = p0 % a.page;
+          } else {
+            *page = w.s;
+            *row = j * TILE;
+          }
+        };
+        int page = 0, row = 0;
+        locate(w.kr.tile(w.m0), &page, &row);
+        for (int m = w.m0; m < w.m1; ++m, ++g) {
+          const int st = g & 1;
+          const uint32_t ph = (g >> 1) & 1;
+          if (lane == 0 && m == w.m0) {
+            const uint32_t bytes = NBOX * p.tile_tokens * a.G * 128;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if ((t ? hi1 : hi0) < 0) continue;
-          ptx::mbar_expect_tx(&q_full[t], NBOX * p.tile_tokens * a.G * 128);
+            for (int t = 0; t < 2; ++t) {
+              if ((t ? w.hi1 : w.hi0) < 0) continue;
+              ptx::mbar_wait(&q_empty[t], ((t ? queries1 : queries0) & 1) ^ 1, abort_flag, a.status, 60);
+              ptx::mbar_expect_tx(&q_full[t], bytes);
 #pragma unroll
-          for (int c = 0; c < NBOX; ++c)
-            tma_load_5d(q_smem + t * TILE_BYTES + c * BOX_BYTES, &map_q, &q_full[t], c * 64, 0,
-                        seq.q_begin + t0 + t * p.tile_tokens, hk, PAGED ? 0 : s);
+              for (int c = 0; c < NBOX; ++c)
+                tma_load_5d(q_smem + t * TILE_BYTES + c * BOX_BYTES, &map_q, &q_full[t], c * 64, 0,
+                            w.seq.q_begin + w.t0 + t * p.tile_tokens, w.hk, PAGED ? 0 : w.s);
+            }
+          }
+          int next_page = 0, next_row = 0;  // (looked up while this step's copies wait for their stage)
+          if (m + 1 < w.m1) locate(w.kr.tile(m + 1), &next_page, &next_row);
+          if (lane == 0) {
+            ptx::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, 61);
+            ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
+          }
+          __syncwarp();
+          if (lane < pieces) {
+#pragma unroll
+            for (int c = 0; c < NBOX; ++c)
+              tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, &map_k, &k_full[st], c * 64, row,
+                          w.hk, page);
+          }
+          const bool fixed_tile = fix && m + 1 == w.m1;
+          uint64_t* vbar = fixed_tile ? &v_raw[st] : &v_full[st];
+          fixed = (fixed & ~(1u << st)) | (fixed_tile ? 1u << st : 0u);
+          if (lane == 0) {
+            ptx::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, 62);
+            ptx::mbar_expect_tx(vbar, TILE_BYTES);
+          }
+          __syncwarp();
+          if (lane < pieces) {
+#pragma unroll
+            for (int c = 0; c < NBOX; ++c)
+              tma_load_4d(v_smem + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, &map_v, vbar, c * 64, row, w.hk, page);
+          }
+          page = next_page;
+          row = next_row;
         }
+        queries0 += w.hi0 >= 0;
+        queries1 += w.hi1 >= 0;
       }
-      const int from = first_key(a, max(base + t0, 0));
-      // page and row of this lane's piece of key tile j (index `pages`: zeros)
-      auto locate = [&](int j, int* page, int* row) {
-        if constexpr (PAGED) {
-          const int p0 = j * TILE + lane * p.piece;
-          int id = -1;
-          if (lane < pieces && p0 < seq.kv_len && (p0 + p.piece > from || p0 < a.sinks))
-            id = a.table[s * a.table_stride + p0 / a.page];
-          *page = id < 0 || id >= a.pages ? a.pages : id;
-          *row = p0 % a.page;
-        } else {
-          *page = s;
-          *row = j * TILE;
-        }
-      };
-      int page = 0, row = 0;
-      if (m1 > m0) locate(kr.tile(m0), &page, &row);
-      for (int m = m0; m < m1; ++m) {
-        const int st = (m - m0) & 1;
-        const uint32_t ph = ((m - m0) >> 1) & 1;
-        int next_page = 0, next_row = 0;  // (looked up while this step's copies wait for their stage)
-        if (m + 1 < m1) locate(kr.tile(m + 1), &next_page, &next_row);
-        if (lane == 0) {
-          ptx::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, 61);
-          ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
-        }
-        __syncwarp();
-        if (lane < pieces) {
-#pragma unroll
-          for (int c = 0; c < NBOX; ++c)
-            tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, &map_k, &k_full[st], c * 64, row, hk,
-                        page);
-        }
-        uint64_t* vbar = fix && m + 1 == m1 ? v_raw : &v_full[st];
-        if (lane == 0) {
-          ptx::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, 62);
-          ptx::mbar_expect_tx(vbar, TILE_BYTES);
-        }
-        __syncwarp();
-        if (lane < pieces) {
-#pragma unroll
-          for (int c = 0; c < NBOX; ++c)
-            tma_load_4d(v_smem + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, &map_v, vbar, c * 64, row, hk, page);
-        }
-        page = next_page;
-        row = next_row;
-      }
-      // Drain: every copy has landed before the CTA gives up its shared memory.
-      if (lane == 0 && m1 > m0) {
-        for (int t = 0; t < 2; ++t)
-          if ((t ? hi1 : hi0) >= 0) ptx::mbar_wait_drain(&q_full[t], 0, abort_flag, a.status, 63);
-        for (int m = m1 - m0 > 2 ? m1 - 2 : m0; m < m1; ++m) {
-          const int st = (m - m0) & 1;
-          const uint32_t ph = ((m - m0) >> 1) & 1;
-          ptx::mbar_wait_drain(&k_full[st], ph, abort_flag, a.status, 64);
-          if (fix && m + 1 == m1)
-            ptx::mbar_wait_drain(v_raw, 0, abort_flag, a.status, 65);
-          else
-            ptx::mbar_wait_drain(&v_full[st], ph, abort_flag, a.status, 65);
+      // Drain: every copy has landed before the CTA gives up its shared memory (warp 3 itself waits for the
+      // copies of the tiles that it completes).
+      if (lane == 0) {
+        if (queries0 > 0) ptx::mbar_wait_drain(&q_full[0], (queries0 - 1) & 1, abort_flag, a.status, 63);
+        if (queries1 > 0) ptx::mbar_wait_drain(&q_full[1], (queries1 - 1) & 1, abort_flag, a.status, 63);
+        for (int i = g > 2 ? g - 2 : 0; i < g; ++i) {
+          ptx::mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1, abort_flag, a.status, 64);
+          if (!((fixed >> (i & 1)) & 1u)) ptx::mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1, abort_flag, a.status, 65);
         }
       }
       __syncwarp();
@@ -264,6 +324,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       const uint64_t dk0 = ptx::make_smem_desc(ptx::smem_u32(k_smem), 16, 1024);
       const uint64_t dv0 = ptx::make_smem_desc(ptx::smem_u32(v_smem), BOX_BYTES, 1024);
       constexpr uint64_t NEXT_TILE = static_cast<uint64_t>(TILE_BYTES >> 4);
+      // Counts of each query tile over all units: score products, value products, units with products.
+      int scores0 = 0, scores1 = 0, values0 = 0, values1 = 0, queries0 = 0, queries1 = 0;
       auto issue_qk = [&](int t, int st) {
         const uint64_t qd = dq0 + (t ? NEXT_TILE : 0), kd = dk0 + (st ? NEXT_TILE : 0);
         const uint32_t d_tmem = tmem_base + COL_S + t * 128;
@@ -273,84 +335,121 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           if (elected) ptx::umma_ss(d_tmem, qd + off, kd + off, IDESC_QK, ks != 0);
         }
       };
-      auto issue_pv = [&](int t, int st, bool accumulate) {
+      auto issue_pv = [&](int t, int st, int ks0, int ks1, bool accumulate) {
         const uint64_t vd = dv0 + (st ? NEXT_TILE : 0);
         const uint32_t d_tmem = tmem_base + COL_O + t * D;
         const uint32_t p_tmem = tmem_base + (P_SPLIT ? COL_P + t * 64 : COL_S + t * 128);
 #pragma unroll
         for (int ks = 0; ks < TILE / 16; ++ks) {
+          if (ks < ks0 || ks >= ks1) continue;
           if (elected)
             ptx::umma_ts(d_tmem, p_tmem + ks * 8, vd + static_cast<uint64_t>((ks * 2048) >> 4), IDESC_PV,
                          accumulate || ks != 0);
         }
       };
-      if (m1 > m0) {
-        int scores[2] = {0, 0}, values[2] = {0, 0};  // products issued so far, per query tile
-        // S of step m for query tile t
-        auto do_scores = [&](int t, int m) {
-          const int st = (m - m0) & 1;
-          if (scores[t] == 0) wait_(&q_full[t], 0, 71 + t);
-          if (P_SPLIT && scores[t] > 0) wait_(&s_free[t], (scores[t] - 1) & 1, 73 + t);
-          wait_(&k_full[st], ((m - m0) >> 1) & 1, 75);
+      int g = 0;  // steps of all units
+      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+        Unit w;
+        if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
+        const int steps = w.m1 - w.m0;
+        bool fresh0 = true, fresh1 = true, first0 = true, first1 = true;  // no scores, no values of the tile yet
+        auto do_scores = [&](auto tag, int i) {  // of step i
+          constexpr int t = decltype(tag)::value;
+          int& scores = t ? scores1 : scores0;
+          bool& fresh = t ? fresh1 : fresh0;
+          if (fresh) wait_(&q_full[t], (t ? queries1 : queries0) & 1, 71 + t);
+          fresh = false;
+          if (P_SPLIT && scores > 0) wait_(&s_free[t], (scores - 1) & 1, 73 + t);
+          wait_(&k_full[(g + i) & 1], ((g + i) >> 1) & 1, 75);
           ptx::tc_fence_after();
-          issue_qk(t, st);
+          issue_qk(t, (g + i) & 1);
           commit_(&s_full[t]);
-          ++scores[t];
+          ++scores;
         };
-        auto do_values = [&](int t, int m) {
-          const int st = (m - m0) & 1;
-          wait_(&p_full[t], values[t] & 1, 76 + t);
-          wait_(&v_full[st], ((m - m0) >> 1) & 1, 78);
+        auto do_values = [&](auto tag, int i) {
+          constexpr int t = decltype(tag)::value;
+          int& values = t ? values1 : values0;
+          bool& first = t ? first1 : first0;
+          if (first && (t ? queries1 : queries0) > 0) wait_(&o_free[t], ((t ? queries1 : queries0) - 1) & 1, 80);
+          wait_(&p_part[t], values & 1, 76 + t);
+          wait_(&v_full[(g + i) & 1], ((g + i) >> 1) & 1, 78);
           ptx::tc_fence_after();
-          issue_pv(t, st, values[t] > 0);
+          issue_pv(t, (g + i) & 1, 0, P_FIRST, !first);
+          wait_(&p_full[t], values & 1, 76 + t);
+          ptx::tc_fence_after();
+          issue_pv(t, (g + i) & 1, P_FIRST, TILE / 16, true);
           commit_(&o_done[t]);
-          ++values[t];
+          first = false;
+          ++values;
         };
+        using T0 = std::integral_constant<int, 0>;
+        using T1 = std::integral_constant<int, 1>;
         {
-          const int j = kr.tile(m0);
-          if (active(0, j)) do_scores(0, m0);
-          if (active(1, j)) do_scores(1, m0);
-          commit_(&k_empty[0]);
+          const int j = w.kr.tile(w.m0);
+          if (w.active(0, j)) do_scores(T0{}, 0);
+          if (w.active(1, j)) do_scores(T1{}, 0);
+          commit_(&k_empty[g & 1]);
         }
-        for (int m = m0; m < m1; ++m) {
-          const int j = kr.tile(m), nj = m + 1 < m1 ? kr.tile(m + 1) : 0;
-          const bool more = m + 1 < m1;
+        for (int i = 0; i < steps; ++i) {
+          const bool more = i + 1 < steps;
+          const int j = w.kr.tile(w.m0 + i), nj = more ? w.kr.tile(w.m0 + i + 1) : 0;
           if constexpr (P_SPLIT) {
             // next scores of a tile before its values
-            if (more && active(0, nj)) do_scores(0, m + 1);
-            if (active(0, j)) do_values(0, m);
-            if (more && active(1, nj)) do_scores(1, m + 1);
-            if (more) commit_(&k_empty[(m + 1 - m0) & 1]);
-            if (active(1, j)) do_values(1, m);
-            commit_(&v_empty[(m - m0) & 1]);
+            if (more && w.active(0, nj)) do_scores(T0{}, i + 1);
+            if (w.active(0, j)) do_values(T0{}, i);
+            if (more && w.active(1, nj)) do_scores(T1{}, i + 1);
+            if (more) commit_(&k_empty[(g + i + 1) & 1]);
+            if (w.active(1, j)) do_values(T1{}, i);
+            commit_(&v_empty[(g + i) & 1]);
           } else {
             // P overwrites S: the next scores follow the values on the in-order pipe
-            if (active(0, j)) do_values(0, m);
-            if (more && active(0, nj)) do_scores(0, m + 1);
-            if (active(1, j)) do_values(1, m);
-            commit_(&v_empty[(m - m0) & 1]);
-            if (more && active(1, nj)) do_scores(1, m + 1);
-            if (more) commit_(&k_empty[(m + 1 - m0) & 1]);
+            if (w.active(0, j)) do_values(T0{}, i);
+            if (more && w.active(0, nj)) do_scores(T0{}, i + 1);
+            if (w.active(1, j)) do_values(T1{}, i);
+            commit_(&v_empty[(g + i) & 1]);
+            if (more && w.active(1, nj)) do_scores(T1{}, i + 1);
+            if (more) commit_(&k_empty[(g + i + 1) & 1]);
           }
+        }
+        g += steps;
+        // (a tile whose queries were brought, but that takes no part in this part of the walk, counts too)
+        if (w.hi0 >= 0) {
+          if (fresh0) wait_(&q_full[0], queries0 & 1, 71);
+          commit_(&q_empty[0]);
+          ++queries0;
+        }
+        if (w.hi1 >= 0) {
+          if (fresh1) wait_(&q_full[1], queries1 & 1, 72);
+          commit_(&q_empty[1]);
+          ++queries1;
         }
       }
       // everything issued has completed before tensor memory is freed
       commit_(mma_drained);
       ptx::mbar_wait_drain(mma_drained, 0, abort_flag, a.status, 79);
       __syncwarp();
-    } else if (PAGED && warp == 3 && fix) {
+    } else if (PAGED && warp == 3) {
       // -------------------------------------------------------------- zeros behind the sequence's end
-      const int st = (m1 - 1 - m0) & 1;
-      ptx::mbar_wait(v_raw, 0, abort_flag, a.status, 66);
-      const int first = seq.kv_len % TILE, end = min(TILE, ((first + p.piece - 1) / p.piece) * p.piece);
-      // (whole pieces behind the end were read as zeros)
-      for (int r = first; r < end; ++r)
+      int g = 0;
+      uint32_t phases = 0;  // bit s: parity of the next completion of stage s
+      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+        Unit w;
+        if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
+        g += w.m1 - w.m0;
+        if (!needs_fix(w)) continue;
+        const int st = (g - 1) & 1;
+        ptx::mbar_wait_drain(&v_raw[st], (phases >> st) & 1u, abort_flag, a.status, 66);
+        phases ^= 1u << st;
+        const int first = w.seq.kv_len % TILE, end = min(TILE, ((first + p.piece - 1) / p.piece) * p.piece);
+        // (whole pieces behind the end were read as zeros)
+        for (int r = first + lane / 8; r < end; r += 4)
 #pragma unroll
-        for (int c = 0; c < NBOX; ++c)
-          if (lane < 8) *reinterpret_cast<uint4*>(v_smem + st * TILE_BYTES + c * BOX_BYTES + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&v_full[st]);
+          for (int c = 0; c < NBOX; ++c)
+            *reinterpret_cast<uint4*>(v_smem + st * TILE_BYTES + c * BOX_BYTES + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&v_full[st]);
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax + epilogue
@@ -358,210 +457,265 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int first_token = t0 + t * p.tile_tokens;
-    const int tokens = min(p.tile_tokens, seq.q_len - first_token);
-    const int rows = tokens > 0 ? tokens * a.G : 0;
-    const bool warp_live = quarter * 32 < rows, live = r < rows;
-    const int token = first_token + r / a.G;  // of the sequence
-    const int pos = live ? base + token : -1;
-    const int pmin = base + first_token, pmax = base + first_token + tokens - 1;
+    const int row_token = r / a.G, row_head = r % a.G;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + COL_S + t * 128;
     const uint32_t o_addr = tmem_base + lane_off + COL_O + t * D;
     const uint32_t p_addr = tmem_base + lane_off + (P_SPLIT ? COL_P + t * 64 : COL_S + t * 128);
-    float m_used = -INFINITY, l = 0.f;
-    int count = 0;
-    for (int m = m0; m < m1; ++m) {
-      const int j = kr.tile(m);
-      if (!active(t, j)) continue;
-      const int c = count++;
-      ptx::mbar_wait(&s_full[t], c & 1, abort_flag, a.status, 81);
-      ptx::tc_fence_after();
-      if (!warp_live) {
-        if constexpr (P_SPLIT) ptx::mbar_arrive(&s_free[t]);
-        // (P(c) of these rows is never read into a stored result; the barrier's phases stay in step)
-        if (P_SPLIT && c > 0) ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 82);
+    int count = 0, turns = 0;  // steps of this tile, units (over all units of the CTA)
+    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+      Unit w;
+      if (!unit_at<PAGED>(p, unit, &w)) continue;
+      const int first_token = w.t0 + t * p.tile_tokens;
+      const int tokens = min(p.tile_tokens, w.seq.q_len - first_token);
+      const int rows = tokens > 0 ? tokens * a.G : 0;
+      const bool warp_live = quarter * 32 < rows, live = r < rows;
+      const int token = first_token + row_token;  // of the sequence
+      const int pos = live ? w.base + token : -1;
+      // positions of the warp's rows
+      const int wmin = w.base + first_token + quarter * 32 / a.G;
+      const int wmax = w.base + first_token + min((quarter * 32 + 31) / a.G, tokens - 1);
+      float m_used = -INFINITY, l = 0.f;
+      const int before = count;
+      for (int m = w.m0; m < w.m1; ++m) {
+        const int j = w.kr.tile(m);
+        if (!w.active(t, j)) continue;
+        const int c = count++;
+        const bool first = c == before;
+        ptx::mbar_wait(&s_full[t], c & 1, abort_flag, a.status, 81);
+        ptx::tc_fence_after();
+        if (!warp_live) {
+          if constexpr (P_SPLIT) ptx::mbar_arrive(&s_free[t]);
+          // (P of these rows is never read into a stored result; the barriers' phases stay in step)
+          if (P_SPLIT && c > 0) ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 82);
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(&p_part[t]);
+          ptx::mbar_arrive(&p_full[t]);
+          continue;
+        }
+        const int j0 = j * TILE;
+        // blocks of 32 columns that no row of the warp sees, and that all see
+        uint32_t none = 0, all = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int b0 = j0 + 32 * q;
+          if (b0 > wmax || (wmin - (b0 + 31) >= a.window && b0 >= a.sinks)) none |= 1u << q;
+          if (b0 + 31 <= wmin && (wmax - b0 < a.window || b0 + 32 <= a.sinks)) all |= 1u << q;
+        }
+        const bool plain = all == 15u && p.scale_log2 >= 0.f;
+        uint32_t sr[4][32];
+        float mx = -INFINITY;
+        if (plain) {
+          float x0 = -INFINITY, x1 = -INFINITY;
+          auto reduce32 = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              x0 = am::max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              x1 = am::max3(x1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+            }
+          };
+          ptx::tmem_ld32(s_addr, sr[0]);
+          am::tmem_ld_wait_dep(sr[0]);
+          ptx::tmem_ld32(s_addr + 32, sr[1]);
+          reduce32(sr[0]);
+          am::tmem_ld_wait_dep(sr[1]);
+          ptx::tmem_ld32(s_addr + 64, sr[2]);
+          reduce32(sr[1]);
+          am::tmem_ld_wait_dep(sr[2]);
+          ptx::tmem_ld32(s_addr + 96, sr[3]);
+          reduce32(sr[2]);
+          am::tmem_ld_wait_dep(sr[3]);
+          reduce32(sr[3]);
+          mx = fmaxf(x0, x1) * p.scale_log2;
+        } else {
+          const uint64_t sc2 = am::pack2f(p.scale_log2, p.scale_log2);
+          float x0 = -INFINITY, x1 = -INFINITY;
+          auto scale32 = [&](uint32_t (&v)[32], int q) {
+            if ((none >> q) & 1u) return;
+            // columns below pos + 1 - b0 are not in the future, those from pos - window + 1 - b0 on in the window
+            const int b0 = j0 + 32 * q;
+            const int64_t low = (int64_t)pos - a.window + 1 - b0;
+            const uint32_t seen = (all >> q) & 1u ? 0xffffffffu
+                                                  : low_bits(pos + 1 - b0) & (~low_bits(low < 0 ? 0 : (int)low) | low_bits(a.sinks - b0));
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float s0, s1;
+              am::unpack2f(am::mul2(am::pack2u(v[i], v[i + 1]), sc2), s0, s1);
+              s0 = seen & (1u << i) ? s0 : -INFINITY;
+              s1 = seen & (2u << i) ? s1 : -INFINITY;
+              if (i & 2) x1 = am::max3(x1, s0, s1);
+              else x0 = am::max3(x0, s0, s1);
+              v[i] = __float_as_uint(s0);
+              v[i + 1] = __float_as_uint(s1);
+            }
+          };
+          ptx::tmem_ld32(s_addr, sr[0]);
+          am::tmem_ld_wait_dep(sr[0]);
+          ptx::tmem_ld32(s_addr + 32, sr[1]);
+          scale32(sr[0], 0);
+          am::tmem_ld_wait_dep(sr[1]);
+          ptx::tmem_ld32(s_addr + 64, sr[2]);
+          scale32(sr[1], 1);
+          am::tmem_ld_wait_dep(sr[2]);
+          ptx::tmem_ld32(s_addr + 96, sr[3]);
+          scale32(sr[2], 2);
+          am::tmem_ld_wait_dep(sr[3]);
+          scale32(sr[3], 3);
+          mx = fmaxf(x0, x1);
+        }
+        if constexpr (P_SPLIT) {
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(&s_free[t]);
+        }
+        const float m_new = fmaxf(m_used, mx);
+        if (first) {
+          m_used = m_new;
+        } else {
+          const bool need = live && m_new > m_used + RESCALE_THRESHOLD;  // (other rows may hold anything)
+          if (__any_sync(0xffffffffu, need)) {
+            ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 83);
+            ptx::tc_fence_after();
+            const float factor = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t v[32];
+              ptx::tmem_ld32(o_addr + q * 32, v);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
+              ptx::tmem_st32(o_addr + q * 32, v);
+            }
+            ptx::tmem_st_wait();
+            l *= factor;
+            m_used = m_new;
+          }
+        }
+        const float m_safe = m_used == -INFINITY ? 0.f : m_used;
+        {
+          const float to_log2 = plain ? p.scale_log2 : 1.f;
+          const uint64_t scale2 = am::pack2f(to_log2, to_log2);
+          const uint64_t negm2 = am::pack2f(-m_safe, -m_safe);
+          uint64_t lsum = am::pack2f(0.f, 0.f), lsum_b = am::pack2f(0.f, 0.f);
+          auto exp32 = [&](const uint32_t (&v)[32], int q) {
+            uint32_t packed[16];
+            if ((none >> q) & 1u) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) packed[i] = 0u;
+              ptx::tmem_st16(p_addr + q * 16, packed);
+              return;
+            }
+            float x[32];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              am::unpack2f(am::fma2(am::pack2u(v[i], v[i + 1]), scale2, negm2), x[i], x[i + 1]);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = am::ex2(x[i]);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              lsum = am::add2(lsum, am::pack2f(x[i], x[i + 1]));
+              lsum_b = am::add2(lsum_b, am::pack2f(x[i + 2], x[i + 3]));
+              packed[i >> 1] = am::cvt_pair<T>(x[i], x[i + 1]);
+              packed[(i >> 1) + 1] = am::cvt_pair<T>(x[i + 2], x[i + 3]);
+            }
+            ptx::tmem_st16(p_addr + q * 16, packed);
+          };
+          if constexpr (P_SPLIT) {
+            if (c > 0) {  // P(c) goes over P(c-1)
+              ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 84);
+              ptx::tc_fence_after();
+            }
+          }
+          exp32(sr[0], 0);
+          exp32(sr[1], 1);
+          exp32(sr[2], 2);
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(&p_part[t]);
+          exp32(sr[3], 3);
+          float l0, l1;
+          am::unpack2f(am::add2(lsum, lsum_b), l0, l1);
+          l += l0 + l1;
+        }
+        ptx::tmem_st_wait();
         ptx::tc_fence_before();
         ptx::mbar_arrive(&p_full[t]);
-        continue;
       }
-      const int j0 = j * TILE;
-      // every row of the tile sees every key of it
-      const bool plain = j0 + TILE - 1 <= pmin && (pmax - j0 < a.window || j0 + TILE <= a.sinks);
-      uint32_t sr[4][32];
-      float mx = -INFINITY;
-      if (plain) {
-        float x0 = -INFINITY, x1 = -INFINITY;
-        auto reduce32 = [&](const uint32_t (&v)[32]) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            x0 = am::max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-            x1 = am::max3(x1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-          }
-        };
-        ptx::tmem_ld32(s_addr, sr[0]);
-        am::tmem_ld_wait_dep(sr[0]);
-        ptx::tmem_ld32(s_addr + 32, sr[1]);
-        reduce32(sr[0]);
-        am::tmem_ld_wait_dep(sr[1]);
-        ptx::tmem_ld32(s_addr + 64, sr[2]);
-        reduce32(sr[1]);
-        am::tmem_ld_wait_dep(sr[2]);
-        ptx::tmem_ld32(s_addr + 96, sr[3]);
-        reduce32(sr[2]);
-        am::tmem_ld_wait_dep(sr[3]);
-        reduce32(sr[3]);
-        if (p.scale_log2 < 0.f) {  // (the largest score is the smallest product)
-          x0 = x1 = INFINITY;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x0 = fminf(x0, __uint_as_float(sr[q][i]));
-        } else {
-          x0 = fmaxf(x0, x1);
-        }
-        mx = x0 * p.scale_log2;
-      } else {
-        const int high = min(pos, seq.kv_len - 1) - j0 + 1;  // columns below `high` are not in the future
-        const int64_t low64 = (int64_t)pos - a.window + 1 - j0;
-        const int low = low64 < 0 ? 0 : (int)low64;          // columns from `low` on are in the window
-        const int sink = a.sinks - j0;                       // columns below `sink` are sinks
-        auto scale32 = [&](uint32_t (&v)[32], int q) {
-          const uint32_t seen = low_bits(high - 32 * q) & (~low_bits(low - 32 * q) | low_bits(sink - 32 * q));
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float sc = (seen >> i) & 1u ? __uint_as_float(v[i]) * p.scale_log2 : -INFINITY;
-            mx = fmaxf(mx, sc);
-            v[i] = __float_as_uint(sc);
-          }
-        };
-        ptx::tmem_ld32(s_addr, sr[0]);
-        am::tmem_ld_wait_dep(sr[0]);
-        ptx::tmem_ld32(s_addr + 32, sr[1]);
-        scale32(sr[0], 0);
-        am::tmem_ld_wait_dep(sr[1]);
-        ptx::tmem_ld32(s_addr + 64, sr[2]);
-        scale32(sr[1], 1);
-        am::tmem_ld_wait_dep(sr[2]);
-        ptx::tmem_ld32(s_addr + 96, sr[3]);
-        scale32(sr[2], 2);
-        am::tmem_ld_wait_dep(sr[3]);
-        scale32(sr[3], 3);
-      }
-      if constexpr (P_SPLIT) {
-        ptx::tc_fence_before();
-        ptx::mbar_arrive(&s_free[t]);
-      }
-      const float m_new = fmaxf(m_used, mx);
-      if (c == 0) {
-        m_used = m_new;
-      } else {
-        const bool need = m_new > m_used + RESCALE_THRESHOLD;
-        if (__any_sync(0xffffffffu, need)) {
-          ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 83);
-          ptx::tc_fence_after();
-          const float factor = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
-#pragma unroll 1
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t v[32];
-            ptx::tmem_ld32(o_addr + q * 32, v);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
-            ptx::tmem_st32(o_addr + q * 32, v);
-          }
-          ptx::tmem_st_wait();
-          l *= factor;
-          m_used = m_new;
-        }
-      }
-      const float m_safe = m_used == -INFINITY ? 0.f : m_used;
-      {
-        const float to_log2 = plain ? p.scale_log2 : 1.f;
-        const uint64_t scale2 = am::pack2f(to_log2, to_log2);
-        const uint64_t negm2 = am::pack2f(-m_safe, -m_safe);
-        uint64_t lsum = am::pack2f(0.f, 0.f), lsum_b = am::pack2f(0.f, 0.f);
-        auto exp32 = [&](const uint32_t (&v)[32], int q) {
-          float x[32];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            am::unpack2f(am::fma2(am::pack2u(v[i], v[i + 1]), scale2, negm2), x[i], x[i + 1]);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = am::ex2(x[i]);
-          uint32_t packed[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            lsum = am::add2(lsum, am::pack2f(x[i], x[i + 1]));
-            lsum_b = am::add2(lsum_b, am::pack2f(x[i + 2], x[i + 3]));
-            packed[i >> 1] = am::cvt_pair<T>(x[i], x[i + 1]);
-            packed[(i >> 1) + 1] = am::cvt_pair<T>(x[i + 2], x[i + 3]);
-          }
-          ptx::tmem_st16(p_addr + q * 16, packed);
-        };
-        if constexpr (P_SPLIT) {
-          if (c > 0) {  // P(c) goes over P(c-1)
-            ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 84);
-            ptx::tc_fence_after();
-          }
-        }
-        exp32(sr[0], 0);
-        exp32(sr[1], 1);
-        exp32(sr[2], 2);
-        exp32(sr[3], 3);
-        float l0, l1;
-        am::unpack2f(am::add2(lsum, lsum_b), l0, l1);
-        l += l0 + l1;
-      }
-      ptx::tmem_st_wait();
-      ptx::tc_fence_before();
-      ptx::mbar_arrive(&p_full[t]);
-    }
-    if (warp_live) {
-      if (count > 0) {
+      const bool counted = count > before;
+      if (counted) {
         ptx::mbar_wait(&o_done[t], (count - 1) & 1, abort_flag, a.status, 85);
         ptx::tc_fence_after();
       }
-      const int head = hk * a.G + r % a.G;
-      const long long tok = seq.q_begin + token;
+      const int head = w.hk * a.G + row_head;
+      const long long tok = w.seq.q_begin + token;
       const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys: zeros
-      const float ls = l > 0.f ? m_used * LN2 + logf(l) : -INFINITY;
-      T* orow = reinterpret_cast<T*>(p.out) + (long long)s * a.os[0] + head * a.os[1] + tok * a.os[2];
-      const long long prow = ((long long)split * a.tokens + tok) * a.H + head;
+      // a full tile leaves through shared memory; copies of the other tile have read it (turn)
+      const bool bulk = w.whole && tokens > 0 && (!PAGED || tokens == p.tile_tokens);
+      if (t == 0) {
+        if (turns > 0) ptx::mbar_wait(&turn[1], (turns - 1) & 1, abort_flag, a.status, 86);
+      } else {
+        ptx::mbar_wait(&turn[0], turns & 1, abort_flag, a.status, 87);
+      }
+      ++turns;
+      if (warp_live) {
+        T* orow = reinterpret_cast<T*>(p.out) + (long long)w.s * a.os[0] + head * a.os[1] + tok * a.os[2];
+        const long long prow = ((long long)w.split * a.tokens + tok) * a.H + head;
 #pragma unroll 1
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t v[32];
-        __syncwarp();
-        if (count > 0) {
-          ptx::tmem_ld32(o_addr + q * 32, v);
-          ptx::tmem_ld_wait();
-        }
-        if (!(l > 0.f)) {  // (nothing was accumulated: the columns hold what was there before)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0;
-        }
-        if (live && whole) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint4 o;
-            o.x = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 0]) * inv, __uint_as_float(v[g * 8 + 1]) * inv);
-            o.y = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 2]) * inv, __uint_as_float(v[g * 8 + 3]) * inv);
-            o.z = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 4]) * inv, __uint_as_float(v[g * 8 + 5]) * inv);
-            o.w = am::cvt_pair<T>(__uint_as_float(v[g * 8 + 6]) * inv, __uint_as_float(v[g * 8 + 7]) * inv);
-            *reinterpret_cast<uint4*>(orow + q * 32 + g * 8) = o;
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t v[32];
+          __syncwarp();
+          if (counted) {
+            ptx::tmem_ld32(o_addr + q * 32, v);
+            ptx::tmem_ld_wait();
           }
-        } else if (live && l > 0.f) {  // (a part without keys is known by its lse)
-          float4* dst = reinterpret_cast<float4*>(a.part_out + prow * D + q * 32);
+          if (!(l > 0.f)) {  // (nothing was accumulated: the columns hold what was there before)
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
-            dst[g] = make_float4(__uint_as_float(v[g * 4]) * inv, __uint_as_float(v[g * 4 + 1]) * inv,
-                                 __uint_as_float(v[g * 4 + 2]) * inv, __uint_as_float(v[g * 4 + 3]) * inv);
+            for (int i = 0; i < 32; ++i) v[i] = 0;
+          }
+          if (w.whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint4 o;
+              o.x = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 0]) * inv, __uint_as_float(v[e * 8 + 1]) * inv);
+              o.y = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 2]) * inv, __uint_as_float(v[e * 8 + 3]) * inv);
+              o.z = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 4]) * inv, __uint_as_float(v[e * 8 + 5]) * inv);
+              o.w = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 6]) * inv, __uint_as_float(v[e * 8 + 7]) * inv);
+              if (bulk) {
+                const int chunk = q * 4 + e;
+                *reinterpret_cast<uint4*>(out_smem + (chunk >> 3) * BOX_BYTES + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = o;
+              } else if (live) {
+                *reinterpret_cast<uint4*>(orow + q * 32 + e * 8) = o;
+              }
+            }
+          } else if (live && l > 0.f) {  // (a part without keys is known by its lse)
+            float4* dst = reinterpret_cast<float4*>(a.part_out + prow * D + q * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_float4(__uint_as_float(v[e * 4]) * inv, __uint_as_float(v[e * 4 + 1]) * inv,
+                                   __uint_as_float(v[e * 4 + 2]) * inv, __uint_as_float(v[e * 4 + 3]) * inv);
+          }
         }
       }
+      ptx::tc_fence_before();
+      if ((t ? w.hi1 : w.hi0) >= 0 && w.m1 > w.m0) ptx::mbar_arrive(&o_free[t]);
+      if (bulk) {
+        ptx::fence_proxy_async_smem();
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+      }
+      if (bulk && (threadIdx.x & 127) == 0) {
+#pragma unroll
+        for (int c = 0; c < NBOX; ++c)
+          ptx::tma_store_5d(&map_out, out_smem + c * BOX_BYTES, c * 64, 0, (int)(w.seq.q_begin + first_token), w.hk, PAGED ? 0 : w.s);
+        ptx::bulk_commit();
+        ptx::bulk_wait_read();
+      }
+      ptx::mbar_arrive(&turn[t]);
       if (live) {
-        if (!whole) a.part_lse[prow] = ls;
-        else if (!PAGED) p.lse[((long long)s * a.H + head) * a.tokens + tok] = ls;
+        const float ls = l > 0.f ? m_used * LN2 + logf(l) : -INFINITY;
+        if (!w.whole) a.part_lse[((long long)w.split * a.tokens + tok) * a.H + head] = ls;
+        else if (!PAGED) p.lse[((long long)w.s * a.H + head) * a.tokens + tok] = ls;
       }
     }
+    if ((threadIdx.x & 127) == 0) ptx::bulk_wait_done();
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -651,9 +805,9 @@ bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void
 namespace {
 
 template <typename T, int D, bool PAGED>
-int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdParams& p, int max_q,
+int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo, const FwdParams& p,
                cudaStream_t st) {
-  constexpr int SMEM = 6 * TILE * D * 2 + 1024 + 256;
+  constexpr int SMEM = 7 * TILE * D * 2 + 1024 + 256;
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
   auto kern = local_fwd_tc_kernel<T, D, PAGED>;
   static std::atomic<unsigned long long> optin_done{0};
@@ -676,8 +830,8 @@ int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
     set_error("local_fwd_tc: kernel compiled with %d registers per thread, the register rebalancing needs %d", regs, REGS_LAUNCH);
     return TB200_ERR_UNSUPPORTED;
   }
-  const dim3 grid((unsigned)ceil_div(max_q, 2 * p.tile_tokens), (unsigned)p.a.KV, (unsigned)(p.a.n * p.a.splits));
-  kern<<<grid, FWD_THREADS, SMEM, st>>>(mq, mk, mv, p);
+  const int sms = sm_count();
+  kern<<<(unsigned)(p.units < sms ? p.units : sms), FWD_THREADS, SMEM, st>>>(mq, mk, mv, mo, p);
   return launch_status("local_fwd_tc");
 }
 
@@ -693,16 +847,21 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   p.scale_log2 = a.scale * LOG2E;
   p.tile_tokens = TILE / a.G;
   p.piece = local_piece(a);
-  p.reverse = a.window == NO_WINDOW;
+  p.pairs = (int)ceil_div(max_q, 2 * p.tile_tokens);
+  const int64_t units = (int64_t)p.pairs * a.KV * a.n * a.splits;
+  TB200_REQUIRE(units < (1ll << 31) - (1 << 20), TB200_ERR_UNSUPPORTED, "local_fwd_tc: %lld units of work", (long long)units);
+  p.units = (int)units;
+  // (walks of a causal training step grow with the tile; those of chunks hardly do, and their last tiles may be empty)
+  p.longest_first = a.window == NO_WINDOW && !a.table;
   p.wait_units = ptx::WAIT_LIMIT_UNITS;
-  CUtensorMap mq, mk, mv;
-  if (!local_map_rows(&mq, q, a.qs, a, p.tile_tokens, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
+  CUtensorMap mq, mk, mv, mo;
+  if (!local_map_rows(&mq, q, a.qs, a, p.tile_tokens, "q") || !local_map_rows(&mo, out, a.os, a, p.tile_tokens, "out") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
       !local_map_keys(&mv, v, a.vs, a, p.piece, "v"))
     return TB200_ERR_UNSUPPORTED;
   auto go = [&](auto tag, auto dsel) -> int {
     using T = decltype(tag);
     constexpr int D = decltype(dsel)::value;
-    return a.table ? launch_fwd<T, D, true>(mq, mk, mv, p, max_q, st) : launch_fwd<T, D, false>(mq, mk, mv, p, max_q, st);
+    return a.table ? launch_fwd<T, D, true>(mq, mk, mv, mo, p, st) : launch_fwd<T, D, false>(mq, mk, mv, mo, p, st);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

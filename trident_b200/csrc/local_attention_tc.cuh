@@ -14,10 +14,19 @@ constexpr int LOCAL_TC_COLS = 96;   // packed query rows of a step of the dK, dV
 bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void* k, const void* v, const void* out);
 int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, const void* v, const LocalArgs& a, int max_q,
                         int dtype, cudaStream_t st);
+// Serving form with few rows (max_q * G <= 64): keys on the tensor-memory lanes. `tokens` of a row tile.
+static inline int local_few_rows(const LocalArgs& a, int max_q) {  // columns of the kernel, 0: too many rows
+  const int64_t rows = (int64_t)max_q * a.G;
+  return !a.table || rows > 64 ? 0 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : 64));
+}
+int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, const LocalArgs& a, int columns, int dtype,
+                        cudaStream_t st);
+
 // Tensor maps (false with the error text set when the driver refuses one) and what they take.
 // (rows: boxes of `tokens` tokens with the heads of a group)
 bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, int tokens, const char* what);
 bool local_map_keys(CUtensorMap* map, const void* k, const int64_t* st, const LocalArgs& a, int piece, const char* what);
+int local_piece(const LocalArgs& a);  // rows of one copy of keys
 bool local_rows_ok(const void* p, const int64_t* st, const LocalArgs& a);
 bool local_keys_ok(const void* p, const int64_t* st, const LocalArgs& a);
 
