@@ -15,7 +15,7 @@
 //               sees, or whose page is outside the pool, are read at a page index past the end: zeros.
 //   warp 1      MMA issuer: S_t = Q_t K^T, O_t += P_t V (P_t from tensor memory, in two parts: the product
 //               starts when three quarters of P_t are there)
-//   warp 2      tensor-memory allocation
+//   warp 2      tensor-memory allocation; issues the bulk copies of output tiles
 //   warp 3      serving form: zeroes the rows of the last V tile behind the sequence's end (a probability
 //               of 0 times what an unused row holds, which may be NaN, would not be 0)
 //   warps 4-7   softmax of query tile 0, warps 8-11 of tile 1: one thread per row; scores stay in registers
@@ -76,6 +76,69 @@ __device__ inline void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* 
 }
 // the lowest n bits
 __device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+
+// Instructions whose order the compiler keeps (see exp_row).
+__device__ inline uint64_t fma2_ordered(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ inline uint64_t add2_ordered(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ inline float ex2_ordered(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ inline uint32_t cvt_ordered(float a, float b);
+template <>
+__device__ inline uint32_t cvt_ordered<__nv_bfloat16>(float a, float b) {
+  uint32_t r;
+  asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <>
+__device__ inline uint32_t cvt_ordered<__half>(float a, float b) {
+  uint32_t r;
+  asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+// P of a whole row of 128 raw scores: p = 2^(v scale - m), 16-bit, to tensor memory; returns the row's sum.
+// One warp of a query tile is alone on its scheduler's exponential unit, which takes an instruction every 8
+// cycles; the arguments, sums and conversions of neighbouring columns are issued in between (as three passes
+// over blocks of 32 columns, one after the other, a row took 1870 cycles instead of the 1024 of its
+// exponentials). `part` is called once the first 96 columns have been stored.
+template <typename T, typename Part>
+__device__ inline float exp_row(const uint32_t (&v)[4][32], uint64_t scale2, uint64_t negm2, uint32_t p_addr, Part part) {
+  constexpr int LAG = 3;  // pairs between an exponential and its use
+  uint64_t sum0 = am::pack2f(0.f, 0.f), sum1 = sum0;
+  float x[128];
+  uint32_t packed[16];
+  am::unpack2f(fma2_ordered(am::pack2u(v[0][0], v[0][1]), scale2, negm2), x[0], x[1]);
+#pragma unroll
+  for (int k = 0; k < 64 + LAG; ++k) {
+    if (k < 64) x[2 * k] = ex2_ordered(x[2 * k]);
+    if (k + 1 < 64)
+      am::unpack2f(fma2_ordered(am::pack2u(v[(k + 1) >> 4][(2 * k + 2) & 31], v[(k + 1) >> 4][(2 * k + 3) & 31]), scale2, negm2),
+                   x[2 * k + 2], x[2 * k + 3]);
+    if (k < 64) x[2 * k + 1] = ex2_ordered(x[2 * k + 1]);
+    if (k >= LAG) {
+      const int d = k - LAG;
+      if (d & 1) sum1 = add2_ordered(sum1, am::pack2f(x[2 * d], x[2 * d + 1]));
+      else sum0 = add2_ordered(sum0, am::pack2f(x[2 * d], x[2 * d + 1]));
+      packed[d & 15] = cvt_ordered<T>(x[2 * d], x[2 * d + 1]);
+      if ((d & 15) == 15) ptx::tmem_st16(p_addr + (d >> 4) * 16, packed);
+      if (d == 47 + 6) part();  // (the stores have had the time of six pairs)
+    }
+  }
+  float s0, s1;
+  am::unpack2f(am::add2(sum0, sum1), s0, s1);
+  return s0 + s1;
+}
 
 // A unit of work, as all roles of the CTA see it.
 struct Unit {
@@ -167,10 +230,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   //   p_full[t]   128 softmax threads, all of P_t stored             MMA issuer: the rest
   //   o_done[t]   tcgen05.commit after P_t V                         softmax: rescale, P_t over P_t, epilogue
   //   o_free[t]   128 softmax threads after the unit's O_t is read   MMA issuer: first P_t V of the next
-  //   turn[t]     128 softmax threads, per unit, the one that issued softmax of the other tile: output tile
-  //               the copy of output tile t once that has been read  into shared memory
-  // (Every barrier's next completion needs all its waiters to have seen the last one. turn counts all threads
-  // of a tile for that: with one arrival per tile, a warp without rows could be two units behind.)
+  //   out_full    128 softmax threads of a tile, per output tile     warp 2: bulk copy
+  //   out_free    warp 2, after the copy has read shared memory      softmax: next output tile into shared memory
+  //               (the output tiles of all units in order, tile 0 of a unit before tile 1)
+  // Every barrier's next completion needs all waiters of the last one to have seen that: a waiter can
+  // never be two phases behind.
   uint64_t* q_full = bars;           // [2]
   uint64_t* k_full = bars + 2;       // [2]
   uint64_t* k_empty = bars + 4;      // [2]
@@ -186,13 +250,19 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   uint64_t* p_part = bars + 21;      // [2]
   uint64_t* s_free = bars + 23;      // [2]
   uint64_t* o_free = bars + 25;      // [2]
-  uint64_t* turn = bars + 27;        // [2]
+  uint64_t* out_full = bars + 27;
+  uint64_t* out_free = bars + 28;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
   volatile uint32_t* abort_flag = tmem_slot + 1;  // [0] abort flag, [1] wait limit (ptx::mbar_wait)
 
   const LocalArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (PAGED && a.zero_tail) zero_tail_rows(reinterpret_cast<T*>(p.out), a, load_sequence(a, a.n - 1));
+  // query tile t's output leaves through shared memory: a full tile of a walk that is not cut
+  auto is_bulk = [&](const Unit& w, int t) {
+    const int tokens = w.seq.q_len - (w.t0 + t * p.tile_tokens);
+    return w.whole && (PAGED ? tokens >= p.tile_tokens : tokens > 0);
+  };
   // the last V tile has rows behind the sequence's end that its copies do not fill with zeros
   auto needs_fix = [&](const Unit& w) {
     return PAGED && w.m1 > w.m0 && w.kr.tile(w.m1 - 1) == (w.seq.kv_len - 1) / TILE && w.seq.kv_len % p.piece != 0;
@@ -200,7 +270,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 19; ++i) ptx::mbar_init(&bars[i], 1);
-    for (int i = 19; i < 29; ++i) ptx::mbar_init(&bars[i], 128);
+    for (int i = 19; i < 28; ++i) ptx::mbar_init(&bars[i], 128);
+    ptx::mbar_init(out_free, 1);
     abort_flag[0] = 0;
     abort_flag[1] = p.wait_units;
     ptx::fence_barrier_init();
@@ -353,6 +424,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
         const int steps = w.m1 - w.m0;
         bool fresh0 = true, fresh1 = true, first0 = true, first1 = true;  // no scores, no values of the tile yet
+        // the last step of each tile: its queries are not needed after that (-1: takes no part)
+        int last0 = steps - 1, last1 = steps - 1;
+        while (last0 >= 0 && !w.active(0, w.kr.tile(w.m0 + last0))) --last0;
+        while (last1 >= 0 && !w.active(1, w.kr.tile(w.m0 + last1))) --last1;
         auto do_scores = [&](auto tag, int i) {  // of step i
           constexpr int t = decltype(tag)::value;
           int& scores = t ? scores1 : scores0;
@@ -364,6 +439,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           ptx::tc_fence_after();
           issue_qk(t, (g + i) & 1);
           commit_(&s_full[t]);
+          if (i == (t ? last1 : last0)) commit_(&q_empty[t]);
           ++scores;
         };
         auto do_values = [&](auto tag, int i) {
@@ -414,19 +490,47 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         g += steps;
         // (a tile whose queries were brought, but that takes no part in this part of the walk, counts too)
         if (w.hi0 >= 0) {
-          if (fresh0) wait_(&q_full[0], queries0 & 1, 71);
-          commit_(&q_empty[0]);
+          if (fresh0) {
+            wait_(&q_full[0], queries0 & 1, 71);
+            commit_(&q_empty[0]);
+          }
           ++queries0;
         }
         if (w.hi1 >= 0) {
-          if (fresh1) wait_(&q_full[1], queries1 & 1, 72);
-          commit_(&q_empty[1]);
+          if (fresh1) {
+            wait_(&q_full[1], queries1 & 1, 72);
+            commit_(&q_empty[1]);
+          }
           ++queries1;
         }
       }
       // everything issued has completed before tensor memory is freed
       commit_(mma_drained);
       ptx::mbar_wait_drain(mma_drained, 0, abort_flag, a.status, 79);
+      __syncwarp();
+    } else if (warp == 2) {
+      // -------------------------------------------------------------- output tiles (one lane)
+      if (lane == 0) {
+        int outs = 0;
+        for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+          Unit w;
+          if (!unit_at<PAGED>(p, unit, &w)) continue;
+#pragma unroll 1
+          for (int t = 0; t < 2; ++t) {
+            if (!is_bulk(w, t)) continue;
+            ptx::mbar_wait(out_full, outs & 1, abort_flag, a.status, 67);
+#pragma unroll
+            for (int c = 0; c < NBOX; ++c)
+              ptx::tma_store_5d(&map_out, out_smem + c * BOX_BYTES, c * 64, 0, w.seq.q_begin + w.t0 + t * p.tile_tokens, w.hk,
+                                PAGED ? 0 : w.s);
+            ptx::bulk_commit();
+            ptx::bulk_wait_read();
+            ptx::mbar_arrive(out_free);
+            ++outs;
+          }
+        }
+        ptx::bulk_wait_done();
+      }
       __syncwarp();
     } else if (PAGED && warp == 3) {
       // -------------------------------------------------------------- zeros behind the sequence's end
@@ -462,10 +566,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const uint32_t s_addr = tmem_base + lane_off + COL_S + t * 128;
     const uint32_t o_addr = tmem_base + lane_off + COL_O + t * D;
     const uint32_t p_addr = tmem_base + lane_off + (P_SPLIT ? COL_P + t * 64 : COL_S + t * 128);
-    int count = 0, turns = 0;  // steps of this tile, units (over all units of the CTA)
-    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
-      Unit w;
-      if (!unit_at<PAGED>(p, unit, &w)) continue;
+    int count = 0, outs = 0;  // steps of this tile, output tiles of both (over all units of the CTA)
+    Unit w;
+    auto next_unit = [&](int unit) {  // the first from `unit` on that has something to do
+      while (unit < p.units && !unit_at<PAGED>(p, unit, &w)) unit += gridDim.x;
+      return unit;
+    };
+    for (int unit = next_unit(blockIdx.x); unit < p.units;) {
       const int first_token = w.t0 + t * p.tile_tokens;
       const int tokens = min(p.tile_tokens, w.seq.q_len - first_token);
       const int rows = tokens > 0 ? tokens * a.G : 0;
@@ -506,27 +613,16 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         uint32_t sr[4][32];
         float mx = -INFINITY;
         if (plain) {
-          float x0 = -INFINITY, x1 = -INFINITY;
-          auto reduce32 = [&](const uint32_t (&v)[32]) {
+          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              x0 = am::max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-              x1 = am::max3(x1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-            }
-          };
-          ptx::tmem_ld32(s_addr, sr[0]);
-          am::tmem_ld_wait_dep(sr[0]);
-          ptx::tmem_ld32(s_addr + 32, sr[1]);
-          reduce32(sr[0]);
-          am::tmem_ld_wait_dep(sr[1]);
-          ptx::tmem_ld32(s_addr + 64, sr[2]);
-          reduce32(sr[1]);
-          am::tmem_ld_wait_dep(sr[2]);
-          ptx::tmem_ld32(s_addr + 96, sr[3]);
-          reduce32(sr[2]);
-          am::tmem_ld_wait_dep(sr[3]);
-          reduce32(sr[3]);
-          mx = fmaxf(x0, x1) * p.scale_log2;
+          for (int q = 0; q < 4; ++q) ptx::tmem_ld32(s_addr + 32 * q, sr[q]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) am::tmem_ld_wait_dep(sr[q]);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = am::max3(x[q], __uint_as_float(sr[q][i]), __uint_as_float(sr[q][i + 1]));
+          mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
         } else {
           const uint64_t sc2 = am::pack2f(p.scale_log2, p.scale_log2);
           float x0 = -INFINITY, x1 = -INFINITY;
@@ -535,8 +631,19 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             // columns below pos + 1 - b0 are not in the future, those from pos - window + 1 - b0 on in the window
             const int b0 = j0 + 32 * q;
             const int64_t low = (int64_t)pos - a.window + 1 - b0;
-            const uint32_t seen = (all >> q) & 1u ? 0xffffffffu
-                                                  : low_bits(pos + 1 - b0) & (~low_bits(low < 0 ? 0 : (int)low) | low_bits(a.sinks - b0));
+            if ((all >> q) & 1u) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float s0, s1;
+                am::unpack2f(am::mul2(am::pack2u(v[i], v[i + 1]), sc2), s0, s1);
+                if (i & 2) x1 = am::max3(x1, s0, s1);
+                else x0 = am::max3(x0, s0, s1);
+                v[i] = __float_as_uint(s0);
+                v[i + 1] = __float_as_uint(s1);
+              }
+              return;
+            }
+            const uint32_t seen = low_bits(pos + 1 - b0) & (~low_bits(low < 0 ? 0 : (int)low) | low_bits(a.sinks - b0));
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float s0, s1;
@@ -591,10 +698,21 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           }
         }
         const float m_safe = m_used == -INFINITY ? 0.f : m_used;
-        {
-          const float to_log2 = plain ? p.scale_log2 : 1.f;
-          const uint64_t scale2 = am::pack2f(to_log2, to_log2);
-          const uint64_t negm2 = am::pack2f(-m_safe, -m_safe);
+        if constexpr (P_SPLIT) {
+          if (c > 0) {  // P(c) goes over P(c-1)
+            ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 84);
+            ptx::tc_fence_after();
+          }
+        }
+        const uint64_t negm2 = am::pack2f(-m_safe, -m_safe);
+        auto first_part = [&]() {
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(&p_part[t]);
+        };
+        if (plain) {
+          l += exp_row<T>(sr, am::pack2f(p.scale_log2, p.scale_log2), negm2, p_addr, first_part);
+        } else {
           uint64_t lsum = am::pack2f(0.f, 0.f), lsum_b = am::pack2f(0.f, 0.f);
           auto exp32 = [&](const uint32_t (&v)[32], int q) {
             uint32_t packed[16];
@@ -607,7 +725,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             float x[32];
 #pragma unroll
             for (int i = 0; i < 32; i += 2)
-              am::unpack2f(am::fma2(am::pack2u(v[i], v[i + 1]), scale2, negm2), x[i], x[i + 1]);
+              am::unpack2f(am::add2(am::pack2u(v[i], v[i + 1]), negm2), x[i], x[i + 1]);
 #pragma unroll
             for (int i = 0; i < 32; ++i) x[i] = am::ex2(x[i]);
 #pragma unroll
@@ -619,18 +737,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             }
             ptx::tmem_st16(p_addr + q * 16, packed);
           };
-          if constexpr (P_SPLIT) {
-            if (c > 0) {  // P(c) goes over P(c-1)
-              ptx::mbar_wait(&o_done[t], (c - 1) & 1, abort_flag, a.status, 84);
-              ptx::tc_fence_after();
-            }
-          }
           exp32(sr[0], 0);
           exp32(sr[1], 1);
           exp32(sr[2], 2);
-          ptx::tmem_st_wait();
-          ptx::tc_fence_before();
-          ptx::mbar_arrive(&p_part[t]);
+          first_part();
           exp32(sr[3], 3);
           float l0, l1;
           am::unpack2f(am::add2(lsum, lsum_b), l0, l1);
@@ -640,82 +750,81 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         ptx::tc_fence_before();
         ptx::mbar_arrive(&p_full[t]);
       }
-      const bool counted = count > before;
+      // What the epilogue needs of this unit; the next one is looked up while the last product runs.
+      const bool counted = count > before, whole = w.whole, bulk0 = is_bulk(w, 0), bulk1 = is_bulk(w, 1), bulk = t ? bulk1 : bulk0;
+      const bool queried = (t ? w.hi1 : w.hi0) >= 0 && w.m1 > w.m0;
+      const int head = w.hk * a.G + row_head;
+      const long long tok = w.seq.q_begin + token;
+      const bool some = l > 0.f;  // (a row without keys: zeros)
+      const float inv = some ? 1.f / l : 0.f;
+      T* orow = reinterpret_cast<T*>(p.out) + (long long)w.s * a.os[0] + head * a.os[1] + tok * a.os[2];
+      const long long prow = ((long long)w.split * a.tokens + tok) * a.H + head;
+      if (live) {
+        const float ls = some ? m_used * LN2 + logf(l) : -INFINITY;
+        if (!whole) a.part_lse[prow] = ls;
+        else if (!PAGED) p.lse[((long long)w.s * a.H + head) * a.tokens + tok] = ls;
+      }
+      unit = next_unit(unit + gridDim.x);
       if (counted) {
         ptx::mbar_wait(&o_done[t], (count - 1) & 1, abort_flag, a.status, 85);
         ptx::tc_fence_after();
       }
-      const int head = w.hk * a.G + row_head;
-      const long long tok = w.seq.q_begin + token;
-      const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys: zeros
-      // a full tile leaves through shared memory; copies of the other tile have read it (turn)
-      const bool bulk = w.whole && tokens > 0 && (!PAGED || tokens == p.tile_tokens);
-      if (t == 0) {
-        if (turns > 0) ptx::mbar_wait(&turn[1], (turns - 1) & 1, abort_flag, a.status, 86);
-      } else {
-        ptx::mbar_wait(&turn[0], turns & 1, abort_flag, a.status, 87);
-      }
-      ++turns;
+      const int mine = outs + (t && bulk0 ? 1 : 0);  // number of this output tile
+      outs += (bulk0 ? 1 : 0) + (bulk1 ? 1 : 0);
+      if (bulk && mine > 0) ptx::mbar_wait(out_free, (mine - 1) & 1, abort_flag, a.status, 86);
       if (warp_live) {
-        T* orow = reinterpret_cast<T*>(p.out) + (long long)w.s * a.os[0] + head * a.os[1] + tok * a.os[2];
-        const long long prow = ((long long)w.split * a.tokens + tok) * a.H + head;
-#pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t v[32];
+        const uint64_t inv2 = am::pack2f(inv, inv);
+        const bool zeros = !__all_sync(0xffffffffu, some || !live);  // (the columns hold what was there before)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          uint32_t v[2][32];
           __syncwarp();
-          if (counted) {
-            ptx::tmem_ld32(o_addr + q * 32, v);
-            ptx::tmem_ld_wait();
-          }
-          if (!(l > 0.f)) {  // (nothing was accumulated: the columns hold what was there before)
+          ptx::tmem_ld32(o_addr + h * 64, v[0]);
+          ptx::tmem_ld32(o_addr + h * 64 + 32, v[1]);
+          am::tmem_ld_wait_dep(v[0]);
+          am::tmem_ld_wait_dep(v[1]);
+          if (zeros) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0;
+            for (int e = 0; e < 64; ++e) v[e >> 5][e & 31] = some ? v[e >> 5][e & 31] : 0u;
           }
-          if (w.whole) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 64; e += 2) {
+            float x, y;
+            am::unpack2f(am::mul2(am::pack2u(v[e >> 5][e & 31], v[e >> 5][(e & 31) + 1]), inv2), x, y);
+            v[e >> 5][e & 31] = __float_as_uint(x);
+            v[e >> 5][(e & 31) + 1] = __float_as_uint(y);
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t* x = &v[e >> 2][(e & 3) * 8];
               uint4 o;
-              o.x = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 0]) * inv, __uint_as_float(v[e * 8 + 1]) * inv);
-              o.y = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 2]) * inv, __uint_as_float(v[e * 8 + 3]) * inv);
-              o.z = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 4]) * inv, __uint_as_float(v[e * 8 + 5]) * inv);
-              o.w = am::cvt_pair<T>(__uint_as_float(v[e * 8 + 6]) * inv, __uint_as_float(v[e * 8 + 7]) * inv);
-              if (bulk) {
-                const int chunk = q * 4 + e;
-                *reinterpret_cast<uint4*>(out_smem + (chunk >> 3) * BOX_BYTES + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = o;
-              } else if (live) {
-                *reinterpret_cast<uint4*>(orow + q * 32 + e * 8) = o;
-              }
+              o.x = am::cvt_pair<T>(__uint_as_float(x[0]), __uint_as_float(x[1]));
+              o.y = am::cvt_pair<T>(__uint_as_float(x[2]), __uint_as_float(x[3]));
+              o.z = am::cvt_pair<T>(__uint_as_float(x[4]), __uint_as_float(x[5]));
+              o.w = am::cvt_pair<T>(__uint_as_float(x[6]), __uint_as_float(x[7]));
+              if (bulk)
+                *reinterpret_cast<uint4*>(out_smem + h * BOX_BYTES + r * 128 + ((e ^ (r & 7)) << 4)) = o;
+              else if (live)
+                *reinterpret_cast<uint4*>(orow + h * 64 + e * 8) = o;
             }
-          } else if (live && l > 0.f) {  // (a part without keys is known by its lse)
-            float4* dst = reinterpret_cast<float4*>(a.part_out + prow * D + q * 32);
+          } else if (live && some) {  // (a part without keys is known by its lse)
+            uint4* dst = reinterpret_cast<uint4*>(a.part_out + prow * D + h * 64);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[e] = make_float4(__uint_as_float(v[e * 4]) * inv, __uint_as_float(v[e * 4 + 1]) * inv,
-                                   __uint_as_float(v[e * 4 + 2]) * inv, __uint_as_float(v[e * 4 + 3]) * inv);
+            for (int e = 0; e < 16; ++e) {
+              const uint32_t* x = &v[e >> 3][(e & 7) * 4];
+              dst[e] = make_uint4(x[0], x[1], x[2], x[3]);
+            }
           }
         }
       }
       ptx::tc_fence_before();
-      if ((t ? w.hi1 : w.hi0) >= 0 && w.m1 > w.m0) ptx::mbar_arrive(&o_free[t]);
+      if (queried) ptx::mbar_arrive(&o_free[t]);
       if (bulk) {
         ptx::fence_proxy_async_smem();
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
-      }
-      if (bulk && (threadIdx.x & 127) == 0) {
-#pragma unroll
-        for (int c = 0; c < NBOX; ++c)
-          ptx::tma_store_5d(&map_out, out_smem + c * BOX_BYTES, c * 64, 0, (int)(w.seq.q_begin + first_token), w.hk, PAGED ? 0 : w.s);
-        ptx::bulk_commit();
-        ptx::bulk_wait_read();
-      }
-      ptx::mbar_arrive(&turn[t]);
-      if (live) {
-        const float ls = l > 0.f ? m_used * LN2 + logf(l) : -INFINITY;
-        if (!w.whole) a.part_lse[((long long)w.split * a.tokens + tok) * a.H + head] = ls;
-        else if (!PAGED) p.lse[((long long)w.s * a.H + head) * a.tokens + tok] = ls;
+        ptx::mbar_arrive(out_full);
       }
     }
-    if ((threadIdx.x & 127) == 0) ptx::bulk_wait_done();
   }
   ptx::tc_fence_before();
   __syncthreads();
