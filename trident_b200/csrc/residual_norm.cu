@@ -248,10 +248,17 @@ __global__ void __launch_bounds__(CTA_ROW ? 512 : 256, CTA_ROW ? 2 : 4)
 
 // Backward: a CTA walks its part of the rows. x, r, dy and dh of a row arrive in a ring of shared-memory
 // stages by bulk copies (one thread issues them stages ahead, so loads stay in flight across the two
-// reductions of a row); a thread takes its vectors into registers, and keeps the column sums of its
-// columns in registers.
-template <typename T, int CHUNKS>
-__global__ void __launch_bounds__(512)
+// reductions of a row). A thread keeps its columns' w2 and gate * w1 (as long as the gate vector stays the
+// same) and their column sums in registers as fp32 pairs; per element of the four inputs that leaves a
+// conversion and about eight two-lane operations, where weights unpacked anew for every row and divisions
+// per thread bounded the kernel at 2.8 TB/s.
+__device__ inline float reciprocal(float v) {  // (one unit in the last place)
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
+  return y;
+}
+template <typename T, int CHUNKS, int THREADS>
+__global__ void __launch_bounds__(THREADS, CHUNKS <= 2 ? 2 : 1)
     resnorm_bwd_vec(T* __restrict__ dx, T* __restrict__ dr, T* __restrict__ dgate_rows, float* __restrict__ part_a,
                     float* __restrict__ part_b, const T* __restrict__ dh, const T* __restrict__ dy, const T* __restrict__ x,
                     const T* __restrict__ r, const T* __restrict__ w1, const T* __restrict__ w2, const T* __restrict__ gate,
@@ -279,8 +286,7 @@ __global__ void __launch_bounds__(512)
   pdl_wait();
   pdl_release();
   const int tensors = 2 + (dh ? 1 : 0) + (dy ? 1 : 0);
-  auto request = [&](int i) {  // (thread 0) row begin + i into its stage
-    const int st = i % stages;
+  auto request = [&](int i, int st) {  // (thread 0) row begin + i into stage st
     uint8_t* dst = ring + (size_t)st * 4 * bytes;
     const int64_t off = (begin + i) * a.cols;
     ptx::mbar_expect_tx(&full[st], (uint32_t)(tensors * bytes));
@@ -296,14 +302,16 @@ __global__ void __launch_bounds__(512)
     if (dy) copy(dy, 3);
   };
   if (threadIdx.x == 0)
-    for (int i = 0; i < stages && i < count; ++i) request(i);
+    for (int i = 0; i < stages && i < count; ++i) request(i, i);
 
-  uint64_t acc_a[CHUNKS][PAIRS], acc_b[CHUNKS][PAIRS];
-#pragma unroll
-  for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-    for (int i = 0; i < PAIRS; ++i) acc_a[c][i] = acc_b[c][i] = 0ull;
+  uint64_t acc_a[CHUNKS][PAIRS], acc_b[CHUNKS][PAIRS], gw[CHUNKS][PAIRS], wv[CHUNKS][PAIRS];
   auto col_of = [&](int c) { return (c * (int)blockDim.x + (int)threadIdx.x) * VEC; };
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) acc_a[c][i] = acc_b[c][i] = gw[c][i] = wv[c][i] = 0ull;
+    if (col_of(c) < cols) unpack2<T>(ld_cached(w2 + col_of(c)), wv[c]);
+  }
   auto flush = [&](float* dst, uint64_t (&acc)[CHUNKS][PAIRS]) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
@@ -319,132 +327,114 @@ __global__ void __launch_bounds__(512)
         }
     }
   };
-  int64_t current = gate_index(a, begin);
+  int64_t current = -1;  // gate vector whose product with w1 is in gw
+  int st = 0;
+  uint32_t ring_phase = 0;
+  float next1 = w1 ? rms1[begin] : 1.f, next2 = rms2[begin];
   for (int i = 0; i < count; ++i) {
     const int64_t row = begin + i, off = row * a.cols, gi = gate_index(a, row);
-    if (part_a && !per_row && gi != current) {  // the previous rows' stretch of one gate vector ends
-      flush(part_a + ((int64_t)blockIdx.x + current) * a.cols, acc_a);
+    if (gi != current) {
+      if (part_a && !per_row && current >= 0) flush(part_a + ((int64_t)blockIdx.x + current) * a.cols, acc_a);
       current = gi;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int col = col_of(c);
+        if (col >= cols) continue;
+        uint64_t w[PAIRS];
+        if (w1) unpack2<T>(ld_cached(w1 + col), gw[c]);
+        if (gate) unpack2<T>(ld_cached(gate + gi * a.cols + col), w);
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+          if (!w1) gw[c][k] = gate ? w[k] : splat2(1.f);
+          else if (gate) gw[c][k] = am::mul2(gw[c][k], w[k]);
+        }
+      }
     }
-    const T* g = gate ? gate + gi * a.cols : nullptr;
-    const float m1 = w1 ? rms1[row] : 1.f, m2 = rms2[row];
-    const float i1 = w1 ? 1.f / (m1 + a.eps) : 1.f, i2 = 1.f / (m2 + a.eps);
+    const float m1 = next1, m2 = next2;
+    if (i + 1 < count) {  // (a row ahead)
+      if (w1) next1 = rms1[row + 1];
+      next2 = rms2[row + 1];
+    }
+    const float i1 = w1 ? reciprocal(m1 + a.eps) : 1.f, i2 = reciprocal(m2 + a.eps);
     const uint64_t i1_2 = splat2(i1), i2_2 = splat2(i2), scale2 = splat2(a.scale);
-    const int st = i % stages;
     const uint8_t* src = ring + (size_t)st * 4 * bytes;
-    ptx::mbar_wait(&full[st], (i / stages) & 1, abort_flag, status, 141);
-    // t = dh w2 (then dY), u = x, v = y
+    ptx::mbar_wait(&full[st], ring_phase, abort_flag, status, 161);
+    // u = x i1, v = y, t = dh w2 i2 (then dY, then dY gate w1)
     uint64_t t[CHUNKS][PAIRS], u[CHUNKS][PAIRS], v[CHUNKS][PAIRS];
     uint4 dyr[CHUNKS];
     uint64_t s2 = 0ull;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int col = col_of(c);
-      if (col < cols) {
-        const uint8_t* at = src + col * (int)sizeof(T);
-        uint64_t w[PAIRS];
-        unpack2<T>(*reinterpret_cast<const uint4*>(at), u[c]);
-        unpack2<T>(*reinterpret_cast<const uint4*>(at + bytes), v[c]);
-        dyr[c] = dy ? *reinterpret_cast<const uint4*>(at + 3 * (size_t)bytes) : make_uint4(0, 0, 0, 0);
-        uint64_t b[PAIRS];  // the branch n * gate
-        if (w1) {
-          unpack2<T>(ld_cached(w1 + col), w);
+      const bool in = col < cols;
+      const uint8_t* at = src + col * (int)sizeof(T);
+      const uint4 none = make_uint4(0, 0, 0, 0);
+      unpack2<T>(in ? *reinterpret_cast<const uint4*>(at) : none, u[c]);
+      unpack2<T>(in ? *reinterpret_cast<const uint4*>(at + bytes) : none, v[c]);
+      dyr[c] = dy && in ? *reinterpret_cast<const uint4*>(at + 3 * (size_t)bytes) : none;
+      unpack2<T>(dh && in ? *reinterpret_cast<const uint4*>(at + 2 * (size_t)bytes) : none, t[c]);
 #pragma unroll
-          for (int k = 0; k < PAIRS; ++k) b[k] = am::mul2(am::mul2(u[c][k], i1_2), w[k]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < PAIRS; ++k) b[k] = u[c][k];
-        }
-        if (g) {
-          unpack2<T>(ld_cached(g + col), w);
-#pragma unroll
-          for (int k = 0; k < PAIRS; ++k) b[k] = am::mul2(b[k], w[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < PAIRS; ++k) v[c][k] = am::fma2(scale2, v[c][k], b[k]);
-        if (dh) {
-          unpack2<T>(*reinterpret_cast<const uint4*>(at + 2 * (size_t)bytes), t[c]);
-          unpack2<T>(ld_cached(w2 + col), w);
-#pragma unroll
-          for (int k = 0; k < PAIRS; ++k) {
-            acc_b[c][k] = am::fma2(t[c][k], am::mul2(v[c][k], i2_2), acc_b[c][k]);
-            t[c][k] = am::mul2(t[c][k], w[k]);
-            s2 = am::fma2(t[c][k], v[c][k], s2);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < PAIRS; ++k) t[c][k] = 0ull;
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < PAIRS; ++k) t[c][k] = u[c][k] = v[c][k] = 0ull;
-        dyr[c] = make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < PAIRS; ++k) {
+        u[c][k] = am::mul2(u[c][k], i1_2);
+        v[c][k] = am::fma2(u[c][k], gw[c][k], am::mul2(scale2, v[c][k]));
+        t[c][k] = am::mul2(t[c][k], i2_2);
+        acc_b[c][k] = am::fma2(t[c][k], v[c][k], acc_b[c][k]);
+        t[c][k] = am::mul2(t[c][k], wv[c][k]);
+        s2 = am::fma2(t[c][k], v[c][k], s2);
       }
     }
     // (the reduction's barrier also says that every thread has taken its part of the stage)
-    ptx::fence_proxy_async_smem();
     const float sum2 = row_reduce<true, false>(hsum2(s2), slot, phase);
-    if (threadIdx.x == 0 && i + stages < count) request(i + stages);
-    const float k2 = m2 > 0.f ? sum2 * i2 * i2 * inv_n / m2 : 0.f;
-    const uint64_t nk2 = splat2(-k2);
+    if (threadIdx.x == 0 && i + stages < count) request(i + stages, st);
+    if (++st == stages) {
+      st = 0;
+      ring_phase ^= 1u;
+    }
+    // k2 = sum(dh w2 y) i2^2 / (N rms2); one factor i2 is in the sum
+    const uint64_t nk2 = splat2(m2 > 0.f ? -(sum2 * i2 * inv_n * reciprocal(m2)) : 0.f);
     uint64_t s1 = 0ull;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int col = col_of(c);
-      if (col < cols) {
-        uint64_t w[PAIRS];
-        unpack2<T>(dyr[c], w);
+      uint64_t w[PAIRS];
+      unpack2<T>(dyr[c], w);
+#pragma unroll
+      for (int k = 0; k < PAIRS; ++k) {
+        t[c][k] = am::fma2(v[c][k], nk2, am::add2(t[c][k], w[k]));
+        v[c][k] = am::mul2(scale2, t[c][k]);
+      }
+      if (col < cols) st_stream(dr + off + col, pack2<T>(v[c]));
+      if (per_row && col < cols) {  // a gate of its own: its gradient, and the sum A with the gate in it
+        uint64_t g[PAIRS];
+        unpack2<T>(ld_cached(gate + gi * a.cols + col), g);
+        if (w1) unpack2<T>(ld_cached(w1 + col), w);
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) {
-          // dY = dy + dh w2 i2 - y k2
-          t[c][k] = am::fma2(t[c][k], i2_2, am::fma2(v[c][k], nk2, w[k]));
-          v[c][k] = am::mul2(scale2, t[c][k]);
+          const uint64_t ax = am::mul2(t[c][k], u[c][k]);
+          v[c][k] = w1 ? am::mul2(ax, w[k]) : ax;
+          acc_a[c][k] = am::fma2(ax, g[k], acc_a[c][k]);
         }
-        st_stream(dr + off + col, pack2<T>(v[c]));
-        // column sum A: dY x i1 (times a gate of its own per row); v = dY g w1
-        uint64_t ax[PAIRS];
+        if (dgate_rows) st_stream(dgate_rows + off + col, pack2<T>(v[c]));
+      }
 #pragma unroll
-        for (int k = 0; k < PAIRS; ++k) ax[k] = am::mul2(t[c][k], am::mul2(u[c][k], i1_2));
-        if (dgate_rows) {
-          uint64_t dg[PAIRS];
-          if (w1) unpack2<T>(ld_cached(w1 + col), w);
-#pragma unroll
-          for (int k = 0; k < PAIRS; ++k) dg[k] = w1 ? am::mul2(ax[k], w[k]) : ax[k];
-          st_stream(dgate_rows + off + col, pack2<T>(dg));
-        }
-        if (g) {
-          unpack2<T>(ld_cached(g + col), w);
-#pragma unroll
-          for (int k = 0; k < PAIRS; ++k) {
-            t[c][k] = am::mul2(t[c][k], w[k]);
-            if (per_row) ax[k] = am::mul2(ax[k], w[k]);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < PAIRS; ++k) acc_a[c][k] = am::add2(acc_a[c][k], ax[k]);
-        if (w1) {
-          unpack2<T>(ld_cached(w1 + col), w);
-#pragma unroll
-          for (int k = 0; k < PAIRS; ++k) {
-            t[c][k] = am::mul2(t[c][k], w[k]);
-            s1 = am::fma2(t[c][k], u[c][k], s1);
-          }
-        }
+      for (int k = 0; k < PAIRS; ++k) {
+        if (!per_row) acc_a[c][k] = am::fma2(t[c][k], u[c][k], acc_a[c][k]);
+        t[c][k] = am::mul2(t[c][k], gw[c][k]);
+        s1 = am::fma2(t[c][k], u[c][k], s1);
       }
     }
+    // dx = i1 (t - u k1'), k1' = sum(t x) i1 / (N rms1): sum(t u) / (N rms1) (w1 null: dx = t)
     uint64_t nk1 = 0ull;
     if (w1) {
       const float sum1 = row_reduce<true, false>(hsum2(s1), slot, phase);
-      nk1 = splat2(m1 > 0.f ? -(sum1 * i1 * i1 * inv_n / m1) : 0.f);
+      nk1 = splat2(m1 > 0.f ? -(sum1 * inv_n * reciprocal(m1) * (m1 + a.eps)) : 0.f);
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int col = col_of(c);
-      if (col < cols) {
 #pragma unroll
-        for (int k = 0; k < PAIRS; ++k) t[c][k] = am::fma2(u[c][k], nk1, am::mul2(t[c][k], i1_2));
-        st_stream(dx + off + col, pack2<T>(t[c]));
-      }
+      for (int k = 0; k < PAIRS; ++k) t[c][k] = am::mul2(i1_2, am::fma2(u[c][k], nk1, t[c][k]));
+      if (col < cols) st_stream(dx + off + col, pack2<T>(t[c]));
     }
   }
   if (part_a) flush(part_a + ((int64_t)blockIdx.x + (per_row ? 0 : current)) * a.cols, acc_a);
@@ -552,7 +542,9 @@ BackwardPlan plan_backward(int64_t cols, bool ptrs_ok) {
   constexpr int VEC = Traits<T>::VEC;
   if (!ptrs_ok || cols % VEC != 0 || cols > 2048 * VEC) return p;
   const int64_t vecs = cols / VEC, stage = 4 * cols * (int64_t)sizeof(T);
-  p.chunks = vecs <= 512 ? 1 : (vecs <= 1024 ? 2 : 4);
+  // Two vectors a thread where the row has them: with one, half of a thread's instructions were the row's
+  // two reductions, barriers and addresses.
+  p.chunks = vecs <= 128 ? 1 : (vecs <= 512 ? 2 : 4);
   p.threads = (int)(ceil_div(ceil_div(vecs, p.chunks), 32) * 32);
   p.stages = (int)(RING_BYTES / stage < 3 ? RING_BYTES / stage : 3);
   int64_t per_sm = 220 * 1024 / (p.stages * stage + 2048);
@@ -654,8 +646,8 @@ extern "C" int tb200_gated_residual_rms_norm_bwd(void* dx, void* dr, void* dw1, 
     float* part_b = want_b ? (float*)workspace + (n + vectors) * cols : nullptr;
     int rc = 0;
     if (plan.chunks) {
-      auto go = [&](auto c) -> int {
-        auto kern = resnorm_bwd_vec<T, decltype(c)::value>;
+      auto go = [&](auto c, auto most) -> int {
+        auto kern = resnorm_bwd_vec<T, decltype(c)::value, decltype(most)::value>;
         static std::atomic<unsigned long long> done{0};
         const cudaError_t e = smem_optin_per_device(done, reinterpret_cast<const void*>(kern), RING_BYTES);
         if (e != cudaSuccess) {
@@ -668,7 +660,10 @@ extern "C" int tb200_gated_residual_rms_norm_bwd(void* dx, void* dr, void* dw1, 
                          device_status_ptr());
         return launch_status("resnorm_bwd_vec");
       };
-      rc = plan.chunks == 1 ? go(IntC<1>{}) : plan.chunks == 2 ? go(IntC<2>{}) : go(IntC<4>{});
+      rc = plan.chunks == 1   ? go(IntC<1>{}, IntC<128>{})
+           : plan.chunks == 2 ? go(IntC<2>{}, IntC<256>{})
+           : plan.threads <= 256 ? go(IntC<4>{}, IntC<256>{})
+                                 : go(IntC<4>{}, IntC<512>{});
     } else {
       resnorm_bwd_generic<T><<<(unsigned)n, 256, 0, st>>>(
           (T*)dx, (T*)dr, per_row ? (T*)dgate : nullptr, part_a, part_b, (const T*)dh, (const T*)dy, (const T*)x, (const T*)r,
