@@ -12,7 +12,8 @@ import os
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-LIB_PATH = os.environ.get("TB200_LIB", os.path.join(_HERE, "libtb200.so"))
+_OWN_LIB = os.path.join(_HERE, "libtb200.so")
+LIB_PATH = os.environ.get("TB200_LIB", _OWN_LIB)
 
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -170,18 +171,29 @@ def _require_cuda(*tensors):
             raise Tb200Error("trident_b200 kernels run on CUDA tensors only (no CPU fallback)")
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    """Entry point `name`, taking stride tuples: the direct one of the _fastcall extension, or a ctypes call
+    where another library than the package's own is used."""
+    function = getattr(load(), name)
+    if LIB_PATH == _OWN_LIB:
+        from trident_b200 import _fastcall
+
+        return getattr(_fastcall, name)
+    return lambda *args: function(*(_stride_array(a) if isinstance(a, tuple) else a for a in args))
+
+
 def _call(name, like, *args):
     """Calls entry point `name` on the device of tensor `like`, made current if it is not (a launch goes
     to the current device), and that device's current stream. (The raw handles of torch._C: a Stream
     object and a device context cost more host time than the launch of a small kernel.)"""
-    function = getattr(load(), name)
     index = like.device.index
     stream = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
-        status = function(*args, stream)
+        status = _entry(name)(*args, stream)
     else:
         with torch.cuda.device(index):
-            status = function(*args, stream)
+            status = _entry(name)(*args, stream)
     if status != 0:
         _check(status, name)
 
@@ -213,10 +225,7 @@ def _stride_array(strides):
 
 
 def _strides4(t):
-    return _stride_array(t.stride())
-
-
-_strides3 = _strides4
+    return (c_i64 * 4)(*t.stride())
 
 
 # --------------------------------------------------------------------------- row ops
@@ -521,7 +530,7 @@ def window_attention_fwd(out, lse, q, k, v, window, sinks, scale):
     B, H, S, D = q.shape
     _call(
         "tb200_window_attention_fwd", q, _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), B, H, k.shape[1], S, D,
-        _strides4(q), _strides4(k), _strides4(v), _strides4(out), window, sinks, scale, dtype_code(q.dtype),
+        q.stride(), k.stride(), v.stride(), out.stride(), window, sinks, scale, dtype_code(q.dtype),
     )
 
 
@@ -537,8 +546,8 @@ def window_attention_bwd(dq, dk, dv, dout, q, k, v, out, lse, workspace, window,
     B, H, S, D = q.shape
     _call(
         "tb200_window_attention_bwd", q, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(q), _ptr(k), _ptr(v),
-        _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel(), B, H, k.shape[1], S, D, _strides4(q), _strides4(k),
-        _strides4(v), _strides4(out), _strides4(dout), _strides4(dq), _strides4(dk), _strides4(dv), window, sinks,
+        _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel(), B, H, k.shape[1], S, D, q.stride(), k.stride(),
+        v.stride(), out.stride(), dout.stride(), dq.stride(), dk.stride(), dv.stride(), window, sinks,
         scale, dtype_code(q.dtype),
     )
 
@@ -559,8 +568,8 @@ def paged_attention(out, q, key_cache, value_cache, table, context, starts, work
     _call(
         "tb200_paged_attention", q, _ptr(out), _ptr(q), _ptr(key_cache), _ptr(value_cache), _ptr(table),
         _ptr(context), _ptr(starts), _ptr(workspace), 0 if workspace is None else workspace.numel(), T, n, H,
-        kv_heads, D, page, pages, blocks, table.stride(0), _strides3(q), _strides4(key_cache),
-        _strides4(value_cache), _strides3(out), max_query_length, max_context_length, window, sinks, scale,
+        kv_heads, D, page, pages, blocks, table.stride(0), q.stride(), key_cache.stride(),
+        value_cache.stride(), out.stride(), max_query_length, max_context_length, window, sinks, scale,
         zero_tail, dtype_code(q.dtype),
     )
 
@@ -571,6 +580,6 @@ def paged_cache_append(key_cache, value_cache, k, v, table, context, starts):
     n, blocks = table.shape
     _call(
         "tb200_paged_cache_append", k, _ptr(key_cache), _ptr(value_cache), _ptr(k), _ptr(v), _ptr(table),
-        _ptr(context), _ptr(starts), T, n, kv_heads, D, page, pages, blocks, table.stride(0), _strides4(key_cache),
-        _strides4(value_cache), _strides3(k), _strides3(v), dtype_code(k.dtype),
+        _ptr(context), _ptr(starts), T, n, kv_heads, D, page, pages, blocks, table.stride(0), key_cache.stride(),
+        value_cache.stride(), k.stride(), v.stride(), dtype_code(k.dtype),
     )

@@ -6,12 +6,14 @@ Usage: python -m trident_b200.build [--force] [--verbose]
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "libtb200.so")
+FASTCALL_PATH = os.path.join(HERE, "_fastcall.so")  # direct Python entry points (csrc/fastcall.c)
 
 SOURCES = [
     "api.cu",
@@ -89,11 +91,27 @@ def build(force=False, verbose=False):
         results = list(pool.map(lambda s: _compile(s, force, verbose), SOURCES))
     objs = [r[0] for r in results]
     if force or _stale(LIB_PATH, objs):
-        cmd = [_nvcc(), "-shared", "-o", LIB_PATH, *objs, "-lcudart", "-Xlinker", "-z,defs"]
+        cmd = [_nvcc(), "-shared", "-o", LIB_PATH, *objs, "-lcudart", "-Xlinker", "-z,defs", "-Xlinker", "-soname,libtb200.so"]
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    _build_fastcall(force)
     return LIB_PATH
+
+
+def _build_fastcall(force):
+    """The CPython extension beside the library, linked against it."""
+    source = os.path.join(CSRC, "fastcall.c")
+    if not force and not _stale(FASTCALL_PATH, [source, LIB_PATH, os.path.join(HERE, "..", "include", "tb200.h")]):
+        return
+    cmd = [
+        os.environ.get("CC", "gcc"), "-std=c11", "-O2", "-Wall", "-shared", "-fPIC",
+        "-I" + sysconfig.get_paths()["include"], source, "-o", FASTCALL_PATH,
+        LIB_PATH, "-Wl,-rpath,$ORIGIN",
+    ]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building the Python entry points failed:\n{res.stdout}\n{res.stderr}")
 
 
 if __name__ == "__main__":

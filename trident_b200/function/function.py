@@ -5,7 +5,7 @@ import math
 
 import torch
 
-from trident_b200 import operation
+from trident_b200 import operation, util
 
 __all__ = [
     "gated_residual_rms_norm",
@@ -49,7 +49,10 @@ def gated_residual_rms_norm(
 
     See GatedResidualRMSNorm for details.
     """
-    return operation.GatedResidualRMSNorm.apply(input, residual, post_weight, pre_weight, gate, residual_scale, eps)
+    args = (input, residual, post_weight, pre_weight, gate, residual_scale, eps)
+    if util.needs_grad(input, residual, post_weight, pre_weight, gate):
+        return operation.GatedResidualRMSNorm.apply(*args)
+    return operation.GatedResidualRMSNorm.run(*args)[0]
 
 
 def geglu(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None, use_accelerator: bool = False):
@@ -230,7 +233,9 @@ def sliding_window_attention(
     See WindowAttention for more details.
     """
     scale = 1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None else softmax_scale
-    return operation.WindowAttention.apply(query, key, value, window_size, num_sinks, scale)
+    if util.needs_grad(query, key, value):
+        return operation.WindowAttention.apply(query, key, value, window_size, num_sinks, scale)
+    return operation.WindowAttention.run(query, key, value, window_size, num_sinks, scale)[0]
 
 
 def softmax(input: torch.Tensor, dim: int = None):

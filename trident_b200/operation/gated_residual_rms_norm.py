@@ -12,10 +12,10 @@ def rows_per_gate(input: torch.Tensor, gate: torch.Tensor) -> int:
     """How many rows of `input` share one gate vector: 0 for one vector in all. `gate` has the features
     of `input` and, if more dimensions, the leading dimensions of `input` with ones from some
     dimension on."""
-    if gate.shape[-1:] != input.shape[-1:] or gate.dim() > input.dim():
-        raise ValueError(f"A gate of shape {tuple(gate.shape)} does not fit an input of shape {tuple(input.shape)}.")
-    if gate.dim() == 1:
+    if gate.dim() == 1 and gate.shape[0] == input.shape[-1]:
         return 0
+    if gate.shape[-1:] != input.shape[-1:]:
+        raise ValueError(f"A gate of shape {tuple(gate.shape)} does not fit an input of shape {tuple(input.shape)}.")
     if gate.dim() != input.dim():
         raise ValueError(f"A gate of shape {tuple(gate.shape)} does not fit an input of shape {tuple(input.shape)}.")
     lead, wanted = gate.shape[:-1], input.shape[:-1]
@@ -38,17 +38,29 @@ def rows_per_gate(input: torch.Tensor, gate: torch.Tensor) -> int:
 class GatedResidualRMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, *args: Any, **kwargs: Any):
-        input, residual, post_weight, pre_weight, gate, residual_scale, eps = args
+        outputs, saved, group = GatedResidualRMSNorm.run(*args)
 
-        if input.dim() < 1 or input.shape[-1] == 0:
+        ctx.save_for_backward(*saved)
+        ctx.set_materialize_grads(False)
+        ctx.group = group
+        ctx.residual_scale = args[5]
+        ctx.eps = args[6]
+
+        return outputs
+
+    @staticmethod
+    def run(input, residual, post_weight, pre_weight, gate, residual_scale, eps):
+        """The forward pass: ((output, output_residual), what the backward pass needs, rows per gate)."""
+        shape = input.shape
+        if len(shape) < 1 or shape[-1] == 0:
             raise ValueError("input should have at least one feature.")
-        if residual.shape != input.shape:
+        if residual.shape != shape:
             raise ValueError("input and residual should have the same shape.")
         if pre_weight is None:
             raise ValueError("pre_weight should be given.")
-        x_size = input.shape[-1]
+        x_size = shape[-1]
         for weight in (post_weight, pre_weight):
-            if weight is not None and weight.shape != (x_size,):
+            if weight is not None and (weight.dim() != 1 or weight.shape[0] != x_size):
                 raise ValueError(f"A weight should have the shape ({x_size},), got {tuple(weight.shape)}.")
         group = 0 if gate is None else rows_per_gate(input, gate)
         for tensor in (residual, post_weight, pre_weight, gate):
@@ -58,9 +70,9 @@ class GatedResidualRMSNorm(torch.autograd.Function):
         _lib.require_one_device(input, residual, post_weight, pre_weight, gate)
 
         util.push_trace("GatedResidualRMSNorm.__forward")
-        input, residual, post_weight, pre_weight, gate = (
-            None if t is None else t.contiguous() for t in (input, residual, post_weight, pre_weight, gate)
-        )
+        input, residual, pre_weight = input.contiguous(), residual.contiguous(), pre_weight.contiguous()
+        post_weight = None if post_weight is None else post_weight.contiguous()
+        gate = None if gate is None else gate.contiguous()
         y_size = input.numel() // x_size
         output, output_residual = torch.empty_like(input), torch.empty_like(input)
         rms = torch.empty(2, y_size, device=input.device, dtype=torch.float32)
@@ -84,13 +96,7 @@ class GatedResidualRMSNorm(torch.autograd.Function):
         util.pop_trace()
         util.pop_trace()
 
-        ctx.save_for_backward(input, residual, post_weight, pre_weight, gate, rms)
-        ctx.set_materialize_grads(False)
-        ctx.group = group
-        ctx.residual_scale = residual_scale
-        ctx.eps = eps
-
-        return output, output_residual
+        return (output, output_residual), (input, residual, post_weight, pre_weight, gate, rms), group
 
     @staticmethod
     def backward(ctx: Any, *grad_outputs: Any):

@@ -32,16 +32,27 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, *args: Any, **kwargs: Any):
-        query, key, value, window_size, num_sinks, softmax_scale = args
+        output, log_sum_exp, window_size, num_sinks = WindowAttention.run(*args)
 
+        ctx.save_for_backward(*args[:3], output, log_sum_exp)
+        ctx.window_size = window_size
+        ctx.num_sinks = num_sinks
+        ctx.softmax_scale = args[5]
+
+        return output
+
+    @staticmethod
+    def run(query, key, value, window_size, num_sinks, softmax_scale):
+        """The forward pass: (output, log-sum-exp of every score row, window and sinks cut to the length)."""
         if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
             raise ValueError("The dimension of query, key and value should be 4.")
         if key.shape != value.shape:
             raise ValueError("key and value should have the same shape.")
         batch, heads, y_size, x_size = query.shape
-        if (key.shape[0], key.shape[2], key.shape[3]) != (batch, y_size, x_size):
+        key_batch, kv_heads, key_length, key_size = key.shape
+        if key_batch != batch or key_length != y_size or key_size != x_size:
             raise ValueError("query and key should have the same batch, length and head size.")
-        check_heads(heads, key.shape[1], x_size)
+        check_heads(heads, kv_heads, x_size)
         check_window(window_size, num_sinks)
         if query.dtype != key.dtype or query.dtype != value.dtype:
             raise ValueError("query, key and value should have the same dtype.")
@@ -52,18 +63,13 @@ class WindowAttention(torch.autograd.Function):
 
         util.push_trace("WindowAttention.__forward")
         output = torch.empty_like(query)  # laid out as query is
-        log_sum_exp = torch.empty(batch, heads, y_size, device=query.device, dtype=torch.float32)
+        log_sum_exp = torch.empty((batch, heads, y_size), device=query.device, dtype=torch.float32)
         util.push_trace("tb200_window_attention_fwd")
         _lib.window_attention_fwd(output, log_sum_exp, query, key, value, window_size, num_sinks, softmax_scale)
         util.pop_trace()
         util.pop_trace()
 
-        ctx.save_for_backward(query, key, value, output, log_sum_exp)
-        ctx.window_size = window_size
-        ctx.num_sinks = num_sinks
-        ctx.softmax_scale = softmax_scale
-
-        return output
+        return output, log_sum_exp, window_size, num_sinks
 
     @staticmethod
     def backward(ctx: Any, *grad_outputs: Any):

@@ -8,6 +8,7 @@ __all__ = [
     "calculate_fan_in_and_fan_out",
     "fill",
     "is_pow2",
+    "needs_grad",
     "size_and_stride",
     "push_trace",
     "pop_trace",
@@ -29,6 +30,15 @@ def fill(inp, val):
 def is_pow2(value):
     """True for 1, 2, 4, ... (trident/util/util.py:61-62)."""
     return value != 0 and (value & (value - 1)) == 0
+
+
+def needs_grad(*tensors):
+    """Whether autograd would record an operation on these tensors (None allowed)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def size_and_stride(input: torch.Tensor, dim: int):
