@@ -324,3 +324,33 @@ def test_no_rows(device):
     h, y = trident.function.gated_residual_rms_norm(x, x, w, w, g)
     (h.sum() + y.sum()).backward()
     assert h.shape == x.shape and torch.all(w.grad == 0) and torch.all(g.grad == 0)
+
+
+@pytest.mark.gpu
+def test_more_than_32_bit_offsets(device):
+    """The last rows of more than 2^31 elements."""
+    cols, dt = 4096, torch.bfloat16
+    rows = 2 ** 31 // cols + 5
+    generator = torch.Generator(device=device).manual_seed(400)
+    x, r, dh, dy = (torch.randn(rows, cols, dtype=dt, device=device, generator=generator) for _ in range(4))
+    w1, w2, g = (torch.randn(cols, dtype=dt, device=device, generator=generator) for _ in range(3))
+    x.requires_grad_(True)
+    r.requires_grad_(True)
+    h, y = trident.function.gated_residual_rms_norm(x, r, w1, w2, g, 0.9, EPS)
+    dx, dr = torch.autograd.grad((h, y), (x, r), (dh, dy))
+    tail = tuple(t.detach()[-6:].cpu() for t in (x, r)) + tuple(t.cpu() for t in (w1, w2, g)) + tuple(t[-6:].cpu() for t in (dh, dy))
+    want = _want(tail, 0.9)
+    for name, got in (("h", h), ("y", y), ("input", dx), ("residual", dr)):
+        _check(got[-6:], want[name], dt, name)
+
+
+def test_library_refuses_before_launch():
+    from trident_b200 import _lib
+
+    call = _lib.load().tb200_gated_residual_rms_norm_fwd
+
+    def fwd(out=8, x=8, post=None, pre=8, gate=None, rows=2, cols=16, group=0, dtype=0):
+        return call(out, 8, 8, 8, x, 8, post, pre, gate, rows, cols, group, 1.0, 1e-6, dtype, None)
+
+    assert fwd(out=None) < 0 and fwd(x=None) < 0 and fwd(pre=None) < 0 and fwd(rows=-1) < 0 and fwd(cols=0) < 0
+    assert fwd(gate=8, group=-1) < 0 and fwd(dtype=9) < 0 and fwd(rows=0) == 0

@@ -374,3 +374,143 @@ def test_nothing_to_do(device):
     out = attend(torch.ones(3, 2, 64, device=device), kc, kc, table, none, torch.zeros(1, dtype=torch.int32, device=device))
     assert torch.all(out == 0)
     append(torch.zeros(0, 1, 64, device=device), torch.zeros(0, 1, 64, device=device), kc, kc, table, none)
+
+
+def _random(low, high, count, seed):
+    return torch.randint(low, high, (count,), generator=util.seeded(seed)).tolist()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window, sinks", [(None, 0), (70, 5)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_sequences(D, window, sinks, dtype, device):
+    """Many more pieces of work than SMs, of very unequal lengths, some of them empty: chunks and single tokens."""
+    n, KV = 90, 6
+    new = _random(0, 40, n, 60)
+    context = [t + c if i % 7 else t for i, (t, c) in enumerate(zip(new, _random(0, 400, n, 61)))]
+    for _ in range(2):
+        _compare(context, new, KV, 2, D, 16, dtype, device, window, sinks, seed=62)
+    _compare([1 + c for c in _random(0, 700, n, 63)], [1] * n, KV, 4, D, 16, dtype, device, window, sinks, seed=64, decode=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G, t", [(1, 17), (4, 6), (16, 2), (1, 64), (8, 8), (5, 9), (64, 1), (33, 1)])
+@pytest.mark.parametrize("window, sinks", [(None, 0), (500, 3)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_up_to_64_rows(D, window, sinks, G, t, dtype, device):
+    """Every width of the kernel for few rows, with the walk whole and cut."""
+    _compare([1500, t, 3], [t, t, 0], 2, G, D, 16, dtype, device, window, sinks, seed=65, max_query_length=t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.3, 0.7])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_scales(D, scale, dtype, device):
+    cache = Cache([700, 150], 1, D, 16, dtype, device, seed=66)
+    for new, decode in (([1, 1], True), ([90, 150], False)):
+        q = util.randn(sum(new), 4, D, seed=67).to(dtype)
+        got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev,
+                     None if decode else _offsets(new, device), softmax_scale=scale)
+        ref.check(got, _want(q, cache, new, 0, 0, scale, dtype), f"{new}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_large_scores(D, dtype, device):
+    """Scores of hundreds: one key takes almost all the weight, the running maximum moves by large steps."""
+    cache = Cache([1700, 300], 2, D, 16, dtype, device, seed=68)
+    for new in ([1, 1], [100, 77]):
+        q = util.randn(sum(new), 4, D, seed=69, std=25.0).to(dtype)
+        got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, _offsets(new, device))
+        ref.check(got, _want(q, cache, new, 0, 0, D ** -0.5, dtype), f"{new}")
+
+
+@pytest.mark.gpu
+def test_offsets_and_contexts_out_of_order(device, dtype):
+    """Offsets that fall and negative contexts count as no tokens and no keys; other sequences keep their results."""
+    D = 64
+    cache = Cache([60, 33, 20], 2, D, 16, dtype, device, seed=70)
+    q = util.randn(9, 4, D, seed=71).to(dtype)
+    offsets = torch.tensor([0, 5, 3, 9], dtype=torch.int32, device=device)  # 5 tokens, none, tokens 3 to 8
+    context = cache.context_dev.clone()
+    context[0] = -(2 ** 31)
+    got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, context, offsets, window_size=10, num_sinks=2)
+    cache.context[0], cache.keys[0], cache.values[0] = 0, cache.keys[0][:0], cache.values[0][:0]
+    assert torch.all(got[:3] == 0) and torch.isfinite(got.float()).all()
+    mine = torch.empty_like(q)
+    mine[3:] = q[3:]
+    want = _want(mine[3:], Third(cache, 2), [6], 10, 2, D ** -0.5, dtype)
+    ref.check(got[5:], tuple(t[2:] for t in want), "third sequence")  # (rows 3 and 4 belong to two sequences)
+    kc = cache.key_cache.clone()
+    k = util.randn(9, 2, D, seed=72).to(dtype).to(device)
+    append(k, k, kc, kc.clone(), cache.table_dev, context, offsets)
+    changed = (kc != cache.key_cache) & ~(torch.isnan(kc.float()) & torch.isnan(cache.key_cache.float()))
+    assert changed.flatten(2).any(-1).sum() == 6  # the third sequence's six tokens
+
+
+class Third:
+    """One sequence of a cache, as _want sees a cache."""
+
+    def __init__(self, cache, s):
+        self.context, self.keys, self.values = [cache.context[s]], [cache.keys[s]], [cache.values[s]]
+        self.key_cache = cache.key_cache
+
+
+@pytest.mark.gpu
+def test_shared_pages(device, dtype):
+    """Sequences may share the pages of a common beginning."""
+    D, page = 128, 16
+    cache = Cache([200], 2, D, page, dtype, device, seed=73)
+    q = util.randn(3, 4, D, seed=74).to(dtype)
+    table = cache.table_dev.expand(3, -1)  # (a stride of zero: one row for all)
+    lengths = [200, 64, 7]
+    got = attend(q.to(device), cache.key_cache, cache.value_cache, table, torch.tensor(lengths, dtype=torch.int32, device=device))
+    for s, c in enumerate(lengths):
+        one = type("One", (), dict(context=[c], keys=[cache.keys[0][:c]], values=[cache.values[0][:c]], key_cache=cache.key_cache))
+        ref.check(got[s:s + 1], _want(q[s:s + 1], one, [1], 0, 0, D ** -0.5, dtype), f"sequence {s}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt, D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)], ids=["bf16", "fp16", "fp32"])
+def test_pool_of_more_than_32_bit_offsets(dt, D, device):
+    """Pages whose elements lie beyond 2^31 and 2^32 elements (bytes, in fp32) from the start of the pool."""
+    KV, page = 8, 16
+    row = KV * page * D
+    beyond = (2 ** 32 if dt != torch.float32 else 2 ** 31) // row
+    pages = beyond + 64
+    kc, vc = (torch.empty(pages, page, KV, D, dtype=dt, device=device) for _ in range(2))
+    numbers = [pages - 1, 3, beyond // 2 + 5, beyond, pages - 7, beyond - 1, beyond // 2 - 1]
+    table = torch.tensor([numbers, numbers[4:] + numbers[:4]], dtype=torch.int32, device=device)
+    context = [55, 40]  # the first four pages, and the other three
+    k, v = (util.randn(95, KV, D, seed=75 + i).to(dt) for i in range(2))
+    args = (kc, vc, table, torch.tensor(context, dtype=torch.int32, device=device))
+    append(k.to(device), v.to(device), *args, _offsets(context, device))
+    for s, (b, c) in enumerate(((0, 55), (55, 40))):
+        for x in (0, c // 2, c - 1):
+            assert torch.equal(kc[table[s, x // page].long(), x % page].cpu(), k[b + x])
+            assert torch.equal(vc[table[s, x // page].long(), x % page].cpu(), v[b + x])
+    cache = type("Both", (), dict(context=context, keys=[k[:55], k[55:]], values=[v[:55], v[55:]], key_cache=kc))
+    for tokens in ([1, 1], [30, 40]):
+        q = util.randn(sum(tokens), 2 * KV, D, seed=77).to(dt)
+        got = attend(q.to(device), *args, _offsets(tokens, device))
+        ref.check(got, _want(q, cache, tokens, 0, 0, D ** -0.5, dt), f"{tokens}")
+
+
+def test_library_refuses_before_launch():
+    import ctypes
+
+    lib = _lib.load()
+    s = (ctypes.c_int64 * 4)(1, 1, 1, 1)
+
+    def call(T=2, n=2, H=4, KV=2, D=64, page=16, max_q=1, max_ctx=10, sinks=0, starts=8, strides=s, ws=0, where=None):
+        return lib.tb200_paged_attention(8, 8, 8, 8, 8, 8, starts, where, ws, T, n, H, KV, D, page, 4, 3, 3, strides, s, s, s,
+                                         max_q, max_ctx, 0, sinks, 1.0, 0, 0, None)
+
+    assert call(H=3) == -1 and call(D=24) == -2 and call(H=130) == -2 and call(page=0) == -1 and call(max_q=0) == -1
+    assert call(max_ctx=-1) == -1 and call(sinks=-1) == -1 and call(T=3, starts=None) == -1 and call(strides=None) == -1
+    assert call(n=70000, T=70000) == -2 and call(T=0) == 0
+    append_call = lib.tb200_paged_cache_append
+    assert append_call(8, 8, 8, 8, 8, 8, 8, 2, 2, 2, 24, 16, 4, 3, 3, s, s, s, s, 0, None) == -2
+    assert append_call(8, 8, 8, 8, 8, 8, None, 3, 2, 2, 64, 16, 4, 3, 3, s, s, s, s, 0, None) == -1
+    assert append_call(None, 8, 8, 8, 8, 8, 8, 2, 2, 2, 64, 16, 4, 3, 3, s, s, s, s, 0, None) == -1
+    assert append_call(8, 8, 8, 8, 8, 8, 8, 2, 2, 2, 64, 16, 4, 3, 3, s, s, None, s, 0, None) == -1

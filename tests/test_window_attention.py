@@ -289,3 +289,66 @@ def test_module(device, dtype):
     q, k, v, dout = (t.to(device) for t in _problem(1, 2, 2, 50, 64, dtype, seed=140))
     assert torch.equal(m(q, k, v), F(q, k, v, 16, 2))
     assert "backend=Trident" in repr(m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, KV, G, S, window, sinks", [(7, 5, 2, 400, 90, 3), (40, 4, 4, 65, 20, 0), (3, 2, 1, 1300, 300, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_tiles_per_sm(B, KV, G, S, window, sinks, D, dtype, device):
+    """Several times more tiles than SMs, walks of unequal lengths."""
+    _compare(_problem(B, KV, G, S, D, dtype, seed=150), window, sinks, device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_heads_and_batches_that_share_keys(D, dtype, device):
+    """Keys expanded over the batch, values over the heads: their gradients are sums over what shares them."""
+    q, k, v, dout = _problem(3, 2, 2, 90, D, dtype, seed=160)
+    k, v = k[:1], v[:, :1]
+    want = ref.batched(q, k.expand(3, -1, -1, -1), v.expand(-1, 2, -1, -1), 30, 2, D ** -0.5, dtype, dout)
+    leaves = [t.to(device).requires_grad_(True) for t in (q, k, v)]
+    out = F(leaves[0], leaves[1].expand(3, -1, -1, -1), leaves[2].expand(-1, 2, -1, -1), 30, 2)
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout.to(device))
+    ref.check(out, want["out"], "out")
+    ref.check(dq, want["dq"], "dq")
+    # the sum of the parts' bounds, and the roundings of the parts' sum (at most three, in the operands' type)
+    u = torch.finfo(dtype).eps / 2
+    for name, got, dim in (("dk", dk, 0), ("dv", dv, 1)):
+        value, bound = (t.sum(dim, keepdim=True) for t in want[name])
+        ref.check(got, (value, bound + 3 * u * (want[name][0].abs().sum(dim, keepdim=True) + bound)), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("needs", [(True, False, False), (False, True, False), (False, False, True)])
+def test_only_one_needs_a_gradient(needs, device):
+    problem = _problem(1, 2, 2, 100, 64, torch.bfloat16, seed=170)
+    full = _run(problem, 40, 2, device)
+    leaves = [t.to(device).requires_grad_(n) for t, n in zip(problem[:3], needs)]
+    out = F(*leaves, 40, 2)
+    out.backward(problem[3].to(device))
+    assert torch.equal(out, full["out"])
+    for leaf, name, need in zip(leaves, ("dq", "dk", "dv"), needs):
+        assert torch.equal(leaf.grad, full[name]) if need else leaf.grad is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_than_32_bit_offsets(D, device):
+    """The last rows of a sequence whose queries are more than 2^31 elements: they see the last keys and the sinks."""
+    G, window, sinks, tail = 64, 60, 3, 40
+    S = 2 ** 31 // (G * D) + 77
+    dt = torch.bfloat16
+    generator = torch.Generator(device=device).manual_seed(180)
+    q, dout = (torch.randn(1, S, G, D, dtype=dt, device=device, generator=generator).transpose(1, 2) for _ in range(2))
+    k, v = (torch.randn(1, 1, S, D, dtype=dt, device=device, generator=generator) for _ in range(2))
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    out = F(q, k, v, window, sinks)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), dout)
+    # tokens that the last ones (and their keys' other queries) see, sinks first, at positions that keep who sees whom
+    near = tail + 2 * window
+    keep = torch.cat([torch.arange(sinks), torch.arange(S - near, S)])
+    cut = [t.detach()[:, :, keep.to(device)].cpu() for t in (q, k, v, dout)]
+    want = ref.batched(*cut[:3], window, sinks, D ** -0.5, dt, cut[3])
+    for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        value, bound = (t[:, :, -tail:] for t in want[name])
+        ref.check(got.detach()[:, :, -tail:], (value, bound), name)

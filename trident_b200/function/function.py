@@ -163,10 +163,11 @@ def paged_attention(
     entries of blocks that no token sees may be anything. block_table, context_lengths and query_offsets
     are int32 tensors on the device and are not read by the host.
 
-    No sequence may have more than max_query_length new tokens (default: all); max_context_length is the
-    longest context expected (default: what the table holds) and only chooses how the work is split. Both
-    have to be given for the best speed, and stay what they are in a captured graph. Rows of query that
-    belong to no sequence give zeros, or leave `output`, where it is given, as it was.
+    No sequence may have more than max_query_length new tokens (default: all; rows beyond are not computed);
+    max_context_length is the longest context expected (default: what the table holds) and only chooses how
+    the work is split. Both have to be given for the best speed, and stay what they are in a captured graph.
+    Rows of query that belong to no sequence give zeros, or leave `output`, where it is given, as it was.
+    What pages hold beyond a context is not read into any result; keys and values inside it have to be finite.
     """
     scale = 1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None else softmax_scale
     return operation.paged_attention(
@@ -186,7 +187,8 @@ def paged_cache_append(
 ):
     """
     Writes the keys and values [tokens, key heads, head size] of new tokens into the pages of a cache, in
-    place: the i-th of t new tokens of a sequence goes to position context_length - t + i.
+    place: the i-th of t new tokens of a sequence goes to position context_length - t + i. Sequences may share
+    pages, but not one that both write: of two tokens written to one place either may stay.
 
     See paged_attention for the other arguments.
     """
@@ -228,7 +230,8 @@ def sliding_window_attention(
 
     query is [batch, heads, length, head size], key and value [batch, key heads, length, head size]; each
     key head serves heads / key heads consecutive query heads. The softmax scale is 1/sqrt(head size)
-    unless given. Any strides are taken; the output is laid out as query is.
+    unless given. Any strides are taken; the output is laid out as query is. Keys and values have to be
+    finite, those of padding too: what a query does not see has the weight 0, and 0 times NaN is NaN.
 
     See WindowAttention for more details.
     """
