@@ -59,6 +59,7 @@ struct FwdParams {
   int piece;        // R: rows of one copy of keys
   int pairs, units; // pairs of query tiles per sequence and key head; pairs * KV * sequences * parts
   int longest_first;
+  Divisor outer, kv, splits;  // of a unit's number (unit_at)
   uint32_t wait_units;
 };
 
@@ -152,24 +153,33 @@ struct Unit {
   // whether query tile t takes part in key tile j: tiles below st_tiles (sinks) or from lo on, up to hi
   __device__ bool active(int t, int j) const { return (j < st_tiles || j >= (t ? lo1 : lo0)) && j <= (t ? hi1 : hi0); }
 };
+// What the MMA issuer needs of one (steps = 0: there are no more). Warp 3 looks it up ahead and hands it over in
+// shared memory: code that runs once per unit is fetched at 5 cycles an instruction, which between one unit's last
+// values and the next one's first scores was 3000 cycles without a product.
+struct Walk {
+  int steps, sink_tiles, skipped, first;  // key tile of step i: first + i, from step sink_tiles on `skipped` further
+  int st_tiles, lo0, lo1, hi0, hi1;
+  int last0, last1;  // last step of each query tile: its queries are not needed after that (-1: takes no part)
+  __device__ int tile(int i) const { return first + i + (first + i < sink_tiles ? 0 : skipped); }
+  __device__ bool active(int t, int j) const { return (j < st_tiles || j >= (t ? lo1 : lo0)) && j <= (t ? hi1 : hi0); }
+};
 // false: nothing to do
 template <bool PAGED>
 __device__ inline bool unit_at(const FwdParams& p, int unit, Unit* w) {
   const LocalArgs& a = p.a;
+  const int high = p.outer.quotient(unit), low = unit - high * (int)p.outer.d;
   int pair, rest;
   if (PAGED || p.longest_first) {
-    const int each = p.units / p.pairs;
-    pair = unit / each;
-    if (p.longest_first) pair = p.pairs - 1 - pair;
-    rest = unit % each;
+    pair = p.longest_first ? p.pairs - 1 - high : high;
+    rest = low;
   } else {  // (neighbouring tiles share keys)
-    pair = unit % p.pairs;
-    rest = unit / p.pairs;
+    pair = low;
+    rest = high;
   }
-  w->hk = rest % a.KV;
-  rest /= a.KV;
-  w->s = rest / a.splits;
-  w->split = rest % a.splits;
+  const int sequence_part = p.kv.quotient(rest);
+  w->hk = rest - sequence_part * a.KV;
+  w->s = p.splits.quotient(sequence_part);
+  w->split = sequence_part - w->s * a.splits;
   w->seq = load_sequence(a, w->s);
   w->t0 = pair * 2 * p.tile_tokens;
   if (w->t0 >= w->seq.q_len) return false;
@@ -229,7 +239,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   //   p_part[t]   128 softmax threads, first part of P_t stored      MMA issuer: first part of P_t V
   //   p_full[t]   128 softmax threads, all of P_t stored             MMA issuer: the rest
   //   o_done[t]   tcgen05.commit after P_t V                         softmax: rescale, P_t over P_t, epilogue
-  //   o_free[t]   128 softmax threads after the unit's O_t is read   MMA issuer: first P_t V of the next
+  //   walk_full   warp 3, after a unit's walk is in shared memory    MMA issuer
+  //   walk_empty  MMA issuer, after it has read the walk             warp 3
   //   out_full    128 softmax threads of a tile, per output tile     warp 2: bulk copy
   //   out_free    warp 2, after the copy has read shared memory      softmax: next output tile into shared memory
   //               (the output tiles of all units in order, tile 0 of a unit before tile 1)
@@ -249,11 +260,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   uint64_t* p_full = bars + 19;      // [2]
   uint64_t* p_part = bars + 21;      // [2]
   uint64_t* s_free = bars + 23;      // [2]
-  uint64_t* o_free = bars + 25;      // [2]
-  uint64_t* out_full = bars + 27;
-  uint64_t* out_free = bars + 28;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  uint64_t* out_full = bars + 25;
+  uint64_t* out_free = bars + 26;
+  uint64_t* walk_full = bars + 27;   // [2]
+  uint64_t* walk_empty = bars + 29;  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
   volatile uint32_t* abort_flag = tmem_slot + 1;  // [0] abort flag, [1] wait limit (ptx::mbar_wait)
+  Walk* walks = reinterpret_cast<Walk*>(bars + 32);  // [2]
 
   const LocalArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -270,8 +283,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 19; ++i) ptx::mbar_init(&bars[i], 1);
-    for (int i = 19; i < 28; ++i) ptx::mbar_init(&bars[i], 128);
-    ptx::mbar_init(out_free, 1);
+    for (int i = 19; i < 26; ++i) ptx::mbar_init(&bars[i], 128);
+    for (int i = 26; i < 31; ++i) ptx::mbar_init(&bars[i], 1);
     abort_flag[0] = 0;
     abort_flag[1] = p.wait_units;
     ptx::fence_barrier_init();
@@ -395,7 +408,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       const uint64_t dk0 = ptx::make_smem_desc(ptx::smem_u32(k_smem), 16, 1024);
       const uint64_t dv0 = ptx::make_smem_desc(ptx::smem_u32(v_smem), BOX_BYTES, 1024);
       constexpr uint64_t NEXT_TILE = static_cast<uint64_t>(TILE_BYTES >> 4);
-      // Counts of each query tile over all units: score products, value products, units with products.
+      // Counts of each query tile over all units: score products, value products, units with queries.
       int scores0 = 0, scores1 = 0, values0 = 0, values1 = 0, queries0 = 0, queries1 = 0;
       auto issue_qk = [&](int t, int st) {
         const uint64_t qd = dq0 + (t ? NEXT_TILE : 0), kd = dk0 + (st ? NEXT_TILE : 0);
@@ -418,76 +431,77 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                          accumulate || ks != 0);
         }
       };
-      int g = 0;  // steps of all units
-      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
-        Unit w;
-        if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
-        const int steps = w.m1 - w.m0;
-        bool fresh0 = true, fresh1 = true, first0 = true, first1 = true;  // no scores, no values of the tile yet
-        // the last step of each tile: its queries are not needed after that (-1: takes no part)
-        int last0 = steps - 1, last1 = steps - 1;
-        while (last0 >= 0 && !w.active(0, w.kr.tile(w.m0 + last0))) --last0;
-        while (last1 >= 0 && !w.active(1, w.kr.tile(w.m0 + last1))) --last1;
-        auto do_scores = [&](auto tag, int i) {  // of step i
-          constexpr int t = decltype(tag)::value;
-          int& scores = t ? scores1 : scores0;
-          bool& fresh = t ? fresh1 : fresh0;
-          if (fresh) wait_(&q_full[t], (t ? queries1 : queries0) & 1, 71 + t);
-          fresh = false;
-          if (P_SPLIT && scores > 0) wait_(&s_free[t], (scores - 1) & 1, 73 + t);
-          wait_(&k_full[(g + i) & 1], ((g + i) >> 1) & 1, 75);
-          ptx::tc_fence_after();
-          issue_qk(t, (g + i) & 1);
-          commit_(&s_full[t]);
-          if (i == (t ? last1 : last0)) commit_(&q_empty[t]);
-          ++scores;
-        };
-        auto do_values = [&](auto tag, int i) {
-          constexpr int t = decltype(tag)::value;
-          int& values = t ? values1 : values0;
-          bool& first = t ? first1 : first0;
-          if (first && (t ? queries1 : queries0) > 0) wait_(&o_free[t], ((t ? queries1 : queries0) - 1) & 1, 80);
-          wait_(&p_part[t], values & 1, 76 + t);
-          wait_(&v_full[(g + i) & 1], ((g + i) >> 1) & 1, 78);
-          ptx::tc_fence_after();
-          issue_pv(t, (g + i) & 1, 0, P_FIRST, !first);
-          wait_(&p_full[t], values & 1, 76 + t);
-          ptx::tc_fence_after();
-          issue_pv(t, (g + i) & 1, P_FIRST, TILE / 16, true);
-          commit_(&o_done[t]);
-          first = false;
-          ++values;
-        };
-        using T0 = std::integral_constant<int, 0>;
-        using T1 = std::integral_constant<int, 1>;
-        {
-          const int j = w.kr.tile(w.m0);
-          if (w.active(0, j)) do_scores(T0{}, 0);
-          if (w.active(1, j)) do_scores(T1{}, 0);
-          commit_(&k_empty[g & 1]);
-        }
-        for (int i = 0; i < steps; ++i) {
-          const bool more = i + 1 < steps;
-          const int j = w.kr.tile(w.m0 + i), nj = more ? w.kr.tile(w.m0 + i + 1) : 0;
+      // One walk over the steps of all units: the scores of step g next to the values of step g - 1, also
+      // where g begins a new unit. The keys and values of both are waited for ahead of the probabilities: a
+      // wait for a barrier that has long completed costs 150 to 250 cycles of this warp, which stood
+      // between a tile's probabilities and its next scores.
+      int g = 0;
+      uint32_t todo = 0;  // values of step g - 1: bit t: of query tile t, bit 2 + t: the first of its unit
+      auto do_values = [&](auto tag, uint32_t which) {
+        constexpr int t = decltype(tag)::value;
+        if (!((which >> t) & 1u)) return;
+        int& values = t ? values1 : values0;
+        const int st = (g - 1) & 1;
+        // (a unit's first probabilities also say that the output of the one before has been read)
+        wait_(&p_part[t], values & 1, 76 + t);
+        ptx::tc_fence_after();
+        issue_pv(t, st, 0, P_FIRST, !((which >> (2 + t)) & 1u));
+        wait_(&p_full[t], values & 1, 76 + t);
+        ptx::tc_fence_after();
+        issue_pv(t, st, P_FIRST, TILE / 16, true);
+        commit_(&o_done[t]);
+        ++values;
+      };
+      using T0 = std::integral_constant<int, 0>;
+      using T1 = std::integral_constant<int, 1>;
+      for (int units = 0;; ++units) {
+        wait_(&walk_full[units & 1], (units >> 1) & 1, 70);
+        const Walk w = walks[units & 1];
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&walk_empty[units & 1]);
+        if (w.steps == 0 || abort_flag[0]) break;
+        const int steps = w.steps;
+        bool fresh0 = true, fresh1 = true;  // no scores of the tile yet
+        for (int i = 0; i < steps; ++i, ++g) {
+          const int j = w.tile(i);
+          const bool active0 = w.active(0, j), active1 = w.active(1, j);
+          const uint32_t old = todo;
+          todo = (active0 ? (fresh0 ? 5u : 1u) : 0u) | (active1 ? (fresh1 ? 10u : 2u) : 0u);
+          if (g > 0) wait_(&v_full[(g - 1) & 1], ((g - 1) >> 1) & 1, 78);
+          if (i > 0) wait_(&k_full[g & 1], (g >> 1) & 1, 75);
+          auto do_scores = [&](auto tag) {
+            constexpr int t = decltype(tag)::value;
+            if (!(t ? active1 : active0)) return;
+            int& scores = t ? scores1 : scores0;
+            bool& fresh = t ? fresh1 : fresh0;
+            if (fresh) wait_(&q_full[t], (t ? queries1 : queries0) & 1, 71 + t);
+            fresh = false;
+            if (P_SPLIT && scores > 0) wait_(&s_free[t], (scores - 1) & 1, 73 + t);
+            if (i == 0) wait_(&k_full[g & 1], (g >> 1) & 1, 75);
+            ptx::tc_fence_after();
+            issue_qk(t, g & 1);
+            commit_(&s_full[t]);
+            if (i == (t ? w.last1 : w.last0)) commit_(&q_empty[t]);
+            ++scores;
+          };
           if constexpr (P_SPLIT) {
             // next scores of a tile before its values
-            if (more && w.active(0, nj)) do_scores(T0{}, i + 1);
-            if (w.active(0, j)) do_values(T0{}, i);
-            if (more && w.active(1, nj)) do_scores(T1{}, i + 1);
-            if (more) commit_(&k_empty[(g + i + 1) & 1]);
-            if (w.active(1, j)) do_values(T1{}, i);
-            commit_(&v_empty[(g + i) & 1]);
+            do_scores(T0{});
+            do_values(T0{}, old);
+            do_scores(T1{});
+            commit_(&k_empty[g & 1]);
+            do_values(T1{}, old);
+            if (g > 0) commit_(&v_empty[(g - 1) & 1]);
           } else {
             // P overwrites S: the next scores follow the values on the in-order pipe
-            if (w.active(0, j)) do_values(T0{}, i);
-            if (more && w.active(0, nj)) do_scores(T0{}, i + 1);
-            if (w.active(1, j)) do_values(T1{}, i);
-            commit_(&v_empty[(g + i) & 1]);
-            if (more && w.active(1, nj)) do_scores(T1{}, i + 1);
-            if (more) commit_(&k_empty[(g + i + 1) & 1]);
+            do_values(T0{}, old);
+            do_scores(T0{});
+            do_values(T1{}, old);
+            if (g > 0) commit_(&v_empty[(g - 1) & 1]);
+            do_scores(T1{});
+            commit_(&k_empty[g & 1]);
           }
         }
-        g += steps;
         // (a tile whose queries were brought, but that takes no part in this part of the walk, counts too)
         if (w.hi0 >= 0) {
           if (fresh0) {
@@ -503,6 +517,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           }
           ++queries1;
         }
+      }
+      if (g > 0) {
+        wait_(&v_full[(g - 1) & 1], ((g - 1) >> 1) & 1, 78);
+        do_values(T0{}, todo);
+        do_values(T1{}, todo);
       }
       // everything issued has completed before tensor memory is freed
       commit_(mma_drained);
@@ -532,19 +551,25 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         ptx::bulk_wait_done();
       }
       __syncwarp();
-    } else if (PAGED && warp == 3) {
-      // -------------------------------------------------------------- zeros behind the sequence's end
-      int g = 0;
+    } else if (warp == 3) {
+      // -------------------------------------------------------------- walks for the issuer, zeros behind the sequence's end
+      int g = 0, n = 0;     // steps, units
       uint32_t phases = 0;  // bit s: parity of the next completion of stage s
-      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
-        Unit w;
-        if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
-        g += w.m1 - w.m0;
-        if (!needs_fix(w)) continue;
+      auto publish = [&](const Walk& w) {
+        ptx::mbar_wait(&walk_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, a.status, 68);
+        if (lane == 0) {
+          walks[n & 1] = w;
+          ptx::mbar_arrive(&walk_full[n & 1]);
+        }
+        __syncwarp();
+        ++n;
+      };
+      // the last V tile of the unit with steps up to g, when its sequence has `keys` keys
+      auto fix = [&](int keys) {
         const int st = (g - 1) & 1;
         ptx::mbar_wait_drain(&v_raw[st], (phases >> st) & 1u, abort_flag, a.status, 66);
         phases ^= 1u << st;
-        const int first = w.seq.kv_len % TILE, end = min(TILE, ((first + p.piece - 1) / p.piece) * p.piece);
+        const int first = keys % TILE, end = min(TILE, ((first + p.piece - 1) / p.piece) * p.piece);
         // (whole pieces behind the end were read as zeros)
         for (int r = first + lane / 8; r < end; r += 4)
 #pragma unroll
@@ -553,7 +578,22 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&v_full[st]);
+      };
+      int fix_keys = 0;  // of the unit before
+      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+        Unit w;
+        if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
+        int last0 = w.m1 - w.m0 - 1, last1 = last0;
+        while (last0 >= 0 && !w.active(0, w.kr.tile(w.m0 + last0))) --last0;
+        while (last1 >= 0 && !w.active(1, w.kr.tile(w.m0 + last1))) --last1;
+        publish(Walk{w.m1 - w.m0, w.kr.sink_tiles, w.kr.lo - w.kr.sink_tiles, w.m0, w.st_tiles, w.lo0, w.lo1, w.hi0, w.hi1,
+                     last0, last1});
+        if (PAGED && fix_keys > 0) fix(fix_keys);
+        g += w.m1 - w.m0;
+        fix_keys = needs_fix(w) ? w.seq.kv_len : 0;
       }
+      publish(Walk{});
+      if (PAGED && fix_keys > 0) fix(fix_keys);
     }
   } else {
     // ---------------------------------------------------------------- softmax + epilogue
@@ -566,6 +606,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const uint32_t s_addr = tmem_base + lane_off + COL_S + t * 128;
     const uint32_t o_addr = tmem_base + lane_off + COL_O + t * D;
     const uint32_t p_addr = tmem_base + lane_off + (P_SPLIT ? COL_P + t * 64 : COL_S + t * 128);
+    const int warp_first = quarter * 32 / a.G, warp_last = (quarter * 32 + 31) / a.G;
     int count = 0, outs = 0;  // steps of this tile, output tiles of both (over all units of the CTA)
     Unit w;
     auto next_unit = [&](int unit) {  // the first from `unit` on that has something to do
@@ -580,8 +621,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       const int token = first_token + row_token;  // of the sequence
       const int pos = live ? w.base + token : -1;
       // positions of the warp's rows
-      const int wmin = w.base + first_token + quarter * 32 / a.G;
-      const int wmax = w.base + first_token + min((quarter * 32 + 31) / a.G, tokens - 1);
+      const int wmin = w.base + first_token + warp_first;
+      const int wmax = w.base + first_token + min(warp_last, tokens - 1);
       float m_used = -INFINITY, l = 0.f;
       const int before = count;
       for (int m = w.m0; m < w.m1; ++m) {
@@ -752,7 +793,6 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       }
       // What the epilogue needs of this unit; the next one is looked up while the last product runs.
       const bool counted = count > before, whole = w.whole, bulk0 = is_bulk(w, 0), bulk1 = is_bulk(w, 1), bulk = t ? bulk1 : bulk0;
-      const bool queried = (t ? w.hi1 : w.hi0) >= 0 && w.m1 > w.m0;
       const int head = w.hk * a.G + row_head;
       const long long tok = w.seq.q_begin + token;
       const bool some = l > 0.f;  // (a row without keys: zeros)
@@ -775,8 +815,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       if (warp_live) {
         const uint64_t inv2 = am::pack2f(inv, inv);
         const bool zeros = !__all_sync(0xffffffffu, some || !live);  // (the columns hold what was there before)
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
+#pragma unroll 1
+        for (int h = 0; h < D / 64; ++h) {  // (not unrolled: run once per unit, its code is fetched anew each time)
           uint32_t v[2][32];
           __syncwarp();
           ptx::tmem_ld32(o_addr + h * 64, v[0]);
@@ -819,7 +859,6 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         }
       }
       ptx::tc_fence_before();
-      if (queried) ptx::mbar_arrive(&o_free[t]);
       if (bulk) {
         ptx::fence_proxy_async_smem();
         ptx::mbar_arrive(out_full);
@@ -916,7 +955,7 @@ namespace {
 template <typename T, int D, bool PAGED>
 int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo, const FwdParams& p,
                cudaStream_t st) {
-  constexpr int SMEM = 7 * TILE * D * 2 + 1024 + 256;
+  constexpr int SMEM = 7 * TILE * D * 2 + 1024 + 384;
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
   auto kern = local_fwd_tc_kernel<T, D, PAGED>;
   static std::atomic<unsigned long long> optin_done{0};
@@ -962,6 +1001,9 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   p.units = (int)units;
   // (walks of a causal training step grow with the tile; those of chunks hardly do, and their last tiles may be empty)
   p.longest_first = a.window == NO_WINDOW && !a.table;
+  p.outer = Divisor(a.table || p.longest_first ? p.units / p.pairs : p.pairs);
+  p.kv = Divisor(a.KV);
+  p.splits = Divisor(a.splits);
   p.wait_units = ptx::WAIT_LIMIT_UNITS;
   CUtensorMap mq, mk, mv, mo;
   if (!local_map_rows(&mq, q, a.qs, a, p.tile_tokens, "q") || !local_map_rows(&mo, out, a.os, a, p.tile_tokens, "out") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||

@@ -9,6 +9,20 @@ namespace tb200 {
 constexpr int LOCAL_TC_TILE = 128;  // packed query rows and keys of a tile
 constexpr int LOCAL_TC_COLS = 96;   // packed query rows of a step of the dK, dV kernel
 
+// Division of 0 <= n < 2^31 by a number that is known at launch: a product, an addition and a shift (the
+// roles of the persistent kernels look up their units of work between one tile and the next, where the five
+// divisions by variables took over 1000 cycles). With 2^(l-1) < d <= 2^l and m = floor(2^32 (2^l - d) / d) + 1
+// the quotient is (floor(m n / 2^32) + n) / 2^l rounded down (Granlund and Montgomery, 1994).
+struct Divisor {
+  uint32_t d = 1, m = 1, l = 0;
+  Divisor() = default;
+  explicit Divisor(int divisor) : d((uint32_t)divisor) {
+    while ((1ull << l) < d) ++l;
+    m = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+  }
+  __device__ int quotient(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> l); }
+};
+
 // What the tensor-core kernels take: 16-bit operands, head size 64 or 128, unit feature strides, other
 // strides multiples of 16 bytes, and (serving form) a page size that shares a factor of at least 8 with 128.
 bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void* k, const void* v, const void* out);
