@@ -87,5 +87,36 @@ __device__ inline void tmem_ld_wait_dep(uint32_t (&r)[16]) {
                : "memory");
 }
 
+// Instructions whose order the compiler keeps, for exponentials with their arithmetic in between.
+__device__ inline uint64_t fma2_ordered(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ inline uint64_t add2_ordered(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ inline float ex2_ordered(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ inline uint32_t cvt_ordered(float a, float b);
+template <>
+__device__ inline uint32_t cvt_ordered<__nv_bfloat16>(float a, float b) {
+  uint32_t r;
+  asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <>
+__device__ inline uint32_t cvt_ordered<__half>(float a, float b) {
+  uint32_t r;
+  asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
 }  // namespace am
 }  // namespace tb200

@@ -228,8 +228,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t ph = i & 1;
         const uint64_t cur = (i % STAGES) * STAGE, nxt = ((i + 1) % STAGES) * STAGE;
         if (i + 1 < steps) {
-          wait_(s_free, ph, 105);
+          // (waiting for what arrived long ago costs 150 cycles: not between the softmax threads and the product)
           wait_(&qdo_full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1, 106);
+          wait_(s_free, ph, 105);
           ptx::tc_fence_after();
           score(COL_S, dk, dq + nxt);
           commit_(s_ready);
@@ -285,35 +286,44 @@ __global__ void __launch_bounds__(THREADS, 1)
       am::tmem_ld_wait_dep(rb);
       ptx::tc_fence_before();
       ptx::mbar_arrive(s_free);
-      auto scaled = [&](int g, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
-        const float4 nl = nlse4[g];
-        am::unpack2f(am::fma2(am::pack2u(v0, v1), scale2, am::pack2f(nl.x, nl.y)), pr[g * 4], pr[g * 4 + 1]);
-        am::unpack2f(am::fma2(am::pack2u(v2, v3), scale2, am::pack2f(nl.z, nl.w)), pr[g * 4 + 2], pr[g * 4 + 3]);
+      uint32_t pa[16], pb[8];
+      // the arguments and conversions of neighbouring columns are issued between the exponentials
+      auto probabilities = [&](auto masked, uint32_t seen0, uint32_t seen1) {
+        constexpr int LAG = 3, PAIRS = HALF / 2;  // pairs between an exponential and its use
+        auto argument = [&](int k) {
+          const float4 nl = nlse4[k >> 1];
+          const uint64_t v = k < 16 ? am::pack2u(ra[2 * k & 31], ra[(2 * k + 1) & 31]) : am::pack2u(rb[2 * k & 15], rb[(2 * k + 1) & 15]);
+          am::unpack2f(am::fma2_ordered(v, scale2, k & 1 ? am::pack2f(nl.z, nl.w) : am::pack2f(nl.x, nl.y)), pr[2 * k], pr[2 * k + 1]);
+        };
+        argument(0);
+#pragma unroll
+        for (int k = 0; k < PAIRS + LAG; ++k) {
+          if (k < PAIRS) pr[2 * k] = am::ex2_ordered(pr[2 * k]);
+          if (k + 1 < PAIRS) argument(k + 1);
+          if (k < PAIRS) pr[2 * k + 1] = am::ex2_ordered(pr[2 * k + 1]);
+          if (k >= LAG) {
+            const int d = k - LAG;
+            if constexpr (decltype(masked)::value) {
+              const uint32_t seen = d < 16 ? seen0 : seen1;
+              if (!(seen & (1u << (2 * d & 31)))) pr[2 * d] = 0.f;
+              if (!(seen & (2u << (2 * d & 31)))) pr[2 * d + 1] = 0.f;
+            }
+            const uint32_t both = am::cvt_ordered<T>(pr[2 * d], pr[2 * d + 1]);
+            if (d < 16) pa[d & 15] = both;
+            else pb[d & 7] = both;
+          }
+        }
       };
-#pragma unroll
-      for (int g = 0; g < 8; ++g) scaled(g, ra[g * 4], ra[g * 4 + 1], ra[g * 4 + 2], ra[g * 4 + 3]);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) scaled(8 + g, rb[g * 4], rb[g * 4 + 1], rb[g * 4 + 2], rb[g * 4 + 3]);
-#pragma unroll
-      for (int e = 0; e < HALF; ++e) pr[e] = am::ex2(pr[e]);
-      if (!plain) {
+      if (plain) {
+        probabilities(std::false_type{}, 0u, 0u);
+      } else {
         // columns from `low` on are not before the key, those below `high` are within its window
         const int low = saturate((int64_t)(key - token0) * a.G) - half * HALF;
         const int high = saturate(((int64_t)key + a.window - token0) * a.G) - half * HALF;
-#pragma unroll
-        for (int q = 0; q < HALF; q += 32) {
-          const uint32_t seen = ~low_bits(low - q) & (low_bits(high - q) | always);
-#pragma unroll
-          for (int e = 0; e < 32 && q + e < HALF; ++e)
-            if (!(seen & (1u << e))) pr[q + e] = 0.f;
-        }
+        probabilities(std::true_type{}, ~low_bits(low) & (low_bits(high) | always),
+                      ~low_bits(low - 32) & (low_bits(high - 32) | always));
       }
       {
-        uint32_t pa[16], pb[8];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pa[e] = am::cvt_pair<T>(pr[2 * e], pr[2 * e + 1]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pb[e] = am::cvt_pair<T>(pr[32 + 2 * e], pr[33 + 2 * e]);
         if (i > 0) {  // P^T(i) goes over P^T(i-1)
           ptx::mbar_wait(dv_done, (i - 1) & 1, abort_flag, p.status, 112);
           ptx::tc_fence_after();
@@ -331,7 +341,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       am::tmem_ld_wait_dep(ra);
       am::tmem_ld_wait_dep(rb);
       {
-        uint32_t pa[16], pb[8];
         auto grad = [&](int g, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, uint32_t& o0, uint32_t& o1) {
           const float4 nd = ndel4[g];
           float d0, d1, d2, d3;

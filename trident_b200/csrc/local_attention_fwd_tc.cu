@@ -78,36 +78,6 @@ __device__ inline void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* 
 // the lowest n bits
 __device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
-// Instructions whose order the compiler keeps (see exp_row).
-__device__ inline uint64_t fma2_ordered(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ inline uint64_t add2_ordered(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ inline float ex2_ordered(float x) {
-  float y;
-  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <typename T>
-__device__ inline uint32_t cvt_ordered(float a, float b);
-template <>
-__device__ inline uint32_t cvt_ordered<__nv_bfloat16>(float a, float b) {
-  uint32_t r;
-  asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
-template <>
-__device__ inline uint32_t cvt_ordered<__half>(float a, float b) {
-  uint32_t r;
-  asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
 // P of a whole row of 128 raw scores: p = 2^(v scale - m), 16-bit, to tensor memory; returns the row's sum.
 // One warp of a query tile is alone on its scheduler's exponential unit, which takes an instruction every 8
 // cycles; the arguments, sums and conversions of neighbouring columns are issued in between (as three passes
@@ -119,19 +89,19 @@ __device__ inline float exp_row(const uint32_t (&v)[4][32], uint64_t scale2, uin
   uint64_t sum0 = am::pack2f(0.f, 0.f), sum1 = sum0;
   float x[128];
   uint32_t packed[16];
-  am::unpack2f(fma2_ordered(am::pack2u(v[0][0], v[0][1]), scale2, negm2), x[0], x[1]);
+  am::unpack2f(am::fma2_ordered(am::pack2u(v[0][0], v[0][1]), scale2, negm2), x[0], x[1]);
 #pragma unroll
   for (int k = 0; k < 64 + LAG; ++k) {
-    if (k < 64) x[2 * k] = ex2_ordered(x[2 * k]);
+    if (k < 64) x[2 * k] = am::ex2_ordered(x[2 * k]);
     if (k + 1 < 64)
-      am::unpack2f(fma2_ordered(am::pack2u(v[(k + 1) >> 4][(2 * k + 2) & 31], v[(k + 1) >> 4][(2 * k + 3) & 31]), scale2, negm2),
+      am::unpack2f(am::fma2_ordered(am::pack2u(v[(k + 1) >> 4][(2 * k + 2) & 31], v[(k + 1) >> 4][(2 * k + 3) & 31]), scale2, negm2),
                    x[2 * k + 2], x[2 * k + 3]);
-    if (k < 64) x[2 * k + 1] = ex2_ordered(x[2 * k + 1]);
+    if (k < 64) x[2 * k + 1] = am::ex2_ordered(x[2 * k + 1]);
     if (k >= LAG) {
       const int d = k - LAG;
-      if (d & 1) sum1 = add2_ordered(sum1, am::pack2f(x[2 * d], x[2 * d + 1]));
-      else sum0 = add2_ordered(sum0, am::pack2f(x[2 * d], x[2 * d + 1]));
-      packed[d & 15] = cvt_ordered<T>(x[2 * d], x[2 * d + 1]);
+      if (d & 1) sum1 = am::add2_ordered(sum1, am::pack2f(x[2 * d], x[2 * d + 1]));
+      else sum0 = am::add2_ordered(sum0, am::pack2f(x[2 * d], x[2 * d + 1]));
+      packed[d & 15] = am::cvt_ordered<T>(x[2 * d], x[2 * d + 1]);
       if ((d & 15) == 15) ptx::tmem_st16(p_addr + (d >> 4) * 16, packed);
       if (d == 47 + 6) part();  // (the stores have had the time of six pairs)
     }
