@@ -7,11 +7,14 @@
 // strides are padded by 4 floats so that the 16-byte reads of a quarter-warp fall into different banks.
 //   forward   resident: 64 (or 16) packed query rows, streamed: 64 keys; running maximum and sum.
 //             16 rows serve single tokens, where 64 would mostly be empty.
-//   dQ        resident: 64 packed query rows (Q, dO), streamed: 32 keys (K, V)
-//   dK, dV    resident: 64 keys (K, V), streamed: 32 packed query rows (Q, dO): the sum over the
+//   dQ        resident: 64 packed query rows (Q, dO), streamed: 64 keys (K, V)
+//   dK, dV    resident: 64 keys (K, V), streamed: 64 packed query rows (Q, dO): the sum over the
 //             heads of a group is part of the walk, in a fixed order
-// Bound by the fp32 pipes and, next to them, shared-memory reads: per 4 features of a score tile a
-// thread issues 8 16-byte reads for 64 multiply-adds.
+// A thread issues 8 16-byte reads for 64 multiply-adds of a score tile's 4 features. At 8 heads, 1024 tokens,
+// window 256, D = 64 (128 CTAs, 8 warps an SM) the kernels wait for those reads and the tiles' loads: dK/dV
+// 77 us with the multiply-adds 30 % and shared memory 44 % busy, dQ 52, forward 40. In the backward kernels a
+// warp covers 4 x 8 threads of the tile (2 x 16 and 32 streamed rows: 92 and 57 us); 8 columns a thread need
+// a quarter fewer reads, but leave 4 warps an SM (110, 71 and 57 us).
 #include <type_traits>
 
 #include "local_attention.cuh"
@@ -328,7 +331,10 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------ backward
-constexpr int BRM = 64, BRS = 32, BTX = 16;
+constexpr int BRM = 64, BRS = 64, BTX = 16;
+// place of a thread in the 16 x 16 threads of a tile, 4 x 8 a warp
+__device__ inline int bwd_tx() { return (threadIdx.x & 7) | ((threadIdx.x >> 2) & 8); }
+__device__ inline int bwd_ty() { return ((threadIdx.x >> 3) & 3) | ((threadIdx.x >> 4) & 12); }
 
 // dQ of 64 packed rows.
 template <typename T, int D>
@@ -343,8 +349,8 @@ __global__ void __launch_bounds__(256)
   float* sd = sq + BRM * LD;
   float* sk = sd + BRM * LD;
   float* sv = sk + BRS * LD;
-  float* sp = sv + BRS * LD;  // [64][36]
-  const int tx = threadIdx.x % BTX, ty = threadIdx.x / BTX;
+  float* sp = sv + BRS * LD;  // [64][68]
+  const int tx = bwd_tx(), ty = bwd_ty();
   const int s = blockIdx.z, hk = blockIdx.y;
   const int tile_tokens = BRM / a.G, t0 = blockIdx.x * tile_tokens;
   const int ntok = min(tile_tokens, a.tokens - t0), rows = ntok * a.G;
@@ -417,10 +423,10 @@ __global__ void __launch_bounds__(256)
   float* sv = sk + BRM * LD;
   float* sq = sv + BRM * LD;
   float* sd = sq + BRS * LD;
-  float* sp = sd + BRS * LD;      // [64][36] probabilities
-  float* sg = sp + BRM * PLD;     // [64][36] score gradients
-  float* srow = sg + BRM * PLD;   // [2][32] lse, delta of the streamed rows
-  const int tx = threadIdx.x % BTX, ty = threadIdx.x / BTX;
+  float* sp = sd + BRS * LD;      // [64][68] probabilities
+  float* sg = sp + BRM * PLD;     // [64][68] score gradients
+  float* srow = sg + BRM * PLD;   // [2][64] lse, delta of the streamed rows
+  const int tx = bwd_tx(), ty = bwd_ty();
   const int s = blockIdx.z, hk = blockIdx.y;
   const int tiles = (a.tokens + BRM - 1) / BRM;
   int kt = blockIdx.x, piece = -1, first, last;  // tokens [first, last)
