@@ -344,6 +344,14 @@ def test_more_than_32_bit_offsets(device):
         _check(got[-6:], want[name], dt, name)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "feature", "sequence", "element"])
+@pytest.mark.parametrize("shape", [(40, 9, 1), (3, 50, 257), (35, 8, 1025), (2, 33, 2049), (5, 7, 4095), (2, 9, 4097)], ids=str)
+def test_odd_widths(shape, gate, dtype, device):
+    """The widths at which the kernels for rows of any alignment change, one and many gate vectors."""
+    _compare(_problem(shape, gate, gate != "feature", dtype, seed=420), 0.9, device, dtype)
+
+
 def test_library_refuses_before_launch():
     from trident_b200 import _lib
 

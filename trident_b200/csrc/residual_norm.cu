@@ -56,7 +56,7 @@ __device__ inline float block_sum(float v, float* slot) {
   return warp_sum(r);
 }
 
-// ------------------------------------------------------------------ any width and alignment
+// ------------------------------------------------------------------ any width and alignment, from 4097 columns on
 // One CTA per row; the row is read again (from L1 or L2) for every pass.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -162,6 +162,161 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------ rows of 16-byte vectors
+// ------------------------------------------------------------------ rows of up to 4096 columns, any alignment
+// Widths that are no multiple of 16 bytes, unaligned views: a CTA holds a row in registers, C columns a thread,
+// a block apart, and reads and writes each element once, one element at a time. At 1665 rows of 1021 fp32 columns
+// (20 MB forward, 41 backward) forward and backward take 9 and 17 us; the kernels above, which read a row again for
+// every pass and keep the column sums in memory, take 15 and 54.
+template <typename T, int C>
+__global__ void __launch_bounds__(512)
+    resnorm_fwd_cols(T* __restrict__ h, T* __restrict__ y, float* __restrict__ rms1, float* __restrict__ rms2,
+                     const T* __restrict__ x, const T* __restrict__ r, const T* __restrict__ w1, const T* __restrict__ w2,
+                     const T* __restrict__ gate, const ResNormArgs a) {
+  using Tr = Traits<T>;
+  __shared__ float slot[32];
+  const int64_t row = blockIdx.x, off = row * a.cols;
+  const T* g = gate ? gate + gate_index(a, row) * a.cols : nullptr;
+  float v[C], rv[C], w[C];
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int c = threadIdx.x + k * blockDim.x;
+    const bool live = c < a.cols;
+    v[k] = live ? Tr::to_f(x[off + c]) : 0.f;
+    rv[k] = live ? Tr::to_f(r[off + c]) : 0.f;
+    w[k] = live ? (w1 ? Tr::to_f(w1[c]) : 1.f) * (g ? Tr::to_f(g[c]) : 1.f) : 0.f;
+  }
+  float i1 = 1.f;
+  if (w1) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < C; ++k) s = fmaf(v[k], v[k], s);
+    const float rms = sqrtf(block_sum(s, slot) / (float)a.cols);
+    i1 = 1.f / (rms + a.eps);
+    if (threadIdx.x == 0) rms1[row] = rms;
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    v[k] = fmaf(a.scale, rv[k], v[k] * i1 * w[k]);
+    s = fmaf(v[k], v[k], s);
+  }
+#pragma unroll
+  for (int k = 0; k < C; ++k) w[k] = threadIdx.x + k * blockDim.x < a.cols ? Tr::to_f(w2[threadIdx.x + k * blockDim.x]) : 0.f;
+  const float rms = sqrtf(block_sum(s, slot) / (float)a.cols), i2 = 1.f / (rms + a.eps);
+  if (threadIdx.x == 0) rms2[row] = rms;
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int c = threadIdx.x + k * blockDim.x;
+    if (c < a.cols) {
+      y[off + c] = Tr::from_f(v[k]);
+      h[off + c] = Tr::from_f(v[k] * i2 * w[k]);
+    }
+  }
+}
+
+// A part of the rows; the next row is read while the sums of this one are formed.
+template <typename T, int C>
+__global__ void __launch_bounds__(512)
+    resnorm_bwd_cols(T* __restrict__ dx, T* __restrict__ dr, T* __restrict__ dgate_rows, float* __restrict__ part_a,
+                     float* __restrict__ part_b, const T* __restrict__ dh, const T* __restrict__ dy, const T* __restrict__ x,
+                     const T* __restrict__ r, const T* __restrict__ w1, const T* __restrict__ w2, const T* __restrict__ gate,
+                     const float* __restrict__ rms1, const float* __restrict__ rms2, const ResNormArgs a, int per_row) {
+  using Tr = Traits<T>;
+  __shared__ float slot[32];
+  const int64_t n = gridDim.x, begin = part_begin(blockIdx.x, n, a.rows), end = part_begin(blockIdx.x + 1, n, a.rows);
+  float W1[C], W2[C], G[C], acc_a[C], acc_b[C], nx[C], nr[C], nh[C], ny[C], nm1 = 1.f, nm2 = 1.f;
+  auto load = [&](int64_t row) {
+    const int64_t off = row * a.cols;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = threadIdx.x + k * blockDim.x;
+      const bool live = c < a.cols;
+      nx[k] = live ? Tr::to_f(x[off + c]) : 0.f;
+      nr[k] = live ? Tr::to_f(r[off + c]) : 0.f;
+      nh[k] = live && dh ? Tr::to_f(dh[off + c]) : 0.f;
+      ny[k] = live && dy ? Tr::to_f(dy[off + c]) : 0.f;
+    }
+    if (w1) nm1 = rms1[row];
+    nm2 = rms2[row];
+  };
+  auto flush = [&](float* part, const float (&acc)[C]) {
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = threadIdx.x + k * blockDim.x;
+      if (c < a.cols) part[c] = acc[k];
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int c = threadIdx.x + k * blockDim.x;
+    const bool live = c < a.cols;
+    W1[k] = live && w1 ? Tr::to_f(w1[c]) : 1.f;
+    W2[k] = live ? Tr::to_f(w2[c]) : 0.f;
+    G[k] = 1.f;
+    acc_a[k] = acc_b[k] = 0.f;
+  }
+  int64_t current = -1;
+  if (begin < end) load(begin);
+  for (int64_t row = begin; row < end; ++row) {
+    const int64_t gi = gate_index(a, row);
+    if (gate && gi != current) {
+      if (part_a && !per_row && current >= 0) {
+        flush(part_a + ((int64_t)blockIdx.x + current) * a.cols, acc_a);
+#pragma unroll
+        for (int k = 0; k < C; ++k) acc_a[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        const int c = threadIdx.x + k * blockDim.x;
+        if (c < a.cols) G[k] = Tr::to_f(gate[gi * a.cols + c]);
+      }
+    }
+    current = gi;
+    const float m1 = nm1, m2 = nm2, i1 = w1 ? 1.f / (m1 + a.eps) : 1.f, i2 = 1.f / (m2 + a.eps);
+    float xv[C], yv[C], hv[C], d[C], s = 0.f;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      xv[k] = nx[k];
+      hv[k] = nh[k];
+      d[k] = ny[k];
+      yv[k] = fmaf(a.scale, nr[k], xv[k] * i1 * W1[k] * G[k]);
+      s = fmaf(hv[k] * W2[k], yv[k], s);
+    }
+    if (row + 1 < end) load(row + 1);
+    float k2 = 0.f;
+    if (dh) {
+      const float s2 = block_sum(s, slot);
+      k2 = m2 > 0.f ? s2 * i2 * i2 / ((float)a.cols * m2) : 0.f;
+    }
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      d[k] += hv[k] * W2[k] * i2 - yv[k] * k2;
+      s = fmaf(d[k] * W1[k] * G[k], xv[k], s);
+    }
+    float k1 = 0.f;
+    if (w1) {
+      const float s1 = block_sum(s, slot);
+      k1 = m1 > 0.f ? s1 * i1 * i1 / ((float)a.cols * m1) : 0.f;
+    }
+    const int64_t off = row * a.cols;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = threadIdx.x + k * blockDim.x;
+      const float ax = d[k] * xv[k] * i1;
+      acc_a[k] += per_row ? ax * G[k] : ax;
+      acc_b[k] = fmaf(hv[k], yv[k] * i2, acc_b[k]);
+      if (c < a.cols) {
+        dr[off + c] = Tr::from_f(a.scale * d[k]);
+        dx[off + c] = Tr::from_f(d[k] * G[k] * W1[k] * i1 - xv[k] * k1);
+        if (dgate_rows) dgate_rows[off + c] = Tr::from_f(ax * W1[k]);
+      }
+    }
+  }
+  if (part_a) flush(part_a + ((int64_t)blockIdx.x + (per_row ? 0 : current)) * a.cols, acc_a);
+  if (part_b) flush(part_b + (int64_t)blockIdx.x * a.cols, acc_b);
+}
+
 // Forward: a row stays in registers (a warp or a CTA owns it, RowPlan); x, r, the weights and the gate
 // are requested together before the first reduction.
 template <typename T, int CHUNKS, bool CTA_ROW>
@@ -477,10 +632,15 @@ __global__ void __launch_bounds__(1024)
           for (int j = 0; j < 8; ++j) acc += v[j];
         }
       } else {
-        for (int64_t c = threadIdx.y; c < n; c += 32) {
-          const int64_t g0 = part_begin(c, n, a.rows) / a.rows_per_gate;
-          const int64_t g1 = (part_begin(c + 1, n, a.rows) - 1) / a.rows_per_gate;
-          for (int64_t g = g0; g <= g1; ++g) acc = fmaf(Tr::to_f(gate[g * a.cols + col]), part_a[(c + g) * a.cols + col], acc);
+        // by gate vectors (the parts of one take two divisions to find): all threads of a column on one vector's
+        // parts, or, of 32 vectors and more, on one vector each
+        const int64_t vectors = a.rows / a.rows_per_gate;
+        const bool apart = vectors >= 32;
+        for (int64_t g = apart ? threadIdx.y : 0; g < vectors; g += apart ? 32 : 1) {
+          const int64_t c0 = part_of(g * a.rows_per_gate, n, a.rows), c1 = part_of((g + 1) * a.rows_per_gate - 1, n, a.rows);
+          float sum = 0.f;
+          for (int64_t c = apart ? c0 : c0 + threadIdx.y; c <= c1; c += apart ? 1 : 32) sum += part_a[(c + g) * a.cols + col];
+          acc = fmaf(Tr::to_f(gate[g * a.cols + col]), sum, acc);
         }
       }
     }
@@ -553,6 +713,9 @@ BackwardPlan plan_backward(int64_t cols, bool ptrs_ok) {
   return p;
 }
 
+// threads of the kernels for any alignment: 4 columns each up to 1024, then 8
+int cols_threads(int64_t cols) { return cols > 2048 && cols <= 4096 ? 512 : 256; }
+
 int check(const char* who, const ResNormArgs& a, const void* gate) {
   TB200_REQUIRE(a.rows >= 0 && a.cols > 0, TB200_ERR_INVALID, "%s: bad shape", who);
   TB200_REQUIRE(a.rows < (1ll << 31) && a.cols < (1ll << 30), TB200_ERR_UNSUPPORTED, "%s: more than 2^31 rows or 2^30 columns", who);
@@ -593,9 +756,10 @@ extern "C" int tb200_gated_residual_rms_norm_fwd(void* h, void* y, float* rms1, 
       if (rc == 0) note_kernel("row_vec", 1);
       return rc;
     }
-    resnorm_fwd_generic<T><<<(unsigned)rows, 256, 0, st>>>((T*)h, (T*)y, rms1, rms2, (const T*)x, (const T*)r,
-                                                           (const T*)w1, (const T*)w2, (const T*)gate, a);
-    const int rc = launch_status("resnorm_fwd_generic");
+    auto kern = cols > 4096 ? resnorm_fwd_generic<T> : (cols <= 1024 ? resnorm_fwd_cols<T, 4> : resnorm_fwd_cols<T, 8>);
+    kern<<<(unsigned)rows, cols_threads(cols), 0, st>>>((T*)h, (T*)y, rms1, rms2, (const T*)x, (const T*)r, (const T*)w1,
+                                                        (const T*)w2, (const T*)gate, a);
+    const int rc = launch_status("resnorm_fwd_cols");
     if (rc == 0) note_kernel("row_generic", 1);
     return rc;
   });
@@ -665,10 +829,11 @@ extern "C" int tb200_gated_residual_rms_norm_bwd(void* dx, void* dr, void* dw1, 
            : plan.threads <= 256 ? go(IntC<4>{}, IntC<256>{})
                                  : go(IntC<4>{}, IntC<512>{});
     } else {
-      resnorm_bwd_generic<T><<<(unsigned)n, 256, 0, st>>>(
+      auto kern = cols > 4096 ? resnorm_bwd_generic<T> : (cols <= 1024 ? resnorm_bwd_cols<T, 4> : resnorm_bwd_cols<T, 8>);
+      kern<<<(unsigned)n, cols_threads(cols), 0, st>>>(
           (T*)dx, (T*)dr, per_row ? (T*)dgate : nullptr, part_a, part_b, (const T*)dh, (const T*)dy, (const T*)x, (const T*)r,
           (const T*)w1, (const T*)w2, (const T*)gate, rms1, rms2, a, per_row ? 1 : 0);
-      rc = launch_status("resnorm_bwd_generic");
+      rc = launch_status("resnorm_bwd_cols");
     }
     if (rc) return rc;
     int launches = 1;
