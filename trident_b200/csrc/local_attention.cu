@@ -123,14 +123,14 @@ void plan_split(LocalArgs* a, int64_t max_q, int64_t max_ctx, int row_tile, int 
 // The kernel family of a serving call and its tiles.
 struct PagedPlan {
   bool tc = false;
-  int few = 0;  // columns of the kernel for few rows
+  bool few = false;  // the kernel for few rows
   int row_tile = 0, key_tile = 0, row_tokens = 0;
 };
 PagedPlan plan_paged(LocalArgs* a, int64_t max_q, int64_t max_ctx, bool tc) {
   PagedPlan p;
   p.tc = tc;
-  p.few = tc ? local_few_rows(*a, (int)max_q) : 0;
-  p.row_tile = p.few ? p.few : (tc ? 2 * LOCAL_TC_TILE : local_simt_row_tile(*a, (int)max_q));
+  p.few = tc && local_few_rows(*a, (int)max_q);
+  p.row_tile = p.few ? LOCAL_FEW_ROWS : (tc ? 2 * LOCAL_TC_TILE : local_simt_row_tile(*a, (int)max_q));
   p.key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
   p.row_tokens = p.few || !tc ? p.row_tile / a->G : local_tc_row_tokens(*a);
   plan_split(a, max_q, max_ctx, p.row_tile, p.key_tile, (int64_t)sm_count() * (p.few ? 8 : 4));
@@ -297,7 +297,7 @@ extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_c
                 "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, split_bytes(a));
   a.part_out = (float*)workspace;
   a.part_lse = a.part_out + (size_t)a.splits * a.tokens * a.H * a.D;
-  int rc = plan.few ? launch_local_few_tc(out, q, key_cache, value_cache, a, plan.few, dtype, st)
+  int rc = plan.few ? launch_local_few_tc(out, q, key_cache, value_cache, a, dtype, st)
            : plan.tc ? launch_local_fwd_tc(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st)
                      : launch_local_fwd_simt(out, nullptr, q, key_cache, value_cache, a, max_q, dtype, st);
   if (rc) return rc;

@@ -1,11 +1,9 @@
-// Attention of few query rows (up to 64 of one sequence and key head: single tokens of a group of heads, or
-// a few tokens) over the pages of a cache, for 16-bit operands with head size 64 or 128.
+// Attention of few query rows (up to 16 of one sequence and key head: single tokens of a group of heads) over
+// the pages of a cache, for 16-bit operands with head size 64 or 128.
 //
-// Everything transposed, so that 128 keys lie on the tensor-memory lanes and the N = 16, 32 or 64 query rows
-// in the columns: a tile of keys is then worked on by 128 threads with N scores each, where a tile with the
-// rows on the lanes would leave all but N of them idle, one thread with 128 exponentials in a row (measured
-// on 64 single tokens over contexts to 8192, 4 heads a group: 5200 cycles a tile, 292 us; HBM gives an SM a
-// tile of keys and values in 2800).
+// Everything transposed, so that 128 keys lie on the tensor-memory lanes and the query rows in N = 16 columns:
+// a tile of keys is then worked on by 128 threads with 16 scores each, where a tile with the rows on the lanes
+// would leave all but 16 of them idle, one thread with 128 exponentials in a row.
 //
 //   S^T = K Q^T        [keys][rows], two buffers
 //   P^T = exp2(S^T scale log2e - m), 16-bit, to shared memory as [row][key] (operand, 128-byte swizzle)
@@ -16,7 +14,7 @@
 // units) above it, which a barrier with a vote finds out: a step costs one barrier, and the shuffles of a
 // row maximum only when it moves. Row sums are kept per thread and added at the end.
 //
-//   warp 0      producer: one ring of four (D = 64: six) tiles, K and V in turn; one lane per piece of a page
+//   warp 0      producer: one ring of three (D = 64: five) tiles, K and V in turn; one lane per piece of a page
 //   warp 1      MMA issuer, tensor-memory allocation
 //   warps 2-5   softmax: lane = key
 // Two CTAs an SM: the start and end of one walk overlap the other's loads. Bound by HBM (the products read
@@ -31,6 +29,7 @@ namespace tb200 {
 namespace {
 
 constexpr int TILE = LOCAL_TC_TILE;
+constexpr int N = LOCAL_FEW_ROWS;
 constexpr int THREADS = 192;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -68,21 +67,8 @@ __device__ inline bool vote128(bool mine) {
 }
 __device__ inline void sync128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
-// N consecutive columns of this thread's lane
-template <int N>
-__device__ inline void load_columns(uint32_t addr, uint32_t (&v)[N]) {
-#pragma unroll
-  for (int c = 0; c < N; c += 16) {
-    uint32_t x[16];
-    ptx::tmem_ld16(addr + c, x);
-    am::tmem_ld_wait_dep(x);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) v[c + e] = x[e];
-  }
-}
-
-template <typename T, int D, int N>
-__global__ void __launch_bounds__(THREADS, N == 64 ? 1 : 2)
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 2)
     local_few_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const FewParams p) {
   constexpr int STAGES = D == 128 ? 3 : 5;  // tiles of the ring
@@ -91,7 +77,7 @@ __global__ void __launch_bounds__(THREADS, N == 64 ? 1 : 2)
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t IDESC_S = ptx::make_idesc(IS_BF16, false, false, TILE, N);  // K-major x K-major
   constexpr uint32_t IDESC_O = ptx::make_idesc(IS_BF16, true, false, TILE, N);   // V^T along the features, P^T K-major
-  constexpr uint32_t TMEM_COLS = N == 16 ? 64 : (N == 32 ? 128 : 256);
+  constexpr uint32_t TMEM_COLS = 64;
   constexpr uint32_t COL_S = 0, COL_O = 2 * N;
 
   extern __shared__ uint8_t smem_raw[];
@@ -265,23 +251,22 @@ __global__ void __launch_bounds__(THREADS, N == 64 ? 1 : 2)
       uint32_t sv[N];
       ptx::mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.status, 149);
       ptx::tc_fence_after();
-      load_columns<N>(tmem_base + lane_off + COL_S + (i & 1) * N, sv);
+      ptx::tmem_ld16(tmem_base + lane_off + COL_S + (i & 1) * N, sv);
+      am::tmem_ld_wait_dep(sv);
       ptx::tc_fence_before();
       ptx::mbar_arrive(&s_free[i & 1]);
       // rows that see this key: from `low` on they are not before it, below `high` within the window
-      uint32_t seen[(N + 31) / 32];
+      uint32_t seen;
       {
         const int low = saturate((int64_t)(j - pos0) * a.G), high = saturate(((int64_t)j - pos0 + a.window) * a.G);
         const uint32_t sink = j < a.sinks ? 0xffffffffu : 0u, exists = j < seq.kv_len ? 0xffffffffu : 0u;
-#pragma unroll
-        for (int q = 0; q < (N + 31) / 32; ++q)
-          seen[q] = exists & low_bits(rows - 32 * q) & ~low_bits(low - 32 * q) & (low_bits(high - 32 * q) | sink);
+        seen = exists & low_bits(rows) & ~low_bits(low) & (low_bits(high) | sink);
       }
       float x[N];
       bool above = false;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        x[n] = (seen[n >> 5] >> (n & 31)) & 1u ? __uint_as_float(sv[n]) * p.scale_log2 : -INFINITY;
+        x[n] = (seen >> n) & 1u ? __uint_as_float(sv[n]) * p.scale_log2 : -INFINITY;
         above = above || x[n] > m_smem[n] + RESCALE_THRESHOLD;
       }
       if (vote128(above)) {  // the maxima move
@@ -308,14 +293,11 @@ __global__ void __launch_bounds__(THREADS, N == 64 ? 1 : 2)
         }
         if (i > 0) {
           uint32_t o[N];
-          load_columns<N>(tmem_base + lane_off + COL_O, o);
+          ptx::tmem_ld16(tmem_base + lane_off + COL_O, o);
+          am::tmem_ld_wait_dep(o);
 #pragma unroll
-          for (int c = 0; c < N; c += 16) {
-            uint32_t y[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(o[c + e]) * f[c + e]);
-            ptx::tmem_st16(tmem_base + lane_off + COL_O + c, y);
-          }
+          for (int n = 0; n < N; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * f[n]);
+          ptx::tmem_st16(tmem_base + lane_off + COL_O, o);
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
         }
@@ -361,7 +343,10 @@ __global__ void __launch_bounds__(THREADS, N == 64 ? 1 : 2)
     }
     sync128();
     uint32_t o[N];
-    if (steps > 0) load_columns<N>(tmem_base + lane_off + COL_O, o);
+    if (steps > 0) {
+      ptx::tmem_ld16(tmem_base + lane_off + COL_O, o);
+      am::tmem_ld_wait_dep(o);
+    }
     // lane = feature
     if (r < D) {
 #pragma unroll
@@ -390,14 +375,14 @@ __global__ void __launch_bounds__(THREADS, N == 64 ? 1 : 2)
   }
 }
 
-template <typename T, int D, int N>
+template <typename T, int D>
 int launch_few(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FewParams& p, cudaStream_t st) {
   constexpr int RING = (D == 128 ? 3 : 5) * TILE * D * 2;
   constexpr int REST = 2 * N * TILE * 2 + N * D * 2 + 5 * N * 4 + 256;
   // (at D = 64 a product on the last stage reads one tile beyond the ring)
   constexpr int SMEM = RING + (D == 64 && REST < TILE * D * 2 ? TILE * D * 2 : REST) + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
-  auto kern = local_few_tc_kernel<T, D, N>;
+  auto kern = local_few_tc_kernel<T, D>;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = smem_optin_per_device(done, reinterpret_cast<const void*>(kern), SMEM);
   if (e != cudaSuccess) {
@@ -410,7 +395,7 @@ int launch_few(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
 
 }  // namespace
 
-int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, const LocalArgs& a, int columns, int dtype,
+int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, const LocalArgs& a, int dtype,
                         cudaStream_t st) {
   FewParams p;
   p.a = a;
@@ -419,15 +404,13 @@ int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, 
   p.scale_log2 = a.scale * LOG2E;
   p.piece = local_piece(a);
   CUtensorMap mq, mk, mv;
-  if (!local_map_rows(&mq, q, a.qs, a, columns / a.G, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
+  if (!local_map_rows(&mq, q, a.qs, a, N / a.G, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
       !local_map_keys(&mv, v, a.vs, a, p.piece, "v"))
     return TB200_ERR_UNSUPPORTED;
   auto go = [&](auto tag, auto dsel) -> int {
     using T = decltype(tag);
     constexpr int D = decltype(dsel)::value;
-    if (columns == 16) return launch_few<T, D, 16>(mq, mk, mv, p, st);
-    if (columns == 32) return launch_few<T, D, 32>(mq, mk, mv, p, st);
-    return launch_few<T, D, 64>(mq, mk, mv, p, st);
+    return launch_few<T, D>(mq, mk, mv, p, st);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

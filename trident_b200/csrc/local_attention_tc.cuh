@@ -28,12 +28,15 @@ struct Divisor {
 bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void* k, const void* v, const void* out);
 int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, const void* v, const LocalArgs& a, int max_q,
                         int dtype, cudaStream_t st);
-// Serving form with few rows (max_q * G <= 64): keys on the tensor-memory lanes. `tokens` of a row tile.
-static inline int local_few_rows(const LocalArgs& a, int max_q) {  // columns of the kernel, 0: too many rows
-  const int64_t rows = (int64_t)max_q * a.G;
-  return !a.table || rows > 64 ? 0 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : 64));
+// Serving form with few rows: keys on the tensor-memory lanes, LOCAL_FEW_ROWS columns. 64 contexts of 4096 bf16
+// keys, 8 key heads: 4, 8, 16 rows take 149, 157, 175 us at D = 64 and 220, 230, 253 at D = 128, the forward
+// kernel 204 to 212 and 247 to 253; 4 contexts of 16384: 68, 73, 83 against 74 to 76, and 87, 93, 103 against 85.
+// (Of 32 and 64 columns the per-row work of every thread outweighs the loads: 304 and 1177 us against 219 and 229.)
+constexpr int LOCAL_FEW_ROWS = 16;
+static inline bool local_few_rows(const LocalArgs& a, int max_q) {
+  return a.table && (int64_t)max_q * a.G <= (a.D == 64 ? LOCAL_FEW_ROWS : 8);
 }
-int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, const LocalArgs& a, int columns, int dtype,
+int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, const LocalArgs& a, int dtype,
                         cudaStream_t st);
 
 // Tensor maps (false with the error text set when the driver refuses one) and what they take.
