@@ -496,6 +496,37 @@ def test_pool_of_more_than_32_bit_offsets(dt, D, device):
         ref.check(got, _want(q, cache, tokens, 0, 0, D ** -0.5, dt), f"{tokens}")
 
 
+@pytest.mark.gpu
+def test_no_room_is_refused(device):
+    q, k = torch.zeros(2, 4, 64, device=device), torch.zeros(2, 2, 64, device=device)
+    lengths = torch.zeros(2, dtype=torch.int32, device=device)
+    for pages, blocks in ((0, 3), (3, 0)):
+        cache = torch.zeros(pages, 16, 2, 64, device=device)
+        table = torch.zeros(2, blocks, dtype=torch.int32, device=device)
+        with pytest.raises(ValueError, match="at least one page"):
+            attend(q, cache, cache, table, lengths)
+        with pytest.raises(ValueError, match="at least one page"):
+            append(k, k, cache, cache, table, lengths)
+
+
+def test_direct_entry_points_check_their_arguments():
+    """The extension module behind the calls: numbers, kinds and lengths of its arguments, before the library."""
+    from trident_b200 import _fastcall
+
+    for name in ("tb200_window_attention_fwd", "tb200_paged_attention", "tb200_paged_cache_append", "tb200_gated_residual_rms_norm_fwd"):
+        entry = getattr(_fastcall, name)
+        count = len(_lib.SIGNATURES[name][1])
+        for args in ((), (0,) * (count - 1), (0,) * (count + 1), ("x",) * count, (2 ** 70,) * count):
+            with pytest.raises((TypeError, OverflowError)):
+                entry(*args)
+    strides = (1, 1, 1, 1)
+    window = _fastcall.tb200_window_attention_fwd
+    for bad in ((1, 1, 1), [1, 1, 1, 1], None, (1, 1, 1, "x"), (1, 1, 1, 2 ** 70)):
+        with pytest.raises((TypeError, OverflowError)):
+            window(8, 8, 8, 8, 8, 1, 2, 2, 8, 16, strides, bad, strides, strides, 4, 0, 1.0, 0, 0)
+    assert window(8, 8, 8, 8, 8, 1, 3, 2, 8, 16, strides, strides, strides, strides, 4, 0, 1.0, 0, 0) == -1
+
+
 def test_library_refuses_before_launch():
     import ctypes
 

@@ -41,6 +41,11 @@ def _check_cache(key_cache, value_cache, block_table, context_lengths, query_off
         raise ValueError("Paged attention has no backward pass: call it under torch.no_grad().")
 
 
+def _check_room(block_table, key_cache):
+    if block_table.shape[1] == 0 or key_cache.shape[0] == 0:
+        raise ValueError("block_table should have a block for every sequence and the cache at least one page.")
+
+
 def _index(tensor):
     """An int32 tensor whose last dimension is dense."""
     return tensor if tensor is None or tensor.numel() == 0 or tensor.stride(-1) == 1 else tensor.contiguous()
@@ -95,6 +100,7 @@ def paged_attention(
     zero_tail = output is None and query_offsets is not None
     if sequences == 0 or tokens == 0:
         return torch.zeros_like(query) if output is None else output
+    _check_room(block_table, key_cache)
     if output is None:
         output = torch.empty_like(query)
     window = 0 if window_size is None else min(window_size, MOST_TOKENS)
@@ -141,6 +147,7 @@ def paged_cache_append(key, value, key_cache, value_cache, block_table, context_
     )
     if key.shape[0] == 0 or block_table.shape[0] == 0:
         return
+    _check_room(block_table, key_cache)
 
     util.push_trace("tb200_paged_cache_append")
     _lib.paged_cache_append(
