@@ -23,8 +23,14 @@
 // The queries beyond the window of a key tile that holds sinks ("far", LocalBwdArgs) are cut into pieces
 // about as long as a walk inside the window, each a CTA of its own: a single CTA would walk all queries.
 //
-// Bound by the compute warps' exponentials and score gradients (the 16 K exponentials of a 128 x 128 tile
-// pair take 1024 cycles), next to them shared-memory reads of the operands and the tensor pipe.
+// P and dS are rounded to 16 bits as operands of their products, as the tensor cores take them: half a step each
+// (2-norm of the error of dq against 64 bits 0.0026 in bf16, 0.00033 in fp16, of which the final rounding alone is
+// 0.0017 and 0.00021). Statistics, delta and all sums are fp32.
+//
+// Bounds, at 2 x 32 heads x 4096 x 128 bf16, window 1024, 8 key heads. dK, dV: 252 us (957 TFLOP/s); a step takes
+// 2350 cycles, of which the products alone, two of them with both operands in shared memory, take about 2200 (dS^T
+// over P^T instead of dP^T, so that the next dP^T need not wait for dK: 302 us, one chain of all four products). dQ:
+// 184 us (983 TFLOP/s); a step takes 2050 cycles, the chain dQ -> dP -> score gradients (1536 of products).
 #include <type_traits>
 
 #include "attn_math.cuh"
@@ -50,6 +56,7 @@ struct BwdParams {
   int row_tiles;
   int col_tokens;       // tokens of a column tile (dK, dV)
   int col_tiles, key_tiles;
+  Divisor heads, kv;    // n * KV, KV
   int* status;
 };
 
@@ -121,13 +128,18 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   const LocalArgs& a = p.b.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int s = blockIdx.z, hk = blockIdx.y;
+  // The longest walks of all sequences and heads first (far pieces, then the key tiles in order, whose walks end
+  // with the sequence): the short ones even out the last CTAs of the SMs. By sequence and head SMs stood idle 15 %
+  // of the time at 512 key tiles and 48 far pieces (262 us, so 252; the dQ kernel's tiles likewise: 189 and 184).
+  const int rank = p.heads.quotient(blockIdx.x), sh = blockIdx.x - rank * (int)p.heads.d;
+  const int s = p.kv.quotient(sh), hk = sh - s * a.KV;
   // the walk: column tiles [i0, i0 + steps)
-  int jt = blockIdx.x, piece = -1, i0, i1;
-  const bool far = jt >= p.key_tiles;
+  const int far_pieces = p.b.sink_tiles * p.b.far;
+  int jt = rank - far_pieces, piece = -1, i0, i1;
+  const bool far = jt < 0;
   if (far) {
-    piece = (jt - p.key_tiles) % p.b.far;
-    jt = (jt - p.key_tiles) / p.b.far;
+    piece = rank % p.b.far;
+    jt = rank / p.b.far;
   }
   const int beyond = (near_end(a, jt, TILE) + p.col_tokens - 1) / p.col_tokens;  // first column tile beyond the window
   if (far) {
@@ -454,12 +466,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   struct Unit {
     int s, hk, t0, ntok;
   };
-  // tile `unit`: longest walks (last tokens) of a sequence and key head first
+  // tile `unit`: longest walks (last tokens) of all sequences and key heads first
   auto unit_at = [&](int unit) {
     Unit w;
-    const int sh = unit / p.row_tiles, it = p.row_tiles - 1 - unit % p.row_tiles;
-    w.s = sh / a.KV;
-    w.hk = sh % a.KV;
+    const int rank = p.heads.quotient(unit), sh = unit - rank * (int)p.heads.d, it = p.row_tiles - 1 - rank;
+    w.s = p.kv.quotient(sh);
+    w.hk = sh - w.s * a.KV;
     w.t0 = it * p.tile_tokens;
     w.ntok = min(p.tile_tokens, a.tokens - w.t0);
     return w;
@@ -845,7 +857,11 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
   p.col_tokens = col_tokens;
   p.col_tiles = (int)ceil_div(a.tokens, col_tokens);
   p.key_tiles = (int)ceil_div(a.tokens, TILE);
+  p.heads = Divisor(a.n * a.KV);
+  p.kv = Divisor(a.KV);
   p.status = device_status_ptr();
+  const int64_t parts = (int64_t)a.n * a.KV * (p.key_tiles + (int64_t)b.sink_tiles * b.far);
+  TB200_REQUIRE(parts < (1ll << 31), TB200_ERR_UNSUPPORTED, "local_dkv_tc: %lld walks", (long long)parts);
   auto go = [&](auto tag, auto dsel) -> int {
     using T = decltype(tag);
     constexpr int D = decltype(dsel)::value;
@@ -860,7 +876,7 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
     const int64_t units = (int64_t)a.n * a.KV * p.row_tiles;
     kq<<<(unsigned)(units < sm_count() ? units : sm_count()), THREADS, DQ_SMEM, st>>>(mq128, md128, mo128, mdq, mk, mv, p);
     if (int rc = launch_status("local_dq_tc")) return rc;
-    kkv<<<dim3((unsigned)(p.key_tiles + b.sink_tiles * b.far), (unsigned)a.KV, (unsigned)a.n), THREADS, DKV_SMEM, st>>>(mq, md, mk, mv, p);
+    kkv<<<(unsigned)parts, THREADS, DKV_SMEM, st>>>(mq, md, mk, mv, p);
     return launch_status("local_dkv_tc");
   };
   using D64 = std::integral_constant<int, 64>;

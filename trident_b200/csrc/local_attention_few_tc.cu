@@ -17,8 +17,9 @@
 //   warp 0      producer: one ring of three (D = 64: five) tiles, K and V in turn; one lane per piece of a page
 //   warp 1      MMA issuer, tensor-memory allocation
 //   warps 2-5   softmax: lane = key
-// Two CTAs an SM: the start and end of one walk overlap the other's loads. Bound by HBM (the products read
-// each key and value once from shared memory: 512 cycles a tile at D = 128).
+// Two CTAs an SM: the start and end of one walk overlap the other's loads. Bound by HBM: 64 single tokens of 8 x 4
+// heads over contexts of 512 to 8192, D = 128 (1.14 GB), 200 us and 5 for joining the parts, 5.7 TB/s. The products
+// read each key and value once from shared memory, 512 cycles a tile, the pipe is 5 % busy.
 #include <type_traits>
 
 #include "attn_math.cuh"

@@ -16,8 +16,9 @@
 //   warp 1      MMA issuer: S_t = Q_t K^T, O_t += P_t V (P_t from tensor memory, in two parts: the product
 //               starts when three quarters of P_t are there)
 //   warp 2      tensor-memory allocation; issues the bulk copies of output tiles
-//   warp 3      serving form: zeroes the rows of the last V tile behind the sequence's end (a probability
-//               of 0 times what an unused row holds, which may be NaN, would not be 0)
+//   warp 3      looks the walks of coming units up for the MMA issuer; serving form: zeroes the rows of the last
+//               V tile behind the sequence's end (a probability of 0 times what an unused row holds, which may
+//               be NaN, would not be 0)
 //   warps 4-7   softmax of query tile 0, warps 8-11 of tile 1: one thread per row; scores stay in registers
 //               between maximum and exponentials. Warps without a row of the sequence only pass the
 //               barriers (a single new token is G rows of one tile). Output tiles leave through shared memory
@@ -29,9 +30,12 @@
 // exactly. The row sum adds the fp32 probabilities; P is rounded to 16 bits for the product with V, as the
 // tensor cores take it.
 //
-// Bound, by size of the problem: the chain scores -> maximum -> exponentials -> P V of each of the two tiles
-// (exponentials of a tile pair take the 16 units of an SM 1024 cycles, as both products together at D = 128)
-// for chunks and training, HBM for single tokens.
+// Bound, by size of the problem: HBM for single tokens, for chunks and training the chain of each of the two
+// tiles. At D = 128 a step of it takes 3700 cycles: 800 from the issue of the scores (operands in shared memory:
+// 94 cycles an instruction instead of 64) to the threads that read them, 800 to the maximum, 1500 for the
+// exponentials (1024 of them the tile's share of the exponential unit), 600 until the next scores are issued behind
+// P V on the in-order pipe; the other tile's step runs beside it. 2 x 32 heads x 4096 x 128 bf16, window 1024, 8 key
+// heads: 169 us (713 TFLOP/s), tensor pipe 45 % busy; 4 chunks of up to 512 tokens over contexts to 16384: 55 us.
 #include <mutex>
 #include <type_traits>
 
@@ -58,7 +62,6 @@ struct FwdParams {
   int tile_tokens;  // tokens of a query tile
   int piece;        // R: rows of one copy of keys
   int pairs, units; // pairs of query tiles per sequence and key head; pairs * KV * sequences * parts
-  int longest_first;
   Divisor outer, kv, splits;  // of a unit's number (unit_at)
   uint32_t wait_units;
 };
@@ -137,15 +140,11 @@ struct Walk {
 template <bool PAGED>
 __device__ inline bool unit_at(const FwdParams& p, int unit, Unit* w) {
   const LocalArgs& a = p.a;
-  const int high = p.outer.quotient(unit), low = unit - high * (int)p.outer.d;
-  int pair, rest;
-  if (PAGED || p.longest_first) {
-    pair = p.longest_first ? p.pairs - 1 - high : high;
-    rest = low;
-  } else {  // (neighbouring tiles share keys)
-    pair = low;
-    rest = high;
-  }
+  const int high = p.outer.quotient(unit), rest = unit - high * (int)p.outer.d;
+  // Walks of a training step grow with the tile up to the window: longest first (3 sequences of 1111 tokens, 2 key
+  // heads: 18.8 us by sequence and head, 17.1 so; 2 of 4096, 8 key heads: 169 and 170). Those of chunks hardly
+  // grow, and their last tiles may be empty.
+  const int pair = PAGED ? high : p.pairs - 1 - high;
   const int sequence_part = p.kv.quotient(rest);
   w->hk = rest - sequence_part * a.KV;
   w->s = p.splits.quotient(sequence_part);
@@ -969,9 +968,7 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   const int64_t units = (int64_t)p.pairs * a.KV * a.n * a.splits;
   TB200_REQUIRE(units < (1ll << 31) - (1 << 20), TB200_ERR_UNSUPPORTED, "local_fwd_tc: %lld units of work", (long long)units);
   p.units = (int)units;
-  // (walks of a causal training step grow with the tile; those of chunks hardly do, and their last tiles may be empty)
-  p.longest_first = a.window == NO_WINDOW && !a.table;
-  p.outer = Divisor(a.table || p.longest_first ? p.units / p.pairs : p.pairs);
+  p.outer = Divisor(p.units / p.pairs);
   p.kv = Divisor(a.KV);
   p.splits = Divisor(a.splits);
   p.wait_units = ptx::WAIT_LIMIT_UNITS;

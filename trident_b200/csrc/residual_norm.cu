@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256)
 // ------------------------------------------------------------------ rows of up to 4096 columns, any alignment
 // Widths that are no multiple of 16 bytes, unaligned views: a CTA holds a row in registers, C columns a thread,
 // a block apart, and reads and writes each element once, one element at a time. At 1665 rows of 1021 fp32 columns
-// (20 MB forward, 41 backward) forward and backward take 9 and 17 us; the kernels above, which read a row again for
+// (27 MB forward, 41 backward) forward and backward take 9 and 17 us; the kernels above, which read a row again for
 // every pass and keep the column sums in memory, take 15 and 54.
 template <typename T, int C>
 __global__ void __launch_bounds__(512)
