@@ -161,7 +161,6 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// ------------------------------------------------------------------ rows of 16-byte vectors
 // ------------------------------------------------------------------ rows of up to 4096 columns, any alignment
 // Widths that are no multiple of 16 bytes, unaligned views: a CTA holds a row in registers, C columns a thread,
 // a block apart, and reads and writes each element once, one element at a time. At 1665 rows of 1021 fp32 columns
@@ -317,8 +316,9 @@ __global__ void __launch_bounds__(512)
   if (part_b) flush(part_b + (int64_t)blockIdx.x * a.cols, acc_b);
 }
 
+// ------------------------------------------------------------------ rows of 16-byte vectors
 // Forward: a row stays in registers (a warp or a CTA owns it, RowPlan); x, r, the weights and the gate
-// are requested together before the first reduction.
+// are requested together before the first reduction. 8192 x 4096 bf16: 48 us, 5.6 TB/s.
 template <typename T, int CHUNKS, bool CTA_ROW>
 __global__ void __launch_bounds__(CTA_ROW ? 512 : 256, CTA_ROW ? 2 : 4)
     resnorm_fwd_vec(T* __restrict__ h, T* __restrict__ y, float* __restrict__ rms1, float* __restrict__ rms2,
@@ -406,7 +406,8 @@ __global__ void __launch_bounds__(CTA_ROW ? 512 : 256, CTA_ROW ? 2 : 4)
 // reductions of a row). A thread keeps its columns' w2 and gate * w1 (as long as the gate vector stays the
 // same) and their column sums in registers as fp32 pairs; per element of the four inputs that leaves a
 // conversion and about eight two-lane operations, where weights unpacked anew for every row and divisions
-// per thread bounded the kernel at 2.8 TB/s.
+// per thread bounded the kernel at 2.8 TB/s. 8192 x 4096 bf16: 93 us, 4.3 TB/s, with half of the issue slots
+// used and two block-wide sums a row in between; joining the parts another 9.
 __device__ inline float reciprocal(float v) {  // (one unit in the last place)
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
