@@ -107,7 +107,7 @@ int tb200_rms_norm_bwd(void* dx, void* dweight, void* dbias /*nullable*/, const 
  *   y = residual_scale * r + gate * n   (gate null: 1)
  *   h = y / (rms(y) + eps) * w2,   rms(v) = sqrt(mean(v^2))
  * x, r, y, h are contiguous [rows, cols]; w1, w2 [cols]; gate is [cols] (rows_per_gate 0) or
- * [rows / rows_per_gate, cols]. rms1 (unused without w1) and rms2 [rows] are kept for backward. */
+ * [rows / rows_per_gate, cols]. rms1 (unused without w1) and rms2 [rows] are kept for backward; null: not written. */
 int tb200_gated_residual_rms_norm_fwd(void* h, void* y, float* rms1, float* rms2, const void* x, const void* r,
                                       const void* w1 /*nullable*/, const void* w2, const void* gate /*nullable*/,
                                       int64_t rows, int64_t cols, int64_t rows_per_gate, float residual_scale,
@@ -259,7 +259,7 @@ int tb200_attention_bwd(void* dq, void* dk, void* dv, void* dmask /*nullable*/,
  * Causal attention of a query at position i over the keys j <= i with i - j < window or j < sinks
  * (the first `sinks` tokens stay visible). q, out: [B,H,S,D]; k, v: [B,KV,S,D], H a multiple of KV
  * (at most 64 times): query head h uses key head h / (H / KV). All with element strides (4 each).
- * lse [B,H,S]: natural-log sum of exponentials of a score row (float32), kept for backward. Keys and
+ * lse [B,H,S]: natural-log sum of exponentials of a score row (float32), kept for backward; null: not written. Keys and
  * values have to be finite: a NaN or infinity may reach queries near it that do not see it. */
 int tb200_window_attention_fwd(void* out, float* lse, const void* q, const void* k, const void* v, int64_t B,
                                int64_t H, int64_t KV, int64_t S, int64_t D, const int64_t* q_strides,

@@ -130,3 +130,18 @@ def test_on_a_second_device(device):
     assert there.device.index == 1 and torch.equal(here.cpu(), there.cpu())
     with pytest.raises(ValueError, match="device"):
         trident.function.sliding_window_attention(q.to("cuda:0"), k.to("cuda:1"), k.to("cuda:1"), 20, 2)
+
+
+@pytest.mark.gpu
+def test_without_gradients_nothing_is_kept_and_nothing_changes(device, dtype):
+    """Calls that autograd does not record keep no statistics and give the same bits."""
+    q, k, v = (util.randn(2, h, 90, 64, seed=130 + h).to(dtype).to(device) for h in (4, 2, 2))
+    for D in (64, 32):
+        plain = trident.function.sliding_window_attention(*(t[..., :D] for t in (q, k, v)), 30, 2)
+        recorded = trident.function.sliding_window_attention(q[..., :D].detach().requires_grad_(True), k[..., :D], v[..., :D], 30, 2)
+        assert recorded.requires_grad and not plain.requires_grad and torch.equal(plain, recorded)
+    for cols in (64, 63, 4500, 9001):
+        x, r, w = (util.randn(*s, seed=140 + i).to(dtype).to(device) for i, s in enumerate(((7, cols), (7, cols), (cols,))))
+        plain = trident.function.gated_residual_rms_norm(x, r, w, w, w, 0.5, EPS)
+        recorded = trident.function.gated_residual_rms_norm(x.clone().requires_grad_(True), r, w, w, w, 0.5, EPS)
+        assert all(torch.equal(a, b) for a, b in zip(plain, recorded))

@@ -300,10 +300,13 @@ def rms_norm_bwd(dx, dweight, dbias, dy, x, weight, rms, workspace, rows, cols, 
 
 
 def gated_residual_rms_norm_fwd(h, y, rms, x, r, w1, w2, gate, rows, cols, rows_per_gate, scale, eps):
-    """rms: [2, rows], of x and of y."""
-    rms1 = rms.data_ptr()
+    """rms: [2, rows], of x and of y, or None."""
+    rms1 = rms2 = None
+    if rms is not None:
+        rms1 = rms.data_ptr()
+        rms2 = rms1 + 4 * rows
     _call(
-        "tb200_gated_residual_rms_norm_fwd", x, _ptr(h), _ptr(y), rms1, rms1 + 4 * rows, _ptr(x), _ptr(r), _ptr(w1),
+        "tb200_gated_residual_rms_norm_fwd", x, _ptr(h), _ptr(y), rms1, rms2, _ptr(x), _ptr(r), _ptr(w1),
         _ptr(w2), _ptr(gate), rows, cols, rows_per_gate, scale, eps, dtype_code(x.dtype),
     )
 

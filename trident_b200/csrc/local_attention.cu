@@ -184,7 +184,7 @@ extern "C" int tb200_window_attention_fwd(void* out, float* lse, const void* q, 
                            sinks, softmax_scale))
     return rc;
   if (B == 0 || S == 0) return 0;
-  TB200_REQUIRE(out && lse && q && k && v, TB200_ERR_INVALID, "window_attention_fwd: null pointer");
+  TB200_REQUIRE(out && q && k && v, TB200_ERR_INVALID, "window_attention_fwd: null pointer");
   const bool tc = local_tc_supported(a, dtype, q, k, v, out);
   int rc = tc ? launch_local_fwd_tc(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream)
               : launch_local_fwd_simt(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream);

@@ -771,7 +771,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       if (live) {
         const float ls = some ? m_used * LN2 + logf(l) : -INFINITY;
         if (!whole) a.part_lse[prow] = ls;
-        else if (!PAGED) p.lse[((long long)w.s * a.H + head) * a.tokens + tok] = ls;
+        else if (!PAGED && p.lse) p.lse[((long long)w.s * a.H + head) * a.tokens + tok] = ls;
       }
       unit = next_unit(unit + gridDim.x);
       if (counted) {

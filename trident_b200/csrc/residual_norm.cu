@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256)
     }
     const float rms = sqrtf(block_sum(s, slot) / (float)a.cols);
     i1 = 1.f / (rms + a.eps);
-    if (threadIdx.x == 0) rms1[row] = rms;
+    if (rms1 && threadIdx.x == 0) rms1[row] = rms;
   }
   auto y_at = [&](int64_t c) {
     float n = Tr::to_f(x[off + c]);
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256)
   }
   const float rms = sqrtf(block_sum(s, slot) / (float)a.cols);
   const float i2 = 1.f / (rms + a.eps);
-  if (threadIdx.x == 0) rms2[row] = rms;
+  if (rms2 && threadIdx.x == 0) rms2[row] = rms;
   for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) h[off + c] = Tr::from_f(y_at(c) * i2 * Tr::to_f(w2[c]));
 }
 
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(512)
     for (int k = 0; k < C; ++k) s = fmaf(v[k], v[k], s);
     const float rms = sqrtf(block_sum(s, slot) / (float)a.cols);
     i1 = 1.f / (rms + a.eps);
-    if (threadIdx.x == 0) rms1[row] = rms;
+    if (rms1 && threadIdx.x == 0) rms1[row] = rms;
   }
   float s = 0.f;
 #pragma unroll
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
   for (int k = 0; k < C; ++k) w[k] = threadIdx.x + k * blockDim.x < a.cols ? Tr::to_f(w2[threadIdx.x + k * blockDim.x]) : 0.f;
   const float rms = sqrtf(block_sum(s, slot) / (float)a.cols), i2 = 1.f / (rms + a.eps);
-  if (threadIdx.x == 0) rms2[row] = rms;
+  if (rms2 && threadIdx.x == 0) rms2[row] = rms;
 #pragma unroll
   for (int k = 0; k < C; ++k) {
     const int c = threadIdx.x + k * blockDim.x;
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(CTA_ROW ? 512 : 256, CTA_ROW ? 2 : 4)
       }
       const float rms = sqrtf(row_reduce<CTA_ROW, false>(hsum2(s2), slot, phase) * inv_n);
       i1 = 1.f / (rms + a.eps);
-      if (rt.tid == 0) rms1[row] = rms;
+      if (rms1 && rt.tid == 0) rms1[row] = rms;
     }
     const uint64_t i1_2 = splat2(i1), scale2 = splat2(a.scale);
     uint64_t s2 = 0ull;
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(CTA_ROW ? 512 : 256, CTA_ROW ? 2 : 4)
     }
     const float rms = sqrtf(row_reduce<CTA_ROW, false>(hsum2(s2), slot, phase) * inv_n);
     const uint64_t i2_2 = splat2(1.f / (rms + a.eps));
-    if (rt.tid == 0) rms2[row] = rms;
+    if (rms2 && rt.tid == 0) rms2[row] = rms;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int col = rt.template col<VEC>(c);
@@ -739,8 +739,7 @@ extern "C" int tb200_gated_residual_rms_norm_fwd(void* h, void* y, float* rms1, 
   a.scale = residual_scale; a.eps = eps;
   if (int rc = check("gated_residual_rms_norm_fwd", a, gate)) return rc;
   if (rows == 0) return 0;
-  TB200_REQUIRE(h && y && rms2 && x && r && w2 && (!w1 || rms1), TB200_ERR_INVALID,
-                "gated_residual_rms_norm_fwd: null pointer");
+  TB200_REQUIRE(h && y && x && r && w2, TB200_ERR_INVALID, "gated_residual_rms_norm_fwd: null pointer");
   cudaStream_t st = (cudaStream_t)stream;
   return dispatch_dtype(dtype, [&](auto tag) -> int {
     using T = decltype(tag);

@@ -52,7 +52,7 @@ def gated_residual_rms_norm(
     args = (input, residual, post_weight, pre_weight, gate, residual_scale, eps)
     if util.needs_grad(input, residual, post_weight, pre_weight, gate):
         return operation.GatedResidualRMSNorm.apply(*args)
-    return operation.GatedResidualRMSNorm.run(*args)[0]
+    return operation.GatedResidualRMSNorm.run(*args, statistics=False)[0]
 
 
 def geglu(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None, use_accelerator: bool = False):
@@ -238,7 +238,7 @@ def sliding_window_attention(
     scale = 1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None else softmax_scale
     if util.needs_grad(query, key, value):
         return operation.WindowAttention.apply(query, key, value, window_size, num_sinks, scale)
-    return operation.WindowAttention.run(query, key, value, window_size, num_sinks, scale)[0]
+    return operation.WindowAttention.run(query, key, value, window_size, num_sinks, scale, statistics=False)[0]
 
 
 def softmax(input: torch.Tensor, dim: int = None):

@@ -49,8 +49,9 @@ class GatedResidualRMSNorm(torch.autograd.Function):
         return outputs
 
     @staticmethod
-    def run(input, residual, post_weight, pre_weight, gate, residual_scale, eps):
-        """The forward pass: ((output, output_residual), what the backward pass needs, rows per gate)."""
+    def run(input, residual, post_weight, pre_weight, gate, residual_scale, eps, statistics=True):
+        """The forward pass: ((output, output_residual), what the backward pass needs, rows per gate). Without
+        `statistics` the rms of the rows is not kept."""
         shape = input.shape
         if len(shape) < 1 or shape[-1] == 0:
             raise ValueError("input should have at least one feature.")
@@ -75,7 +76,7 @@ class GatedResidualRMSNorm(torch.autograd.Function):
         gate = None if gate is None else gate.contiguous()
         y_size = input.numel() // x_size
         output, output_residual = torch.empty_like(input), torch.empty_like(input)
-        rms = torch.empty(2, y_size, device=input.device, dtype=torch.float32)
+        rms = torch.empty(2, y_size, device=input.device, dtype=torch.float32) if statistics else None
 
         util.push_trace("tb200_gated_residual_rms_norm_fwd")
         _lib.gated_residual_rms_norm_fwd(

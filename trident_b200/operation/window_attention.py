@@ -42,8 +42,9 @@ class WindowAttention(torch.autograd.Function):
         return output
 
     @staticmethod
-    def run(query, key, value, window_size, num_sinks, softmax_scale):
-        """The forward pass: (output, log-sum-exp of every score row, window and sinks cut to the length)."""
+    def run(query, key, value, window_size, num_sinks, softmax_scale, statistics=True):
+        """The forward pass: (output, log-sum-exp of every score row or, without `statistics`, None, window and
+        sinks cut to the length)."""
         if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
             raise ValueError("The dimension of query, key and value should be 4.")
         if key.shape != value.shape:
@@ -63,7 +64,9 @@ class WindowAttention(torch.autograd.Function):
 
         util.push_trace("WindowAttention.__forward")
         output = torch.empty_like(query)  # laid out as query is
-        log_sum_exp = torch.empty((batch, heads, y_size), device=query.device, dtype=torch.float32)
+        log_sum_exp = None
+        if statistics:
+            log_sum_exp = torch.empty((batch, heads, y_size), device=query.device, dtype=torch.float32)
         util.push_trace("tb200_window_attention_fwd")
         _lib.window_attention_fwd(output, log_sum_exp, query, key, value, window_size, num_sinks, softmax_scale)
         util.pop_trace()
