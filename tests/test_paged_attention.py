@@ -403,6 +403,18 @@ def test_up_to_64_rows(D, window, sinks, G, t, dtype, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_no_announced_lengths(D, dtype, device):
+    """Hundreds of ragged chunks in one call whose longest is not given: almost all planned pieces of work are empty,
+    and the roles of a kernel wait for one another while they pass over them."""
+    n, KV = 400, 2
+    new = _random(0, 60, n, 80)
+    context = [t + c for t, c in zip(new, _random(0, 90, n, 81))]
+    for _ in range(3):
+        _compare(context, new, KV, 4, D, 16, dtype, device, None, 0, seed=82)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [0.0, -0.3, 0.7])
 @pytest.mark.parametrize("D", [32, 64, 128])
 def test_scales(D, scale, dtype, device):

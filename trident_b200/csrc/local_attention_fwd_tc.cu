@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   uint64_t* walk_empty = bars + 29;  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
   volatile uint32_t* abort_flag = tmem_slot + 1;  // [0] abort flag, [1] wait limit (ptx::mbar_wait)
-  Walk* walks = reinterpret_cast<Walk*>(bars + 32);  // [2]
+  Walk* walks = reinterpret_cast<Walk*>(bars + 33);  // [2], behind the two words of abort_flag
 
   const LocalArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -924,7 +924,8 @@ namespace {
 template <typename T, int D, bool PAGED>
 int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo, const FwdParams& p,
                cudaStream_t st) {
-  constexpr int SMEM = 7 * TILE * D * 2 + 1024 + 384;
+  constexpr int SMEM = 7 * TILE * D * 2 + 1024 + 384;  // (tiles, alignment, barriers and what follows them)
+  static_assert(33 * 8 + 2 * sizeof(Walk) <= 384, "barriers, flags and walks");
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
   auto kern = local_fwd_tc_kernel<T, D, PAGED>;
   static std::atomic<unsigned long long> optin_done{0};
