@@ -22,7 +22,7 @@ C = 64.0
 
 
 def visible(q_pos, n_keys, window, sinks):
-    j = torch.arange(n_keys)
+    j = torch.arange(n_keys, device=q_pos.device)
     i = q_pos[:, None]
     seen = j <= i
     if window:
@@ -93,7 +93,7 @@ def batched(q, k, v, window, sinks, scale, dtype, dout=None):
 
 
 def check(got, want, what):
-    value, bound = want
+    value, bound = (t.cpu() for t in want)
     got = got.detach().double().cpu()
     assert got.shape == value.shape, (what, got.shape, value.shape)
     assert torch.isfinite(got).all(), f"{what}: not finite"

@@ -415,6 +415,17 @@ def test_no_announced_lengths(D, dtype, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("G, KV", [(16, 3), (4, 2), (64, 1)])
+@pytest.mark.parametrize("window, sinks", [(None, 0), (4, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_new_tokens_than_keys(D, window, sinks, G, KV, dtype, device):
+    """Long chunks over short contexts: most rows lie at positions below zero, whole tiles of them next to tiles
+    with keys."""
+    n = 100
+    _compare(_random(0, 30, n, 90), _random(0, 130, n, 91), KV, G, D, 16, dtype, device, window, sinks, seed=92)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [0.0, -0.3, 0.7])
 @pytest.mark.parametrize("D", [32, 64, 128])
 def test_scales(D, scale, dtype, device):

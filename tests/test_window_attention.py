@@ -352,3 +352,21 @@ def test_more_than_32_bit_offsets(D, device):
     for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
         value, bound = (t[:, :, -tail:] for t in want[name])
         ref.check(got.detach()[:, :, -tail:], (value, bound), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, KV, G, S, window, sinks", [(12, 2, 64, 988, 116, 55), (40, 3, 33, 200, 1, 0), (30, 1, 64, 600, 20, 4)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_short_walks(B, KV, G, S, window, sinks, D, device):
+    """Tiles of two or three tokens, dozens of them one after the other on every SM (the formula on the device, in
+    64 bits too)."""
+    dt = torch.bfloat16
+    q, k, v, _ = (t.to(device) for t in _problem(B, KV, G, S, D, dt, seed=190))
+    out = F(q, k, v, window, sinks)
+    assert _lib.device_status() == 0
+    at = torch.arange(S, device=device)
+    for b in range(B):
+        for h in range(KV):
+            heads = slice(h * G, (h + 1) * G)
+            want = ref.attention(q[b, heads].double(), k[b, h].double(), v[b, h].double(), at, window, sinks, D ** -0.5, dt)["out"]
+            ref.check(out[b, heads], want, f"sequence {b}, key head {h}")

@@ -114,6 +114,24 @@ __device__ inline float exp_row(const uint32_t (&v)[4][32], uint64_t scale2, uin
   return s0 + s1;
 }
 
+// Until `count` output tiles have been read from shared memory (a bounded wait, as ptx::mbar_wait).
+__device__ inline void wait_copied(const uint32_t* copied, int count, volatile uint32_t* abort_flag, int* status) {
+  const long long start = clock64();
+  for (uint32_t polls = 1;; ++polls) {
+    uint32_t now;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(now) : "r"(ptx::smem_u32(copied)) : "memory");
+    if ((int)now >= count) return;
+    if ((polls & 1023u) == 0) {
+      if (abort_flag[0]) return;
+      if (clock64() - start > (static_cast<long long>(abort_flag[1]) << 16)) {
+        abort_flag[0] = 1;
+        if (status) atomicCAS(status, 0, 86);
+        return;
+      }
+    }
+  }
+}
+
 // A unit of work, as all roles of the CTA see it.
 struct Unit {
   int s, hk, split, t0;   // t0: first token (within the sequence) of query tile 0
@@ -211,8 +229,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   //   walk_full   warp 3, after a unit's walk is in shared memory    MMA issuer
   //   walk_empty  MMA issuer, after it has read the walk             warp 3
   //   out_full    128 softmax threads of a tile, per output tile     warp 2: bulk copy
-  //   out_free    warp 2, after the copy has read shared memory      softmax: next output tile into shared memory
-  //               (the output tiles of all units in order, tile 0 of a unit before tile 1)
+  //   copied      (a counter) warp 2, output tiles whose copy has    softmax: next output tile into shared memory
+  //               read shared memory; the tiles of all units in order, tile 0 of a unit before tile 1. (Not a
+  //               barrier: a query tile waits for every other number only, and one without keys to walk gets
+  //               to its next output while its last is being copied, two phases before the one it waits for.)
   // Every barrier's next completion needs all waiters of the last one to have seen that: a waiter can
   // never be two phases behind.
   uint64_t* q_full = bars;           // [2]
@@ -230,7 +250,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   uint64_t* p_part = bars + 21;      // [2]
   uint64_t* s_free = bars + 23;      // [2]
   uint64_t* out_full = bars + 25;
-  uint64_t* out_free = bars + 26;
+  uint32_t* copied = reinterpret_cast<uint32_t*>(bars + 26);
   uint64_t* walk_full = bars + 27;   // [2]
   uint64_t* walk_empty = bars + 29;  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
@@ -253,7 +273,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 19; ++i) ptx::mbar_init(&bars[i], 1);
     for (int i = 19; i < 26; ++i) ptx::mbar_init(&bars[i], 128);
-    for (int i = 26; i < 31; ++i) ptx::mbar_init(&bars[i], 1);
+    for (int i = 27; i < 31; ++i) ptx::mbar_init(&bars[i], 1);
+    *copied = 0;
     abort_flag[0] = 0;
     abort_flag[1] = p.wait_units;
     ptx::fence_barrier_init();
@@ -513,8 +534,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                                 PAGED ? 0 : w.s);
             ptx::bulk_commit();
             ptx::bulk_wait_read();
-            ptx::mbar_arrive(out_free);
             ++outs;
+            asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(ptx::smem_u32(copied)), "r"(outs) : "memory");
           }
         }
         ptx::bulk_wait_done();
@@ -780,7 +801,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       }
       const int mine = outs + (t && bulk0 ? 1 : 0);  // number of this output tile
       outs += (bulk0 ? 1 : 0) + (bulk1 ? 1 : 0);
-      if (bulk && mine > 0) ptx::mbar_wait(out_free, (mine - 1) & 1, abort_flag, a.status, 86);
+      if (bulk) wait_copied(copied, mine, abort_flag, a.status);
       if (warp_live) {
         const uint64_t inv2 = am::pack2f(inv, inv);
         const bool zeros = !__all_sync(0xffffffffu, some || !live);  // (the columns hold what was there before)
