@@ -96,6 +96,28 @@ __device__ inline void accumulate(float (&acc)[4][Shape<D, RM, RS, TX>::DC][Shap
   }
 }
 
+// The same with a sum of its own for the step, added at its end: one running sum over the rows of 64 heads and 600
+// tokens was off by 4e-6 of the result, 10 times a matrix product's error.
+template <int D, int RM, int RS, int TX>
+__device__ inline void accumulate_step(float (&acc)[4][Shape<D, RM, RS, TX>::DC][Shape<D, RM, RS, TX>::W], const float* p,
+                                       const float* b, int ty, int tx) {
+  using Sh = Shape<D, RM, RS, TX>;
+  float sum[4][Sh::DC][Sh::W];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < Sh::DC; ++c)
+#pragma unroll
+      for (int w = 0; w < Sh::W; ++w) sum[i][c][w] = 0.f;
+  accumulate<D, RM, RS, TX>(sum, p, b, ty, tx);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < Sh::DC; ++c)
+#pragma unroll
+      for (int w = 0; w < Sh::W; ++w) acc[i][c][w] += sum[i][c][w];
+}
+
 // Rows [0, rows) of a tile into shared memory as fp32; row_ptr(r) is null for rows that do not exist.
 template <typename T, int D, int THREADS, typename RowPtr>
 __device__ inline void load_rows(float* dst, int rows, int64_t feature_stride, bool vec, RowPtr row_ptr) {
@@ -486,8 +508,8 @@ __global__ void __launch_bounds__(256)
         sg[(ty * 4 + i) * PLD + r] = p * (dp[i][j] - srow[BRS + r]);
       }
     __syncthreads();
-    accumulate<D, BRM, BRS, BTX>(av, sp, sd, ty, tx);
-    accumulate<D, BRM, BRS, BTX>(ak, sg, sq, ty, tx);
+    accumulate_step<D, BRM, BRS, BTX>(av, sp, sd, ty, tx);
+    accumulate_step<D, BRM, BRS, BTX>(ak, sg, sq, ty, tx);
   }
   const bool parted = kt < b.sink_tiles;
 #pragma unroll
