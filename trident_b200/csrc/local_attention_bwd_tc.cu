@@ -838,6 +838,7 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
   const LocalArgs& a = b.f;
   const int col_tokens = COLS / a.G;
   CUtensorMap mq, md, mq128, md128, mo128, mk, mv, mdq;
+  bind_primary_context();
   if (!local_map_rows(&mq, q, a.qs, a, col_tokens, "q") || !local_map_rows(&md, dout, b.dos, a, col_tokens, "dout") ||
       !local_map_rows(&mq128, q, a.qs, a, TILE / a.G, "q") || !local_map_rows(&md128, dout, b.dos, a, TILE / a.G, "dout") ||
       !local_map_rows(&mo128, out, a.os, a, TILE / a.G, "out") ||

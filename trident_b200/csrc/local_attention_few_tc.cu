@@ -405,6 +405,7 @@ int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, 
   p.scale_log2 = a.scale * LOG2E;
   p.piece = local_piece(a);
   CUtensorMap mq, mk, mv;
+  bind_primary_context();
   if (!local_map_rows(&mq, q, a.qs, a, N / a.G, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
       !local_map_keys(&mv, v, a.vs, a, p.piece, "v"))
     return TB200_ERR_UNSUPPORTED;

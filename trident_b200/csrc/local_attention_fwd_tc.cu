@@ -883,7 +883,6 @@ EncodeFn encode_fn() {
 
 bool encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
             const cuuint32_t* box, const char* what) {
-  bind_primary_context();
   cuuint32_t elem[5] = {1, 1, 1, 1, 1};
   const CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides,
                                  box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -995,6 +994,7 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   p.splits = Divisor(a.splits);
   p.wait_units = ptx::WAIT_LIMIT_UNITS;
   CUtensorMap mq, mk, mv, mo;
+  bind_primary_context();
   if (!local_map_rows(&mq, q, a.qs, a, p.tile_tokens, "q") || !local_map_rows(&mo, out, a.os, a, p.tile_tokens, "out") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||
       !local_map_keys(&mv, v, a.vs, a, p.piece, "v"))
     return TB200_ERR_UNSUPPORTED;

@@ -39,7 +39,8 @@ static inline bool local_few_rows(const LocalArgs& a, int max_q) {
 int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, const LocalArgs& a, int dtype,
                         cudaStream_t st);
 
-// Tensor maps (false with the error text set when the driver refuses one) and what they take.
+// Tensor maps (false with the error text set when the driver refuses one; the caller has bound the primary
+// context) and what they take.
 // (rows: boxes of `tokens` tokens with the heads of a group)
 bool local_map_rows(CUtensorMap* map, const void* q, const int64_t* st, const LocalArgs& a, int tokens, const char* what);
 bool local_map_keys(CUtensorMap* map, const void* k, const int64_t* st, const LocalArgs& a, int piece, const char* what);
