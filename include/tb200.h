@@ -288,7 +288,8 @@ int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, c
  * A token without a visible key (position below 0) gets zeros. Rows that belong to no sequence (behind
  * starts[n]) are left alone, or set to zero with zero_tail != 0. table, context and starts are read on
  * the device; values out of range are cut to the buffers (a page outside the pool reads as zeros), and
- * table entries of blocks that no query sees are not read. max_query_length: no sequence has more new
+ * table entries of blocks that no query sees are not read. A context beyond the table keeps its positions: the keys
+ * behind the table do not exist, no token is moved onto an earlier place. max_query_length: no sequence has more new
  * tokens. max_context_length: the longest context expected (longer ones are still right). The workspace
  * holds the parts of walks that are cut along the keys. */
 size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t H, int64_t KV, int64_t D,

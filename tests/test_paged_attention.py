@@ -568,3 +568,64 @@ def test_library_refuses_before_launch():
     assert append_call(8, 8, 8, 8, 8, 8, None, 3, 2, 2, 64, 16, 4, 3, 3, s, s, s, s, 0, None) == -1
     assert append_call(None, 8, 8, 8, 8, 8, 8, 2, 2, 2, 64, 16, 4, 3, 3, s, s, s, s, 0, None) == -1
     assert append_call(8, 8, 8, 8, 8, 8, 8, 2, 2, 2, 64, 16, 4, 3, 3, s, s, None, s, 0, None) == -1
+
+
+# ------------------------------------------------------------------------------------ contexts beyond the table
+def _full(room, beyond, KV, D, page, dtype, device, seed):
+    """A sequence whose table is full, its context `beyond` tokens longer, next to one with room left."""
+    cache = Cache([room, 50], KV, D, page, dtype, device, seed)
+    cache.table = cache.table[:, : room // page].contiguous()
+    cache.table_dev = cache.table.to(device)
+    cache.context = [room + beyond, 50]
+    cache.context_dev = torch.tensor(cache.context, dtype=torch.int32, device=device)
+    return cache
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beyond", [0, 1, 30, 500, 2 ** 31 - 97])
+@pytest.mark.parametrize("window, sinks", [(None, 0), (40, 3), (5, 0), (200, 130)])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_contexts_beyond_the_table(D, window, sinks, beyond, dtype, device):
+    """Tokens keep their positions: they see the keys that the table holds, as far as window and sinks reach."""
+    cache = _full(96, beyond, 2, D, 16, dtype, device, 110)
+    for new in ([1, 1], [3, 1], [70, 50], [150, 10]):
+        q = util.randn(sum(new), 4, D, seed=111).to(dtype)
+        got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, _offsets(new, device),
+                     max_query_length=max(new), window_size=window, num_sinks=sinks)
+        ref.check(got, _want(q, cache, new, window or 0, sinks, D ** -0.5, dtype), f"{new}")
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_contexts_beyond_the_table(D, dtype, device):
+    """The same where the walk along the keys is cut."""
+    cache = _full(4000, 150, 1, D, 16, dtype, device, 112)
+    for new in ([1, 1], [200, 5]):
+        for window, sinks in ((None, 0), (3000, 5), (160, 1500)):
+            q = util.randn(sum(new), 4, D, seed=113).to(dtype)
+            got = attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, _offsets(new, device),
+                         max_query_length=max(new), window_size=window, num_sinks=sinks)
+            ref.check(got, _want(q, cache, new, window or 0, sinks, D ** -0.5, dtype), f"{new} {window}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beyond", [1, 2, 6, 500, 2 ** 31 - 65])
+@pytest.mark.parametrize("D", [16, 64])
+def test_append_beyond_the_table(D, beyond, dtype, device):
+    """Tokens behind the table's last place are left out, and nothing else in the pool changes."""
+    cache = _full(64, beyond, 2, D, 16, dtype, device, 114)
+    new = [4, 3]
+    k, v = (util.randn(7, 2, D, seed=115 + i).to(dtype).to(device) for i in range(2))
+    kc, vc = cache.key_cache.clone(), cache.value_cache.clone()
+    append(k, v, kc, vc, cache.table_dev, cache.context_dev, _offsets(new, device))
+    for got, before, rows in ((kc, cache.key_cache, k), (vc, cache.value_cache, v)):
+        want = before.clone()
+        at = 0
+        for s, t in enumerate(new):
+            for i in range(t):
+                pos = cache.context[s] - t + i
+                if pos < 64:
+                    want[cache.table[s, pos // 16].long(), pos % 16] = rows[at + i]
+            at += t
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))

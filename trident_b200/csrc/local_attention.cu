@@ -16,12 +16,11 @@ __global__ void __launch_bounds__(256)
   const int s = blockIdx.z;
   const Sequence sq = load_sequence(a, s);
   const int per_row = a.D / N, per_token = a.KV * per_row;
-  const int base = sq.kv_len - sq.q_len;
   const int64_t total = (int64_t)sq.q_len * per_token;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int t = (int)(i / per_token), rest = (int)(i % per_token), h = rest / per_row, d = rest % per_row * N;
-    const int pos = base + t;
-    if (pos < 0) continue;
+    const int pos = sq.base + t;
+    if (pos < 0 || pos >= sq.kv_len) continue;  // (a context may go beyond the table)
     const int page = a.table[s * a.table_stride + pos / a.page];
     if (page < 0 || page >= a.pages) continue;
     const int64_t off = pos % a.page, tok = sq.q_begin + t;

@@ -44,15 +44,17 @@ struct LocalArgs {
   int* status = nullptr;
 };
 
-// New tokens [q_begin, q_begin + q_len) of a sequence and its number of keys. Values out of range are
-// cut to what the buffers hold.
+// New tokens [q_begin, q_begin + q_len) of a sequence, the position of the first of them and the number of keys that
+// the table has room for. Offsets out of range are cut to the rows that there are; a context beyond the table
+// moves no token: its positions are counted from the context's own end, and the keys behind the table do not exist.
 struct Sequence {
-  int q_begin, q_len, kv_len;
+  int q_begin, q_len, base, kv_len;
 };
+constexpr int MOST_KEYS = 0x7ffff000;  // (positions and a tile's columns behind them stay within 32 bits)
 __device__ inline Sequence load_sequence(const LocalArgs& a, int s) {
   Sequence r;
   if (a.table == nullptr) {
-    r.q_begin = 0;
+    r.q_begin = r.base = 0;
     r.q_len = r.kv_len = a.tokens;
     return r;
   }
@@ -66,9 +68,10 @@ __device__ inline Sequence load_sequence(const LocalArgs& a, int s) {
     r.q_len = s < a.tokens ? 1 : 0;
   }
   const int64_t room = (int64_t)a.table_cols * a.page;
-  int kv = a.context[s];
-  if (kv > room) kv = (int)room;
-  r.kv_len = kv < 0 ? 0 : kv;
+  int context = a.context[s];
+  context = context < 0 ? 0 : (context > MOST_KEYS ? MOST_KEYS : context);
+  r.base = context - r.q_len;
+  r.kv_len = context > room ? (int)room : context;
   return r;
 }
 
@@ -88,6 +91,7 @@ __device__ inline KeyRange key_range(const LocalArgs& a, int pmin, int pmax, int
   if (a.window != NO_WINDOW && a.sinks > 0) {
     const int st = (a.sinks + tile - 1) / tile;
     r.sink_tiles = st < r.lo ? st : r.lo;
+    if (r.sink_tiles > hi) r.sink_tiles = hi;  // (a window that lies behind the table's end)
   }
   r.count = r.sink_tiles + (hi > r.lo ? hi - r.lo : 0);
   return r;

@@ -105,9 +105,9 @@ __global__ void __launch_bounds__(THREADS, 2)
   const Sequence seq = load_sequence(a, s);
   if (a.zero_tail && s == a.n - 1 && hk == 0) zero_tail_rows(reinterpret_cast<T*>(p.out), a, seq);
   if (seq.q_len == 0) return;
-  const int base = seq.kv_len - seq.q_len;
+  const int base = seq.base;
   const int rows = min(seq.q_len, N / a.G) * a.G;
-  const KeyRange kr = key_range(a, base, seq.kv_len - 1, seq.kv_len, TILE);
+  const KeyRange kr = key_range(a, base, base + seq.q_len - 1, seq.kv_len, TILE);
   int m0, m1;
   split_range(a, kr.count, split, &m0, &m1);
   if (split > 0 && m0 >= m1) return;

@@ -170,7 +170,7 @@ __device__ inline bool unit_at(const FwdParams& p, int unit, Unit* w) {
   w->seq = load_sequence(a, w->s);
   w->t0 = pair * 2 * p.tile_tokens;
   if (w->t0 >= w->seq.q_len) return false;
-  w->base = w->seq.kv_len - w->seq.q_len;
+  w->base = w->seq.base;
   const int last_token = min(w->t0 + 2 * p.tile_tokens, w->seq.q_len) - 1;
   w->kr = key_range(a, w->base + w->t0, w->base + last_token, w->seq.kv_len, TILE);
   split_range(a, w->kr.count, w->split, &w->m0, &w->m1);
@@ -613,6 +613,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       // positions of the warp's rows
       const int wmin = w.base + first_token + warp_first;
       const int wmax = w.base + first_token + min(warp_last, tokens - 1);
+      // (positions may lie behind the last key: see load_sequence)
+      const int end = PAGED ? w.seq.kv_len - 1 : MOST_KEYS, pos_end = min(pos, end), wmin_end = min(wmin, end), wmax_end = min(wmax, end);
       float m_used = -INFINITY, l = 0.f;
       const int before = count;
       for (int m = w.m0; m < w.m1; ++m) {
@@ -637,8 +639,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int b0 = j0 + 32 * q;
-          if (b0 > wmax || (wmin - (b0 + 31) >= a.window && b0 >= a.sinks)) none |= 1u << q;
-          if (b0 + 31 <= wmin && (wmax - b0 < a.window || b0 + 32 <= a.sinks)) all |= 1u << q;
+          if (b0 > wmax_end || (wmin - (b0 + 31) >= a.window && b0 >= a.sinks)) none |= 1u << q;
+          if (b0 + 31 <= wmin_end && (wmax - b0 < a.window || b0 + 32 <= a.sinks)) all |= 1u << q;
         }
         const bool plain = all == 15u && p.scale_log2 >= 0.f;
         uint32_t sr[4][32];
@@ -674,7 +676,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
               }
               return;
             }
-            const uint32_t seen = low_bits(pos + 1 - b0) & (~low_bits(low < 0 ? 0 : (int)low) | low_bits(a.sinks - b0));
+            const uint32_t seen = low_bits(pos_end + 1 - b0) & (~low_bits(low < 0 ? 0 : (int)low) | low_bits(a.sinks - b0));
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float s0, s1;

@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(Shape<D, RM, KEY_TILE, TX>::THREADS)
   const int tile_tokens = RM / a.G, t0 = blockIdx.x * tile_tokens;
   const int ntok = min(tile_tokens, sq_.q_len - t0);
   if (ntok <= 0) return;
-  const int base = sq_.kv_len - sq_.q_len;  // position of the sequence's first new token
+  const int base = sq_.base;
   const KeyRange kr = key_range(a, base + t0, base + t0 + ntok - 1, sq_.kv_len, KEY_TILE);
   int m0, m1;
   split_range(a, kr.count, split, &m0, &m1);
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(256)
   const int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int t = item / a.H, head = item % a.H;
   if (t >= sq.q_len) return;
-  const int base = sq.kv_len - sq.q_len, t0 = t / row_tokens * row_tokens;
+  const int base = sq.base, t0 = t / row_tokens * row_tokens;
   const int t1 = min(t0 + row_tokens, sq.q_len) - 1;
   const KeyRange kr = key_range(a, base + t0, base + t1, sq.kv_len, key_tile);
   if (kr.count <= a.split_tiles) return;  // written whole

@@ -161,7 +161,8 @@ def paged_attention(
     [tokens, heads, head size]; without query_offsets there is one per sequence. A token sees the positions
     up to its own; with window_size, those less than window_size back and the first num_sinks, and table
     entries of blocks that no token sees may be anything. block_table, context_lengths and query_offsets
-    are int32 tensors on the device and are not read by the host.
+    are int32 tensors on the device and are not read by the host. A context longer than the table has room for keeps
+    its positions: the keys behind the table do not exist, and are not written by paged_cache_append.
 
     No sequence may have more than max_query_length new tokens (default: all; rows beyond are not computed);
     max_context_length is the longest context expected (default: what the table holds) and only chooses how
