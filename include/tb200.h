@@ -285,12 +285,13 @@ int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, c
  * included; its new tokens are the rows [starts[s], starts[s+1]) of q [T,H,D] (3 strides; starts
  * null: token s), and the i-th of t new tokens has position context - t + i. It sees the positions
  * up to its own, with a window (> 0) those less than `window` back and the first `sinks`.
- * A token without a visible key (position below 0) gets zeros. Rows that belong to no sequence (behind
- * starts[n]) are left alone, or set to zero with zero_tail != 0. table, context and starts are read on
+ * A token without a visible key (position below 0) gets zeros. Rows that belong to no sequence (before
+ * starts[0], behind starts[n]) and the rows of a sequence beyond max_query_length are left alone, or set to zero with
+ * zero_rest != 0. table, context and starts are read on
  * the device; values out of range are cut to the buffers (a page outside the pool reads as zeros), and
  * table entries of blocks that no query sees are not read. A context beyond the table keeps its positions: the keys
- * behind the table do not exist, no token is moved onto an earlier place. max_query_length: no sequence has more new
- * tokens. max_context_length: the longest context expected (longer ones are still right). The workspace
+ * behind the table do not exist, no token is moved onto an earlier place. max_query_length: of a sequence's new tokens
+ * the first so many are computed. max_context_length: the longest context expected (longer ones are still right). The workspace
  * holds the parts of walks that are cut along the keys. */
 size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t H, int64_t KV, int64_t D,
                                        int64_t max_query_length, int64_t max_context_length, int64_t window,
@@ -301,7 +302,7 @@ int tb200_paged_attention(void* out, const void* q, const void* key_cache, const
                           int64_t D, int64_t page, int64_t pages, int64_t table_cols, int64_t table_stride,
                           const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                           const int64_t* out_strides, int64_t max_query_length, int64_t max_context_length,
-                          int64_t window, int64_t sinks, float softmax_scale, int zero_tail, int dtype, void* stream);
+                          int64_t window, int64_t sinks, float softmax_scale, int zero_rest, int dtype, void* stream);
 /* Writes the keys and values of the new tokens, k and v [T,KV,D] (3 strides), to their places in the
  * pages (same table, context and starts). Tokens at positions below 0, beyond the table or on pages
  * outside the pool are left out. */

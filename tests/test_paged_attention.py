@@ -629,3 +629,57 @@ def test_append_beyond_the_table(D, beyond, dtype, device):
                     want[cache.table[s, pos // 16].long(), pos % 16] = rows[at + i]
             at += t
         assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+# ------------------------------------------------------------------------------------ rows that are not computed
+def _poisoned(call, shape, dtype, device):
+    """`call`, with NaN in the memory that its output is most likely made from."""
+    block = torch.full(shape, float("nan"), dtype=dtype, device=device)
+    torch.cuda.synchronize()
+    del block
+    return call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new, at, tokens", [([4, 6], 9, 40), ([1, 1], 5, 8), ([1, 1], 300, 302), ([150, 70], 1, 600), ([0, 3], 200, 203)])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_rows_before_the_first_sequence(D, new, at, tokens, dtype, device):
+    cache = Cache([160, 75], 2, D, 16, dtype, device, seed=120)
+    q = util.randn(tokens, 4, D, seed=121).to(dtype).to(device)
+    offsets = _offsets(new, device) + at
+    last = at + sum(new)
+    want = _want(q[at:last].cpu(), cache, new, 20, 2, D ** -0.5, dtype)
+
+    def call(**more):
+        return attend(q, cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, offsets,
+                      max_query_length=max(new), window_size=20, num_sinks=2, **more)
+
+    got = _poisoned(call, q.shape, dtype, device)
+    ref.check(got[at:last], want, "rows of the sequences")
+    assert torch.all(got[:at] == 0) and torch.all(got[last:] == 0)
+    mine = torch.full_like(q, 5.0)
+    call(output=mine)
+    assert torch.equal(mine[at:last], got[at:last]) and torch.all(mine[:at] == 5.0) and torch.all(mine[last:] == 5.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("longest", [1, 5, 40, 100])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_rows_beyond_max_query_length(D, longest, dtype, device):
+    """A sequence's first max_query_length tokens are computed, at their positions among all of its tokens."""
+    new = [3, 60, 1, 200, 0, 41] * 8
+    cache = Cache([t + 30 for t in new], 1, D, 16, dtype, device, seed=122)
+    q = util.randn(sum(new) + 3, 4, D, seed=123).to(dtype)
+    kept = torch.cat([torch.arange(t) < longest for t in new] + [torch.zeros(3, dtype=torch.bool)])
+    value, bound = _want(q[:-3], cache, new, 50, 1, D ** -0.5, dtype)
+
+    def call(**more):
+        return attend(q.to(device), cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, _offsets(new, device),
+                      max_query_length=longest, window_size=50, num_sinks=1, **more)
+
+    got = _poisoned(call, q.shape, dtype, device).cpu()
+    ref.check(got[kept], (value[kept[:-3]], bound[kept[:-3]]), "rows that are computed")
+    assert torch.all(got[~kept] == 0)
+    mine = torch.full_like(q.to(device), 5.0)
+    call(output=mine)
+    assert torch.equal(mine.cpu()[kept], got[kept]) and torch.all(mine.cpu()[~kept] == 5.0)

@@ -564,7 +564,7 @@ def paged_attention_workspace(q, kv_heads, n, max_query_length, max_context_leng
 
 
 def paged_attention(out, q, key_cache, value_cache, table, context, starts, workspace, max_query_length,
-                    max_context_length, window, sinks, scale, zero_tail):
+                    max_context_length, window, sinks, scale, zero_rest):
     T, H, D = q.shape
     pages, page, kv_heads, _ = key_cache.shape
     n, blocks = table.shape
@@ -573,7 +573,7 @@ def paged_attention(out, q, key_cache, value_cache, table, context, starts, work
         _ptr(context), _ptr(starts), _ptr(workspace), 0 if workspace is None else workspace.numel(), T, n, H,
         kv_heads, D, page, pages, blocks, table.stride(0), q.stride(), key_cache.stride(),
         value_cache.stride(), out.stride(), max_query_length, max_context_length, window, sinks, scale,
-        zero_tail, dtype_code(q.dtype),
+        zero_rest, dtype_code(q.dtype),
     )
 
 

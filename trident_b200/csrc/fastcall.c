@@ -147,10 +147,10 @@ static PyObject* paged_attention(PyObject* self, PyObject* const* args, Py_ssize
   strides(&a, o, 3);
   for (int i = 0; i < 4; ++i) m[i] = integer(&a);
   float scale = real(&a);
-  int zero_tail = (int)integer(&a), dtype = (int)integer(&a);
+  int zero_rest = (int)integer(&a), dtype = (int)integer(&a);
   void* stream = pointer(&a);
   CALL(tb200_paged_attention(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], bytes, d[0], d[1], d[2], d[3], d[4], d[5], d[6], d[7],
-                             d[8], q, k, v, o, m[0], m[1], m[2], m[3], scale, zero_tail, dtype, stream));
+                             d[8], q, k, v, o, m[0], m[1], m[2], m[3], scale, zero_rest, dtype, stream));
 }
 
 static PyObject* paged_cache_append(PyObject* self, PyObject* const* args, Py_ssize_t n) {

@@ -270,7 +270,7 @@ extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_c
                                      int64_t page, int64_t pages, int64_t table_cols, int64_t table_stride,
                                      const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                                      const int64_t* out_strides, int64_t max_query_length, int64_t max_context_length,
-                                     int64_t window, int64_t sinks, float softmax_scale, int zero_tail, int dtype,
+                                     int64_t window, int64_t sinks, float softmax_scale, int zero_rest, int dtype,
                                      void* stream) {
   LocalArgs a;
   if (int rc = fill_paged(&a, "paged_attention", T, n, H, KV, D, table, context, starts, table_cols, table_stride, page,
@@ -289,9 +289,10 @@ extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_c
   }
   set_window(&a, window, sinks);
   a.scale = softmax_scale;
-  a.zero_tail = zero_tail;
+  a.zero_rest = zero_rest;
   cudaStream_t st = (cudaStream_t)stream;
   const int max_q = (int)(max_query_length < T ? max_query_length : T);
+  a.max_q = max_q;
   const PagedPlan plan = plan_paged(&a, max_q, max_context_length, local_tc_supported(a, dtype, q, key_cache, value_cache, out));
   TB200_REQUIRE(workspace_bytes >= split_bytes(a) && (workspace || a.split_tiles == 0), TB200_ERR_WORKSPACE,
                 "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, split_bytes(a));

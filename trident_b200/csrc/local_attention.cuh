@@ -33,6 +33,7 @@ struct LocalArgs {
   const int* table = nullptr;    // [n, table_cols]: page of each block of a sequence
   const int* context = nullptr;  // [n]: keys of a sequence, new tokens included
   const int* starts = nullptr;   // [n + 1] first new token of each sequence; null: one token each
+  int max_q = 0x7fffffff;        // new tokens of a sequence beyond these are not computed
   int table_cols = 0;
   int64_t table_stride = 0;
   int page = 0, pages = 0;       // keys per page, pages in the pool
@@ -40,37 +41,39 @@ struct LocalArgs {
   int split_tiles = 0, splits = 1;
   float* part_out = nullptr;     // [splits][tokens * H][D]
   float* part_lse = nullptr;     // [splits][tokens * H]
-  int zero_tail = 0;             // rows of no sequence (behind the last one) are set to zero
+  int zero_rest = 0;             // rows that are not computed (of no sequence, beyond max_q) are set to zero
   int* status = nullptr;
 };
 
-// New tokens [q_begin, q_begin + q_len) of a sequence, the position of the first of them and the number of keys that
-// the table has room for. Offsets out of range are cut to the rows that there are; a context beyond the table
+// New tokens [q_begin, q_begin + q_len) of a sequence that are computed, the end of all that it has, the position of
+// the first of them and the number of keys that the table has room for. Offsets out of range are cut to the rows that there are; a context beyond the table
 // moves no token: its positions are counted from the context's own end, and the keys behind the table do not exist.
 struct Sequence {
-  int q_begin, q_len, base, kv_len;
+  int q_begin, q_len, q_end, base, kv_len;
 };
 constexpr int MOST_KEYS = 0x7ffff000;  // (positions and a tile's columns behind them stay within 32 bits)
 __device__ inline Sequence load_sequence(const LocalArgs& a, int s) {
   Sequence r;
   if (a.table == nullptr) {
     r.q_begin = r.base = 0;
-    r.q_len = r.kv_len = a.tokens;
+    r.q_len = r.q_end = r.kv_len = a.tokens;
     return r;
   }
   if (a.starts) {
     const int b = a.starts[s], e = a.starts[s + 1];
     r.q_begin = b < 0 ? 0 : (b > a.tokens ? a.tokens : b);
     const int end = e > a.tokens ? a.tokens : e;
-    r.q_len = end > r.q_begin ? end - r.q_begin : 0;
+    r.q_end = end > r.q_begin ? end : r.q_begin;
   } else {
     r.q_begin = s;
-    r.q_len = s < a.tokens ? 1 : 0;
+    r.q_end = s < a.tokens ? s + 1 : s;
   }
+  const int count = r.q_end - r.q_begin;
+  r.q_len = count < a.max_q ? count : a.max_q;
   const int64_t room = (int64_t)a.table_cols * a.page;
   int context = a.context[s];
   context = context < 0 ? 0 : (context > MOST_KEYS ? MOST_KEYS : context);
-  r.base = context - r.q_len;
+  r.base = context - count;
   r.kv_len = context > room ? (int)room : context;
   return r;
 }
@@ -103,12 +106,19 @@ __device__ inline bool visible(const LocalArgs& a, int p, int j) {
 // excepted, are seen by no row of the tile: their pages may have been given away).
 __device__ inline int first_key(const LocalArgs& a, int pmin) { return a.window > pmin ? 0 : pmin - a.window + 1; }
 
-// Sets the rows behind the last sequence to zero; called by all CTAs of (last sequence, first head, first part).
+// Sets rows [begin, end) of the output to zero: every `parts`-th of them from `part` on, by `threads` threads.
 template <typename T>
-__device__ inline void zero_tail_rows(T* out, const LocalArgs& a, const Sequence& last) {
-  for (int64_t t = (int64_t)last.q_begin + last.q_len + blockIdx.x; t < a.tokens; t += gridDim.x)
-    for (int i = threadIdx.x; i < a.H * a.D; i += blockDim.x)
+__device__ inline void zero_rows(T* out, const LocalArgs& a, int64_t begin, int64_t end, int part, int parts, int thread, int threads) {
+  for (int64_t t = begin + part; t < end; t += parts)
+    for (int i = thread; i < a.H * a.D; i += threads)
       out[t * a.os[2] + (int64_t)(i / a.D) * a.os[1] + (int64_t)(i % a.D) * a.os[3]] = Traits<T>::from_f(0.f);
+}
+// Rows that no sequence computes, by the CTAs (part of parts) of sequence s: those of s beyond max_q, and before the
+// first and behind the last sequence.
+template <typename T>
+__device__ inline void zero_rest_of(T* out, const LocalArgs& a, int s, const Sequence& seq, int part, int parts) {
+  if (s == 0) zero_rows(out, a, 0, seq.q_begin, part, parts, threadIdx.x, blockDim.x);
+  zero_rows(out, a, (int64_t)seq.q_begin + seq.q_len, s == a.n - 1 ? a.tokens : seq.q_end, part, parts, threadIdx.x, blockDim.x);
 }
 
 // Key tiles of the walk that split `s` of a row tile takes.

@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x, hk = blockIdx.y, s = blockIdx.z;
   const Sequence seq = load_sequence(a, s);
-  if (a.zero_tail && s == a.n - 1 && hk == 0) zero_tail_rows(reinterpret_cast<T*>(p.out), a, seq);
+  if (a.zero_rest && hk == 0) zero_rest_of(reinterpret_cast<T*>(p.out), a, s, seq, split, gridDim.x);
   if (seq.q_len == 0) return;
   const int base = seq.base;
   const int rows = min(seq.q_len, N / a.G) * a.G;

@@ -259,7 +259,6 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 
   const LocalArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (PAGED && a.zero_tail) zero_tail_rows(reinterpret_cast<T*>(p.out), a, load_sequence(a, a.n - 1));
   // query tile t's output leaves through shared memory: a full tile of a walk that is not cut
   auto is_bulk = [&](const Unit& w, int t) {
     const int tokens = w.seq.q_len - (w.t0 + t * p.tile_tokens);
@@ -588,6 +587,26 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   } else {
     // ---------------------------------------------------------------- softmax + epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    if (PAGED && a.zero_rest) {  // (these warps have nothing else to do until the first scores are there)
+      T* out = reinterpret_cast<T*>(p.out);
+      const int thread = threadIdx.x - 128;
+      zero_rows(out, a, 0, load_sequence(a, 0).q_begin, blockIdx.x, gridDim.x, thread, 256);
+      zero_rows(out, a, load_sequence(a, a.n - 1).q_end, a.tokens, blockIdx.x, gridDim.x, thread, 256);
+      if (a.max_q < a.tokens)  // a warp looks 32 sequences up, and takes the rows beyond max_q of each in turn
+        for (int s0 = thread & ~31; s0 < a.n; s0 += 256) {
+          int begin = 0, end = 0;
+          if (s0 + lane < a.n) {
+            const Sequence seq = load_sequence(a, s0 + lane);
+            begin = seq.q_begin + seq.q_len;
+            end = seq.q_end;
+          }
+          for (uint32_t some = __ballot_sync(0xffffffffu, begin < end); some; some &= some - 1) {
+            const int l = __ffs(some) - 1;
+            const int from = __shfl_sync(0xffffffffu, begin, l), to = __shfl_sync(0xffffffffu, end, l);
+            zero_rows(out, a, from, to, blockIdx.x, gridDim.x, lane, 32);
+          }
+        }
+    }
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;

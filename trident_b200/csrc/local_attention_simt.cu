@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(Shape<D, RM, KEY_TILE, TX>::THREADS)
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const int s = blockIdx.z / a.splits, split = blockIdx.z % a.splits, hk = blockIdx.y;
   const Sequence sq_ = load_sequence(a, s);
-  if (a.zero_tail && s == a.n - 1 && hk == 0 && split == 0) zero_tail_rows(out, a, sq_);
+  if (a.zero_rest && hk == 0 && split == 0) zero_rest_of(out, a, s, sq_, blockIdx.x, gridDim.x);
   // the packed rows of this tile: row r is token r / G of the tile, head r % G of the group
   const int tile_tokens = RM / a.G, t0 = blockIdx.x * tile_tokens;
   const int ntok = min(tile_tokens, sq_.q_len - t0);

@@ -164,10 +164,11 @@ def paged_attention(
     are int32 tensors on the device and are not read by the host. A context longer than the table has room for keeps
     its positions: the keys behind the table do not exist, and are not written by paged_cache_append.
 
-    No sequence may have more than max_query_length new tokens (default: all; rows beyond are not computed);
+    Of each sequence the first max_query_length new tokens are computed (default: all of them);
     max_context_length is the longest context expected (default: what the table holds) and only chooses how
     the work is split. Both have to be given for the best speed, and stay what they are in a captured graph.
-    Rows of query that belong to no sequence give zeros, or leave `output`, where it is given, as it was.
+    Rows of query that belong to no sequence or lie beyond max_query_length give zeros, or leave `output`, where it
+    is given, as it was.
     What pages hold beyond a context is not read into any result; keys and values inside it have to be finite.
     """
     scale = 1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None else softmax_scale

@@ -97,7 +97,7 @@ def paged_attention(
     max_query_length = max(1, min(max_query_length, tokens, MOST_TOKENS))
     max_context_length = min(max_context_length, MOST_TOKENS)
     sequences = block_table.shape[0]
-    zero_tail = output is None and query_offsets is not None
+    zero_rest = output is None and query_offsets is not None
     if sequences == 0 or tokens == 0:
         return torch.zeros_like(query) if output is None else output
     _check_room(block_table, key_cache)
@@ -126,7 +126,7 @@ def paged_attention(
         window,
         sinks,
         softmax_scale,
-        zero_tail,
+        zero_rest,
     )
     util.pop_trace()
     util.pop_trace()
