@@ -39,6 +39,17 @@ def _check_cache(key_cache, value_cache, block_table, context_lengths, query_off
     _lib.dtype_code(dtype)
     if grad and torch.is_grad_enabled():
         raise ValueError("Paged attention has no backward pass: call it under torch.no_grad().")
+    if util.is_watched():
+        _check_unwatched(key_cache, value_cache, *tensors.values())
+
+
+def _check_unwatched(*tensors):
+    if torch._C._get_tracing_state() is not None:
+        raise ValueError("Paged attention cannot be traced: a trace records no call of the library.")
+    if torch._C._are_functorch_transforms_active():
+        raise ValueError("Paged attention cannot be called under function transforms (vmap, jvp, ...).")
+    if any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("Paged attention has no forward-mode derivative.")
 
 
 def _check_room(block_table, key_cache):

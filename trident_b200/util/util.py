@@ -8,6 +8,7 @@ __all__ = [
     "calculate_fan_in_and_fan_out",
     "fill",
     "is_pow2",
+    "is_watched",
     "needs_grad",
     "size_and_stride",
     "push_trace",
@@ -33,12 +34,23 @@ def is_pow2(value):
 
 
 def needs_grad(*tensors):
-    """Whether autograd would record an operation on these tensors (None allowed)."""
+    """Whether an operation on these tensors (None allowed) has to go through its autograd Function: autograd
+    would record it, or something else that only sees Functions is looking on."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    return is_watched()
+
+
+def is_watched():
+    """Whether a trace, a function transform or forward-mode differentiation is under way: they would take the
+    output of a kernel that is called directly for an empty tensor, or for one without a tangent."""
+    return (
+        torch._C._get_tracing_state() is not None
+        or torch._C._are_functorch_transforms_active()
+        or torch.autograd.forward_ad._current_level >= 0
+    )
 
 
 def size_and_stride(input: torch.Tensor, dim: int):
