@@ -21,7 +21,8 @@ def calls(monkeypatch):
         def run(*args):
             seen.append(name)
             for t in args[:outputs]:
-                t.fill_(1.0)
+                with torch.inference_mode(t.is_inference()):
+                    t.data.fill_(1.0)  # (as a kernel: autograd sees nothing of it)
 
         monkeypatch.setattr(_lib, name, run)
 
@@ -104,3 +105,30 @@ def test_ordinary_calls_are_direct(calls):
     for call, name in ((_window, "window_attention_fwd"), (_norm, "gated_residual_rms_norm_fwd")):
         assert call(Q).grad_fn is None and calls[-1] == name
         assert call(Q.clone().requires_grad_(True)).grad_fn is not None
+
+
+@pytest.mark.parametrize("which", ["key_cache", "value_cache", "a view", "output"])
+def test_autograd_sees_what_is_written(which, calls):
+    """A graph that saved a tensor which a call writes in place refuses its backward pass."""
+    keys, values, out, x = torch.randn(4, 8, 2, 16), torch.randn(4, 8, 2, 16), torch.randn(3, 2, 16), torch.randn(3, 2, 16)
+    saved = {"key_cache": keys, "value_cache": values, "a view": keys[1], "output": out}[which]
+    leaf = torch.randn_like(saved, requires_grad=True)
+    loss = (saved * leaf).sum()
+    F.paged_attention(x, keys, values, TABLE, LENGTHS)  # reads
+    torch.autograd.grad(loss, leaf, retain_graph=True)
+    if which == "output":
+        F.paged_attention(x, keys, values, TABLE, LENGTHS, output=out)
+    else:
+        F.paged_cache_append(x, x, keys, values, TABLE, LENGTHS)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_inference_tensors_are_written(calls):
+    with torch.inference_mode():
+        keys, x = torch.zeros(4, 8, 2, 16), torch.zeros(3, 2, 16)
+        out = F.paged_attention(x, keys, keys, TABLE, LENGTHS, output=x)
+    with torch.no_grad():
+        F.paged_cache_append(x, x, keys, keys, TABLE, LENGTHS)
+        assert F.paged_attention(x, keys, keys, TABLE, LENGTHS, output=out) is out
+    assert len(calls) == 3

@@ -112,7 +112,8 @@ def paged_attention(
     if sequences == 0 or tokens == 0:
         return torch.zeros_like(query) if output is None else output
     _check_room(block_table, key_cache)
-    if output is None:
+    given = output is not None
+    if not given:
         output = torch.empty_like(query)
     window = 0 if window_size is None else min(window_size, MOST_TOKENS)
     sinks = min(num_sinks, MOST_TOKENS)
@@ -139,6 +140,8 @@ def paged_attention(
         softmax_scale,
         zero_rest,
     )
+    if given:
+        util.written(output)
     util.pop_trace()
     util.pop_trace()
 
@@ -164,4 +167,5 @@ def paged_cache_append(key, value, key_cache, value_cache, block_table, context_
     _lib.paged_cache_append(
         key_cache, value_cache, key, value, _index(block_table), _index(context_lengths), _index(query_offsets)
     )
+    util.written(key_cache, value_cache)
     util.pop_trace()

@@ -1,6 +1,7 @@
 """Host-side helpers of the operation layer; counterparts of trident/util/util.py."""
 
 import torch
+from torch.autograd import forward_ad
 
 from trident_b200 import config
 
@@ -13,6 +14,7 @@ __all__ = [
     "size_and_stride",
     "push_trace",
     "pop_trace",
+    "written",
     "uniform",
     "zero",
 ]
@@ -33,6 +35,12 @@ def is_pow2(value):
     return value != 0 and (value & (value - 1)) == 0
 
 
+# (looked up once: the calls that ask take 10 us of host time in all)
+_increment_version = torch.autograd.graph.increment_version
+_tracing_state = torch._C._get_tracing_state
+_transforms_active = torch._C._are_functorch_transforms_active
+
+
 def needs_grad(*tensors):
     """Whether an operation on these tensors (None allowed) has to go through its autograd Function: autograd
     would record it, or something else that only sees Functions is looking on."""
@@ -43,14 +51,19 @@ def needs_grad(*tensors):
     return is_watched()
 
 
+def written(*tensors):
+    """Tells autograd that these tensors were written in place by a kernel: a graph that saved one of them refuses its
+    backward pass, as after an in-place operation of torch. (Inference tensors are never saved and keep no version.)"""
+    try:
+        _increment_version(tensors)
+    except RuntimeError:  # (an inference tensor outside of inference mode)
+        _increment_version([t for t in tensors if not t.is_inference()])
+
+
 def is_watched():
     """Whether a trace, a function transform or forward-mode differentiation is under way: they would take the
     output of a kernel that is called directly for an empty tensor, or for one without a tangent."""
-    return (
-        torch._C._get_tracing_state() is not None
-        or torch._C._are_functorch_transforms_active()
-        or torch.autograd.forward_ad._current_level >= 0
-    )
+    return _tracing_state() is not None or _transforms_active() or forward_ad._current_level >= 0
 
 
 def size_and_stride(input: torch.Tensor, dim: int):
