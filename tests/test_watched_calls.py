@@ -20,7 +20,7 @@ def calls(monkeypatch):
     def stand_in(name, outputs):
         def run(*args):
             seen.append(name)
-            for t in args[:outputs]:
+            for t in filter(torch.is_tensor, args[:outputs]):
                 with torch.inference_mode(t.is_inference()):
                     t.data.fill_(1.0)  # (as a kernel: autograd sees nothing of it)
 
@@ -30,6 +30,10 @@ def calls(monkeypatch):
     monkeypatch.setattr(_lib, "paged_attention_workspace", lambda *args: 0)
     stand_in("window_attention_fwd", 1)
     stand_in("gated_residual_rms_norm_fwd", 2)
+    for name in ("window_attention_bwd_workspace", "gated_residual_rms_norm_bwd_workspace"):
+        monkeypatch.setattr(_lib, name, lambda *args: 16)
+    stand_in("window_attention_bwd", 3)
+    stand_in("gated_residual_rms_norm_bwd", 5)
     stand_in("paged_attention", 1)
     stand_in("paged_cache_append", 0)
     return seen
@@ -132,3 +136,19 @@ def test_inference_tensors_are_written(calls):
         F.paged_cache_append(x, x, keys, keys, TABLE, LENGTHS)
         assert F.paged_attention(x, keys, keys, TABLE, LENGTHS, output=out) is out
     assert len(calls) == 3
+
+
+@pytest.mark.parametrize("call", [_window, _norm])
+def test_a_second_derivative_is_refused(call, calls):
+    """Its part of a sum is not dropped without a word, whether or not the gradient that comes in needs one itself."""
+    for ask in (False, True):
+        x = Q.clone().requires_grad_(True)
+        out = call(x)
+        dout = torch.ones_like(out, requires_grad=ask)
+        (dx,) = torch.autograd.grad(out, x, dout, create_graph=True)
+        assert dx.requires_grad
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(dx.square().sum() + x.square().sum(), x)
+    x = Q.clone().requires_grad_(True)
+    call(x).sum().backward()
+    assert not x.grad.requires_grad

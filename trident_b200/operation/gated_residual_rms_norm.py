@@ -117,6 +117,8 @@ class GatedResidualRMSNorm(torch.autograd.Function):
         )
         util.pop_trace()
 
+        grads = util.first_order("Gated residual RMSNorm", grads, *grad_outputs, *ctx.saved_tensors)
+
         return (*grads, None, None)
 
     @staticmethod

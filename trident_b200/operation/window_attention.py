@@ -84,7 +84,7 @@ class WindowAttention(torch.autograd.Function):
         )
         util.pop_trace()
 
-        return (*grads, None, None, None)
+        return (*util.first_order("Window attention", grads, grad_output, *ctx.saved_tensors), None, None, None)
 
     @staticmethod
     def __backward(grad_output, query, key, value, output, log_sum_exp, window_size, num_sinks, softmax_scale):

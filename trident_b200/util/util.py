@@ -8,6 +8,7 @@ from trident_b200 import config
 __all__ = [
     "calculate_fan_in_and_fan_out",
     "fill",
+    "first_order",
     "is_pow2",
     "is_watched",
     "needs_grad",
@@ -49,6 +50,28 @@ def needs_grad(*tensors):
             if t is not None and t.requires_grad:
                 return True
     return is_watched()
+
+
+class _FirstOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, count, *tensors):
+        ctx.what = what
+        return tuple(t.view_as(t) for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} has no second derivative.")
+
+
+def first_order(what, grads, *sources):
+    """The gradients (None allowed) of a backward pass that cannot be differentiated itself, computed from `sources`.
+    Under create_graph=True they are tied to these by a node that refuses: without one a second derivative would
+    lose their part of a sum without a word."""
+    if not torch.is_grad_enabled():
+        return grads
+    given = [g for g in grads if g is not None]
+    tied = iter(_FirstOrder.apply(what, len(given), *given, *(t for t in sources if t is not None)))
+    return tuple(None if g is None else next(tied) for g in grads)
 
 
 def written(*tensors):
