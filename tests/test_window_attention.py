@@ -370,3 +370,20 @@ def test_many_short_walks(B, KV, G, S, window, sinks, D, device):
             heads = slice(h * G, (h + 1) * G)
             want = ref.attention(q[b, heads].double(), k[b, h].double(), v[b, h].double(), at, window, sinks, D ** -0.5, dt)["out"]
             ref.check(out[b, heads], want, f"sequence {b}, key head {h}")
+
+
+def test_workspace_of_many_sinks():
+    """The parts of the sinks' gradients: at most eight far pieces an SM in all, or one of each tile, and its window part."""
+    bytes_of = _lib.load().tb200_window_attention_bwd_workspace
+    for B, H, KV, S, D, window, sinks in ((1, 32, 8, 65536, 128, 1024, 8192), (4, 8, 8, 100000, 64, 128, 50000), (1, 8, 1, 65536, 128, 1024, 4)):
+        tiles = B * KV * -(-sinks // 64)  # (of the CUDA-core kernels; those of the tensor cores are twice as long)
+        rows = 2 * B * KV * -(-S // (96 // (H // KV))) * 96 * 4 + 256
+        assert bytes_of(B, H, KV, S, D, window, sinks, 2) <= rows + (8 * 148 + 2 * tiles) * 2 * 128 * D * 4
+    assert bytes_of(1, 32, 8, 65536, 128, 1024, 8192, 2) < 600e6  # (dk and dv are 270 MB)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt, D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)], ids=["bf16", "fp16", "fp32"])
+def test_many_sinks(dt, D, device):
+    """More tiles with sinks than the far pieces are cut for."""
+    _compare(_problem(8, 4, 1, 1600, D, dt, seed=80), 60, 1100, device)

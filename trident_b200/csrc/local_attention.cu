@@ -69,8 +69,12 @@ int fill_window(LocalArgs* a, const char* who, int64_t B, int64_t H, int64_t KV,
   return 0;
 }
 
-// Far pieces of the backward pass (see LocalBwdArgs), each about as long as a key tile's walk inside
-// the window.
+// Far pieces of the backward pass (see LocalBwdArgs), each about as long as a key tile's walk inside the window, and
+// of all sequences, heads and sink tiles together no more than FAR_PER_SM an SM: beyond that they no longer even out
+// the work, but each takes a tile of fp32 gradients of the workspace (backward pass of 32 heads on 8 key heads, 65536 x
+// 128 bf16, window 1024, 8192 sinks: 2 pieces 26.8 ms and 0.2 GB, 56 pieces 31.5 ms and 4.1 GB; 8 heads x 32768, window
+// 256, 2048 sinks: 9 pieces 1.28 ms, 64 pieces 2.04).
+constexpr int64_t FAR_PER_SM = 8;
 void plan_far(LocalBwdArgs* b, int key_tile) {
   const LocalArgs& a = b->f;
   b->sink_tiles = b->far = 0;
@@ -79,8 +83,11 @@ void plan_far(LocalBwdArgs* b, int key_tile) {
   while (b->sink_tiles < st && near_end(a, b->sink_tiles, key_tile) < a.tokens) ++b->sink_tiles;
   if (b->sink_tiles == 0) return;
   const int64_t span = a.tokens - near_end(a, 0, key_tile), walk = (int64_t)a.window + key_tile;
-  const int64_t pieces = ceil_div(span, walk);
-  b->far = (int)(pieces < 64 ? pieces : 64);
+  int64_t pieces = ceil_div(span, walk);
+  if (pieces > 64) pieces = 64;
+  const int64_t most = FAR_PER_SM * sm_count() / ((int64_t)a.n * a.KV * b->sink_tiles);
+  if (pieces > most) pieces = most;
+  b->far = pieces > 1 ? (int)pieces : 1;
 }
 size_t far_bytes(const LocalBwdArgs& b, int key_tile) {
   return (size_t)b.f.n * b.f.KV * b.sink_tiles * (b.far + 1) * 2 * key_tile * b.f.D * sizeof(float);
