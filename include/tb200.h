@@ -331,11 +331,12 @@ int tb200_device_status(int reset);
  * the calling thread and applies to the norm backward calls that thread makes; other threads
  * keep their own. Returns the old value. */
 int tb200_set_norm_fused_finalize(int on);
-/* Test hook of the calling thread for the bounded waits of the tensor-core kernels. mode 1: the
- * attention forward launches this thread makes next run with a wait limit of about a
- * millisecond and the producer of CTA (0, 0) leaves out the copy of its second key tile, so one
- * wait runs out: the launch must still complete, free its tensor memory and leave a non-zero
- * code in the device status word (tb200_device_status); its output is invalid. mode 0: normal
+/* Test hook of the calling thread for the bounded waits of the tensor-core and bulk-copy kernels. mode 1: the launches
+ * this thread makes next of the attention forward, the window attention forward, paged attention, the first kernel of the
+ * window attention backward (dQ) and the gated residual RMSNorm backward run with a wait limit of about a
+ * millisecond, and the producer of their first CTA leaves out one copy, so one wait runs out: the launch must still
+ * complete, free its tensor memory and leave a non-zero code in the device status word (tb200_device_status); its
+ * output is invalid. mode 2: the same for the second kernel of the window attention backward (dK, dV). mode 0: normal
  * operation. Returns the old mode. No memory is touched that a normal launch would not touch. */
 int tb200_test_wait_fault(int mode);
 

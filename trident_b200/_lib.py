@@ -137,7 +137,7 @@ def set_norm_fused_finalize(on):
 
 
 def test_wait_fault(mode):
-    """Test hook (calling thread): 1 makes one bounded wait of the next attention forward launches
+    """Test hook (calling thread): 1 (or 2) makes one bounded wait of the next launches of some kernels
     run out (see include/tb200.h); 0 restores normal operation. Returns the old mode."""
     return load().tb200_test_wait_fault(int(mode))
 

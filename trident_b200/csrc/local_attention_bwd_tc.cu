@@ -58,6 +58,7 @@ struct BwdParams {
   int col_tiles, key_tiles;
   Divisor heads, kv;    // n * KV, KV
   int* status;
+  WaitTest test_dq, test_dkv;
 };
 
 __device__ inline void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < 1 + 2 * STAGES + 4; ++i) ptx::mbar_init(&bars[i], 1);
     for (int i = 0; i < 3; ++i) ptx::mbar_init(s_free + i, 256);
     abort_flag[0] = 0;
-    abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
+    abort_flag[1] = p.test_dkv.units;
     ptx::fence_barrier_init();
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_do);
@@ -185,9 +186,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         tma_load_4d(k_smem + c * KEY_BOX, &map_k, kv_full, c * 64, jt * TILE, hk, s);
         tma_load_4d(v_smem + c * KEY_BOX, &map_v, kv_full, c * 64, jt * TILE, hk, s);
       }
+      int brought = 0;
       for (int i = 0; i < steps; ++i) {
         const int st = i % STAGES, it = i0 + i;
         ptx::mbar_wait(&qdo_empty[st], ((i / STAGES) & 1) ^ 1, abort_flag, p.status, 101);
+        if (abort_flag[0]) break;  // a wait has run out: nothing more is brought
+        brought = i + 1;
+        if (i == p.test_dkv.skip && blockIdx.x == 0) continue;  // (test hook)
         ptx::mbar_expect_tx(&qdo_full[st], 2 * NBOX * rows * 128 + 2 * COLS * 4);
 #pragma unroll
         for (int c = 0; c < NBOX; ++c) {
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // every copy has landed before the CTA gives up its shared memory
       ptx::mbar_wait_drain(kv_full, 0, abort_flag, p.status, 102);
-      for (int i = steps > STAGES ? steps - STAGES : 0; i < steps; ++i)
+      for (int i = brought > STAGES ? brought - STAGES : 0; i < brought; ++i)
         ptx::mbar_wait_drain(&qdo_full[i % STAGES], (i / STAGES) & 1, abort_flag, p.status, 102);
     }
     __syncwarp();
@@ -485,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 17; i < 19; ++i) ptx::mbar_init(&bars[i], 64);
     ptx::mbar_init(out_free, 1);
     abort_flag[0] = 0;
-    abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
+    abort_flag[1] = p.test_dq.units;
     if ((ptx::smem_u32(smem) & 1023u) != 0) {  // swizzled tiles need a 1024-byte aligned base
       abort_flag[0] = 1;
       atomicCAS(p.status, 0, 120);
@@ -518,18 +523,24 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_load_5d(out_smem + c * BOX_BYTES, &map_out, land_full, c * 64, 0, w.t0, w.hk, w.s);
         }
       };
-      int g = 0, u = 0;
+      int g = 0, u = 0, keys = 0, landed = 1;  // steps, tiles; K tiles (g, or one more) and landings brought
+      bool stop = false;                       // a wait has run out: nothing more is brought
       land(blockIdx.x);
-      for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
+      for (int unit = blockIdx.x; unit < units && !stop; unit += gridDim.x, ++u) {
         const Unit w = unit_at(unit);
         const KeyRange kr = walk_of(w);
         for (int i = 0; i < kr.count; ++i, ++g) {
           const int st = g & 1, j0 = kr.tile(i) * TILE;
           ptx::mbar_wait(&k_empty[st], ((g >> 1) & 1) ^ 1, abort_flag, p.status, 121);
-          ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
+          if ((stop = abort_flag[0] != 0)) break;
+          ++keys;
+          if (!(g == p.test_dq.skip && blockIdx.x == 0)) {  // (test hook)
+            ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
 #pragma unroll
-          for (int c = 0; c < NBOX; ++c) tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES, &map_k, &k_full[st], c * 64, j0, w.hk, w.s);
+            for (int c = 0; c < NBOX; ++c) tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES, &map_k, &k_full[st], c * 64, j0, w.hk, w.s);
+          }
           ptx::mbar_wait(&v_empty[st], ((g >> 1) & 1) ^ 1, abort_flag, p.status, 122);
+          if ((stop = abort_flag[0] != 0)) break;
           ptx::mbar_expect_tx(&v_full[st], TILE_BYTES);
 #pragma unroll
           for (int c = 0; c < NBOX; ++c) tma_load_4d(v_smem + st * TILE_BYTES + c * BOX_BYTES, &map_v, &v_full[st], c * 64, j0, w.hk, w.s);
@@ -538,16 +549,19 @@ __global__ void __launch_bounds__(THREADS, 1)
             ptx::mbar_wait(q_ready, u & 1, abort_flag, p.status, 123);
             ptx::mbar_wait(&stats_full[u & 1], (u >> 1) & 1, abort_flag, p.status, 123);
             ptx::mbar_wait(out_free, u & 1, abort_flag, p.status, 123);
+            if ((stop = abort_flag[0] != 0)) {
+              ++g;  // (this step's V is under way)
+              break;
+            }
             land(unit + gridDim.x);
+            ++landed;
           }
         }
       }
       // every copy has landed before the CTA gives up its shared memory
-      ptx::mbar_wait_drain(land_full, (u - 1) & 1, abort_flag, p.status, 124);
-      for (int i = g > 2 ? g - 2 : 0; i < g; ++i) {
-        ptx::mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 124);
-        ptx::mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 124);
-      }
+      ptx::mbar_wait_drain(land_full, (landed - 1) & 1, abort_flag, p.status, 124);
+      for (int i = keys > 2 ? keys - 2 : 0; i < keys; ++i) ptx::mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 124);
+      for (int i = g > 2 ? g - 2 : 0; i < g; ++i) ptx::mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1, abort_flag, p.status, 124);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -861,6 +875,8 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
   p.heads = Divisor(a.n * a.KV);
   p.kv = Divisor(a.KV);
   p.status = device_status_ptr();
+  p.test_dq = WaitTest::of_this_thread(1, 1);
+  p.test_dkv = WaitTest::of_this_thread(2, 1);
   const int64_t parts = (int64_t)a.n * a.KV * (p.key_tiles + (int64_t)b.sink_tiles * b.far);
   TB200_REQUIRE(parts < (1ll << 31), TB200_ERR_UNSUPPORTED, "local_dkv_tc: %lld walks", (long long)parts);
   auto go = [&](auto tag, auto dsel) -> int {

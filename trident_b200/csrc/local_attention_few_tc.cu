@@ -41,6 +41,7 @@ struct FewParams {
   void* out;
   float scale_log2;
   int piece;  // rows of one copy of keys
+  WaitTest test;
 };
 
 __device__ inline void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     for (int i = 0; i < 2 * STAGES + 5; ++i) ptx::mbar_init(&bars[i], 1);
     for (int i = 0; i < 4; ++i) ptx::mbar_init(s_free + i, 128);
     abort_flag[0] = 0;
-    abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
+    abort_flag[1] = p.test.units;
     ptx::fence_barrier_init();
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
@@ -154,18 +155,23 @@ __global__ void __launch_bounds__(THREADS, 2)
           tma_load_5d(q_smem + c * (N * 128), &map_q, q_full, c * 64, 0, seq.q_begin, hk, 0);
       }
     }
-    for (int i = 0; i < steps; ++i) {
+    int brought = 0;    // tiles
+    bool stop = false;  // a wait has run out: nothing more is brought
+    for (int i = 0; i < steps && !stop; ++i) {
       int next_page = 0, next_row = 0;
       if (i + 1 < steps) locate(kr.tile(m0 + i + 1), &next_page, &next_row);
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         const int g = 2 * i + kv, st = g % STAGES;
-        if (lane == 0) {
-          ptx::mbar_wait(&empty[st], ((g / STAGES) & 1) ^ 1, abort_flag, a.status, 141);
-          ptx::mbar_expect_tx(&full[st], TILE_BYTES);
-        }
+        if (stop) continue;
+        if (lane == 0) ptx::mbar_wait(&empty[st], ((g / STAGES) & 1) ^ 1, abort_flag, a.status, 141);
+        stop = __shfl_sync(0xffffffffu, lane == 0 ? abort_flag[0] : 0u, 0) != 0;
+        if (stop) continue;
+        brought = g + 1;
+        const bool left_out = g == p.test.skip && blockIdx.x + blockIdx.y + blockIdx.z == 0;  // (test hook)
+        if (lane == 0 && !left_out) ptx::mbar_expect_tx(&full[st], TILE_BYTES);
         __syncwarp();
-        if (lane < pieces) {
+        if (lane < pieces && !left_out) {
 #pragma unroll
           for (int c = 0; c < NBOX; ++c)
             tma_load_4d(ring + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, kv ? &map_v : &map_k, &full[st], c * 64, row,
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     // every copy has landed before the CTA gives up its shared memory
     if (lane == 0 && steps > 0) {
       ptx::mbar_wait_drain(q_full, 0, abort_flag, a.status, 142);
-      for (int g = 2 * steps > STAGES ? 2 * steps - STAGES : 0; g < 2 * steps; ++g)
+      for (int g = brought > STAGES ? brought - STAGES : 0; g < brought; ++g)
         ptx::mbar_wait_drain(&full[g % STAGES], (g / STAGES) & 1, abort_flag, a.status, 142);
     }
     __syncwarp();
@@ -404,6 +410,7 @@ int launch_local_few_tc(void* out, const void* q, const void* k, const void* v, 
   p.out = out;
   p.scale_log2 = a.scale * LOG2E;
   p.piece = local_piece(a);
+  p.test = WaitTest::of_this_thread(1, 2);
   CUtensorMap mq, mk, mv;
   bind_primary_context();
   if (!local_map_rows(&mq, q, a.qs, a, N / a.G, "q") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||

@@ -63,7 +63,7 @@ struct FwdParams {
   int piece;        // R: rows of one copy of keys
   int pairs, units; // pairs of query tiles per sequence and key head; pairs * KV * sequences * parts
   Divisor outer, kv, splits;  // of a unit's number (unit_at)
-  uint32_t wait_units;
+  WaitTest test;
 };
 
 __device__ inline void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     for (int i = 27; i < 31; ++i) ptx::mbar_init(&bars[i], 1);
     *copied = 0;
     abort_flag[0] = 0;
-    abort_flag[1] = p.wait_units;
+    abort_flag[1] = p.test.units;
     ptx::fence_barrier_init();
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
@@ -299,9 +299,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     if (warp == 0) {
       // -------------------------------------------------------------- producer (whole warp)
       const int pieces = TILE / p.piece;
-      int g = 0, queries0 = 0, queries1 = 0;  // steps, units of each query tile so far
-      uint32_t fixed = 0;                     // bit s: the last V tile of stage s is completed by warp 3
-      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+      int g = 0, queries0 = 0, queries1 = 0;  // steps so far, queries brought of each tile (lane 0)
+      int keys = 0;                           // K tiles: g, or one more
+      uint32_t fixed = 0;                     // bit s: the last V tile of stage s is completed by warp 3; 2 + s: parity
+                                              // of that completion (of v_raw)
+      bool stop = false;                      // a wait has run out: nothing more is brought
+      auto stopped = [&]() { return __shfl_sync(0xffffffffu, lane == 0 ? abort_flag[0] : 0u, 0) != 0; };
+      for (int unit = blockIdx.x; unit < p.units && !stop; unit += gridDim.x) {
         Unit w;
         if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
         const bool fix = needs_fix(w);
@@ -331,6 +335,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             for (int t = 0; t < 2; ++t) {
               if ((t ? w.hi1 : w.hi0) < 0) continue;
               ptx::mbar_wait(&q_empty[t], ((t ? queries1 : queries0) & 1) ^ 1, abort_flag, a.status, 60);
+              if (abort_flag[0]) break;
+              ++(t ? queries1 : queries0);
               ptx::mbar_expect_tx(&q_full[t], bytes);
 #pragma unroll
               for (int c = 0; c < NBOX; ++c)
@@ -340,12 +346,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           }
           int next_page = 0, next_row = 0;  // (looked up while this step's copies wait for their stage)
           if (m + 1 < w.m1) locate(w.kr.tile(m + 1), &next_page, &next_row);
-          if (lane == 0) {
-            ptx::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, 61);
-            ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
-          }
+          if (lane == 0) ptx::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, 61);
+          if ((stop = stopped())) break;
+          const bool left_out = g == p.test.skip && blockIdx.x == 0;  // (test hook)
+          if (lane == 0 && !left_out) ptx::mbar_expect_tx(&k_full[st], TILE_BYTES);
           __syncwarp();
-          if (lane < pieces) {
+          ++keys;
+          if (lane < pieces && !left_out) {
 #pragma unroll
             for (int c = 0; c < NBOX; ++c)
               tma_load_4d(k_smem + st * TILE_BYTES + c * BOX_BYTES + lane * p.piece * 128, &map_k, &k_full[st], c * 64, row,
@@ -353,11 +360,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           }
           const bool fixed_tile = fix && m + 1 == w.m1;
           uint64_t* vbar = fixed_tile ? &v_raw[st] : &v_full[st];
-          fixed = (fixed & ~(1u << st)) | (fixed_tile ? 1u << st : 0u);
-          if (lane == 0) {
-            ptx::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, 62);
-            ptx::mbar_expect_tx(vbar, TILE_BYTES);
-          }
+          if (lane == 0) ptx::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, 62);
+          if ((stop = stopped())) break;
+          fixed = ((fixed & ~(1u << st)) | (fixed_tile ? 1u << st : 0u)) ^ (fixed_tile ? 4u << st : 0u);
+          if (lane == 0) ptx::mbar_expect_tx(vbar, TILE_BYTES);
           __syncwarp();
           if (lane < pieces) {
 #pragma unroll
@@ -367,17 +373,16 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           page = next_page;
           row = next_row;
         }
-        queries0 += w.hi0 >= 0;
-        queries1 += w.hi1 >= 0;
       }
-      // Drain: every copy has landed before the CTA gives up its shared memory (warp 3 itself waits for the
-      // copies of the tiles that it completes).
+      // Drain: every copy has landed before the CTA gives up its shared memory.
       if (lane == 0) {
         if (queries0 > 0) ptx::mbar_wait_drain(&q_full[0], (queries0 - 1) & 1, abort_flag, a.status, 63);
         if (queries1 > 0) ptx::mbar_wait_drain(&q_full[1], (queries1 - 1) & 1, abort_flag, a.status, 63);
-        for (int i = g > 2 ? g - 2 : 0; i < g; ++i) {
+        for (int i = keys > 2 ? keys - 2 : 0; i < keys; ++i)
           ptx::mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1, abort_flag, a.status, 64);
-          if (!((fixed >> (i & 1)) & 1u)) ptx::mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1, abort_flag, a.status, 65);
+        for (int i = g > 2 ? g - 2 : 0; i < g; ++i) {
+          if (((fixed >> (i & 1)) & 1u)) ptx::mbar_wait_drain(&v_raw[i & 1], ((fixed >> (2 + (i & 1))) & 1u) ^ 1u, abort_flag, a.status, 65);
+          else ptx::mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1, abort_flag, a.status, 65);
         }
       }
       __syncwarp();
@@ -448,7 +453,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         const Walk w = walks[units & 1];
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&walk_empty[units & 1]);
-        if (w.steps == 0 || abort_flag[0]) break;
+        if (__any_sync(0xffffffffu, w.steps == 0 || abort_flag[0])) break;
         const int steps = w.steps;
         bool fresh0 = true, fresh1 = true;  // no scores of the tile yet
         for (int i = 0; i < steps; ++i, ++g) {
@@ -522,6 +527,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         int outs = 0;
         for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
           Unit w;
+          if (abort_flag[0]) break;
           if (!unit_at<PAGED>(p, unit, &w)) continue;
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
@@ -571,6 +577,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       int fix_keys = 0;  // of the unit before
       for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
         Unit w;
+        if (__any_sync(0xffffffffu, abort_flag[0] != 0)) break;
         if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
         int last0 = w.m1 - w.m0 - 1, last1 = last0;
         while (last0 >= 0 && !w.active(0, w.kr.tile(w.m0 + last0))) --last0;
@@ -623,6 +630,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       return unit;
     };
     for (int unit = next_unit(blockIdx.x); unit < p.units;) {
+      if (__any_sync(0xffffffffu, abort_flag[0] != 0)) break;
       const int first_token = w.t0 + t * p.tile_tokens;
       const int tokens = min(p.tile_tokens, w.seq.q_len - first_token);
       const int rows = tokens > 0 ? tokens * a.G : 0;
@@ -1013,7 +1021,7 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   p.outer = Divisor(p.units / p.pairs);
   p.kv = Divisor(a.KV);
   p.splits = Divisor(a.splits);
-  p.wait_units = ptx::WAIT_LIMIT_UNITS;
+  p.test = WaitTest::of_this_thread(1, 1);
   CUtensorMap mq, mk, mv, mo;
   bind_primary_context();
   if (!local_map_rows(&mq, q, a.qs, a, p.tile_tokens, "q") || !local_map_rows(&mo, out, a.os, a, p.tile_tokens, "out") || !local_map_keys(&mk, k, a.ks, a, p.piece, "k") ||

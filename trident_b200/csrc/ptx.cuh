@@ -287,5 +287,19 @@ bool make_tensor_map_3d(CUtensorMap* map, const void* base, uint64_t batch, uint
 int* device_status_ptr();
 // Test hook of the calling thread (tb200_test_wait_fault): 0 = normal operation.
 int test_wait_fault_mode();
+// What a kernel needs of it: the limit of its waits, and the copy (step, row) that its first CTA leaves out, -1: none.
+struct WaitTest {
+  uint32_t units = ptx::WAIT_LIMIT_UNITS;
+  int skip = -1;
+  // `mode`: the one that means this kernel
+  static WaitTest of_this_thread(int mode, int skip) {
+    WaitTest w;
+    if (test_wait_fault_mode() == mode) {
+      w.units = 30;  // x 65536 cycles: about a millisecond
+      w.skip = skip;
+    }
+    return w;
+  }
+};
 
 }  // namespace tb200

@@ -419,12 +419,12 @@ __global__ void __launch_bounds__(THREADS, CHUNKS <= 2 ? 2 : 1)
                     float* __restrict__ part_b, const T* __restrict__ dh, const T* __restrict__ dy, const T* __restrict__ x,
                     const T* __restrict__ r, const T* __restrict__ w1, const T* __restrict__ w2, const T* __restrict__ gate,
                     const float* __restrict__ rms1, const float* __restrict__ rms2, const ResNormArgs a, int per_row,
-                    int stages, int* status) {
+                    int stages, int* status, const WaitTest test) {
   constexpr int VEC = Traits<T>::VEC, PAIRS = VEC / 2;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float slot[64];
   __shared__ uint64_t full[4];
-  __shared__ uint32_t abort_words[2];
+  __shared__ uint32_t abort_words[3];  // abort flag, wait limit (ptx::mbar_wait), rows requested
   volatile uint32_t* abort_flag = abort_words;
   const int cols = (int)a.cols;
   const int bytes = cols * (int)sizeof(T);
@@ -434,8 +434,8 @@ __global__ void __launch_bounds__(THREADS, CHUNKS <= 2 ? 2 : 1)
   int phase = 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) ptx::mbar_init(&full[i], 1);
-    abort_flag[0] = 0;
-    abort_flag[1] = ptx::WAIT_LIMIT_UNITS;
+    abort_flag[0] = abort_flag[2] = 0;
+    abort_flag[1] = test.units;
     ptx::fence_barrier_init();
   }
   __syncthreads();
@@ -443,6 +443,8 @@ __global__ void __launch_bounds__(THREADS, CHUNKS <= 2 ? 2 : 1)
   pdl_release();
   const int tensors = 2 + (dh ? 1 : 0) + (dy ? 1 : 0);
   auto request = [&](int i, int st) {  // (thread 0) row begin + i into stage st
+    abort_flag[2] = i + 1;
+    if (i == test.skip && blockIdx.x == 0) return;  // (test hook)
     uint8_t* dst = ring + (size_t)st * 4 * bytes;
     const int64_t off = (begin + i) * a.cols;
     ptx::mbar_expect_tx(&full[st], (uint32_t)(tensors * bytes));
@@ -541,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, CHUNKS <= 2 ? 2 : 1)
     }
     // (the reduction's barrier also says that every thread has taken its part of the stage)
     const float sum2 = row_reduce<true, false>(hsum2(s2), slot, phase);
-    if (threadIdx.x == 0 && i + stages < count) request(i + stages, st);
+    if (threadIdx.x == 0 && i + stages < count && !abort_flag[0]) request(i + stages, st);  // (not after an expired wait)
     if (++st == stages) {
       st = 0;
       ring_phase ^= 1u;
@@ -595,6 +597,10 @@ __global__ void __launch_bounds__(THREADS, CHUNKS <= 2 ? 2 : 1)
   }
   if (part_a) flush(part_a + ((int64_t)blockIdx.x + (per_row ? 0 : current)) * a.cols, acc_a);
   if (part_b) flush(part_b + (int64_t)blockIdx.x * a.cols, acc_b);
+  // Every copy has landed before the CTA gives up its shared memory (without an expired wait all have been waited for).
+  if (threadIdx.x == 0 && abort_flag[0])
+    for (int requested = abort_flag[2], i = requested > stages ? requested - stages : 0; i < requested; ++i)
+      ptx::mbar_wait_drain(&full[i % stages], (i / stages) & 1, abort_flag, status, 162);
 }
 
 // blockIdx.y 0: dw1 (and dgate where one vector serves all rows), 1: dw2, 2..: dgate of one vector each.
@@ -821,7 +827,7 @@ extern "C" int tb200_gated_residual_rms_norm_bwd(void* dx, void* dr, void* dw1, 
         (void)launch_pdl(kern, dim3((unsigned)n), dim3(plan.threads), (size_t)plan.stages * 4 * cols * sizeof(T), st, false,
                          (T*)dx, (T*)dr, per_row ? (T*)dgate : nullptr, part_a, part_b, (const T*)dh, (const T*)dy, (const T*)x,
                          (const T*)r, (const T*)w1, (const T*)w2, (const T*)gate, rms1, rms2, a, per_row ? 1 : 0, plan.stages,
-                         device_status_ptr());
+                         device_status_ptr(), WaitTest::of_this_thread(1, 1));
         return launch_status("resnorm_bwd_vec");
       };
       rc = plan.chunks == 1   ? go(IntC<1>{}, IntC<128>{})
