@@ -141,3 +141,38 @@ def test_workload_work_figures_at_full_size():
     assert W["geglu"].work({"x": Meta((8192, 4096), 2), "w": Meta((22016, 4096), 2)}) == 4432406249472
     assert W["attention_causal"].work({"q": Meta((4, 32, 4096, 128), 2)}) == 1924145348608
     assert W["attention_masked"].work({"q": Meta((8, 16, 16384, 64), 2)}) == 30786325577728
+
+
+def test_calls_without_the_extension_go_through_ctypes(monkeypatch):
+    import sys
+
+    import trident_b200
+
+    monkeypatch.delattr(trident_b200, "_fastcall", raising=False)
+    monkeypatch.setitem(sys.modules, "trident_b200._fastcall", None)  # (an import of it fails)
+    _lib._entry.cache_clear()
+    try:
+        window = _lib._entry("tb200_window_attention_fwd")
+        strides = (1, 1, 1, 1)
+        assert window(8, 8, 8, 8, 8, 1, 3, 2, 8, 16, strides, strides, strides, strides, 4, 0, 1.0, 0, 0) == -1
+        assert "multiple" in _lib.last_error()
+        paged = _lib._entry("tb200_paged_attention")
+        assert paged(8, 8, 8, 8, 8, 8, None, None, 0, 0, 0, 4, 2, 64, 16, 4, 3, 3, strides[:3], strides, strides,
+                     strides[:3], 1, 10, 0, 0, 1.0, True, 0, 0) == 0
+    finally:
+        _lib._entry.cache_clear()
+
+
+def test_the_extension_is_not_needed_to_build(monkeypatch, tmp_path, capsys):
+    import sysconfig
+
+    from trident_b200 import build
+
+    assert build.FASTCALL_PATH.endswith(sysconfig.get_config_var("EXT_SUFFIX"))  # (another interpreter passes it by)
+    path = tmp_path / "_fastcall.so"
+    monkeypatch.setattr(build, "FASTCALL_PATH", str(path))
+    for compiler in ("/no/such/compiler", "false"):
+        path.write_text("of another build")
+        monkeypatch.setenv("CC", compiler)
+        build._build_fastcall(True)
+        assert not path.exists() and "through ctypes" in capsys.readouterr().err

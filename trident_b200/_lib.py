@@ -173,13 +173,16 @@ def _require_cuda(*tensors):
 
 @functools.lru_cache(maxsize=None)
 def _entry(name):
-    """Entry point `name`, taking stride tuples: the direct one of the _fastcall extension, or a ctypes call
-    where another library than the package's own is used."""
+    """Entry point `name`, taking stride tuples: the direct one of the _fastcall extension, or a ctypes call of the
+    same function where the extension is not built, or another library than the package's own is used."""
     function = getattr(load(), name)
     if LIB_PATH == _OWN_LIB:
-        from trident_b200 import _fastcall
+        try:
+            from trident_b200 import _fastcall
 
-        return getattr(_fastcall, name)
+            return getattr(_fastcall, name)
+        except ImportError:
+            pass
     return lambda *args: function(*(_stride_array(a) if isinstance(a, tuple) else a for a in args))
 
 
