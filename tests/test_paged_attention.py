@@ -683,3 +683,21 @@ def test_rows_beyond_max_query_length(D, longest, dtype, device):
     mine = torch.full_like(q.to(device), 5.0)
     call(output=mine)
     assert torch.equal(mine.cpu()[kept], got[kept]) and torch.all(mine.cpu()[~kept] == 5.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_error_of_long_sums(D, device):
+    """fp32 values of one sign with equal weights, walks of 2^16 keys that are not cut (many sequences on the same pages):
+    partial sums grow along the walk. Each addition is off by e / sqrt(3) of the sum at most in the mean (e = 2^-24), so
+    a sum per 64 keys and their sum are off by about sqrt(n / 64) e / 3, one running sum by sqrt(n) e / 3. The
+    bound is between the two: sqrt(n / 64) e, and 4 e for the division and the last rounding."""
+    n, sequences, page = 2 ** 16, 600, 256
+    v = util.randn(n, D, seed=130) + 6.0
+    vc = v.view(n // page, page, 1, D).to(device)
+    table = torch.arange(n // page, dtype=torch.int32, device=device).expand(sequences, -1)
+    lengths = torch.full((sequences,), n, dtype=torch.int32, device=device)
+    got = attend(torch.zeros(sequences, 1, D, device=device), torch.ones_like(vc), vc, table, lengths)
+    want = v.double().mean(0)
+    off = (got[0, 0].double().cpu() / want - 1).square().mean().sqrt() / 2.0 ** -24
+    assert off < (n / 64) ** 0.5 + 4, off

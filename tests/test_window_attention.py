@@ -387,3 +387,30 @@ def test_workspace_of_many_sinks():
 def test_many_sinks(dt, D, device):
     """More tiles with sinks than the far pieces are cut for."""
     _compare(_problem(8, 4, 1, 1600, D, dt, seed=80), 60, 1100, device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [16, 64])
+def test_error_of_long_sums(D, device):
+    """dq of the last tokens where the score gradients of the first half of the keys have one sign and those of the
+    second half the other: the partial sums rise to P and fall. As in the test of paged attention, a sum per 64 keys is
+    off by about sqrt(n / 64) e / 3 of P, one running sum by sqrt(n) e / 3. The weights are exp(-log n), the same for
+    all keys: their error, 20 e with the sums' last roundings, is doubled for the two halves."""
+    n, last = 2 ** 16, 64
+    sign = torch.where(torch.arange(n) < n // 2, 1.0, -1.0)
+    k = util.randn(n, D, seed=90) + 6.0
+    v = sign[:, None] * (1.0 + 0.1 * util.randn(n, D, seed=91).abs())
+    dout = torch.zeros(n, D)
+    dout[-last:] = 1.0
+    q = torch.zeros(n, D)
+    leaves = [t[None, None].to(device).requires_grad_(True) for t in (q, k, v)]
+    F(*leaves, n, 0, 1.0).backward(dout[None, None].to(device))
+    got = leaves[0].grad[0, 0, -last:].double()
+    k, v = k.double().to(device), v.double().to(device)
+    i = torch.arange(n - last, n, device=device)[:, None]
+    p = (torch.arange(n, device=device) <= i).double() / (i + 1.0)
+    dp = v.sum(-1)
+    g = p * (dp - (p * dp).sum(-1, keepdim=True))
+    most = (g.clamp(min=0) @ k)  # P
+    off = ((got - g @ k) / most).square().mean().sqrt().item() / 2.0 ** -24
+    assert off < (n / 64) ** 0.5 + 40, off

@@ -97,7 +97,8 @@ __device__ inline void accumulate(float (&acc)[4][Shape<D, RM, RS, TX>::DC][Shap
 }
 
 // The same with a sum of its own for the step, added at its end: one running sum over the rows of 64 heads and 600
-// tokens was off by 4e-6 of the result, 10 times a matrix product's error.
+// tokens was off by 4e-6 of the result, 10 times a matrix product's error, one over 65536 keys of a forward walk by 3.6e-6
+// in the mean (now 0.5e-6).
 template <int D, int RM, int RS, int TX>
 __device__ inline void accumulate_step(float (&acc)[4][Shape<D, RM, RS, TX>::DC][Shape<D, RM, RS, TX>::W], const float* p,
                                        const float* b, int ty, int tx) {
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(Shape<D, RM, KEY_TILE, TX>::THREADS)
         for (int w = 0; w < Sh::W; ++w) acc[i][c][w] *= shrink;
     }
     __syncthreads();
-    accumulate<D, RM, KEY_TILE, TX>(acc, sp, sv, ty, tx);
+    accumulate_step<D, RM, KEY_TILE, TX>(acc, sp, sv, ty, tx);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(256)
         sp[(ty * 4 + i) * PLD + tx + BTX * j] = p * (dp[i][j] - de[i]);
       }
     __syncthreads();
-    accumulate<D, BRM, BRS, BTX>(acc, sp, sk, ty, tx);
+    accumulate_step<D, BRM, BRS, BTX>(acc, sp, sk, ty, tx);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
