@@ -292,7 +292,7 @@ int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, c
  * table entries of blocks that no query sees are not read. A context beyond the table keeps its positions: the keys
  * behind the table do not exist, no token is moved onto an earlier place. max_query_length: of a sequence's new tokens
  * the first so many are computed. max_context_length: the longest context expected (longer ones are still right). The workspace
- * holds the parts of walks that are cut along the keys. */
+ * (16-byte aligned) holds the parts of walks that are cut along the keys, or a list of the row tiles. */
 size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t H, int64_t KV, int64_t D,
                                        int64_t max_query_length, int64_t max_context_length, int64_t window,
                                        int64_t sinks, int dtype);

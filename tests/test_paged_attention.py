@@ -701,3 +701,78 @@ def test_error_of_long_sums(D, device):
     want = v.double().mean(0)
     off = (got[0, 0].double().cpu() / want - 1).square().mean().sqrt() / 2.0 ** -24
     assert off < (n / 64) ** 0.5 + 4, off
+
+
+# ------------------------------------------------------------------------------------ listed pieces of work
+def _tokens_of_few(new, KV, G, D, dtype, device, seed):
+    """Many sequences on the pages of a small pool: (arguments of the call, longest, one that checks given sequences)."""
+    n, page, pages = len(new), 8, 64
+    blocks = 5
+    g = util.seeded(seed)
+    kc, vc = (torch.randn(pages, page, KV, D, generator=g).to(dtype) for _ in range(2))
+    table = torch.randint(0, pages, (n, blocks), generator=g, dtype=torch.int32)
+    context = torch.randint(0, blocks * page + 1, (n,), generator=g, dtype=torch.int32)
+    q = torch.randn(sum(new), KV * G, D, generator=g).to(dtype)
+    offsets = torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32)
+
+    def check(got, sequences, window, sinks):
+        for s in sequences:
+            c, (a, b) = int(context[s]), offsets[s:s + 2].tolist()
+            if a == b:
+                continue
+            rows = [t[table[s].long()].flatten(0, 1)[:c] for t in (kc, vc)]
+            one = type("One", (), dict(context=[c], keys=[rows[0]], values=[rows[1]], key_cache=kc))
+            ref.check(got[a:b], _want(q[a:b], one, [b - a], window, sinks, D ** -0.5, dtype), f"sequence {s}")
+
+    return [t.to(device) for t in (q, kc, vc, table, context, offsets)], max(new), check
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 300, 1025, 5000])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_one_long_chunk_among_many_sequences(D, n, dtype, device):
+    """Most pieces of work that the longest chunk plans for every sequence are empty: they are listed first. The same
+    results as announced exactly; rows of no sequence and beyond the longest length as ever."""
+    new = _random(0, 4, n, 140)
+    new[-1] = 0
+    new[n // 2] = 3000
+    args, longest, check = _tokens_of_few(new, 2, 4, D, dtype, device, 141)
+    got = attend(*args, window_size=30, num_sinks=2)
+    check(got, sorted({0, 1 % n, n // 2, max(n - 2, 0), n - 1}), 30, 2)
+    assert torch.equal(got, attend(*args, max_query_length=longest, window_size=30, num_sinks=2))
+    short = _poisoned(lambda: attend(*args, max_query_length=1000, window_size=30, num_sinks=2), got.shape, dtype, device)
+    at = sum(new[: n // 2])
+    assert torch.equal(short[: at + 1000], got[: at + 1000]) and torch.equal(short[at + 3000:], got[at + 3000:])
+    assert torch.all(short[at + 1000: at + 3000] == 0)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_more_planned_pieces_than_31_bits(dt, device):
+    """60000 sequences of 0 to 6 tokens whose longest is not announced."""
+    new = _random(0, 7, 60000, 142)
+    new[7] = 0
+    args, longest, check = _tokens_of_few(new, 1, 64 if dt == torch.bfloat16 else 16, 64, dt, device, 143)
+    args[0] = args[0].contiguous()
+    got = attend(*args)
+    check(got, (0, 1, 7, 30011, 59998, 59999), 0, 0)
+    assert torch.equal(got, attend(*args, max_query_length=longest))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_listed_pieces_in_a_graph(device):
+    """The list is made anew at every replay: offsets and contexts may change."""
+    dt = torch.bfloat16
+    args, _, check = _tokens_of_few([1500] + [1] * 300, 2, 4, 64, dt, device, 144)
+    attend(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend(*args)
+    for new in ([1] * 300 + [1500], [6] * 300 + [0], [0] * 300 + [1800]):
+        args[5].copy_(_offsets(new, device))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[: sum(new)], attend(*args)[: sum(new)])
+    assert _lib.device_status() == 0

@@ -39,6 +39,30 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Fills the list form's array. One CTA: a stretch of sequences a thread, then the stretches' sums.
+__global__ void __launch_bounds__(1024) list_tiles(int* before, const LocalArgs a, const int tile_tokens) {
+  __shared__ int64_t sums[1024];
+  const int per = (a.n + 1023) / 1024, s0 = threadIdx.x * per, s1 = min(s0 + per, a.n);
+  int64_t own = 0;
+  for (int s = s0; s < s1; ++s) own += (load_sequence(a, s).q_len + tile_tokens - 1) / tile_tokens;
+  sums[threadIdx.x] = own;
+  __syncthreads();
+  for (int d = 1; d < 1024; d <<= 1) {
+    const int64_t left = (int)threadIdx.x >= d ? sums[threadIdx.x - d] : 0;
+    __syncthreads();
+    sums[threadIdx.x] += left;
+    __syncthreads();
+  }
+  // (sequences that overlap, which no call should have, may add up to more: the rest is not computed)
+  constexpr int64_t MOST = (1ll << 31) - (1 << 20);
+  int64_t at = sums[threadIdx.x] - own;
+  for (int s = s0; s < s1; ++s) {
+    before[s] = (int)(at < MOST ? at : MOST);
+    at += (load_sequence(a, s).q_len + tile_tokens - 1) / tile_tokens;
+  }
+  if (threadIdx.x == 1023) before[a.n] = (int)(sums[1023] < MOST ? sums[1023] : MOST);
+}
+
 int check_heads(const char* who, int64_t H, int64_t KV, int64_t D) {
   TB200_REQUIRE(H > 0 && KV > 0 && H % KV == 0, TB200_ERR_INVALID, "%s: %lld query heads are no multiple of %lld key heads",
                 who, (long long)H, (long long)KV);
@@ -132,7 +156,13 @@ struct PagedPlan {
   bool tc = false;
   bool few = false;  // the kernel for few rows
   int row_tile = 0, key_tile = 0, row_tokens = 0;
+  bool list = false;  // row tiles are listed on the device first
 };
+// As many row tiles are planned for each sequence as the longest announced one has. Where most of them would be empty
+// (no length announced, or one long chunk among many sequences) they are listed first: a launch of 2 us, and a search
+// for each tile. n sequences of 64 tokens, not announced, 8 x 4 heads, D = 128, bf16: 8 sequences (3 empty tiles an SM)
+// 31 us listed and 29 not, 16 (13 an SM) 33 and 35, 64 (218) 101 and 198, 128 (880) 169 and 609.
+constexpr int64_t LIST_FROM = 8;  // empty tiles an SM
 PagedPlan plan_paged(LocalArgs* a, int64_t max_q, int64_t max_ctx, bool tc) {
   PagedPlan p;
   p.tc = tc;
@@ -141,9 +171,14 @@ PagedPlan plan_paged(LocalArgs* a, int64_t max_q, int64_t max_ctx, bool tc) {
   p.key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
   p.row_tokens = p.few || !tc ? p.row_tile / a->G : local_tc_row_tokens(*a);
   plan_split(a, max_q, max_ctx, p.row_tile, p.key_tile, (int64_t)sm_count() * (p.few ? 8 : 4));
+  if (a->starts && !p.few && a->split_tiles == 0) {
+    const int64_t planned = a->n * ceil_div(max_q, p.row_tokens), most = a->tokens / p.row_tokens + a->n;  // (per key head)
+    p.list = (planned - most) * a->KV > LIST_FROM * sm_count();
+  }
   return p;
 }
-size_t split_bytes(const LocalArgs& a) {
+size_t paged_bytes(const LocalArgs& a, const PagedPlan& p) {
+  if (p.list) return (size_t)(a.n + 1) * sizeof(int);
   return a.split_tiles == 0 ? 0 : (size_t)a.splits * a.tokens * a.H * (a.D + 1) * sizeof(float);
 }
 
@@ -266,9 +301,8 @@ extern "C" size_t tb200_paged_attention_workspace(int64_t T, int64_t n, int64_t 
   if (max_q <= 0) return 0;
   // (which kernel family takes the call depends on strides and alignment: enough for either)
   LocalArgs b = a;
-  plan_paged(&a, max_q, max_context_length, false);
-  plan_paged(&b, max_q, max_context_length, true);
-  return split_bytes(a) > split_bytes(b) ? split_bytes(a) : split_bytes(b);
+  const PagedPlan simt = plan_paged(&a, max_q, max_context_length, false), tc = plan_paged(&b, max_q, max_context_length, true);
+  return paged_bytes(a, simt) > paged_bytes(b, tc) ? paged_bytes(a, simt) : paged_bytes(b, tc);
 }
 
 extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_cache, const void* value_cache,
@@ -301,8 +335,14 @@ extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_c
   const int max_q = (int)(max_query_length < T ? max_query_length : T);
   a.max_q = max_q;
   const PagedPlan plan = plan_paged(&a, max_q, max_context_length, local_tc_supported(a, dtype, q, key_cache, value_cache, out));
-  TB200_REQUIRE(workspace_bytes >= split_bytes(a) && (workspace || a.split_tiles == 0), TB200_ERR_WORKSPACE,
-                "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, split_bytes(a));
+  const size_t need = paged_bytes(a, plan);
+  TB200_REQUIRE(workspace_bytes >= need && (workspace || need == 0), TB200_ERR_WORKSPACE,
+                "paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (plan.list) {
+    list_tiles<<<1, 1024, 0, st>>>((int*)workspace, a, plan.row_tokens);
+    if (int rc = launch_status("list_tiles")) return rc;
+    a.before = (const int*)workspace;
+  }
   a.part_out = (float*)workspace;
   a.part_lse = a.part_out + (size_t)a.splits * a.tokens * a.H * a.D;
   int rc = plan.few ? launch_local_few_tc(out, q, key_cache, value_cache, a, dtype, st)
@@ -311,7 +351,7 @@ extern "C" int tb200_paged_attention(void* out, const void* q, const void* key_c
   if (rc) return rc;
   if (a.split_tiles > 0)
     if ((rc = launch_local_combine(out, a, max_q, plan.row_tokens, plan.key_tile, dtype, st))) return rc;
-  note_kernel(plan.tc ? "local_tcgen05" : "local_simt", a.split_tiles > 0 ? 2 : 1);
+  note_kernel(plan.tc ? "local_tcgen05" : "local_simt", a.split_tiles > 0 || plan.list ? 2 : 1);
   return 0;
 }
 

@@ -41,6 +41,8 @@ struct LocalArgs {
   int split_tiles = 0, splits = 1;
   float* part_out = nullptr;     // [splits][tokens * H][D]
   float* part_lse = nullptr;     // [splits][tokens * H]
+  // list form: row tiles (units of work) of the sequences before s, [n + 1]; null: as many for each as for the longest
+  const int* before = nullptr;
   int zero_rest = 0;             // rows that are not computed (of no sequence, beyond max_q) are set to zero
   int* status = nullptr;
 };
@@ -119,6 +121,18 @@ template <typename T>
 __device__ inline void zero_rest_of(T* out, const LocalArgs& a, int s, const Sequence& seq, int part, int parts) {
   if (s == 0) zero_rows(out, a, 0, seq.q_begin, part, parts, threadIdx.x, blockDim.x);
   zero_rows(out, a, (int64_t)seq.q_begin + seq.q_len, s == a.n - 1 ? a.tokens : seq.q_end, part, parts, threadIdx.x, blockDim.x);
+}
+
+// Sequence and row tile of number `tile` (below before[n]) of the list form.
+__device__ inline void listed_tile(const LocalArgs& a, int tile, int* s, int* t) {
+  int lo = 0, hi = a.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.before[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  *s = lo;
+  *t = tile - a.before[lo];
 }
 
 // Key tiles of the walk that split `s` of a row tile takes.

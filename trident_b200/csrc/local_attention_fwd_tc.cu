@@ -53,6 +53,7 @@ constexpr int REGS_LAUNCH = 168, REGS_SERVICE = 72, REGS_SOFTMAX = 216;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float RESCALE_THRESHOLD = 8.f;
+constexpr int64_t MOST_UNITS = (1ll << 31) - (1 << 20);
 
 struct FwdParams {
   LocalArgs a;
@@ -158,15 +159,23 @@ struct Walk {
 template <bool PAGED>
 __device__ inline bool unit_at(const FwdParams& p, int unit, Unit* w) {
   const LocalArgs& a = p.a;
-  const int high = p.outer.quotient(unit), rest = unit - high * (int)p.outer.d;
-  // Walks of a training step grow with the tile up to the window: longest first (3 sequences of 1111 tokens, 2 key
-  // heads: 18.8 us by sequence and head, 17.1 so; 2 of 4096, 8 key heads: 169 and 170). Those of chunks hardly
-  // grow, and their last tiles may be empty.
-  const int pair = PAGED ? high : p.pairs - 1 - high;
-  const int sequence_part = p.kv.quotient(rest);
-  w->hk = rest - sequence_part * a.KV;
-  w->s = p.splits.quotient(sequence_part);
-  w->split = sequence_part - w->s * a.splits;
+  int pair;
+  if (PAGED && a.before) {
+    const int tile = p.kv.quotient(unit);
+    w->hk = unit - tile * a.KV;
+    w->split = 0;
+    listed_tile(a, tile, &w->s, &pair);
+  } else {
+    const int high = p.outer.quotient(unit), rest = unit - high * (int)p.outer.d;
+    // Walks of a training step grow with the tile up to the window: longest first (3 sequences of 1111 tokens, 2 key
+    // heads: 18.8 us by sequence and head, 17.1 so; 2 of 4096, 8 key heads: 169 and 170). Those of chunks hardly
+    // grow, and their last tiles may be empty.
+    pair = PAGED ? high : p.pairs - 1 - high;
+    const int sequence_part = p.kv.quotient(rest);
+    w->hk = rest - sequence_part * a.KV;
+    w->s = p.splits.quotient(sequence_part);
+    w->split = sequence_part - w->s * a.splits;
+  }
   w->seq = load_sequence(a, w->s);
   w->t0 = pair * 2 * p.tile_tokens;
   if (w->t0 >= w->seq.q_len) return false;
@@ -294,6 +303,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   static_assert(REGS_LAUNCH * FWD_THREADS <= 65536, "launch allocation");
   static_assert(4 * 32 * REGS_SERVICE + 8 * 32 * REGS_SOFTMAX <= REGS_LAUNCH * FWD_THREADS,
                 "register pool of the CTA exceeded: setmaxnreg.inc would never return");
+  int units = p.units;
+  if (PAGED && a.before) {
+    const int64_t listed = (int64_t)a.before[a.n] * a.KV;
+    units = (int)(listed < MOST_UNITS ? listed : MOST_UNITS);
+  }
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_SERVICE));
     if (warp == 0) {
@@ -305,7 +319,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                                               // of that completion (of v_raw)
       bool stop = false;                      // a wait has run out: nothing more is brought
       auto stopped = [&]() { return __shfl_sync(0xffffffffu, lane == 0 ? abort_flag[0] : 0u, 0) != 0; };
-      for (int unit = blockIdx.x; unit < p.units && !stop; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < units && !stop; unit += gridDim.x) {
         Unit w;
         if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
         const bool fix = needs_fix(w);
@@ -525,7 +539,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       // -------------------------------------------------------------- output tiles (one lane)
       if (lane == 0) {
         int outs = 0;
-        for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
           Unit w;
           if (abort_flag[0]) break;
           if (!unit_at<PAGED>(p, unit, &w)) continue;
@@ -575,7 +589,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         if (lane == 0) ptx::mbar_arrive(&v_full[st]);
       };
       int fix_keys = 0;  // of the unit before
-      for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
         Unit w;
         if (__any_sync(0xffffffffu, abort_flag[0] != 0)) break;
         if (!unit_at<PAGED>(p, unit, &w) || w.m1 <= w.m0) continue;
@@ -626,10 +640,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     int count = 0, outs = 0;  // steps of this tile, output tiles of both (over all units of the CTA)
     Unit w;
     auto next_unit = [&](int unit) {  // the first from `unit` on that has something to do
-      while (unit < p.units && !unit_at<PAGED>(p, unit, &w)) unit += gridDim.x;
+      while (unit < units && !unit_at<PAGED>(p, unit, &w)) unit += gridDim.x;
       return unit;
     };
-    for (int unit = next_unit(blockIdx.x); unit < p.units;) {
+    for (int unit = next_unit(blockIdx.x); unit < units;) {
       if (__any_sync(0xffffffffu, abort_flag[0] != 0)) break;
       const int first_token = w.t0 + t * p.tile_tokens;
       const int tokens = min(p.tile_tokens, w.seq.q_len - first_token);
@@ -1016,9 +1030,9 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   p.piece = local_piece(a);
   p.pairs = (int)ceil_div(max_q, 2 * p.tile_tokens);
   const int64_t units = (int64_t)p.pairs * a.KV * a.n * a.splits;
-  TB200_REQUIRE(units < (1ll << 31) - (1 << 20), TB200_ERR_UNSUPPORTED, "local_fwd_tc: %lld units of work", (long long)units);
-  p.units = (int)units;
-  p.outer = Divisor(p.units / p.pairs);
+  TB200_REQUIRE(a.before || units < MOST_UNITS, TB200_ERR_UNSUPPORTED, "local_fwd_tc: %lld units of work", (long long)units);
+  p.units = (int)(units < MOST_UNITS ? units : MOST_UNITS);  // (list form: the kernel finds the number)
+  p.outer = Divisor(a.before ? 1 : p.units / p.pairs);
   p.kv = Divisor(a.KV);
   p.splits = Divisor(a.splits);
   p.test = WaitTest::of_this_thread(1, 1);

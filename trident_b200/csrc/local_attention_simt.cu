@@ -189,11 +189,26 @@ __global__ void __launch_bounds__(Shape<D, RM, KEY_TILE, TX>::THREADS)
   float* sp = D >= 64 ? sk : sv + KEY_TILE * LD;
 
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
-  const int s = blockIdx.z / a.splits, split = blockIdx.z % a.splits, hk = blockIdx.y;
+  int s = blockIdx.z / a.splits, tile = blockIdx.x;
+  const int split = blockIdx.z % a.splits, hk = blockIdx.y;
+  if (a.before == nullptr) {
+    if (a.zero_rest && hk == 0 && split == 0) zero_rest_of(out, a, s, load_sequence(a, s), blockIdx.x, gridDim.x);
+  } else {
+    const bool zero = a.zero_rest && hk == 0;
+    if (zero) {
+      zero_rows(out, a, 0, load_sequence(a, 0).q_begin, blockIdx.x, gridDim.x, threadIdx.x, THREADS);
+      zero_rows(out, a, load_sequence(a, a.n - 1).q_end, a.tokens, blockIdx.x, gridDim.x, threadIdx.x, THREADS);
+    }
+    if (tile >= a.before[a.n]) return;
+    listed_tile(a, tile, &s, &tile);
+    if (zero) {  // (a sequence with rows beyond max_q has tiles)
+      const Sequence seq = load_sequence(a, s);
+      zero_rows(out, a, (int64_t)seq.q_begin + seq.q_len, seq.q_end, tile, a.before[s + 1] - a.before[s], threadIdx.x, THREADS);
+    }
+  }
   const Sequence sq_ = load_sequence(a, s);
-  if (a.zero_rest && hk == 0 && split == 0) zero_rest_of(out, a, s, sq_, blockIdx.x, gridDim.x);
   // the packed rows of this tile: row r is token r / G of the tile, head r % G of the group
-  const int tile_tokens = RM / a.G, t0 = blockIdx.x * tile_tokens;
+  const int tile_tokens = RM / a.G, t0 = tile * tile_tokens;
   const int ntok = min(tile_tokens, sq_.q_len - t0);
   if (ntok <= 0) return;
   const int base = sq_.base;
@@ -590,7 +605,9 @@ int launch_fwd(T* out, float* lse, const T* q, const T* k, const T* v, const Loc
   static std::atomic<unsigned long long> done{0};
   if (int rc = optin(kern, SMEM, done, "local_fwd_simt")) return rc;
   const int qvec = rows_vectorised<T>(q, a.qs), kvec = rows_vectorised<T>(k, a.ks) && rows_vectorised<T>(v, a.vs);
-  const dim3 grid((unsigned)ceil_div(max_q, RM / a.G), (unsigned)a.KV, (unsigned)(a.n * a.splits));
+  // (list form: no sequence has more tiles than its tokens fill, and one that is not full)
+  const int64_t tiles = a.before ? a.tokens / (RM / a.G) + a.n : ceil_div(max_q, RM / a.G);
+  const dim3 grid((unsigned)tiles, (unsigned)a.KV, (unsigned)(a.before ? 1 : a.n * a.splits));
   kern<<<grid, Sh::THREADS, SMEM, st>>>(out, lse, q, k, v, a, qvec, kvec);
   return launch_status("local_fwd_simt");
 }
