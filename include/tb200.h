@@ -260,14 +260,20 @@ int tb200_attention_bwd(void* dq, void* dk, void* dv, void* dmask /*nullable*/,
  * (the first `sinks` tokens stay visible). q, out: [B,H,S,D]; k, v: [B,KV,S,D], H a multiple of KV
  * (at most 64 times): query head h uses key head h / (H / KV). All with element strides (4 each).
  * lse [B,H,S]: natural-log sum of exponentials of a score row (float32), kept for backward; null: not written. Keys and
- * values have to be finite: a NaN or infinity may reach queries near it that do not see it. */
+ * values have to be finite: a NaN or infinity may reach queries near it that do not see it.
+ * The form with out_low (nullable; 16-bit types) also writes out minus its rounded value there, in the type and strides
+ * of out, for a backward pass whose delta = sum out dout is not off by out's rounding. */
 int tb200_window_attention_fwd(void* out, float* lse, const void* q, const void* k, const void* v, int64_t B,
                                int64_t H, int64_t KV, int64_t S, int64_t D, const int64_t* q_strides,
                                const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
                                int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream);
+int tb200_window_attention_fwd_low(void* out, void* out_low, float* lse, const void* q, const void* k, const void* v,
+                                   int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D, const int64_t* q_strides,
+                                   const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
+                                   int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream);
 /* dq [B,H,S,D], dk, dv [B,KV,S,D] (summed over the query heads of a key head) from dout. No atomics:
  * the same inputs give the same bits. The workspace (16-byte aligned) holds a float per score row and
- * the parts of the sinks' gradients. */
+ * the parts of the sinks' gradients. out_low (nullable) is that of the forward pass. */
 size_t tb200_window_attention_bwd_workspace(int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D, int64_t window,
                                             int64_t sinks, int dtype);
 int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k,
@@ -277,6 +283,13 @@ int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const void* dout, c
                                const int64_t* out_strides, const int64_t* dout_strides, const int64_t* dq_strides,
                                const int64_t* dk_strides, const int64_t* dv_strides, int64_t window, int64_t sinks,
                                float softmax_scale, int dtype, void* stream);
+int tb200_window_attention_bwd_low(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k,
+                                   const void* v, const void* out, const void* out_low, const float* lse,
+                                   void* workspace, size_t workspace_bytes, int64_t B, int64_t H, int64_t KV, int64_t S,
+                                   int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                                   const int64_t* v_strides, const int64_t* out_strides, const int64_t* dout_strides,
+                                   const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
+                                   int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream);
 
 /* ---- Paged attention (not in the reference) --------------------------------
  * Keys and values of n sequences lie in pages of a pool, key_cache and value_cache
@@ -332,11 +345,11 @@ int tb200_device_status(int reset);
  * keep their own. Returns the old value. */
 int tb200_set_norm_fused_finalize(int on);
 /* Test hook of the calling thread for the bounded waits of the tensor-core and bulk-copy kernels. mode 1: the launches
- * this thread makes next of the attention forward, the window attention forward, paged attention, the first kernel of the
- * window attention backward (dQ) and the gated residual RMSNorm backward run with a wait limit of about a
+ * this thread makes next of the attention forward, the window attention forward, paged attention, the dQ kernel of the
+ * window attention backward and the gated residual RMSNorm backward run with a wait limit of about a
  * millisecond, and the producer of their first CTA leaves out one copy, so one wait runs out: the launch must still
  * complete, free its tensor memory and leave a non-zero code in the device status word (tb200_device_status); its
- * output is invalid. mode 2: the same for the second kernel of the window attention backward (dK, dV). mode 0: normal
+ * output is invalid. mode 2: the same for the dK, dV kernel of the window attention backward. mode 0: normal
  * operation. Returns the old mode. No memory is touched that a normal launch would not touch. */
 int tb200_test_wait_fault(int mode);
 

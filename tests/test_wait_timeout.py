@@ -49,7 +49,7 @@ def test_expired_wait_sets_the_status_word_and_the_context_stays_usable(device):
 
 
 # ------------------------------------------------------------------ window and paged attention, norms between blocks
-# (the hook's mode 1 means the first kernel of a call, mode 2 the second of the window attention backward)
+# (the hook's mode 1 means the kernel of a call, of the window attention backward that of dQ, mode 2 that of dK, dV)
 def _expires(call, outputs, mode, kernel):
     """`call` fills `outputs`: right, then with a wait that runs out, then right again, to the bit."""
     _lib.device_status(reset=True)

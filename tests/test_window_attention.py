@@ -414,3 +414,25 @@ def test_error_of_long_sums(D, device):
     most = (g.clamp(min=0) @ k)  # P
     off = ((got - g @ k) / most).square().mean().sqrt().item() / 2.0 ** -24
     assert off < (n / 64) ** 0.5 + 40, off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("KV, G", [(4, 1), (2, 3), (2, 4)])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_error_of_short_windows(D, KV, G, dt, device):
+    """The score gradients of a row sum to zero: what delta = sum out dout is off by goes to dq as a common part of them
+    times the sum of p k, the more the shorter the window is. With delta of the unrounded output the roundings of the
+    score gradients (an operand of the tensor cores: not at D = 32) and of dq itself remain. A rounding is off by at most
+    half a step of 2 u of its value, spread over it evenly by 2 u / sqrt(12) in the mean, and less for mantissas
+    above 1; the two of them by sqrt(2) times that. (delta of the rounded output: 0.0044 at a window of 2 in bf16.)"""
+    u = torch.finfo(dt).eps / 2
+    bound = 2 * u / 12 ** 0.5 * (2 ** 0.5 if D >= 64 else 1.0)
+    for window in (2, 3):
+        problem = _problem(2, KV, G, 900, D, dt, seed=95)
+        want = ref.batched(*problem[:3], window, 0, D ** -0.5, dt, problem[3])
+        got = _run(problem, window, 0, device)
+        for name in ("dq", "dk"):
+            value = want[name][0]
+            off = ((got[name].double().cpu() - value).norm() / value.norm()).item()
+            assert off < bound, (window, name, off, bound)

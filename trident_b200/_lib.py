@@ -75,6 +75,14 @@ SIGNATURES = {
         c_int,
         [c_ptr] * 10 + [c_size] + [c_i64] * 5 + [c_ptr] * 8 + [c_i64] * 2 + [c_f32, c_int, c_ptr],
     ),
+    "tb200_window_attention_fwd_low": (
+        c_int,
+        [c_ptr] * 6 + [c_i64] * 5 + [c_ptr] * 4 + [c_i64] * 2 + [c_f32, c_int, c_ptr],
+    ),
+    "tb200_window_attention_bwd_low": (
+        c_int,
+        [c_ptr] * 11 + [c_size] + [c_i64] * 5 + [c_ptr] * 8 + [c_i64] * 2 + [c_f32, c_int, c_ptr],
+    ),
     "tb200_paged_attention_workspace": (c_size, [c_i64] * 9 + [c_int]),
     "tb200_paged_attention": (
         c_int,
@@ -532,10 +540,11 @@ def attention_bwd(dq, dk, dv, dmask, dout, q, k, v, out, lse, mask, workspace, i
     )
 
 
-def window_attention_fwd(out, lse, q, k, v, window, sinks, scale):
+def window_attention_fwd(out, lse, q, k, v, window, sinks, scale, low=None):
+    """low: laid out as out, or None."""
     B, H, S, D = q.shape
     _call(
-        "tb200_window_attention_fwd", q, _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), B, H, k.shape[1], S, D,
+        "tb200_window_attention_fwd_low", q, _ptr(out), _ptr(low), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), B, H, k.shape[1], S, D,
         q.stride(), k.stride(), v.stride(), out.stride(), window, sinks, scale, dtype_code(q.dtype),
     )
 
@@ -548,11 +557,11 @@ def window_attention_bwd_workspace(q, k, window, sinks):
     )
 
 
-def window_attention_bwd(dq, dk, dv, dout, q, k, v, out, lse, workspace, window, sinks, scale):
+def window_attention_bwd(dq, dk, dv, dout, q, k, v, out, lse, workspace, window, sinks, scale, low=None):
     B, H, S, D = q.shape
     _call(
-        "tb200_window_attention_bwd", q, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(q), _ptr(k), _ptr(v),
-        _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel(), B, H, k.shape[1], S, D, q.stride(), k.stride(),
+        "tb200_window_attention_bwd_low", q, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(q), _ptr(k), _ptr(v),
+        _ptr(out), _ptr(low), _ptr(lse), _ptr(workspace), workspace.numel(), B, H, k.shape[1], S, D, q.stride(), k.stride(),
         v.stride(), out.stride(), dout.stride(), dq.stride(), dk.stride(), dv.stride(), window, sinks,
         scale, dtype_code(q.dtype),
     )

@@ -134,6 +134,37 @@ static PyObject* window_attention_bwd(PyObject* self, PyObject* const* args, Py_
                                   s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], window, sinks, scale, dtype, stream));
 }
 
+static PyObject* window_attention_fwd_low(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  BEGIN;
+  void *out = pointer(&a), *low = pointer(&a), *lse = pointer(&a), *q = pointer(&a), *k = pointer(&a), *v = pointer(&a);
+  int64_t d[5], s[4][4];
+  for (int i = 0; i < 5; ++i) d[i] = integer(&a);
+  for (int i = 0; i < 4; ++i) strides(&a, s[i], 4);
+  int64_t window = integer(&a), sinks = integer(&a);
+  float scale = real(&a);
+  int dtype = (int)integer(&a);
+  void* stream = pointer(&a);
+  CALL(tb200_window_attention_fwd_low(out, low, lse, q, k, v, d[0], d[1], d[2], d[3], d[4], s[0], s[1], s[2], s[3], window, sinks,
+                                      scale, dtype, stream));
+}
+
+static PyObject* window_attention_bwd_low(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  BEGIN;
+  void* p[11];
+  for (int i = 0; i < 11; ++i) p[i] = pointer(&a);
+  size_t bytes = (size_t)integer(&a);
+  int64_t d[5], s[8][4];
+  for (int i = 0; i < 5; ++i) d[i] = integer(&a);
+  for (int i = 0; i < 8; ++i) strides(&a, s[i], 4);
+  int64_t window = integer(&a), sinks = integer(&a);
+  float scale = real(&a);
+  int dtype = (int)integer(&a);
+  void* stream = pointer(&a);
+  CALL(tb200_window_attention_bwd_low(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], bytes, d[0], d[1], d[2],
+                                      d[3], d[4], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], window, sinks, scale, dtype,
+                                      stream));
+}
+
 static PyObject* paged_attention(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   BEGIN;
   void* p[8];
@@ -172,7 +203,8 @@ static PyObject* paged_cache_append(PyObject* self, PyObject* const* args, Py_ss
 #define METHOD(name) {"tb200_" #name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {
     METHOD(gated_residual_rms_norm_fwd), METHOD(gated_residual_rms_norm_bwd), METHOD(window_attention_fwd),
-    METHOD(window_attention_bwd),        METHOD(paged_attention),             METHOD(paged_cache_append),
+    METHOD(window_attention_bwd),        METHOD(window_attention_fwd_low),    METHOD(window_attention_bwd_low),
+    METHOD(paged_attention),             METHOD(paged_cache_append),
     {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__fastcall(void) { return PyModule_Create(&module); }

@@ -490,11 +490,10 @@ extern "C" int tb200_device_status(int reset) {
 }
 
 // Test hook of the calling thread. mode 1: the next launches of this thread of the attention and window attention
-// forward, paged attention, the first kernel of the window attention backward (dQ) or the gated residual RMSNorm
-// backward run with a wait limit of about one millisecond, and the producer of the first CTA leaves out one copy into
+// forward, paged attention, the dQ kernel of the window attention backward or the gated residual RMSNorm backward run with a wait limit of about one millisecond, and the producer of the first CTA leaves out one copy into
 // shared memory (it touches no memory it would not otherwise touch), so that the wait for it runs out: the
 // kernel must still end, free its tensor memory and leave a non-zero code in the device status word. mode 2: the
-// second kernel of the window attention backward (dK, dV). mode 0: normal operation. Returns the old mode.
+// dK, dV kernel of the window attention backward. mode 0: normal operation. Returns the old mode.
 extern "C" int tb200_test_wait_fault(int mode) {
   const int old = tb200::g_test_wait_fault;
   tb200::g_test_wait_fault = mode;

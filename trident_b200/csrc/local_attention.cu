@@ -220,13 +220,23 @@ extern "C" int tb200_window_attention_fwd(void* out, float* lse, const void* q, 
                                           int64_t H, int64_t KV, int64_t S, int64_t D, const int64_t* q_strides,
                                           const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
                                           int64_t window, int64_t sinks, float softmax_scale, int dtype, void* stream) {
+  return tb200_window_attention_fwd_low(out, nullptr, lse, q, k, v, B, H, KV, S, D, q_strides, k_strides, v_strides, out_strides,
+                                        window, sinks, softmax_scale, dtype, stream);
+}
+
+extern "C" int tb200_window_attention_fwd_low(void* out, void* out_low, float* lse, const void* q, const void* k, const void* v,
+                                              int64_t B, int64_t H, int64_t KV, int64_t S, int64_t D,
+                                              const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                              const int64_t* out_strides, int64_t window, int64_t sinks, float softmax_scale,
+                                              int dtype, void* stream) {
   LocalArgs a;
   if (int rc = fill_window(&a, "window_attention_fwd", B, H, KV, S, D, q_strides, k_strides, v_strides, out_strides, window,
                            sinks, softmax_scale))
     return rc;
   if (B == 0 || S == 0) return 0;
   TB200_REQUIRE(out && q && k && v, TB200_ERR_INVALID, "window_attention_fwd: null pointer");
-  const bool tc = local_tc_supported(a, dtype, q, k, v, out);
+  a.low = dtype == TB200_F32 ? nullptr : out_low;
+  const bool tc = local_tc_supported(a, dtype, q, k, v, out) && (!a.low || aligned16(a.low));
   int rc = tc ? launch_local_fwd_tc(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream)
               : launch_local_fwd_simt(out, lse, q, k, v, a, (int)S, dtype, (cudaStream_t)stream);
   if (rc == 0) note_kernel(tc ? "local_tcgen05" : "local_simt", 1);
@@ -252,6 +262,19 @@ extern "C" int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const vo
                                           const int64_t* dq_strides, const int64_t* dk_strides,
                                           const int64_t* dv_strides, int64_t window, int64_t sinks, float softmax_scale,
                                           int dtype, void* stream) {
+  return tb200_window_attention_bwd_low(dq, dk, dv, dout, q, k, v, out, nullptr, lse, workspace, workspace_bytes, B, H, KV, S, D,
+                                        q_strides, k_strides, v_strides, out_strides, dout_strides, dq_strides, dk_strides,
+                                        dv_strides, window, sinks, softmax_scale, dtype, stream);
+}
+
+extern "C" int tb200_window_attention_bwd_low(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k,
+                                              const void* v, const void* out, const void* out_low, const float* lse,
+                                              void* workspace, size_t workspace_bytes, int64_t B, int64_t H, int64_t KV,
+                                              int64_t S, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                                              const int64_t* v_strides, const int64_t* out_strides,
+                                              const int64_t* dout_strides, const int64_t* dq_strides,
+                                              const int64_t* dk_strides, const int64_t* dv_strides, int64_t window,
+                                              int64_t sinks, float softmax_scale, int dtype, void* stream) {
   LocalBwdArgs b;
   if (int rc = fill_window(&b.f, "window_attention_bwd", B, H, KV, S, D, q_strides, k_strides, v_strides, out_strides, window,
                            sinks, softmax_scale))
@@ -263,7 +286,8 @@ extern "C" int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const vo
                 "window_attention_bwd: null pointer");
   copy4(b.dos, dout_strides); copy4(b.dqs, dq_strides); copy4(b.dks, dk_strides); copy4(b.dvs, dv_strides);
   cudaStream_t st = (cudaStream_t)stream;
-  const bool tc = local_bwd_tc_supported(b, dtype, q, k, v, out, dout, dq, dk, dv);
+  b.f.low = dtype == TB200_F32 ? nullptr : const_cast<void*>(out_low);
+  const bool tc = local_bwd_tc_supported(b, dtype, q, k, v, out, dout, dq, dk, dv) && (!b.f.low || aligned16(b.f.low));
   const int key_tile = tc ? LOCAL_TC_TILE : local_simt_key_tile();
   const size_t need = bwd_bytes(b, tc);
   plan_far(&b, key_tile);
@@ -278,7 +302,7 @@ extern "C" int tb200_window_attention_bwd(void* dq, void* dk, void* dv, const vo
     if (int rc = launch_local_delta(row_scratch, out, dout, b.dos, b.f, dtype, st)) return rc;
     if (int rc = launch_local_bwd_simt(dq, dk, dv, dout, q, k, v, lse, row_scratch, b, dtype, st)) return rc;
   }
-  int launches = tc ? 2 : 3;
+  int launches = 3;
   if (b.sink_tiles > 0) {
     if (int rc = launch_local_far_sum(dk, dv, b, key_tile, dtype, st)) return rc;
     ++launches;

@@ -45,6 +45,8 @@ struct LocalArgs {
   const int* before = nullptr;
   int zero_rest = 0;             // rows that are not computed (of no sequence, beyond max_q) are set to zero
   int* status = nullptr;
+  // training form, 16-bit operands: what the rounding of out leaves, in the same type and layout; null: not kept
+  void* low = nullptr;
 };
 
 // New tokens [q_begin, q_begin + q_len) of a sequence that are computed, the end of all that it has, the position of

@@ -2,7 +2,7 @@
 //
 // Two kernels, each of which owns what it sums, so that nothing is added with atomics and the same inputs
 // give the same bits (one kernel for all three gradients would need 5 products a tile pair instead of 7,
-// but has to add dQ across CTAs):
+// but has to add dQ across CTAs), behind one over the rows (local_rows_tc_kernel):
 //
 //   dQ      tiles of 128 packed query rows (token * G + head); a persistent CTA takes every gridDim-th of
 //           them. Q and dO of the tile are put into tensor memory as operands (their products then read only
@@ -10,8 +10,7 @@
 //           took the pipe 120 cycles an instruction instead of 64); along the keys of the tile's walk
 //             S = Q K^T, dP = dO V^T, P = exp2(S scale log2e - lse log2e), dS = P (dP - delta), dQ += dS K
 //           (dS 16-bit in tensor memory over dP). S(i+1) is computed as soon as S(i) is in registers, dP(i+1)
-//           after dQ(i), so that exponentials and score gradients follow each other without a pause. Two
-//           more warps compute delta = sum_d out dout of the next tile, also for the other kernel.
+//           after dQ(i), so that exponentials and score gradients follow each other without a pause.
 //   dK, dV  a CTA owns 128 keys (K_j, V_j resident in shared memory) and walks the tiles of 96 packed query
 //           rows that see any of them; the sum over the heads of a group is part of the walk. All
 //           transposed, keys on the tensor-memory lanes:
@@ -24,13 +23,14 @@
 // about as long as a walk inside the window, each a CTA of its own: a single CTA would walk all queries.
 //
 // P and dS are rounded to 16 bits as operands of their products, as the tensor cores take them: half a step each
-// (2-norm of the error of dq against 64 bits 0.0026 in bf16, 0.00033 in fp16, of which the final rounding alone is
-// 0.0017 and 0.00021). Statistics, delta and all sums are fp32.
+// (2-norm of the error of dq against 64 bits 0.0024 in bf16, 0.00031 in fp16 at any window, of which the final rounding
+// alone is 0.0017 and 0.00021; with delta of the rounded output it was 0.0026 at a window of 1024 and 0.0044 at 2).
+// fp16 score gradients below 2^-14 are multiples of 2^-24. Statistics, delta and all sums are fp32.
 //
 // Bounds, at 2 x 32 heads x 4096 x 128 bf16, window 1024, 8 key heads. dK, dV: 252 us (957 TFLOP/s); a step takes
 // 2350 cycles, of which the products alone, two of them with both operands in shared memory, take about 2200 (dS^T
 // over P^T instead of dP^T, so that the next dP^T need not wait for dK: 302 us, one chain of all four products). dQ:
-// 184 us (983 TFLOP/s); a step takes 2050 cycles, the chain dQ -> dP -> score gradients (1536 of products).
+// 180 us (1008 TFLOP/s); a step takes 2050 cycles, the chain dQ -> dP -> score gradients (1536 of products).
 #include <type_traits>
 
 #include "attn_math.cuh"
@@ -49,7 +49,7 @@ struct BwdParams {
   LocalBwdArgs b;
   void *dk, *dv;
   const float* lse;
-  float* nlse2;         // [n * KV][column tiles][96]  -lse * log2(e), written by the dQ kernel for the other
+  float* nlse2;         // [n * KV][column tiles][96]  -lse * log2(e), written by the kernel of the rows
   float* ndelta;        // [n * KV][column tiles][96]  -delta
   float scale_log2;
   int tile_tokens;      // tokens of a row tile (dQ)
@@ -87,6 +87,62 @@ __device__ inline void zero_rows(uint8_t* smem, int boxes, int rows) {
   const int per_box = (COLS - rows) * 8;  // 16-byte chunks
   for (int i = threadIdx.x; i < boxes * per_box; i += THREADS)
     *reinterpret_cast<uint4*>(smem + (i / per_box) * (COLS * 128) + rows * 128 + (i % per_box) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// ------------------------------------------------------------------ -lse log2e, -delta
+// Of all packed rows, in the order in which the other kernels read them (entries of column tiles that belong to no row:
+// zeros; the products that meet them see rows of zeros). delta = sum_d out dout in fp32, of the output before its
+// rounding where what that left was kept (LocalArgs::low): the score gradients of a row sum to zero, and an error of delta
+// goes to dq as a common part of them times sum p k, which does not average out over a short window. Bounded by HBM:
+// reads out, low and dout once (2 x 32 heads x 4096 x 128: 201 MB, 36 us, 5.5 TB/s; two warps of the dQ
+// kernel, which did this before for out alone, were 85 us slower with low: a row's loads there are not under way together).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) local_rows_tc_kernel(const T* out, const T* dout, const BwdParams p) {
+  constexpr int LANES = D / 8, ROWS = 32 / LANES, AHEAD = 4, EACH = 16;  // lanes and rows of a load; rows of a warp
+  const LocalArgs& a = p.b.f;
+  const T* low = reinterpret_cast<const T*>(a.low);
+  const int lane = threadIdx.x & 31, sub = lane / LANES, at = lane % LANES * 8;
+  const int64_t warp = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), row0 = warp * EACH;
+  static_assert(COLS % EACH == 0 && EACH % (ROWS * AHEAD) == 0, "a column tile is a whole number of warps");
+  const int64_t tile = row0 / COLS;
+  if (tile >= (int64_t)a.n * a.KV * p.col_tiles) return;
+  const int it = (int)(tile % p.col_tiles), sh = (int)(tile / p.col_tiles), hk = sh % a.KV, s = sh / a.KV;
+#pragma unroll
+  for (int b = 0; b < EACH; b += ROWS * AHEAD) {
+    uint4 o[AHEAD], l[AHEAD], g[AHEAD];
+    float lse[AHEAD];
+    bool live[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int c = (int)(row0 % COLS) + b + k * ROWS + sub, t = it * p.col_tokens + c / a.G, h = hk * a.G + c % a.G;
+      live[k] = c < p.col_tokens * a.G && t < a.tokens;
+      o[k] = l[k] = g[k] = make_uint4(0, 0, 0, 0);
+      lse[k] = 0.f;
+      if (live[k]) {
+        const int64_t from = (int64_t)s * a.os[0] + (int64_t)h * a.os[1] + (int64_t)t * a.os[2] + at;
+        o[k] = ld_stream(out + from);
+        if (low) l[k] = ld_stream(low + from);
+        g[k] = *reinterpret_cast<const uint4*>(dout + (int64_t)s * p.b.dos[0] + (int64_t)h * p.b.dos[1] + (int64_t)t * p.b.dos[2] + at);
+        lse[k] = p.lse[((int64_t)s * a.H + h) * a.tokens + t];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      float x[8], y[8], z[8], sum = 0.f;
+      unpack<T>(o[k], x);
+      unpack<T>(l[k], y);
+      unpack<T>(g[k], z);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(x[e] + y[e], z[e], sum);
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (at == 0) {
+        const int64_t row = row0 + b + k * ROWS + sub;
+        p.nlse2[row] = live[k] ? -lse[k] * LOG2E : 0.f;
+        p.ndelta[row] = live[k] ? -sum : 0.f;
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------ dK, dV
@@ -424,13 +480,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // ------------------------------------------------------------------ dQ
-// warp 0: producer (rings of two K and two V tiles across all tiles of the CTA; Q, dO and out of the next tile
-// land in shared memory during this one); warp 1: MMA issuer; warps 2, 3: -lse log2e and -delta of the next
-// tile's rows, also for the other kernel; warps 4-11: compute.
+// warp 0: producer (rings of two K and two V tiles across all tiles of the CTA; Q and dO of the next tile land in
+// shared memory during this one); warp 1: MMA issuer; warps 2, 3: -lse log2e and -delta of the next tile's rows; warps
+// 4-11: compute.
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
     local_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-                       const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_dq,
+                       const __grid_constant__ CUtensorMap map_dq,
                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const BwdParams p) {
   constexpr int TILE_BYTES = TILE * D * 2, NBOX = D / 64, BOX_BYTES = TILE * 128;
@@ -444,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* k_smem = smem;                     // [2]
   uint8_t* v_smem = smem + 2 * TILE_BYTES;    // [2]
   uint8_t* land_smem = smem + 4 * TILE_BYTES; // Q, dO of the next tile
-  uint8_t* out_smem = smem + 6 * TILE_BYTES;  // dQ of the last tile on its way out, then out of the next one
+  uint8_t* out_smem = smem + 6 * TILE_BYTES;  // dQ of a tile on its way out
   float* stats = reinterpret_cast<float*>(smem + 7 * TILE_BYTES);  // [2][nlse, ndelta][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(stats + 4 * TILE);
   // Per step (g counts the steps of all tiles of this CTA), per tile (u): parity of g or u; rings: of g / 2.
@@ -515,12 +571,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       auto land = [&](int unit) {
         const Unit w = unit_at(unit);
-        ptx::mbar_expect_tx(land_full, 3 * NBOX * p.tile_tokens * a.G * 128);
+        ptx::mbar_expect_tx(land_full, 2 * NBOX * p.tile_tokens * a.G * 128);
 #pragma unroll
         for (int c = 0; c < NBOX; ++c) {
           tma_load_5d(land_smem + c * BOX_BYTES, &map_q, land_full, c * 64, 0, w.t0, w.hk, w.s);
           tma_load_5d(land_smem + TILE_BYTES + c * BOX_BYTES, &map_do, land_full, c * 64, 0, w.t0, w.hk, w.s);
-          tma_load_5d(out_smem + c * BOX_BYTES, &map_out, land_full, c * 64, 0, w.t0, w.hk, w.s);
         }
       };
       int g = 0, u = 0, keys = 0, landed = 1;  // steps, tiles; K tiles (g, or one more) and landings brought
@@ -547,8 +602,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           // the next tile's rows, once this tile's have been taken out (after the copies that are needed first)
           if (i == min(1, kr.count - 1) && unit + (int)gridDim.x < units) {
             ptx::mbar_wait(q_ready, u & 1, abort_flag, p.status, 123);
-            ptx::mbar_wait(&stats_full[u & 1], (u >> 1) & 1, abort_flag, p.status, 123);
-            ptx::mbar_wait(out_free, u & 1, abort_flag, p.status, 123);
             if ((stop = abort_flag[0] != 0)) {
               ++g;  // (this step's V is under way)
               break;
@@ -625,15 +678,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else if (warp < 4) {
     // -------------------------------------------------------------- -lse log2e, -delta
-    // entries of column tiles that belong to no row: zeros (the products that meet them see rows of zeros)
     const int t = threadIdx.x - 64;
-    {
-      const int64_t tiles = (int64_t)a.n * a.KV * p.col_tiles;
-      for (int64_t i = (int64_t)blockIdx.x * 64 + t; i < tiles; i += (int64_t)gridDim.x * 64) {
-        const int left = a.tokens - (int)(i % p.col_tiles) * p.col_tokens;
-        for (int c = min(left, p.col_tokens) * a.G; c < COLS; ++c) p.nlse2[i * COLS + c] = p.ndelta[i * COLS + c] = 0.f;
-      }
-    }
     int u = 0;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++u) {
       const Unit w = unit_at(unit);
@@ -641,23 +686,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {  // rows t and t + 64
         const int r = t + 64 * i;
-        nlse[i] = r < w.ntok * a.G ? -p.lse[((int64_t)w.s * a.H + w.hk * a.G + r % a.G) * a.tokens + w.t0 + r / a.G] * LOG2E : 0.f;
-      }
-      ptx::mbar_wait(land_full, u & 1, abort_flag, p.status, 131);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = t + 64 * i;
-        float acc = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          const int at = (c >> 3) * BOX_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-          float x[8], y[8];
-          unpack<T>(*reinterpret_cast<const uint4*>(out_smem + at), x);
-          unpack<T>(*reinterpret_cast<const uint4*>(land_smem + TILE_BYTES + at), y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc = fmaf(x[e], y[e], acc);
+        nlse[i] = ndelta[i] = 0.f;
+        if (r < w.ntok * a.G) {
+          const int pos = w.t0 + r / a.G;
+          const int64_t at = (((int64_t)w.s * a.KV + w.hk) * p.col_tiles + pos / p.col_tokens) * COLS + (pos % p.col_tokens) * a.G + r % a.G;
+          nlse[i] = p.nlse2[at];
+          ndelta[i] = p.ndelta[at];
         }
-        ndelta[i] = -acc;
       }
       ptx::mbar_wait(&stats_empty[u & 1], ((u >> 1) & 1) ^ 1, abort_flag, p.status, 131);
 #pragma unroll
@@ -665,14 +700,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int r = t + 64 * i;
         stats[(u & 1) * 2 * TILE + r] = nlse[i];
         stats[((u & 1) * 2 + 1) * TILE + r] = ndelta[i];
-        if (r < w.ntok * a.G) {
-          const int pos = w.t0 + r / a.G;
-          const int64_t at = (((int64_t)w.s * a.KV + w.hk) * p.col_tiles + pos / p.col_tokens) * COLS + (pos % p.col_tokens) * a.G + r % a.G;
-          p.nlse2[at] = nlse[i];
-          p.ndelta[at] = ndelta[i];
-        }
       }
-      ptx::fence_proxy_async_smem();  // (the landing zone is next written by copies)
       ptx::mbar_arrive(&stats_full[u & 1]);
     }
   } else {
@@ -787,10 +815,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         ptx::tc_fence_before();
         ptx::mbar_arrive(ds_ready);
       }
-      // dQ out through shared memory, where `out` of the next tile has been read (its statistics are there):
-      // each half of the warps takes half of the features
-      if (unit + (int)gridDim.x < units)
-        ptx::mbar_wait(&stats_full[(u + 1) & 1], ((u + 1) >> 1) & 1, abort_flag, p.status, 137);
+      // dQ out through shared memory, once the last tile's has left it: each half of the warps takes half of the features
+      ptx::mbar_wait(out_free, u & 1, abort_flag, p.status, 137);
       ptx::mbar_wait(tile_done, u & 1, abort_flag, p.status, 136);
       ptx::tc_fence_after();
 #pragma unroll
@@ -851,11 +877,10 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
                         cudaStream_t st) {
   const LocalArgs& a = b.f;
   const int col_tokens = COLS / a.G;
-  CUtensorMap mq, md, mq128, md128, mo128, mk, mv, mdq;
+  CUtensorMap mq, md, mq128, md128, mk, mv, mdq;
   bind_primary_context();
   if (!local_map_rows(&mq, q, a.qs, a, col_tokens, "q") || !local_map_rows(&md, dout, b.dos, a, col_tokens, "dout") ||
       !local_map_rows(&mq128, q, a.qs, a, TILE / a.G, "q") || !local_map_rows(&md128, dout, b.dos, a, TILE / a.G, "dout") ||
-      !local_map_rows(&mo128, out, a.os, a, TILE / a.G, "out") ||
       !local_map_rows(&mdq, dq, b.dqs, a, TILE / a.G, "dq") || !local_map_keys(&mk, k, a.ks, a, TILE, "k") ||
       !local_map_keys(&mv, v, a.vs, a, TILE, "v"))
     return TB200_ERR_UNSUPPORTED;
@@ -891,7 +916,9 @@ int launch_local_bwd_tc(void* dq, void* dk, void* dv, const void* dout, const vo
     if (int rc = optin(kkv, DKV_SMEM, done_kv)) return rc;
     if (int rc = optin(kq, DQ_SMEM, done_q)) return rc;
     const int64_t units = (int64_t)a.n * a.KV * p.row_tiles;
-    kq<<<(unsigned)(units < sm_count() ? units : sm_count()), THREADS, DQ_SMEM, st>>>(mq128, md128, mo128, mdq, mk, mv, p);
+    local_rows_tc_kernel<T, D><<<(unsigned)ceil_div(local_tc_rows(a), 16 * 8), 256, 0, st>>>((const T*)out, (const T*)dout, p);
+    if (int rc = launch_status("local_rows_tc")) return rc;
+    kq<<<(unsigned)(units < sm_count() ? units : sm_count()), THREADS, DQ_SMEM, st>>>(mq128, md128, mdq, mk, mv, p);
     if (int rc = launch_status("local_dq_tc")) return rc;
     kkv<<<(unsigned)parts, THREADS, DKV_SMEM, st>>>(mq, md, mk, mv, p);
     return launch_status("local_dkv_tc");

@@ -198,7 +198,9 @@ __device__ inline bool unit_at(const FwdParams& p, int unit, Unit* w) {
   return true;
 }
 
-template <typename T, int D, bool PAGED>
+// LOW: also writes what the rounding of the output leaves (training form), by the threads themselves: 179 us instead of
+// 167 at 2 x 32 heads x 4096 x 128, window 1024, 87 instead of 74 at a window of 128.
+template <typename T, int D, bool PAGED, bool LOW>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
     local_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
@@ -830,7 +832,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       const long long tok = w.seq.q_begin + token;
       const bool some = l > 0.f;  // (a row without keys: zeros)
       const float inv = some ? 1.f / l : 0.f;
-      T* orow = reinterpret_cast<T*>(p.out) + (long long)w.s * a.os[0] + head * a.os[1] + tok * a.os[2];
+      const long long oat = (long long)w.s * a.os[0] + head * a.os[1] + tok * a.os[2];
+      T* orow = reinterpret_cast<T*>(p.out) + oat;
       const long long prow = ((long long)w.split * a.tokens + tok) * a.H + head;
       if (live) {
         const float ls = some ? m_used * LN2 + logf(l) : -INFINITY;
@@ -876,6 +879,16 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
               o.y = am::cvt_pair<T>(__uint_as_float(x[2]), __uint_as_float(x[3]));
               o.z = am::cvt_pair<T>(__uint_as_float(x[4]), __uint_as_float(x[5]));
               o.w = am::cvt_pair<T>(__uint_as_float(x[6]), __uint_as_float(x[7]));
+              if (LOW && live) {  // what the rounding leaves
+                float y[8];
+                unpack<T>(o, y);
+                uint4 low;
+                low.x = am::cvt_pair<T>(__uint_as_float(x[0]) - y[0], __uint_as_float(x[1]) - y[1]);
+                low.y = am::cvt_pair<T>(__uint_as_float(x[2]) - y[2], __uint_as_float(x[3]) - y[3]);
+                low.z = am::cvt_pair<T>(__uint_as_float(x[4]) - y[4], __uint_as_float(x[5]) - y[5]);
+                low.w = am::cvt_pair<T>(__uint_as_float(x[6]) - y[6], __uint_as_float(x[7]) - y[7]);
+                *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.low) + oat + h * 64 + e * 8) = low;
+              }
               if (bulk)
                 *reinterpret_cast<uint4*>(out_smem + h * BOX_BYTES + r * 128 + ((e ^ (r & 7)) << 4)) = o;
               else if (live)
@@ -984,13 +997,13 @@ bool local_tc_supported(const LocalArgs& a, int dtype, const void* q, const void
 
 namespace {
 
-template <typename T, int D, bool PAGED>
+template <typename T, int D, bool PAGED, bool LOW>
 int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo, const FwdParams& p,
                cudaStream_t st) {
   constexpr int SMEM = 7 * TILE * D * 2 + 1024 + 384;  // (tiles, alignment, barriers and what follows them)
   static_assert(33 * 8 + 2 * sizeof(Walk) <= 384, "barriers, flags and walks");
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
-  auto kern = local_fwd_tc_kernel<T, D, PAGED>;
+  auto kern = local_fwd_tc_kernel<T, D, PAGED, LOW>;
   static std::atomic<unsigned long long> optin_done{0};
   static std::atomic<int> regs_cached{0};
   cudaError_t e = smem_optin_per_device(optin_done, reinterpret_cast<const void*>(kern), SMEM);
@@ -1044,7 +1057,8 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
   auto go = [&](auto tag, auto dsel) -> int {
     using T = decltype(tag);
     constexpr int D = decltype(dsel)::value;
-    return a.table ? launch_fwd<T, D, true>(mq, mk, mv, mo, p, st) : launch_fwd<T, D, false>(mq, mk, mv, mo, p, st);
+    return a.table ? launch_fwd<T, D, true, false>(mq, mk, mv, mo, p, st)
+           : a.low ? launch_fwd<T, D, false, true>(mq, mk, mv, mo, p, st) : launch_fwd<T, D, false, false>(mq, mk, mv, mo, p, st);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

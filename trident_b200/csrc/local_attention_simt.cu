@@ -291,6 +291,16 @@ __global__ void __launch_bounds__(Shape<D, RM, KEY_TILE, TX>::THREADS)
       for (int c = 0; c < Sh::DC; ++c)
 #pragma unroll
         for (int w = 0; w < Sh::W; ++w) o[((c * TX + tx) * Sh::W + w) * a.os[3]] = Traits<T>::from_f(acc[i][c][w] * inv);
+      if (a.low) {
+        T* low = reinterpret_cast<T*>(a.low) + (o - out);
+#pragma unroll
+        for (int c = 0; c < Sh::DC; ++c)
+#pragma unroll
+          for (int w = 0; w < Sh::W; ++w) {
+            const float x = acc[i][c][w] * inv;
+            low[((c * TX + tx) * Sh::W + w) * a.os[3]] = Traits<T>::from_f(x - Traits<T>::to_f(Traits<T>::from_f(x)));
+          }
+      }
       if (lse && tx == 0) lse[((int64_t)s * a.H + head) * a.tokens + token] = ls;
     } else {
       const int64_t row = ((int64_t)split * a.tokens + token) * a.H + head;
@@ -352,6 +362,7 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------ delta = sum_d out * dout
+// (out with what its rounding left, where that was kept)
 template <typename T>
 __global__ void __launch_bounds__(256)
     local_delta(float* delta, const T* out, const T* dout, const LocalArgs a, const LocalBwdArgs strides) {
@@ -363,7 +374,11 @@ __global__ void __launch_bounds__(256)
   const T* o = out + b * a.os[0] + h * a.os[1] + t * a.os[2];
   const T* g = dout + b * strides.dos[0] + h * strides.dos[1] + t * strides.dos[2];
   float acc = 0.f;
-  for (int d = lane; d < a.D; d += 32) acc = fmaf(Traits<T>::to_f(o[d * a.os[3]]), Traits<T>::to_f(g[d * strides.dos[3]]), acc);
+  const T* low = a.low ? reinterpret_cast<const T*>(a.low) + (o - out) : nullptr;
+  for (int d = lane; d < a.D; d += 32) {
+    const float x = Traits<T>::to_f(o[d * a.os[3]]) + (low ? Traits<T>::to_f(low[d * a.os[3]]) : 0.f);
+    acc = fmaf(x, Traits<T>::to_f(g[d * strides.dos[3]]), acc);
+  }
   acc = warp_sum(acc);
   if (lane == 0) delta[row] = acc;
 }

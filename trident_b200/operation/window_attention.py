@@ -32,9 +32,9 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, *args: Any, **kwargs: Any):
-        output, log_sum_exp, window_size, num_sinks = WindowAttention.run(*args)
+        output, low, log_sum_exp, window_size, num_sinks = WindowAttention.run(*args)
 
-        ctx.save_for_backward(*args[:3], output, log_sum_exp)
+        ctx.save_for_backward(*args[:3], output, low, log_sum_exp)
         ctx.window_size = window_size
         ctx.num_sinks = num_sinks
         ctx.softmax_scale = args[5]
@@ -43,8 +43,8 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def run(query, key, value, window_size, num_sinks, softmax_scale, statistics=True):
-        """The forward pass: (output, log-sum-exp of every score row or, without `statistics`, None, window and
-        sinks cut to the length)."""
+        """The forward pass: (output, what its rounding to 16 bits left, log-sum-exp of every score row, window and
+        sinks cut to the length). Without `statistics`, and the second of 32-bit operands, those of backward are None."""
         if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
             raise ValueError("The dimension of query, key and value should be 4.")
         if key.shape != value.shape:
@@ -64,15 +64,17 @@ class WindowAttention(torch.autograd.Function):
 
         util.push_trace("WindowAttention.__forward")
         output = torch.empty_like(query)  # laid out as query is
-        log_sum_exp = None
+        low = log_sum_exp = None
         if statistics:
+            if query.dtype != torch.float32:
+                low = torch.empty_like(output)
             log_sum_exp = torch.empty((batch, heads, y_size), device=query.device, dtype=torch.float32)
         util.push_trace("tb200_window_attention_fwd")
-        _lib.window_attention_fwd(output, log_sum_exp, query, key, value, window_size, num_sinks, softmax_scale)
+        _lib.window_attention_fwd(output, log_sum_exp, query, key, value, window_size, num_sinks, softmax_scale, low)
         util.pop_trace()
         util.pop_trace()
 
-        return output, log_sum_exp, window_size, num_sinks
+        return output, low, log_sum_exp, window_size, num_sinks
 
     @staticmethod
     def backward(ctx: Any, *grad_outputs: Any):
@@ -87,7 +89,7 @@ class WindowAttention(torch.autograd.Function):
         return (*util.first_order("Window attention", grads, grad_output, *ctx.saved_tensors), None, None, None)
 
     @staticmethod
-    def __backward(grad_output, query, key, value, output, log_sum_exp, window_size, num_sinks, softmax_scale):
+    def __backward(grad_output, query, key, value, output, low, log_sum_exp, window_size, num_sinks, softmax_scale):
         """delta, dq, dk and dv (and, with sinks, the sum of their parts)."""
         if 0 in grad_output.stride():
             # (an expanded gradient, as that of a sum: the kernels read whole rows)
@@ -114,6 +116,7 @@ class WindowAttention(torch.autograd.Function):
             window_size,
             num_sinks,
             softmax_scale,
+            low,
         )
         util.pop_trace()
 
