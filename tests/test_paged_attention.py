@@ -776,3 +776,33 @@ def test_listed_pieces_in_a_graph(device):
         torch.cuda.synchronize()
         assert torch.equal(out[: sum(new)], attend(*args)[: sum(new)])
     assert _lib.device_status() == 0
+
+
+# ------------------------------------------------------------------------------------ what is written
+def test_expanded_tensors_are_not_written():
+    args = _cpu_call()
+    one = torch.randn(3, 1, 16)
+    with pytest.raises(ValueError, match="output should not be expanded"):
+        attend(**args, output=one.expand(3, 4, 16))
+    del args["query"]
+    k = torch.randn(3, 2, 16)
+    for name in ("key_cache", "value_cache"):
+        for shape in ((1, 8, 2, 16), (5, 8, 1, 16)):
+            with pytest.raises(ValueError, match=f"{name} should not be expanded"):
+                append(k, k, **{**args, name: torch.zeros(shape).expand(5, 8, 2, 16)})
+    with pytest.raises(_lib.Tb200Error, match="CUDA tensors only"):  # (a dimension of one may have any stride)
+        append(k[:, :1], k[:, :1], **{**args, "key_cache": torch.zeros(5, 8, 16).unsqueeze(2).as_strided((5, 8, 1, 16), (128, 16, 0, 1)),
+                                     "value_cache": torch.zeros(5, 8, 1, 16)})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_output_may_be_the_query(D, dtype, device):
+    """Each row is read by the pieces of work that write it, before they do."""
+    for new in ([1, 1], [3, 200]):
+        cache = Cache([2500, 300], 2, D, 16, dtype, device, seed=150)
+        q = util.randn(sum(new), 8, D, seed=151).to(dtype)
+        mine = q.to(device)
+        attend(mine, cache.key_cache, cache.value_cache, cache.table_dev, cache.context_dev, _offsets(new, device),
+               max_query_length=max(new), output=mine)
+        ref.check(mine, _want(q, cache, new, 0, 0, D ** -0.5, dtype), f"{new}")

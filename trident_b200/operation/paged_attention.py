@@ -57,6 +57,12 @@ def _check_room(block_table, key_cache):
         raise ValueError("block_table should have a block for every sequence and the cache at least one page.")
 
 
+def _check_written(name, tensor):
+    """A tensor that is written must have a place of its own for each element."""
+    if 0 in tensor.stride() and any(st == 0 and size > 1 for st, size in zip(tensor.stride(), tensor.shape)):
+        raise ValueError(f"{name} should not be expanded: some of its elements share their memory.")
+
+
 def _index(tensor):
     """An int32 tensor whose last dimension is dense."""
     return tensor if tensor is None or tensor.numel() == 0 or tensor.stride(-1) == 1 else tensor.contiguous()
@@ -91,6 +97,8 @@ def paged_attention(
         check_window(window_size, num_sinks)
     if output is not None and output.shape != query.shape:
         raise ValueError("output and query should have the same shape.")
+    if output is not None:
+        _check_written("output", output)
     if query_offsets is None:
         max_query_length = 1
     elif max_query_length is None:
@@ -156,6 +164,8 @@ def paged_cache_append(key, value, key_cache, value_cache, block_table, context_
     if key.shape[1:] != key_cache.shape[2:]:
         raise ValueError("key and key_cache should have the same heads and head size.")
     check_heads(key.shape[1], key.shape[1], key.shape[2])
+    _check_written("key_cache", key_cache)
+    _check_written("value_cache", value_cache)
     _lib.require_one_device(
         key_cache, value_cache, block_table, context_lengths, query_offsets, *tensors.values()
     )
