@@ -425,7 +425,7 @@ def test_error_of_short_windows(D, KV, G, dt, device):
     times the sum of p k, the more the shorter the window is. With delta of the unrounded output the roundings of the
     score gradients (an operand of the tensor cores: not at D = 32) and of dq itself remain. A rounding is off by at most
     half a step of 2 u of its value, spread over it evenly by 2 u / sqrt(12) in the mean, and less for mantissas
-    above 1; the two of them by sqrt(2) times that. (delta of the rounded output: 0.0044 at a window of 2 in bf16.)"""
+    above 1; the two of them by sqrt(2) times that. (delta of the rounded output: 0.0038 at a window of 2 in bf16.)"""
     u = torch.finfo(dt).eps / 2
     bound = 2 * u / 12 ** 0.5 * (2 ** 0.5 if D >= 64 else 1.0)
     for window in (2, 3):

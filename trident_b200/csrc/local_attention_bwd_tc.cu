@@ -23,8 +23,8 @@
 // about as long as a walk inside the window, each a CTA of its own: a single CTA would walk all queries.
 //
 // P and dS are rounded to 16 bits as operands of their products, as the tensor cores take them: half a step each
-// (2-norm of the error of dq against 64 bits 0.0024 in bf16, 0.00031 in fp16 at any window, of which the final rounding
-// alone is 0.0017 and 0.00021; with delta of the rounded output it was 0.0026 at a window of 1024 and 0.0044 at 2).
+// (2-norm of the error of dq against 64 bits 0.0025 in bf16, 0.00031 in fp16 at any window, of which the final rounding
+// alone is 0.0017 and 0.00021; with delta of the rounded output it was 0.0026 at a window of 1024 and 0.0038 at 2).
 // fp16 score gradients below 2^-14 are multiples of 2^-24. Statistics, delta and all sums are fp32.
 //
 // Bounds, at 2 x 32 heads x 4096 x 128 bf16, window 1024, 8 key heads. dK, dV: 252 us (957 TFLOP/s); a step takes
