@@ -12,7 +12,7 @@
 //             heads of a group is part of the walk, in a fixed order
 // A thread issues 8 16-byte reads for 64 multiply-adds of a score tile's 4 features. At 8 heads, 1024 tokens,
 // window 256, D = 64 (128 CTAs, 8 warps an SM) the kernels wait for those reads and the tiles' loads: dK/dV
-// 77 us with the multiply-adds 30 % and shared memory 44 % busy, dQ 52, forward 40. In the backward kernels a
+// 77 us, dQ 52, forward 40, the multiply-adds 30 % and the issue slots 42 % busy in each. In the backward kernels a
 // warp covers 4 x 8 threads of the tile (2 x 16 and 32 streamed rows: 92 and 57 us); 8 columns a thread need
 // a quarter fewer reads, but leave 4 warps an SM (110, 71 and 57 us).
 #include <type_traits>

@@ -31,6 +31,8 @@ int launch_local_fwd_tc(void* out, float* lse, const void* q, const void* k, con
 // Serving form with few rows: keys on the tensor-memory lanes, LOCAL_FEW_ROWS columns. 64 contexts of 4096 bf16
 // keys, 8 key heads: 4, 8, 16 rows take 149, 157, 175 us at D = 64 and 220, 230, 253 at D = 128, the forward
 // kernel 204 to 212 and 247 to 253; 4 contexts of 16384: 68, 73, 83 against 74 to 76, and 87, 93, 103 against 85.
+// The rule sees rows and head size alone (the lengths lie on the device, and the announced longest says little of the
+// others): where a few long contexts are all there is, it costs up to 12 %.
 // (Of 32 and 64 columns the per-row work of every thread outweighs the loads: 304 and 1177 us against 219 and 229.)
 constexpr int LOCAL_FEW_ROWS = 16;
 static inline bool local_few_rows(const LocalArgs& a, int max_q) {
