@@ -436,3 +436,33 @@ def test_error_of_short_windows(D, KV, G, dt, device):
             value = want[name][0]
             off = ((got[name].double().cpu() - value).norm() / value.norm()).item()
             assert off < bound, (window, name, off, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt, D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 32), (torch.float32, 64)], ids=str)
+def test_entry_points_without_the_rest_of_the_output(dt, D, device):
+    """The C entry points that keep nothing of what the output's rounding leaves: the same output, gradients in bounds."""
+    q, k, v, dout = problem = _problem(2, 2, 2, 500, D, dt, seed=97)
+    q, k, v, dout = (t.to(device) for t in problem)
+    window, sinks, scale = 40, 3, D ** -0.5
+    out, dq, dk, dv = (torch.empty_like(t) for t in (q, q, k, v))
+    lse = torch.empty(2, 4, 500, device=device)
+    code = _lib.dtype_code(dt)
+    sizes, strides = (2, 4, 2, 500, D), [t.stride() for t in (q, k, v, out)]
+    _lib._call("tb200_window_attention_fwd", q, *(t.data_ptr() for t in (out, lse, q, k, v)), *sizes, *strides, window, sinks, scale, code)
+    work = torch.empty(_lib.window_attention_bwd_workspace(q, k, window, sinks), dtype=torch.uint8, device=device)
+    _lib._call("tb200_window_attention_bwd", q, *(t.data_ptr() for t in (dq, dk, dv, dout, q, k, v, out, lse, work)), work.numel(),
+               *sizes, *strides, *(t.stride() for t in (dout, dq, dk, dv)), window, sinks, scale, code)
+    assert torch.equal(out, F(q, k, v, window, sinks))
+    want = ref.batched(*problem[:3], window, sinks, scale, dt, problem[3])
+    for name, got in (("out", out), ("dv", dv), ("dq", dq), ("dk", dk)):
+        ref.check(got, want[name], name)
+
+
+def test_entry_points_with_the_rest_of_the_output_refuse():
+    strides = (1, 1, 1, 1)
+    forward, backward = (_lib._entry(f"tb200_window_attention_{name}_low") for name in ("fwd", "bwd"))
+    assert forward(8, 8, 8, 8, 8, 8, 1, 3, 2, 8, 16, *[strides] * 4, 4, 0, 1.0, 0, 0) == -1  # heads
+    assert forward(None, 8, 8, 8, 8, 8, 1, 2, 2, 8, 16, *[strides] * 4, 4, 0, 1.0, 0, 0) == -1
+    assert backward(*[8] * 11, 0, 1, 2, 2, 8, 16, *[strides] * 8, 4, 0, 1.0, 0, 0) == -3  # no workspace
+    assert backward(*[8] * 7, None, *[8] * 3, 1 << 20, 1, 2, 2, 8, 16, *[strides] * 8, 4, 0, 1.0, 0, 0) == -1
